@@ -42,6 +42,11 @@
  *                                forward.rs:1745-1761), with the pick fused into its epilogue:
  *                                the GEMM's tiles publish mxs_epilogue.h statistics and the
  *                                finish-only pick reads those and the tiles a head can reach.
+ *   mxs_beam_select,          <- (no counterpart: the reference decodes one sequence per
+ *   mxs_beam_reorder             request.)  Beam search: the selection over beams and
+ *                                vocabulary, and the move of the beams' states.
+ *   mxs_linear_bf16           <- the projections around the lm_head (forward.rs:1745-1761)
+ *                                with bias, activation and residual in the epilogue.
  *   mxs_sync                  <- Qwen3TokenPicks::wait (picks.rs:390-401).
  *   mxs_last_error            <- KernelError's message (mlx-kernels/src/lib.rs:444-450).
  *
@@ -96,7 +101,8 @@ enum {
   MXS_ROW_INVALID_BIAS = -12,
   MXS_ROW_TOKEN_OUT_OF_RANGE = -13,
   MXS_ROW_PROBABILITIES = -14,
-  MXS_ROW_UNSUPPORTED_RULE = -15  /* mxs_finish_tiles: a rule other than greedy or top-k <= 4096 */
+  MXS_ROW_UNSUPPORTED_RULE = -15, /* mxs_finish_tiles: a rule other than greedy or top-k <= 4096 */
+  MXS_ROW_INVALID_PARENT = -16    /* mxs_beam_reorder: a parent outside the group */
 };
 
 typedef enum { MXS_F32 = 0, MXS_BF16 = 1 } mxs_dtype;
@@ -282,6 +288,114 @@ int mxs_lmhead_bf16(mxs_ctx* ctx, const void* hidden, const void* weight, uint32
  * than mxs_sample; a row with k above the tile count reads its row twice in
  * one workgroup, slower than mxs_sample's chunked read. */
 int mxs_finish_tiles(mxs_ctx* ctx, const mxs_batch* batch, const void* tile_stats, const mxs_out* out);
+/* Beam search (no counterpart in the reference, which decodes one sequence
+ * per request).  A batch is `groups` requests of `beams` sequences; row
+ * g * beams + b is beam b of group g.
+ *
+ * mxs_beam_select picks each group's n best continuations over all its beams
+ * and the vocabulary.  A live beam's candidate for token v has the score
+ * score[row] + (l[v] - ln sum_u exp(l[u])) in f64, over the row's logits l;
+ * an ended beam (`ended` nonzero) is one candidate with end_token and its own
+ * score, and its logits are not read.  Candidates are ordered by
+ * score * scale[row] (a length penalty; NULL => by score), largest first;
+ * equal ones by lower beam, larger logit, lower token.  The logarithm of the
+ * sum is within 2^-39 of exact, so candidates of different beams closer than
+ * that may come in either order.
+ *
+ * A score of -inf is a beam that is not there (the first step has one live
+ * beam a group).  A logit of -inf is a token that cannot follow: it weighs
+ * nothing and is no candidate.  The mask removes candidates; the sum is over
+ * the whole row, or over the legal tokens when legal_norm is nonzero (then
+ * the logits of other tokens are not looked at).  A beam left without legal
+ * tokens has no candidates.  Where a group has fewer than n, the rest of its
+ * entries are token -1, beam -1, score -inf, ended 0.
+ *
+ * status[g]: 0, MXS_ROW_PROBABILITIES (a score NaN or +inf, a scale not
+ * finite and positive), MXS_ROW_NON_FINITE_LOGIT (a NaN or +inf among the
+ * logits that count) or MXS_ROW_EMPTY_SUPPORT (no candidate).  With the first
+ * two every entry is token -1, beam -1, score NaN, ended 0. */
+#define MXS_BEAM_MAX 64    /* beams per group */
+#define MXS_BEAM_N_MAX 128 /* candidates per group */
+typedef struct {
+  const void* logits;             /* groups * beams rows of row_stride elements of `dtype` */
+  int32_t dtype;                  /* mxs_dtype */
+  uint32_t groups;                /* groups * beams <= the context's max_rows */
+  uint32_t beams;                 /* 1..MXS_BEAM_MAX */
+  uint32_t vocab;
+  uint64_t row_stride;            /* elements between row starts; multiple of 4 */
+  const double* score;            /* required: groups x beams cumulative log probabilities */
+  const uint8_t* ended;           /* groups x beams; NULL => none has ended */
+  const double* scale;            /* groups x beams; NULL => 1 */
+  const uint32_t* mask_words;     /* as mxs_batch's; NULL => every token is legal */
+  uint64_t mask_stride;
+  uint32_t tokenizer_vocab;       /* with a mask: tokens at or past it are never legal */
+  uint32_t legal_norm;            /* with a mask: nonzero => probabilities over the legal tokens */
+  uint32_t n;                     /* candidates per group, 1..MXS_BEAM_N_MAX */
+  int32_t end_token;              /* the token that ends a beam; -1 => none (then `ended` must be NULL) */
+} mxs_beam;
+typedef struct {
+  int32_t* token;                 /* groups x n, best first */
+  int32_t* beam;                  /* groups x n: the candidate's beam within its group */
+  double* score;                  /* groups x n, without the scale; with n == beams it may be the input scores' array */
+  uint8_t* ended;                 /* groups x n: 1 when the candidate has ended; with n == beams it may be the input's array; NULL => not written */
+  int32_t* status;                /* groups */
+} mxs_beam_out;
+int mxs_beam_select(mxs_ctx* ctx, const mxs_beam* beam, const mxs_beam_out* out);
+/* Moves what each beam carries (key-value caches, recurrent states, token
+ * histories) to the beams that a selection made of it, in place: row
+ * g * beams + b of every state becomes what row g * beams + parent[g][b] was.
+ * A parent of -1 leaves its row as it is; a group with any other parent
+ * outside 0..beams-1 is left as it is, with status MXS_ROW_INVALID_PARENT.
+ * A row of a state is `segments` pieces of segment_bytes, segment_stride
+ * apart; all lengths in bytes, at any alignment.  With `lengths`, only the
+ * first lengths[g] * position_bytes bytes of each segment move (states with
+ * position_bytes 0 move whole).  Each surviving row is read once and each
+ * changed row written once, whatever the permutation.  Rows and segments of
+ * a state must not overlap, nor two states (the latter is not checked). */
+typedef struct {
+  void* data;
+  uint64_t row_stride;
+  uint64_t segment_stride;
+  uint64_t segment_bytes;
+  uint64_t position_bytes;
+  uint32_t segments;
+  uint32_t reserved;
+} mxs_state;
+typedef struct {
+  const mxs_state* states;        /* host array of `count`, read during the call */
+  uint32_t count;
+  uint32_t groups, beams;         /* beams 1..MXS_BEAM_MAX */
+  uint32_t parent_stride;         /* entries between the groups' parents, >= beams */
+  const int32_t* parent;          /* device: groups x parent_stride */
+  const int32_t* lengths;         /* device: groups, the positions in use; NULL => whole segments */
+  int32_t* status;                /* device: groups; 0 or MXS_ROW_INVALID_PARENT */
+} mxs_reorder;
+int mxs_beam_reorder(mxs_ctx* ctx, const mxs_reorder* reorder);
+/* A bf16 matrix product with its epilogue:
+ *   out[r][o] = act(sum_k x[r][k] weight[o][k] + bias[o]) + residual[r][o]
+ * x rows x in_features and weight out_features x in_features row-major bf16
+ * (16-byte aligned, strides multiples of 8 elements; nothing past a row's
+ * in_features is read), products summed in f32, the epilogue in f32 with
+ * one rounding to the output type.  Any number of rows and features.  bias
+ * f32 or bf16 (bias_dtype) or NULL; residual of out's type or NULL; it may be
+ * out itself (same stride), otherwise out may overlap no input. */
+enum { MXS_ACT_NONE = 0, MXS_ACT_RELU = 1, MXS_ACT_SILU = 2, MXS_ACT_GELU = 3 /* erf */, MXS_ACT_GELU_TANH = 4 };
+typedef struct {
+  const void* x;
+  uint64_t x_stride;
+  const void* weight;
+  uint64_t weight_stride;
+  const void* bias;
+  const void* residual;
+  uint64_t residual_stride;
+  void* out;
+  uint64_t out_stride;
+  uint32_t rows, in_features, out_features;
+  int32_t act;                    /* MXS_ACT_* */
+  int32_t out_dtype;              /* mxs_dtype of out and residual */
+  int32_t bias_dtype;             /* mxs_dtype of bias */
+} mxs_linear;
+int mxs_linear_bf16(mxs_ctx* ctx, const mxs_linear* linear);
 int mxs_mask_host(mxs_ctx* ctx, uint32_t slot, uint32_t** words, uint64_t* stride_words);
 int mxs_mask_upload(mxs_ctx* ctx, uint32_t slot, uint32_t rows, const uint32_t** device_words);
 int mxs_sync(mxs_ctx* ctx);

@@ -6,11 +6,14 @@ host binding used by tests and the benchmark; device memory and streams come
 from PyTorch.  There is no CPU fallback: every entry point fails loudly when
 the built library or a GPU is missing.
 """
+from .beam import BeamSearch, Hypothesis  # noqa: F401
 from .sampler import (  # noqa: F401
+    ACTIVATIONS,
     LIB_PATH,
     MXS_BF16,
     MXS_F32,
     ROW_STATUS,
+    BeamResult,
     Sampler,
     SamplerError,
     load_library,

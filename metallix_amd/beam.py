@@ -1,0 +1,99 @@
+"""Beam search on the device: a batch of requests, several sequences each.
+
+The reference decodes one sequence per request (EngineLoop::decode_now,
+crates/app/cli/src/engine_loop.rs:1080-1134); this is the step that stands in
+its place for requests that search.  `BeamSearch.step` takes the logits of all
+live sequences and queues the selection (mxs_beam_select) and the move of what
+each sequence carries (mxs_beam_reorder: the caller's states, the token
+histories, the lengths) on the sampler's stream; nothing is read back until
+`result`.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import List, Optional
+
+from .sampler import BeamResult
+
+
+@dataclass
+class Hypothesis:
+    """One sequence a search found: its tokens (the end token included when
+    it ended), its cumulative log probability and whether it ended."""
+    tokens: List[int]
+    score: float
+    ended: bool
+
+
+class BeamSearch:
+    """groups x beams sequences over one Sampler.  Row g * beams + b of every
+    tensor is beam b of group g; a group starts with one live beam, beam 0.
+    Ended beams stay in the race with their score.  length_penalty a orders
+    the candidates by score * ((5 + length) / 6) ** -a."""
+
+    def __init__(self, sampler, groups: int, beams: int, max_new: int, *, end_token: Optional[int] = None,
+                 length_penalty: float = 0.0):
+        torch = sampler.torch
+        self.sampler, self.groups, self.beams, self.max_new = sampler, groups, beams, max_new
+        self.end_token, self.length_penalty = end_token, float(length_penalty)
+        self.steps = 0
+        dev = torch.device("cuda", sampler.device)
+        rows = groups * beams
+        with torch.cuda.stream(sampler.stream):
+            self.score = torch.full((groups, beams), float("-inf"), dtype=torch.float64, device=dev)
+            self.score[:, 0] = 0.0
+            self.ended = torch.zeros((groups, beams), dtype=torch.bool, device=dev)
+            self.tokens = torch.full((rows, max_new), -1, dtype=torch.int32, device=dev)
+            self.length = torch.zeros((rows, 1), dtype=torch.int32, device=dev)
+            e = lambda *s: torch.empty(s, dtype=torch.int32, device=dev)
+            self.picked = BeamResult(token=e(groups, beams), beam=e(groups, beams), score=self.score, ended=self.ended,
+                                     status=e(groups))
+            self.moved = e(groups)
+
+    def step(self, logits, states=(), *, lengths=None, length_dim=None, **rule):
+        """Queues one step over `logits` [groups * beams, vocab]: picks each
+        group's best continuations (`rule`: mask, legal_norm, ... of
+        Sampler.beam_select), moves `states` (tensors of groups * beams rows,
+        the first lengths[g] positions of their length_dim) and the search's
+        own rows to them.  Returns the rows' next tokens, int32[groups *
+        beams] on the device (-1: no sequence; an ended one's end token)."""
+        if self.steps >= self.max_new:
+            raise ValueError(f"the search holds {self.max_new} tokens")
+        s, torch = self.sampler, self.sampler.torch
+        with torch.cuda.stream(s.stream):
+            if self.end_token is not None:
+                rule = dict(rule, ended=self.ended, end_token=self.end_token)
+            if self.length_penalty:
+                n = torch.where(self.ended, self.length.view(self.groups, self.beams), self.steps + 1)
+                rule = dict(rule, scale=((5.0 + n.double()) / 6.0) ** -self.length_penalty)
+            if self.end_token is not None:
+                self.length.masked_fill_(~self.ended.view(-1, 1), self.steps + 1)
+            else:
+                self.length.fill_(self.steps + 1)
+            s.beam_select(logits, self.score, self.beams, out=self.picked, **rule)
+            dims = list(length_dim) if isinstance(length_dim, (list, tuple)) else [length_dim] * len(states)
+            s.beam_reorder([*states, self.tokens, self.length], self.picked.beam, lengths=lengths,
+                           length_dim=[*dims, None, None], status=self.moved)
+            self.tokens[:, self.steps] = self.picked.token.view(-1)
+        self.steps += 1
+        return self.picked.token.view(-1)
+
+    def done(self) -> bool:
+        """Whether every sequence has ended or is not there (reads back)."""
+        self.sampler.sync()
+        return bool((self.ended | (self.score == float("-inf")) | self.score.isnan()).all())
+
+    def result(self) -> List[List[Hypothesis]]:
+        """Each group's hypotheses, best first (reads back)."""
+        self.sampler.sync()
+        tokens, length = self.tokens.cpu().tolist(), self.length.cpu().view(-1).tolist()
+        score, ended = self.score.cpu().tolist(), self.ended.cpu().tolist()
+        out = []
+        for g in range(self.groups):
+            hyps = []
+            for b in range(self.beams):
+                r = g * self.beams + b
+                if score[g][b] > float("-inf"):
+                    hyps.append(Hypothesis(tokens[r][: length[r]], score[g][b], ended[g][b]))
+            out.append(hyps)
+        return out

@@ -7019,6 +7019,7 @@ const char* mxs_status_string(int32_t s) {
     case MXS_ROW_TOKEN_OUT_OF_RANGE: return "drafted token outside the vocabulary";
     case MXS_ROW_PROBABILITIES: return "invalid probability vectors";
     case MXS_ROW_UNSUPPORTED_RULE: return "the finish-only pick serves greedy and top-k (k <= 4096) rows";
+    case MXS_ROW_INVALID_PARENT: return "a beam's parent must be -1 or a beam of its group";
     default: return "unknown status";
   }
 }
@@ -7065,6 +7066,9 @@ int mxs_create(int device, void* stream, uint32_t max_rows, uint32_t max_vocab, 
   e = e ? e : hipMalloc(&ctx->race_scratch, mxs::race_scratch_bytes(max_rows, max_vocab));
   e = e ? e : hipMalloc(&ctx->race_kept, (size_t)max_rows * ((max_vocab + 31u) / 32u) * sizeof(uint32_t));
   e = e ? e : hipMalloc(&ctx->race_m, (size_t)max_rows * sizeof(float));
+  e = e ? e : hipMalloc(&ctx->beam_ctr, (size_t)max_rows * mxs::CTR_STRIDE * sizeof(uint32_t));
+  e = e ? e : hipMemset(ctx->beam_ctr, 0, (size_t)max_rows * mxs::CTR_STRIDE * sizeof(uint32_t));
+  e = e ? e : hipMalloc(&ctx->beam_scratch, mxs::beam_scratch_bytes(max_rows));
   const size_t nr = (size_t)max_rows + 1, nwords = (size_t)max_vocab / 32 + 2;
   e = e ? e : hipMalloc(&ctx->d_zero_u32, nr * sizeof(uint32_t));
   e = e ? e : hipMalloc(&ctx->d_one_f64, nr * sizeof(double));
@@ -7121,6 +7125,8 @@ int mxs_destroy(mxs_ctx* ctx) {
   hipFree(ctx->race_scratch);
   hipFree(ctx->race_kept);
   hipFree(ctx->race_m);
+  hipFree(ctx->beam_ctr);
+  hipFree(ctx->beam_scratch);
   mxs::mask_release(ctx);
   hipSetDevice(prev);
   delete ctx;

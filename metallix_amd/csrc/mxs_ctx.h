@@ -45,6 +45,7 @@ size_t topn_scratch_bytes(uint32_t max_rows);
 const char* noalloc_last_error();   // this thread's last mxs_logsoftmax_topn_noalloc error, or nullptr
 size_t spec_scratch_bytes(uint32_t max_rows, uint32_t max_vocab);
 size_t race_scratch_bytes(uint32_t max_rows, uint32_t max_vocab);
+size_t beam_scratch_bytes(uint32_t max_rows);
 constexpr uint32_t SPEC_COUNTERS_PER_ROW = 10;   // one per (row, position <= 8), one per row
 
 // Rows' counters and exchange words sit on their own 128-byte lines, so the
@@ -99,6 +100,9 @@ struct mxs_ctx {
   void* race_scratch = nullptr;
   uint32_t* race_kept = nullptr;
   float* race_m = nullptr;   // each row's largest adjusted logit, from the finisher to the race kernel
+  // mxs_beam_select: per-group arrival counters, per-chunk results
+  uint32_t* beam_ctr = nullptr;
+  void* beam_scratch = nullptr;
   // the uniform of the inverse-CDF draw mxs_sample_race discards (below)
   double* d_race_u = nullptr;
   // grammar-mask staging (mxs_mask_host / mxs_mask_upload, mx_mask.hip):

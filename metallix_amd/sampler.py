@@ -38,6 +38,7 @@ ROW_STATUS = {
     -13: "TokenOutOfRange",
     -14: "Probabilities",
     -15: "UnsupportedRule",   # mxs_finish_tiles: a rule other than greedy or top-k
+    -16: "InvalidParent",     # mxs_beam_reorder: a parent outside the group
 }
 
 _vp = ctypes.c_void_p
@@ -74,6 +75,46 @@ class MxsReceipts(ctypes.Structure):
     ]
 
 
+class MxsBeam(ctypes.Structure):
+    _fields_ = [
+        ("logits", _vp), ("dtype", ctypes.c_int32), ("groups", ctypes.c_uint32), ("beams", ctypes.c_uint32),
+        ("vocab", ctypes.c_uint32), ("row_stride", ctypes.c_uint64),
+        ("score", _vp), ("ended", _vp), ("scale", _vp),
+        ("mask_words", _vp), ("mask_stride", ctypes.c_uint64), ("tokenizer_vocab", ctypes.c_uint32),
+        ("legal_norm", ctypes.c_uint32), ("n", ctypes.c_uint32), ("end_token", ctypes.c_int32),
+    ]
+
+
+class MxsBeamOut(ctypes.Structure):
+    _fields_ = [("token", _vp), ("beam", _vp), ("score", _vp), ("ended", _vp), ("status", _vp)]
+
+
+class MxsState(ctypes.Structure):
+    _fields_ = [
+        ("data", _vp), ("row_stride", ctypes.c_uint64), ("segment_stride", ctypes.c_uint64),
+        ("segment_bytes", ctypes.c_uint64), ("position_bytes", ctypes.c_uint64),
+        ("segments", ctypes.c_uint32), ("reserved", ctypes.c_uint32),
+    ]
+
+
+class MxsReorder(ctypes.Structure):
+    _fields_ = [
+        ("states", ctypes.POINTER(MxsState)), ("count", ctypes.c_uint32), ("groups", ctypes.c_uint32),
+        ("beams", ctypes.c_uint32), ("parent_stride", ctypes.c_uint32), ("parent", _vp), ("lengths", _vp),
+        ("status", _vp),
+    ]
+
+
+class MxsLinear(ctypes.Structure):
+    _fields_ = [
+        ("x", _vp), ("x_stride", ctypes.c_uint64), ("weight", _vp), ("weight_stride", ctypes.c_uint64),
+        ("bias", _vp), ("residual", _vp), ("residual_stride", ctypes.c_uint64), ("out", _vp),
+        ("out_stride", ctypes.c_uint64), ("rows", ctypes.c_uint32), ("in_features", ctypes.c_uint32),
+        ("out_features", ctypes.c_uint32), ("act", ctypes.c_int32), ("out_dtype", ctypes.c_int32),
+        ("bias_dtype", ctypes.c_int32),
+    ]
+
+
 # Exported symbols and their prototypes, as declared in include/mx_sampler.h.
 PROTOTYPES = {
     "mxs_abi_version": (ctypes.c_int, []),
@@ -99,6 +140,9 @@ PROTOTYPES = {
     "mxs_lmhead_bf16": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32, _vp,
                                        ctypes.c_uint64, _vp]),
     "mxs_finish_tiles": (ctypes.c_int, [_vp, ctypes.POINTER(MxsBatch), _vp, ctypes.POINTER(MxsOut)]),
+    "mxs_beam_select": (ctypes.c_int, [_vp, ctypes.POINTER(MxsBeam), ctypes.POINTER(MxsBeamOut)]),
+    "mxs_beam_reorder": (ctypes.c_int, [_vp, ctypes.POINTER(MxsReorder)]),
+    "mxs_linear_bf16": (ctypes.c_int, [_vp, ctypes.POINTER(MxsLinear)]),
     "mxs_debug_set_timing": (ctypes.c_int, [_vp, _vp]),
     "mxs_debug_floor": (ctypes.c_int, [_vp, _vp, ctypes.c_int32, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32,
                                        ctypes.c_uint32, _vp, _vp]),
@@ -117,6 +161,11 @@ ABI_VERSION = 2                 # MXS_ABI_VERSION of include/mx_sampler.h
 RECEIPT_NONE = 0xFFFFFFFF       # MXS_RECEIPT_NONE: a receipt_top entry for "no receipt"
 TILE_TOKENS = 256               # MXS_TILE_TOKENS: vocabulary entries per epilogue-statistics tile
 TILE_STAT_BYTES = 8             # MXS_TILE_STAT_BYTES: bytes per (row, tile)
+
+
+BEAM_MAX = 64                   # MXS_BEAM_MAX: beams per group
+BEAM_N_MAX = 128                # MXS_BEAM_N_MAX: candidates per group
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}   # MXS_ACT_*
 
 
 def load_library(path: Optional[Path] = None):
@@ -182,6 +231,174 @@ def _ptr(t) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+def _need(t, name: str, device, dtypes, shape) -> None:
+    """Raises ValueError unless `t` is a tensor on `device` of one of the
+    dtypes and of the shape (None: any size)."""
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}, not {t.device}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, not {t.dtype}")
+    if t.dim() != len(shape) or any(want is not None and got != want for got, want in zip(t.shape, shape)):
+        raise ValueError(f"{name} must have the shape {list(shape)}, not {list(t.shape)}")
+
+
+def _dense(t, name: str) -> None:
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _float_code(torch, dtype) -> int:
+    return MXS_BF16 if dtype == torch.bfloat16 else MXS_F32
+
+
+def beam_struct(torch, device, logits, score, n: int, *, ended=None, end_token: Optional[int] = None, scale=None,
+                mask=None, tokenizer_vocab: Optional[int] = None, legal_norm: bool = False,
+                vocab: Optional[int] = None) -> MxsBeam:
+    """The mxs_beam of a call, its tensors checked against `device` and each
+    other (ValueError)."""
+    _need(score, "score", device, (torch.float64,), (None, None))
+    groups, beams = score.shape
+    V = logits.shape[-1] if vocab is None else int(vocab)
+    _need(logits, "logits", device, (torch.float32, torch.bfloat16), (groups * beams, None))
+    if not 0 < V <= logits.shape[1] or logits.stride(1) != 1:
+        raise ValueError("logits rows must hold `vocab` consecutive elements")
+    _dense(score, "score")
+    if ended is not None:
+        _need(ended, "ended", device, (torch.bool, torch.uint8), (groups, beams))
+        _dense(ended, "ended")
+    if scale is not None:
+        _need(scale, "scale", device, (torch.float64,), (groups, beams))
+        _dense(scale, "scale")
+    b = MxsBeam()
+    b.logits, b.dtype = logits.data_ptr(), _float_code(torch, logits.dtype)
+    b.groups, b.beams, b.vocab = groups, beams, V
+    # (a single row's stride says nothing: any multiple of 4 that holds it)
+    b.row_stride = logits.stride(0) if groups * beams > 1 else (V + 3) // 4 * 4
+    b.score, b.ended, b.scale = score.data_ptr(), _ptr(ended), _ptr(scale)
+    if mask is not None:
+        if not isinstance(mask, DeviceWords):
+            _need(mask, "mask", device, (torch.int32,), (groups * beams, None))
+            if mask.shape[1] < (V + 31) // 32 or mask.stride(1) != 1:
+                raise ValueError("mask rows must hold ceil(vocab / 32) consecutive words")
+        elif mask.rows < groups * beams:
+            raise ValueError("mask holds fewer rows than the batch")
+        b.mask_words = mask.data_ptr()
+        b.mask_stride = mask.stride(0) if groups * beams > 1 else (V + 31) // 32
+        b.tokenizer_vocab = V if tokenizer_vocab is None else int(tokenizer_vocab)
+    b.legal_norm = 1 if legal_norm else 0
+    b.n = n
+    b.end_token = -1 if end_token is None else int(end_token)
+    return b
+
+
+def state_struct(t, rows: int, length_dim: Optional[int] = None) -> MxsState:
+    """The mxs_state of a tensor whose dimension 0 is the rows: the pieces of
+    a row from `length_dim` on (or the longest run of dimensions that lie
+    consecutively in memory), one per index of the dimensions before, which
+    must be evenly spaced.  ValueError for any other layout."""
+    if t.dim() < 1 or t.shape[0] != rows:
+        raise ValueError(f"a state must have {rows} rows, not {list(t.shape)}")
+    size, stride = list(t.shape), list(t.stride())
+    if 0 in size:
+        raise ValueError("a state must not be empty")
+    es, nd = t.element_size(), t.dim()
+    if length_dim is not None and not 1 <= length_dim < nd:
+        raise ValueError(f"length_dim must be in 1..{nd - 1}")
+
+    def run(d):   # elements of dimensions d.. when they are consecutive, else 0
+        n = 1
+        for i in range(nd - 1, d - 1, -1):
+            if size[i] != 1 and stride[i] != n:
+                return 0
+            n *= size[i]
+        return n
+
+    if length_dim is None:
+        first = nd
+        while first > 1 and run(first - 1):
+            first -= 1
+    else:
+        first = length_dim
+        if not run(first):
+            raise ValueError("a state's elements from length_dim on must be consecutive")
+    outer = [(n, s) for n, s in zip(size[1:first], stride[1:first]) if n != 1]
+    for (_, s), (n1, s1) in zip(outer, outer[1:]):
+        if s != n1 * s1:
+            raise ValueError("a state's dimensions before its pieces must be evenly spaced")
+    m = MxsState()
+    m.data = t.data_ptr()
+    m.segment_bytes = run(first) * es
+    m.segments = 1
+    for n, _ in outer:
+        m.segments *= n
+    m.segment_stride = outer[-1][1] * es if outer else m.segment_bytes
+    m.row_stride = stride[0] * es if rows > 1 else m.segments * m.segment_stride
+    m.position_bytes = 0 if length_dim is None else run(first) * es // size[first]
+    return m
+
+
+def reorder_struct(torch, device, states, parent, status, *, beams: Optional[int] = None, lengths=None,
+                   length_dim=None) -> MxsReorder:
+    """The mxs_reorder of a call, its tensors checked against `device` and
+    each other (ValueError)."""
+    _need(parent, "parent", device, (torch.int32,), (None, None))
+    groups = parent.shape[0]
+    W = parent.shape[1] if beams is None else int(beams)
+    if not 0 < W <= parent.shape[1] or (parent.shape[1] > 1 and parent.stride(1) != 1):
+        raise ValueError("parent rows must hold `beams` consecutive entries")
+    if lengths is not None:
+        _need(lengths, "lengths", device, (torch.int32,), (groups,))
+        _dense(lengths, "lengths")
+    dims = list(length_dim) if isinstance(length_dim, (list, tuple)) else [length_dim] * len(states)
+    if len(dims) != len(states):
+        raise ValueError("length_dim must be one dimension or one per state")
+    arr = (MxsState * max(1, len(states)))()
+    for i, (t, d) in enumerate(zip(states, dims)):
+        if t.device != device:
+            raise ValueError(f"states must be on {device}, not {t.device}")
+        arr[i] = state_struct(t, groups * W, d)
+    r = MxsReorder()
+    r.states, r.count = ctypes.cast(arr, ctypes.POINTER(MxsState)), len(states)
+    r.groups, r.beams = groups, W
+    r.parent, r.parent_stride = parent.data_ptr(), parent.stride(0) if groups > 1 else parent.shape[1]
+    r.lengths, r.status = _ptr(lengths), status.data_ptr()
+    r.keep = arr
+    return r
+
+
+def linear_struct(torch, device, x, weight, bias, residual, out, activation) -> MxsLinear:
+    """The mxs_linear of a call, its tensors checked against `device` and each
+    other (ValueError)."""
+    _need(x, "x", device, (torch.bfloat16,), (None, None))
+    R, K = x.shape
+    _need(weight, "weight", device, (torch.bfloat16,), (None, K))
+    N = weight.shape[0]
+    _need(out, "out", device, (torch.bfloat16, torch.float32), (R, N))
+    if bias is not None:
+        _need(bias, "bias", device, (torch.bfloat16, torch.float32), (N,))
+        _dense(bias, "bias")
+    if residual is not None:
+        _need(residual, "residual", device, (out.dtype,), (R, N))
+    for t, name in ((x, "x"), (weight, "weight"), (out, "out"), (residual, "residual")):
+        if t is not None and t.shape[1] > 1 and t.stride(1) != 1:
+            raise ValueError(f"{name} rows must be consecutive elements")
+    act = ACTIVATIONS.get("none" if activation is None else activation)
+    if act is None:
+        raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}")
+    # a single row's stride says nothing
+    rows_of = lambda t, unit: t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // unit) * unit
+    a = MxsLinear()
+    a.x, a.x_stride = x.data_ptr(), rows_of(x, 8)
+    a.weight, a.weight_stride = weight.data_ptr(), rows_of(weight, 8)
+    a.bias, a.residual = _ptr(bias), _ptr(residual)
+    a.residual_stride = rows_of(residual, 1) if residual is not None else 0
+    a.out, a.out_stride = out.data_ptr(), rows_of(out, 1)
+    a.rows, a.in_features, a.out_features, a.act = R, K, N, act
+    a.out_dtype = _float_code(torch, out.dtype)
+    a.bias_dtype = _float_code(torch, bias.dtype) if bias is not None else MXS_F32
+    return a
+
+
 class DeviceWords:
     """A staging slot's device mask words, as `Sampler.sample(mask=...)`
     takes them (a data pointer and a row stride in words)."""
@@ -203,6 +420,17 @@ class ReceiptResult:
     ids: "object"
     logprobs: "object"
     token_logprob: "object"
+    status: "object"
+
+
+@dataclass
+class BeamResult:
+    """Device tensors of one selection (mxs_beam_out), [groups, n] and, the
+    status, [groups]."""
+    token: "object"
+    beam: "object"
+    score: "object"
+    ended: "object"
     status: "object"
 
 
@@ -593,6 +821,120 @@ class Sampler:
                 self._check(rc, "mxs_spec_verify")
 
         launch.out = out
+        return launch
+
+    def _device(self):
+        return self.torch.device("cuda", self.device)
+
+    def beam_select(self, logits, score, n: int, *, out: Optional[BeamResult] = None, **kw) -> BeamResult:
+        """Queues one beam-search selection (mxs_beam_select): logits
+        [groups * beams, >= vocab] f32 or bf16, score f64[groups, beams]; the
+        n best (beam, token) candidates of each group, best first.  ended:
+        bool[groups, beams] (with end_token); scale: f64[groups, beams], the
+        length penalty that orders the candidates; mask: allowed-token words
+        as `sample` takes them, with legal_norm for probabilities over the
+        legal tokens."""
+        return self.beam_launcher(logits, score, n, out=out, **kw).out
+
+    def beam_launcher(self, logits, score, n: int, *, out: Optional[BeamResult] = None, **kw):
+        """Pre-built beam_select for repeated selections with the same
+        outputs (the first of them queued here): returns f(logits) that only
+        swaps the logits pointer (f.out holds the outputs).  `out` may hold
+        the input's own score and ended tensors when n == beams."""
+        torch, dev = self.torch, self._device()
+        b = beam_struct(torch, dev, logits, score, n, **kw)
+        groups = score.shape[0]
+        if out is None:
+            with torch.cuda.stream(self.stream):
+                e = lambda dt: torch.empty((groups, n), dtype=dt, device=dev)
+                out = BeamResult(token=e(torch.int32), beam=e(torch.int32), score=e(torch.float64),
+                                 ended=e(torch.bool), status=torch.empty(groups, dtype=torch.int32, device=dev))
+        else:
+            for name, dts in (("token", (torch.int32,)), ("beam", (torch.int32,)), ("score", (torch.float64,)),
+                              ("ended", (torch.bool, torch.uint8))):
+                t = getattr(out, name)
+                if t is not None or name != "ended":
+                    _need(t, f"out.{name}", dev, dts, (groups, n))
+                    _dense(t, f"out.{name}")
+            _need(out.status, "out.status", dev, (torch.int32,), (groups,))
+        o = MxsBeamOut()
+        o.token, o.beam, o.score = out.token.data_ptr(), out.beam.data_ptr(), out.score.data_ptr()
+        o.ended, o.status = _ptr(out.ended), out.status.data_ptr()
+        fn, ctx, bp, op = self.lib.mxs_beam_select, self.ctx, ctypes.byref(b), ctypes.byref(o)
+
+        def launch(t):
+            b.logits = t.data_ptr()
+            rc = fn(ctx, bp, op)
+            if rc != 0:
+                self._check(rc, "mxs_beam_select")
+
+        launch(logits)
+        launch.out, launch.keep = out, (b, o, score, kw)
+        return launch
+
+    def beam_reorder(self, states, parent, *, status=None, **kw):
+        """Queues the move of the beams' states to their children
+        (mxs_beam_reorder), in place: row g * beams + b of every tensor of
+        `states` becomes what row g * beams + parent[g, b] was (-1: stays).
+        parent: int32[groups, >= beams] (its first `beams` columns; default
+        all).  lengths: int32[groups], the positions in use along each
+        state's length_dim (one dimension, or one per state, None for states
+        that move whole).  Returns the status, int32[groups]."""
+        f = self.reorder_launcher(states, parent, status=status, **kw)
+        f()
+        return f.status
+
+    def reorder_launcher(self, states, parent, *, status=None, **kw):
+        """Pre-built beam_reorder for repeated moves of the same states:
+        returns f() that re-issues mxs_beam_reorder with what parent and
+        lengths then hold (f.status holds the status)."""
+        torch, dev = self.torch, self._device()
+        if status is None:
+            with torch.cuda.stream(self.stream):
+                status = torch.empty(parent.shape[0], dtype=torch.int32, device=dev)
+        else:
+            _need(status, "status", dev, (torch.int32,), (parent.shape[0],))
+        r = reorder_struct(torch, dev, states, parent, status, **kw)
+        fn, ctx, rp = self.lib.mxs_beam_reorder, self.ctx, ctypes.byref(r)
+
+        def launch():
+            rc = fn(ctx, rp)
+            if rc != 0:
+                self._check(rc, "mxs_beam_reorder")
+
+        launch.status, launch.keep = status, (r, states, parent, kw)
+        return launch
+
+    def linear(self, x, weight, bias=None, *, activation=None, residual=None, out=None, out_dtype=None):
+        """Queues out = act(x @ weight.T + bias) + residual (mxs_linear_bf16):
+        x bf16[rows, in_features], weight bf16[out_features, in_features],
+        row strides multiples of 8; bias f32 or bf16; activation none, relu,
+        silu, gelu or gelu_tanh; residual of out's type (bf16 by default; it
+        may be out itself).  Returns out."""
+        return self.linear_launcher(x, weight, bias, activation=activation, residual=residual, out=out,
+                                    out_dtype=out_dtype).out
+
+    def linear_launcher(self, x, weight, bias=None, *, activation=None, residual=None, out=None, out_dtype=None):
+        """Pre-built linear for repeated products into the same output (the
+        first of them queued here): returns f(x) that only swaps x's pointer
+        (f.out holds the output)."""
+        torch, dev = self.torch, self._device()
+        if out is None:
+            with torch.cuda.stream(self.stream):
+                out = torch.empty((x.shape[0], weight.shape[0]), dtype=out_dtype or torch.bfloat16, device=dev)
+        elif out_dtype is not None and out.dtype != out_dtype:
+            raise ValueError(f"out must be {out_dtype}, not {out.dtype}")
+        a = linear_struct(torch, dev, x, weight, bias, residual, out, activation)
+        fn, ctx, ap = self.lib.mxs_linear_bf16, self.ctx, ctypes.byref(a)
+
+        def launch(t):
+            a.x = t.data_ptr()
+            rc = fn(ctx, ap)
+            if rc != 0:
+                self._check(rc, "mxs_linear_bf16")
+
+        launch(x)
+        launch.out, launch.keep = out, (a, weight, bias, residual)
         return launch
 
     def mask_host(self, slot: int):
