@@ -2,6 +2,8 @@
 // continuations over its beams and the vocabulary (mxs_beam_select), and the
 // move of the beams' states to their children (mxs_beam_reorder).
 #include <hip/hip_runtime.h>
+
+#include <float.h>
 #include <math.h>
 #include <stdint.h>
 
@@ -16,167 +18,655 @@
 namespace mxs {
 
 constexpr int BNT = 256;                  // threads per workgroup
-constexpr int BNW = BNT / 64;
+constexpr int BNW = BNT / 64;             // waves
+constexpr int BQ = 4;                     // quads per thread and tile
+constexpr uint32_t BSL = BNT * 4;         // tokens per slice (one quad per thread)
+constexpr uint32_t BTILE = BSL * BQ;      // tokens per tile (4096)
+constexpr uint32_t BCAP = 256;            // candidate slots per wave
+constexpr uint32_t BLIST = 512;           // entries a chunk publishes at most
+constexpr uint32_t BDENSE = 1024;         // entries a group's finisher ranks by counting
+constexpr uint32_t BWGS = 2048;           // chunks a call aims at
+constexpr uint32_t BGCH = 512;            // chunks per group at most (or one per beam)
+static_assert(BLIST >= BNW * MXS_BEAM_N_MAX && BCAP >= MXS_BEAM_N_MAX + 64, "a compacted list fits");
 
-struct BeamRow {
-  double norm;          // ln sum exp of the row's logits that count
-  uint32_t bad;         // a NaN or +inf among them
-  uint32_t pad;
+struct BeamStat {
+  double ref, sum;      // the chunk's weights: sum of exp(l - ref); ref -inf: no weight
+  uint32_t thr;         // order key that n of the chunk's candidates reach (0: fewer than n)
+  uint32_t top;         // order key of its largest candidate (0: none)
+  uint32_t count;       // entries listed
+  uint32_t bad;         // a NaN or +inf among the logits that count
 };
 
 struct BeamArgs {
   const void* logits;
   uint64_t stride;
   uint32_t G, W, V, n;
+  uint32_t C, T;                          // chunks per row, tiles per chunk
   const double* score;
   const uint8_t* ended;
   const double* scale;
   const uint32_t* mask;
   uint64_t mask_stride;
-  uint32_t tok_vocab, legal_norm;
+  uint32_t tok_vocab;
   int32_t end_token;
   int32_t* token;
   int32_t* beam;
   double* oscore;
   uint8_t* oended;
   int32_t* status;
-  BeamRow* rows;
+  BeamStat* stat;                         // [G * W * C]
+  unsigned long long* list;               // [G * W * C * BLIST]: (order key << 32) | ~token
+  uint32_t* ctr;                          // [G * CTR_STRIDE]
 };
 
-__device__ __forceinline__ bool beam_legal(const BeamArgs& A, uint32_t row, uint32_t v) {
-  if (!A.mask) return true;
-  return v < A.tok_vocab && ((A.mask[(uint64_t)row * A.mask_stride + (v >> 5)] >> (v & 31u)) & 1u);
+// What the sum and the candidates are taken over.
+enum { BEAM_ALL = 0, BEAM_MASK = 1, BEAM_MASK_NORM = 2 };   // no mask; candidates masked; both masked
+
+__device__ __forceinline__ unsigned long long beam_entry(uint32_t key, uint32_t token) {
+  return ((unsigned long long)key << 32) | (unsigned long long)(~token);
 }
+__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// 2^(n - n0) e^r for x = n ln 2 + r, |r| <= ln 2 / 2, in f64: `magic` is 1.5
+// 2^52 - n0, so the low word of fma(x, log2 e, magic) is n - n0.  e^r by the
+// polynomial of degree 8 through its values at the Chebyshev nodes (relative
+// error below 2^-39.7).  For |x| <= 2400 the reduction adds 2^-44.
+__device__ __forceinline__ double beam_weight(float xf, double magic) {
+  const double x = (double)xf;
+  const double t = __builtin_fma(x, 1.4426950408889634, magic);
+  const double r = __builtin_fma(magic - t, 0.6931471805599453, x);
+  double p = 0x1.a15a4f98eb4cep-16;
+  p = __builtin_fma(p, r, 0x1.a1aa7f143c63cp-13);
+  p = __builtin_fma(p, r, 0x1.6c164df443c8cp-10);
+  p = __builtin_fma(p, r, 0x1.111080ae06089p-7);
+  p = __builtin_fma(p, r, 0x1.5555557428d91p-5);
+  p = __builtin_fma(p, r, 0x1.555555a26dedbp-3);
+  p = __builtin_fma(p, r, 0x1.fffffffff71cfp-2);
+  p = __builtin_fma(p, r, 0x1.ffffffffd38c1p-1);
+  p = __builtin_fma(p, r, 1.0);
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, p);
+  const uint32_t n = (uint32_t)__builtin_bit_cast(unsigned long long, t);
+  const uint32_t up = (uint32_t)(b >> 32) + (n << 20);
+  return __builtin_bit_cast(double, ((unsigned long long)up << 32) | (uint32_t)b);
+}
+
+struct alignas(16) BeamCand {
+  double rank;              // score * scale
+  unsigned long long tie;   // place among equal ranks (beam_tie)
+};
+
+struct alignas(16) BeamSmem {
+  union {
+    unsigned long long cand[BNW][BCAP];                                    // the chunk's candidates, per wave
+    struct { double ref[BGCH], sum[BGCH]; } c;                             // the finisher: chunks' weights
+    BeamCand d[BDENSE];                                                    // ... and its candidates
+  } u;
+  double wref[BNW], wsum[BNW];
+  uint32_t wthr[2][BNW], wcnt[2][BNW], wtop[BNW], wbad[BNW];
+  double score[MXS_BEAM_MAX], scale[MXS_BEAM_MAX], norm[MXS_BEAM_MAX];
+  uint16_t surv[BGCH], cnt[BGCH];
+  uint8_t kind[MXS_BEAM_MAX];                                              // 0: not there, 1: live, 2: ended
+  uint32_t flags, nsurv, m, last;
+};
 
 __device__ __forceinline__ bool beam_live(const BeamArgs& A, uint32_t row) {
   const double s = A.score[row];
   return s > -INFINITY && !(A.ended && A.ended[row]);
 }
 
-template <typename In>
-__global__ __launch_bounds__(BNT) void beam_norm_kernel(BeamArgs A) {
-  __shared__ double red[BNW];
-  __shared__ float redf[BNW];
-  __shared__ uint32_t redu[BNW];
-  const uint32_t row = blockIdx.x;
-  if (!beam_live(A, row)) return;
+// One wave's candidates down to the n largest, sorted; returns how many are
+// left and raises `lim` to the n-th.
+__device__ __noinline__ uint32_t beam_compact(unsigned long long* c, uint32_t count, uint32_t n, unsigned long long* lim) {
+  unsigned long long e[BCAP / 64];
+  uint32_t r[BCAP / 64];
+#pragma unroll
+  for (uint32_t k = 0; k < BCAP / 64u; ++k) {
+    e[k] = lane() + 64u * k < count ? c[lane() + 64u * k] : 0ull;
+    r[k] = 0u;
+  }
+  for (uint32_t i = 0; i < count; ++i) {
+    const unsigned long long v = c[i];
+#pragma unroll
+    for (uint32_t k = 0; k < BCAP / 64u; ++k) r[k] += v > e[k] ? 1u : 0u;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (uint32_t k = 0; k < BCAP / 64u; ++k)
+    if (lane() + 64u * k < count && r[k] < n) c[r[k]] = e[k];
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  if (count >= n) *lim = max(*lim, c[n - 1u]);
+  return min(count, n);
+}
+
+// A chunk of one live row: its weights' sum, and a list that holds its n
+// largest candidates.
+template <typename In, int MODE>
+__device__ __forceinline__ void beam_chunk(const BeamArgs& A, BeamSmem& S, uint32_t row, uint32_t chunk) {
+  const uint32_t tid = threadIdx.x, V = A.V, n = A.n;
+  const uint32_t c0 = chunk * A.T * BTILE, c1 = min(V, c0 + A.T * BTILE);
+  const uint32_t tiles = (c1 - c0 + BTILE - 1u) / BTILE;
   const In* src = reinterpret_cast<const In*>(A.logits) + (uint64_t)row * A.stride;
-  float m = -INFINITY;
-  uint32_t bad = 0;
-  for (uint32_t v = threadIdx.x; v < A.V; v += BNT) {
-    if (A.legal_norm && !beam_legal(A, row, v)) continue;
-    const float x = Quad<In>::one(src + v);
-    bad |= !(x < INFINITY);
-    m = fmaxf(m, x);
-  }
-  m = wave_max_f32(m);
-  bad = wave_or_u32(bad);
-  if (lane() == 0) { redf[wave()] = m; redu[wave()] = bad; }
-  __syncthreads();
-  for (int w = 0; w < BNW; ++w) { m = fmaxf(m, redf[w]); bad |= redu[w]; }
-  double sum = 0.0;
-  if (m > -INFINITY && !bad)
-    for (uint32_t v = threadIdx.x; v < A.V; v += BNT) {
-      if (A.legal_norm && !beam_legal(A, row, v)) continue;
-      sum += exp_neg_p((double)Quad<In>::one(src + v) - (double)m);
+  const uint32_t* mrow = MODE == BEAM_ALL ? nullptr : A.mask + (uint64_t)row * A.mask_stride;
+  const uint32_t vm = MODE == BEAM_ALL ? V : min(V, A.tok_vocab);
+  typename Quad<In>::Raw cur[BQ], nxt[BQ];
+  uint32_t mcur[BQ] = {}, mnxt[BQ] = {};
+  auto load = [&](typename Quad<In>::Raw (&d)[BQ], uint32_t (&mw)[BQ], uint32_t tile) {
+    const uint32_t b = c0 + tile * BTILE;
+    if (b + BTILE <= V) {   // uniform
+#pragma unroll
+      for (int q = 0; q < BQ; ++q) d[q] = Quad<In>::load(src + b + (uint32_t)q * BSL + tid * 4u);
+      if (MODE != BEAM_ALL)
+#pragma unroll
+        for (int q = 0; q < BQ; ++q) mw[q] = mrow[(b + (uint32_t)q * BSL + tid * 4u) >> 5];
+    } else {                // the row's last tile: nothing past the row is read, what is missing is -inf
+#pragma unroll
+      for (int q = 0; q < BQ; ++q) {
+        const uint32_t e0 = b + (uint32_t)q * BSL + tid * 4u;
+        In v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = Quad<In>::ninf();
+        if (e0 + 4u <= V) {
+          d[q] = Quad<In>::load(src + e0);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (e0 + (uint32_t)e < V) v[e] = src[e0 + (uint32_t)e];
+          d[q] = Quad<In>::pack(v);
+        }
+        if (MODE != BEAM_ALL) mw[q] = e0 < V ? mrow[e0 >> 5] : 0u;
+      }
     }
+  };
+  load(cur, mcur, 0u);
+
+  unsigned long long* cand = S.u.cand[wave()];
+  uint32_t woff = 0u;                 // this wave's candidates (uniform)
+  unsigned long long lim = 0ull;      // entries below cannot be among the chunk's n largest
+  float fthr = -INFINITY;             // ... as a logit
+  uint32_t thr = 0u;                  // an order key that n of the chunk's candidates reach
+  float lm = -INFINITY;               // this lane's largest candidate
+  bool bad = false;
+  double sum = 0.0, unit = -INFINITY; // the weights are relative to e^unit
+  float ref = -INFINITY, hi = -INFINITY, lo = 0.0f;
+  double magic = 0.0;
+  bool wide = false;
+  uint32_t slot = 0u;
+  for (uint32_t tile = 0; tile < tiles; ++tile) {
+    if (tile + 1u < tiles) load(nxt, mnxt, tile + 1u);
+    const uint32_t tb = c0 + tile * BTILE + tid * 4u;
+    float x[BQ][4], qm[BQ], tm;       // the logits weighed; the quads' largest candidates; the largest weighed
+    uint32_t nib[BQ];
+    if (MODE == BEAM_ALL) {
+#pragma unroll
+      for (int q = 0; q < BQ; ++q) {
+        Quad<In>::unpack(cur[q], x[q]);
+        qm[q] = max_nan(max_nan(max_nan(x[q][0], x[q][1]), x[q][2]), x[q][3]);
+      }
+      tm = max_nan(max_nan(qm[0], qm[1]), max_nan(qm[2], qm[3]));
+    } else {
+      tm = -INFINITY;
+#pragma unroll
+      for (int q = 0; q < BQ; ++q) {
+        const uint32_t e0 = tb + (uint32_t)q * BSL;
+        nib[q] = (mcur[q] >> (e0 & 31u)) & 15u;
+        const uint32_t have = vm > e0 ? vm - e0 : 0u;
+        if (have < 4u) nib[q] &= (1u << have) - 1u;
+        Quad<In>::unpack(cur[q], x[q]);
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = ((nib[q] >> e) & 1u) ? x[q][e] : -INFINITY;
+        qm[q] = max_nan(max_nan(max_nan(y[0], y[1]), y[2]), y[3]);
+        if (MODE == BEAM_MASK_NORM) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[q][e] = y[e];
+          tm = max_nan(tm, qm[q]);
+        } else {
+          tm = max_nan(tm, max_nan(max_nan(max_nan(x[q][0], x[q][1]), x[q][2]), x[q][3]));
+        }
+      }
+      if (MODE == BEAM_MASK) bad |= !(tm < INFINITY);
+    }
+    lm = fmaxf(lm, fmaxf(fmaxf(qm[0], qm[1]), fmaxf(qm[2], qm[3])));
+    if (((tile + 1u) & tile) == 0u) {
+      // After 1, 2, 4, ... tiles: a key that at least n of the chunk's lanes
+      // have reached, so n of its candidates have: each wave's n/4-th largest
+      // lane maximum (0 where fewer lanes hold a candidate), the smallest over
+      // the waves, to its upper 18 bits (a few candidates more, 14 ballots
+      // less).
+      const uint32_t sh = (n + (uint32_t)BNW - 1u) / (uint32_t)BNW;
+      const bool any = lm > -INFINITY;
+      uint32_t wthr = 0u;
+      if ((uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(any)) >= sh) {
+        const uint32_t ak = any ? okey(lm) : 0u;
+#pragma unroll
+        for (int bit = 31; bit >= 14; --bit) {
+          const uint32_t c = wthr | (1u << bit);
+          if ((uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(ak >= c)) >= sh) wthr = c;
+        }
+      }
+      if (lane() == 0) S.wthr[slot][wave()] = wthr;
+      lds_barrier();
+      uint32_t t = 0xffffffffu;
+#pragma unroll
+      for (int w = 0; w < BNW; ++w) t = min(t, S.wthr[slot][w]);
+      slot ^= 1u;
+      thr = max(thr, t);
+      lim = max(lim, (unsigned long long)thr << 32);
+      // (a key below the finite ones' is no logit)
+      fthr = okey_value(max((uint32_t)(lim >> 32), okey(-FLT_MAX)));
+    }
+#pragma unroll
+    for (int q = 0; q < BQ; ++q) {
+      if (__builtin_amdgcn_ballot_w64(!(qm[q] < fthr)) == 0ull) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool legal = MODE == BEAM_ALL || ((nib[q] >> e) & 1u);
+        const float v = x[q][e];
+        bad |= legal && !(v < INFINITY);
+        const unsigned long long entry = beam_entry(okey(v + 0.0f), tb + (uint32_t)q * BSL + (uint32_t)e);   // -0 as +0
+        bool c = legal && v > -INFINITY && entry >= lim;
+        uint64_t bal = __builtin_amdgcn_ballot_w64(c);
+        if (bal == 0ull) continue;
+        if (woff + (uint32_t)__builtin_popcountll(bal) > BCAP) {
+          woff = beam_compact(cand, woff, n, &lim);
+          fthr = okey_value(max((uint32_t)(lim >> 32), okey(-FLT_MAX)));
+          c = c && entry >= lim;
+          bal = __builtin_amdgcn_ballot_w64(c);
+        }
+        if (c) cand[woff + lanes_below(bal)] = entry;
+        woff += (uint32_t)__builtin_popcountll(bal);
+      }
+    }
+    // The weights, relative to a power of two near the first maximum the wave
+    // meets: f64 holds e^-700..e^600 of it, so it moves only for a later
+    // maximum 600 above.
+    if (__builtin_amdgcn_ballot_w64(tm > hi)) {
+      const float wm = wave_max_f32(tm);
+      wide = !(fabsf(wm) <= 1000.0f);
+      const double n0 = rint((double)wm * 1.4426950408889634);
+      const double u = wide ? (double)wm : n0 * 0.6931471805599453;
+      if (ref > -INFINITY) sum *= exp_neg_p(unit - u);
+      ref = wm;
+      unit = u;
+      hi = wm + 600.0f;
+      lo = wm - 700.0f;
+      magic = 0x1.8p52 - n0;
+    }
+    if (ref > -INFINITY) {
+      if (!wide) {
+#pragma unroll
+        for (int q = 0; q < BQ; ++q) {
+          double w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = beam_weight(vmax(x[q][e], lo), magic);
+          sum += (w[0] + w[1]) + (w[2] + w[3]);
+        }
+      } else {
+#pragma unroll 1
+        for (int q = 0; q < BQ; ++q)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum += exp_neg_p((double)x[q][e] - unit);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < BQ; ++q) {
+      cur[q] = nxt[q];
+      mcur[q] = mnxt[q];
+    }
+  }
+
+  // ---- the chunk's results
   sum = wave_sum_f64(sum);
-  if (lane() == 0) red[wave()] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    sum = 0.0;
-    for (int w = 0; w < BNW; ++w) sum += red[w];
-    A.rows[row].norm = (double)m + log(sum);
-    A.rows[row].bad = bad;
+  const uint32_t top = wave_max_u32(lm > -INFINITY ? okey(lm + 0.0f) : 0u);
+  const bool wbad = __builtin_amdgcn_ballot_w64(bad) != 0ull;
+  uint32_t kept = 0u;
+#pragma unroll
+  for (uint32_t k = 0; k < BCAP / 64u; ++k) {
+    const uint32_t i = lane() + 64u * k;
+    kept += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(i < woff && cand[i < woff ? i : 0u] >= lim));
   }
-}
-
-// A candidate and its place in the order: larger rank, lower beam, larger
-// logit, lower token.
-struct BeamCand {
-  double rank;
-  double score;
-  uint32_t beam, key, token;
-};
-__device__ __forceinline__ bool before(const BeamCand& a, const BeamCand& b) {
-  if (a.rank != b.rank) return a.rank > b.rank;
-  if (a.beam != b.beam) return a.beam < b.beam;
-  if (a.key != b.key) return a.key > b.key;
-  return a.token < b.token;
-}
-
-template <typename In>
-__global__ __launch_bounds__(BNT) void beam_pick_kernel(BeamArgs A) {
-  __shared__ BeamCand best[BNT];
-  const uint32_t g = blockIdx.x, W = A.W, n = A.n;
-  uint32_t st = 0;
-  for (uint32_t b = 0; b < W; ++b) {
-    const uint32_t row = g * W + b;
-    const double s = A.score[row], c = A.scale ? A.scale[row] : 1.0;
-    if (!(s < INFINITY) || !(c > 0.0 && c < INFINITY)) st |= 1u;
-    else if (beam_live(A, row) && A.rows[row].bad) st |= 2u;
+  if (lane() == 0) {
+    S.wsum[wave()] = sum;
+    S.wref[wave()] = unit;
+    S.wtop[wave()] = top;
+    S.wbad[wave()] = wbad ? 1u : 0u;
+    S.wcnt[0][wave()] = kept;
   }
-  __syncthreads();   // the inputs are read before an output that shares their array is written
-  if (st) {
-    for (uint32_t j = threadIdx.x; j < n; j += BNT) {
-      A.token[g * n + j] = -1;
-      A.beam[g * n + j] = -1;
-      A.oscore[g * n + j] = __builtin_nan("");
-      if (A.oended) A.oended[g * n + j] = 0;
+  lds_barrier();
+  uint32_t before = 0u, total = 0u, ctop = 0u, cbad = 0u;
+#pragma unroll
+  for (int w = 0; w < BNW; ++w) {
+    before += (uint32_t)w < wave() ? S.wcnt[0][w] : 0u;
+    total += S.wcnt[0][w];
+    ctop = max(ctop, S.wtop[w]);
+    cbad |= S.wbad[w];
+  }
+  if (total > BLIST) {   // near-ties: each wave's n largest
+    if (woff > n) woff = beam_compact(cand, woff, n, &lim);
+    kept = 0u;
+#pragma unroll
+    for (uint32_t k = 0; k < BCAP / 64u; ++k) {
+      const uint32_t i = lane() + 64u * k;
+      kept += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(i < woff && cand[i < woff ? i : 0u] >= lim));
     }
-    if (threadIdx.x == 0) A.status[g] = (st & 1u) ? MXS_ROW_PROBABILITIES : MXS_ROW_NON_FINITE_LOGIT;
+    if (lane() == 0) S.wcnt[1][wave()] = kept;
+    lds_barrier();
+    before = total = 0u;
+#pragma unroll
+    for (int w = 0; w < BNW; ++w) {
+      before += (uint32_t)w < wave() ? S.wcnt[1][w] : 0u;
+      total += S.wcnt[1][w];
+    }
+  }
+  const uint64_t at = (uint64_t)row * A.C + chunk;
+#pragma unroll
+  for (uint32_t k = 0; k < BCAP / 64u; ++k) {
+    const uint32_t i = lane() + 64u * k;
+    const unsigned long long e = i < woff ? cand[i] : 0ull;
+    const bool c = i < woff && e >= lim;
+    const uint64_t bal = __builtin_amdgcn_ballot_w64(c);
+    if (c) st_dev(&A.list[at * BLIST + before + lanes_below(bal)], e);
+    before += (uint32_t)__builtin_popcountll(bal);
+  }
+  if (wave() == 0) {   // the waves' sums, each lane one
+    const double r = lane() < (uint32_t)BNW ? S.wref[lane()] : -INFINITY;
+    const double cr = wave_max_f64(r);
+    const double e = r > -INFINITY ? S.wsum[lane()] * exp_neg_p(r - cr) : 0.0;
+    const double cs = ((readlane_t(e, 0) + readlane_t(e, 1)) + readlane_t(e, 2)) + readlane_t(e, 3);
+    if (lane() == 0) {
+      BeamStat* st = &A.stat[at];
+      st_dev(&st->ref, cr);
+      st_dev(&st->sum, cs);
+      st_dev(&st->thr, thr);
+      st_dev(&st->top, ctop);
+      st_dev(&st->count, total);
+      st_dev(&st->bad, cbad);
+    }
+  }
+}
+
+// A candidate's place among equal ranks as one number: lower beam, larger
+// logit, lower token.  An ended beam's key is 1, below every logit's.
+__device__ __forceinline__ unsigned long long beam_tie(uint32_t beam, uint32_t key, uint32_t token) {
+  return ((unsigned long long)(MXS_BEAM_MAX - 1u - beam) << 53) | ((unsigned long long)key << 21) |
+         (unsigned long long)(BEAM_MAX_VOCAB - 1u - token);
+}
+__device__ __forceinline__ double beam_score(const BeamSmem& S, uint32_t b, uint32_t key) {
+  return S.kind[b] == 2 ? S.score[b] : S.score[b] + ((double)okey_value(key) - S.norm[b]);
+}
+
+__device__ __forceinline__ bool beam_before(const BeamCand& a, const BeamCand& b) {
+  return (a.rank > b.rank) | ((a.rank == b.rank) & (a.tie > b.tie));   // (no branch around the second read)
+}
+
+// At most the wave's k-th largest of the lanes' ranks (-inf: none), -inf when
+// it has fewer: a value near it that k of them reach.
+template <int OWN>
+__device__ __forceinline__ double beam_wave_nth(const double (&r)[OWN], uint32_t k) {
+  uint32_t key[OWN], most = 0u, have = 0u;   // the upper halves of order keys (0: none)
+#pragma unroll
+  for (int i = 0; i < OWN; ++i) {
+    const unsigned long long b = __builtin_bit_cast(unsigned long long, r[i]);
+    key[i] = r[i] > -INFINITY ? (uint32_t)(((b >> 63) ? ~b : (b | 1ull << 63)) >> 32) : 0u;
+    most = max(most, key[i]);
+    have += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(key[i] != 0u));
+  }
+  if (have < k) return -INFINITY;
+  most = wave_max_u32(most);
+  uint32_t least = 0xffffffffu;
+#pragma unroll
+  for (int i = 0; i < OWN; ++i) least = key[i] ? min(least, key[i]) : least;
+  least = ~wave_max_u32(~least);
+  // the bits all keys share, then the twelve after them: within 2^-11 of the
+  // ranks' spread
+  const int first = most == least ? -1 : 31 - __builtin_clz(most ^ least);
+  uint32_t t = first < 0 ? most : most & ~((2u << first) - 1u);
+  for (int bit = first; bit >= max(0, first - 11); --bit) {
+    const uint32_t c = t | (1u << bit);
+    uint32_t count = 0u;
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) count += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(key[i] >= c));
+    if (count >= k) t = c;
+  }
+  const unsigned long long b = (unsigned long long)t << 32;
+  return __builtin_bit_cast(double, (t >> 31) ? b & ~(1ull << 63) : ~b);
+}
+
+// The group's n best, by its last workgroup: the rows' norms from their
+// chunks, a rank that n candidates reach (the best chunk threshold), the
+// entries of the chunks that reach it, their order by counting.
+__device__ __forceinline__ void beam_finish(const BeamArgs& A, BeamSmem& S, uint32_t g) {
+  const uint32_t tid = threadIdx.x, W = A.W, C = A.C, n = A.n, NC = W * C;
+  constexpr int OWN = (int)(BGCH / BNT);
+  // (a row's chunks fall to all four waves)
+  auto own = [&](int i) { return lane() * (uint32_t)BNW + wave() + (uint32_t)i * BNT; };
+  double ref[OWN], sum[OWN];
+  uint32_t cthr[OWN], ctop[OWN], ccnt[OWN], cbad[OWN];
+#pragma unroll
+  for (int i = 0; i < OWN; ++i) {
+    const uint32_t c = own(i);
+    const BeamStat* st = &A.stat[(uint64_t)g * NC + min(c, NC - 1u)];   // (a row that is not live has none: not used)
+    ref[i] = ld_dev(&st->ref);
+    sum[i] = ld_dev(&st->sum);
+    cthr[i] = ld_dev(&st->thr);
+    ctop[i] = ld_dev(&st->top);
+    ccnt[i] = ld_dev(&st->count);
+    cbad[i] = ld_dev(&st->bad);
+  }
+  if (tid == 0) {
+    S.flags = 0u;
+    S.nsurv = 0u;
+    S.m = 0u;
+  }
+  uint32_t err = 0u;
+  if (tid < W) {
+    const uint32_t row = g * W + tid;
+    const double s = A.score[row], c = A.scale ? A.scale[row] : 1.0;
+    const bool e = A.ended && A.ended[row];
+    S.score[tid] = s;
+    S.scale[tid] = c;
+    S.kind[tid] = !(s > -INFINITY) ? 0 : e ? 2 : 1;
+    if (!(s < INFINITY) || !(c > 0.0 && c < INFINITY)) err = 1u;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < OWN; ++i) {
+    const uint32_t c = own(i);
+    if (c >= NC || S.kind[c / C] != 1) {
+      ccnt[i] = 0u;
+      cthr[i] = 0u;
+    } else if (cbad[i]) {
+      err |= 2u;
+    }
+    if (c < NC) {
+      S.u.c.ref[c] = ref[i];
+      S.u.c.sum[c] = sum[i];
+      S.cnt[c] = (uint16_t)ccnt[i];
+    }
+  }
+  if (err) atomicOr(&S.flags, err);
+  __syncthreads();
+  if (S.flags) {   // uniform
+    for (uint32_t j = tid; j < n; j += BNT) {
+      const uint64_t at = (uint64_t)g * n + j;
+      A.token[at] = -1;
+      A.beam[at] = -1;
+      A.oscore[at] = __builtin_nan("");
+      if (A.oended) A.oended[at] = 0;
+    }
+    if (tid == 0) A.status[g] = (S.flags & 1u) ? MXS_ROW_PROBABILITIES : MXS_ROW_NON_FINITE_LOGIT;
     return;
   }
-  const BeamCand none{-INFINITY, -INFINITY, 0xffffffffu, 0u, 0xffffffffu};
-  BeamCand last{INFINITY, 0.0, 0u, 0xffffffffu, 0u};
-  BeamCand keep = none;   // thread j holds candidate j
-  uint32_t count = 0;
-  for (uint32_t j = 0; j < n; ++j) {
-    BeamCand mine = none;
-    for (uint32_t b = 0; b < W; ++b) {
-      const uint32_t row = g * W + b;
-      const double s = A.score[row], c = A.scale ? A.scale[row] : 1.0;
-      if (!(s > -INFINITY)) continue;
-      if (A.ended && A.ended[row]) {
-        const BeamCand e{s * c, s, b, 0u, (uint32_t)A.end_token};
-        if (threadIdx.x == 0 && (j == 0 || before(last, e)) && before(e, mine)) mine = e;
-        continue;
-      }
-      const In* src = reinterpret_cast<const In*>(A.logits) + (uint64_t)row * A.stride;
-      const double norm = A.rows[row].norm;
-      for (uint32_t v = threadIdx.x; v < A.V; v += BNT) {
-        const float x = Quad<In>::one(src + v) + 0.0f;   // -0 and +0 are equal logits
-        if (!(x > -INFINITY) || !beam_legal(A, row, v)) continue;
-        const double sc = s + ((double)x - norm);
-        const BeamCand e{sc * c, sc, b, okey(x), v};
-        if ((j == 0 || before(last, e)) && before(e, mine)) mine = e;
-      }
+  // each chunk's sum relative to its row's largest unit, then the row's sum in chunk order
+  double rel[OWN];
+#pragma unroll
+  for (int i = 0; i < OWN; ++i) {
+    const uint32_t c = own(i);
+    rel[i] = 0.0;
+    if (c < NC && S.kind[c / C] == 1 && ref[i] > -INFINITY) {
+      const uint32_t c0 = c / C * C;
+      double m = ref[i];
+      for (uint32_t k = 0; k < C; ++k) m = fmax(m, S.u.c.ref[c0 + k]);
+      rel[i] = sum[i] * exp_neg_p(ref[i] - m);
     }
-    best[threadIdx.x] = mine;
-    __syncthreads();
-    for (uint32_t h = BNT / 2; h > 0; h >>= 1) {
-      if (threadIdx.x < h && before(best[threadIdx.x + h], best[threadIdx.x])) best[threadIdx.x] = best[threadIdx.x + h];
-      __syncthreads();
-    }
-    last = best[0];
-    __syncthreads();
-    if (last.beam == 0xffffffffu) break;
-    if (threadIdx.x == j) keep = last;
-    ++count;
   }
-  if (threadIdx.x < n) {
-    const uint32_t j = threadIdx.x;
-    const bool there = j < count;
+#pragma unroll
+  for (int i = 0; i < OWN; ++i) {
+    const uint32_t c = own(i);
+    if (c < NC) S.u.c.sum[c] = rel[i];
+  }
+  __syncthreads();
+  if (tid < W && S.kind[tid] == 1) {
+    double m = -INFINITY, t = 0.0;
+    for (uint32_t k = 0; k < C; ++k) {
+      m = fmax(m, S.u.c.ref[tid * C + k]);
+      t += S.u.c.sum[tid * C + k];
+    }
+    S.norm[tid] = m + log(t);   // (a row without weight has no candidates either)
+  }
+  __syncthreads();
+  // A rank that n candidates reach: the best chunk threshold, or the n-th
+  // largest of the chunks' largest (by wave: its n/4-th largest, the smallest
+  // over the waves), whichever is more.
+  double gthr = -INFINITY, ctr[OWN];
+#pragma unroll
+  for (int i = 0; i < OWN; ++i) {
+    const uint32_t b = min(own(i), NC - 1u) / C;
+    ctr[i] = ccnt[i] ? beam_score(S, b, ctop[i]) * S.scale[b] : -INFINITY;
+    if (cthr[i]) gthr = fmax(gthr, beam_score(S, b, max(cthr[i], okey(-FLT_MAX))) * S.scale[b]);
+  }
+  gthr = wave_max_f64(gthr);
+  const double nth = beam_wave_nth(ctr, (n + (uint32_t)BNW - 1u) / (uint32_t)BNW);
+  if (lane() == 0) {
+    S.wref[wave()] = gthr;
+    S.wsum[wave()] = nth;
+  }
+  __syncthreads();
+  double tops = S.wsum[0];
+#pragma unroll
+  for (int w = 0; w < BNW; ++w) {
+    gthr = fmax(gthr, S.wref[w]);
+    tops = fmin(tops, S.wsum[w]);
+  }
+  gthr = fmax(gthr, tops);
+#pragma unroll
+  for (int i = 0; i < OWN; ++i)
+    if (ccnt[i] && ctr[i] >= gthr) S.surv[atomicAdd(&S.nsurv, 1u)] = (uint16_t)own(i);
+  if (tid < W && S.kind[tid] == 2) {
+    const double r = S.score[tid] * S.scale[tid];
+    if (r >= gthr) S.u.d[atomicAdd(&S.m, 1u)] = BeamCand{r, beam_tie(tid, 1u, (uint32_t)A.end_token)};   // at most 64
+  }
+  __syncthreads();
+  const uint32_t ns = S.nsurv;
+  auto each = [&](auto&& f) {   // every listed entry that reaches gthr, 16 lanes to a chunk
+    for (uint32_t k = tid >> 4; k < ns; k += BNT / 16u) {
+      const uint32_t c = S.surv[k], b = c / C;
+      const uint32_t count = S.cnt[c];
+      const double* list = reinterpret_cast<const double*>(&A.list[((uint64_t)g * NC + c) * BLIST]);
+      for (uint32_t j0 = tid & 15u; j0 < count; j0 += 64u) {
+        double d[4];   // (four loads in flight)
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i) d[i] = ld_dev(&list[min(j0 + 16u * i, count - 1u)]);
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i) {
+          const unsigned long long e = __builtin_bit_cast(unsigned long long, d[i]);
+          const uint32_t key = (uint32_t)(e >> 32);
+          const double r = beam_score(S, b, key) * S.scale[b];
+          if (j0 + 16u * i < count && r >= gthr) f(r, beam_tie(b, key, ~(uint32_t)e));
+        }
+      }
+    }
+  };
+  each([&](double r, unsigned long long t) {
+    const uint32_t at = atomicAdd(&S.m, 1u);
+    if (at < BDENSE) S.u.d[at] = BeamCand{r, t};
+  });
+  __syncthreads();
+  const uint32_t m = S.m;
+  auto put = [&](uint32_t j, unsigned long long t) {
     const uint64_t at = (uint64_t)g * n + j;
-    A.token[at] = there ? (int32_t)keep.token : -1;
-    A.beam[at] = there ? (int32_t)keep.beam : -1;
-    A.oscore[at] = there ? keep.score : -INFINITY;
-    if (A.oended) A.oended[at] = there && (int32_t)keep.token == A.end_token ? 1 : 0;
+    const uint32_t b = MXS_BEAM_MAX - 1u - (uint32_t)(t >> 53);
+    const int32_t token = (int32_t)(BEAM_MAX_VOCAB - 1u - ((uint32_t)t & (BEAM_MAX_VOCAB - 1u)));
+    A.token[at] = token;
+    A.beam[at] = (int32_t)b;
+    A.oscore[at] = beam_score(S, b, (uint32_t)(t >> 21));
+    if (A.oended) A.oended[at] = token == A.end_token ? 1 : 0;
+  };
+  if (m <= BDENSE) {
+    for (uint32_t i = tid; i < m; i += BNT) {
+      const BeamCand e = S.u.d[i];
+      uint32_t at = 0, k = 0;
+      for (; k + 8u <= m; k += 8u)   // (eight reads in flight)
+#pragma unroll
+        for (uint32_t j = 0; j < 8u; ++j) at += beam_before(S.u.d[k + j], e) ? 1u : 0u;
+      for (; k < m; ++k) at += beam_before(S.u.d[k], e) ? 1u : 0u;
+      if (at < n) put(at, e.tie);
+    }
+  } else {
+    // more near-ties than fit: the best after the last one, n times
+    BeamCand last{INFINITY, ~0ull};
+    for (uint32_t j = 0; j < n; ++j) {
+      BeamCand best{-INFINITY, 0ull};
+      auto take = [&](double r, unsigned long long t) {
+        const BeamCand e{r, t};
+        if (beam_before(last, e) && beam_before(e, best)) best = e;
+      };
+      each(take);
+      if (tid < W && S.kind[tid] == 2) take(S.score[tid] * S.scale[tid], beam_tie(tid, 1u, (uint32_t)A.end_token));
+      __syncthreads();
+      S.u.d[tid] = best;
+      __syncthreads();
+      for (uint32_t h = BNT / 2; h > 0; h >>= 1) {
+        if (tid < h && beam_before(S.u.d[tid + h], S.u.d[tid])) S.u.d[tid] = S.u.d[tid + h];
+        __syncthreads();
+      }
+      last = S.u.d[0];
+      if (tid == 0) put(j, last.tie);   // (m > BDENSE >= n candidates: there is always one)
+    }
   }
-  if (threadIdx.x == 0) A.status[g] = count ? 0 : MXS_ROW_EMPTY_SUPPORT;
+  for (uint32_t j = m + tid; j < n; j += BNT) {
+    const uint64_t at = (uint64_t)g * n + j;
+    A.token[at] = -1;
+    A.beam[at] = -1;
+    A.oscore[at] = -INFINITY;
+    if (A.oended) A.oended[at] = 0;
+  }
+  if (tid == 0) A.status[g] = m ? MXS_ROW_OK : MXS_ROW_EMPTY_SUPPORT;
 }
 
-size_t beam_scratch_bytes(uint32_t max_rows) { return (size_t)max_rows * sizeof(BeamRow); }
+template <typename In, int MODE>
+__global__ __launch_bounds__(BNT, 4) void beam_kernel(BeamArgs A) {
+  __shared__ BeamSmem S;
+  const uint32_t row = blockIdx.x / A.C, chunk = blockIdx.x - row * A.C, g = row / A.W;
+  if (beam_live(A, row)) beam_chunk<In, MODE>(A, S, row, chunk);
+  if (!arrive_last(&A.ctr[g * CTR_STRIDE], A.W * A.C, &S.last)) return;
+  beam_finish(A, S, g);
+}
+
+// Chunks per row and tiles per chunk: enough workgroups to fill the chip
+// (BWGS), no more per group than its finisher's threads hold.
+static void beam_layout(uint32_t rows, uint32_t W, uint32_t V, uint32_t* C, uint32_t* T) {
+  const uint32_t tiles = (V + BTILE - 1u) / BTILE;
+  uint32_t c = BWGS / rows;
+  if (c > BGCH / W) c = BGCH / W;
+  if (c > tiles) c = tiles;
+  if (c < 1u) c = 1u;
+  *T = (tiles + c - 1u) / c;
+  *C = (tiles + *T - 1u) / *T;
+}
+
+size_t beam_scratch_bytes(uint32_t max_rows) {   // rows * C <= BWGS + max_rows
+  return ((size_t)BWGS + max_rows) * (sizeof(BeamStat) + BLIST * sizeof(unsigned long long));
+}
+
+template <int MODE>
+static void beam_go(hipStream_t stream, int32_t dtype, const BeamArgs& A) {
+  const dim3 grid(A.G * A.W * A.C);
+  if (dtype == MXS_F32) hipLaunchKernelGGL((beam_kernel<float, MODE>), grid, dim3(BNT), 0, stream, A);
+  else hipLaunchKernelGGL((beam_kernel<uint16_t, MODE>), grid, dim3(BNT), 0, stream, A);
+}
 
 // ---------------------------------------------------------------------------
 // The move of the states.
@@ -191,24 +681,25 @@ struct ReorderArgs {
   uint32_t W, pstride;
 };
 
-// Sixteen bytes at any alignment (global memory takes unaligned accesses).
-struct __attribute__((packed, aligned(1))) Piece16 { uint32_t w[4]; };
-struct __attribute__((packed, aligned(1))) Piece8 { uint32_t w[2]; };
-struct __attribute__((packed, aligned(1))) Piece4 { uint32_t w; };
-struct __attribute__((packed, aligned(1))) Piece2 { uint16_t w; };
-struct __attribute__((packed, aligned(1))) Piece1 { uint8_t w; };
+// Pieces of a row at any alignment (global memory takes unaligned accesses),
+// as values in registers.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <typename T>
+struct Unaligned { typedef T type __attribute__((aligned(1))); };
 
 // Moves one T at `at` (offset `at` of row 0 of the group) between the rows,
 // in the lanes where `act`.  p: lane j holds row j's parent.  Every lane of
 // the wave comes here, so that the ballots see all parents.
 template <typename T, int WMAX>
 __device__ __forceinline__ void move_piece(char* at, uint64_t stride, int32_t p, bool act) {
+  typedef typename Unaligned<T>::type U;
   const uint32_t l = threadIdx.x & 63u;
   T v[WMAX];
 #pragma unroll
   for (int j = 0; j < WMAX; ++j) {
     const uint64_t to = __builtin_amdgcn_ballot_w64(p == j && l != (uint32_t)j);
-    if (to && act) v[j] = *reinterpret_cast<const T*>(at + (uint64_t)j * stride);
+    if (to && act) v[j] = *reinterpret_cast<const U*>(at + (uint64_t)j * stride);
   }
 #pragma unroll
   for (int j = 0; j < WMAX; ++j) {
@@ -216,7 +707,7 @@ __device__ __forceinline__ void move_piece(char* at, uint64_t stride, int32_t p,
     while (to) {
       const uint32_t d = (uint32_t)__builtin_ctzll(to);
       to &= to - 1u;
-      if (act) *reinterpret_cast<T*>(at + (uint64_t)d * stride) = v[j];
+      if (act) *reinterpret_cast<U*>(at + (uint64_t)d * stride) = v[j];
     }
   }
 }
@@ -248,15 +739,15 @@ __global__ __launch_bounds__(RO_NT) void reorder_kernel(ReorderArgs A) {
   char* at = reinterpret_cast<char*>(s.data) + (uint64_t)g * W * s.row_stride + (uint64_t)seg * s.segment_stride +
              (uint64_t)pc * 16u;
   const uint32_t have = !in ? 0u : (uint32_t)min((uint64_t)16u, used - (uint64_t)pc * 16u);
-  move_piece<Piece16, WMAX>(at, s.row_stride, p, have == 16u);
+  move_piece<u32x4, WMAX>(at, s.row_stride, p, have == 16u);
   if (__builtin_amdgcn_ballot_w64(have & 15u)) {   // a segment's last bytes
-    move_piece<Piece8, WMAX>(at, s.row_stride, p, (have & 8u) != 0u);
+    move_piece<u32x2, WMAX>(at, s.row_stride, p, (have & 8u) != 0u);
     at += have & 8u;
-    move_piece<Piece4, WMAX>(at, s.row_stride, p, (have & 4u) != 0u);
+    move_piece<uint32_t, WMAX>(at, s.row_stride, p, (have & 4u) != 0u);
     at += have & 4u;
-    move_piece<Piece2, WMAX>(at, s.row_stride, p, (have & 2u) != 0u);
+    move_piece<uint16_t, WMAX>(at, s.row_stride, p, (have & 2u) != 0u);
     at += have & 2u;
-    move_piece<Piece1, WMAX>(at, s.row_stride, p, (have & 1u) != 0u);
+    move_piece<uint8_t, WMAX>(at, s.row_stride, p, (have & 1u) != 0u);
   }
 }
 
@@ -286,24 +777,22 @@ extern "C" int mxs_beam_select(mxs_ctx* ctx, const mxs_beam* beam, const mxs_bea
   A.mask = b.mask_words;
   A.mask_stride = b.mask_stride;
   A.tok_vocab = b.tokenizer_vocab;
-  A.legal_norm = b.mask_words ? b.legal_norm : 0u;
   A.end_token = b.end_token;
   A.token = out->token;
   A.beam = out->beam;
   A.oscore = out->score;
   A.oended = out->ended;
   A.status = out->status;
-  A.rows = reinterpret_cast<BeamRow*>(ctx->beam_scratch);
+  beam_layout(A.G * A.W, A.W, A.V, &A.C, &A.T);
+  A.stat = reinterpret_cast<BeamStat*>(ctx->beam_scratch);
+  A.list = reinterpret_cast<unsigned long long*>(A.stat + ((size_t)BWGS + ctx->max_rows));
+  A.ctr = ctx->beam_ctr;
   int prev = 0;
   (void)hipGetDevice(&prev);
   if (prev != ctx->device) (void)hipSetDevice(ctx->device);
-  if (b.dtype == MXS_F32) {
-    hipLaunchKernelGGL(beam_norm_kernel<float>, dim3(A.G * A.W), dim3(BNT), 0, ctx->stream, A);
-    hipLaunchKernelGGL(beam_pick_kernel<float>, dim3(A.G), dim3(BNT), 0, ctx->stream, A);
-  } else {
-    hipLaunchKernelGGL(beam_norm_kernel<uint16_t>, dim3(A.G * A.W), dim3(BNT), 0, ctx->stream, A);
-    hipLaunchKernelGGL(beam_pick_kernel<uint16_t>, dim3(A.G), dim3(BNT), 0, ctx->stream, A);
-  }
+  if (!b.mask_words) beam_go<BEAM_ALL>(ctx->stream, b.dtype, A);
+  else if (!b.legal_norm) beam_go<BEAM_MASK>(ctx->stream, b.dtype, A);
+  else beam_go<BEAM_MASK_NORM>(ctx->stream, b.dtype, A);
   const hipError_t e = hipGetLastError();
   if (prev != ctx->device) (void)hipSetDevice(prev);
   if (e != hipSuccess) return hip_fail(ctx, e, "beam launch");

@@ -246,6 +246,8 @@ struct Quad<float> {
   __device__ static Raw load(const float* p) { return *reinterpret_cast<const float4*>(p); }
   __device__ static void unpack(const Raw& r, float x[4]) { x[0] = r.x; x[1] = r.y; x[2] = r.z; x[3] = r.w; }
   __device__ static float one(const float* p) { return *p; }
+  __device__ static float ninf() { return -INFINITY; }
+  __device__ static Raw pack(const float (&v)[4]) { return make_float4(v[0], v[1], v[2], v[3]); }
 };
 template <>
 struct Quad<uint16_t> {
@@ -256,6 +258,10 @@ struct Quad<uint16_t> {
     x[2] = bf16_to_f32((uint16_t)(r.y & 0xffffu)); x[3] = bf16_to_f32((uint16_t)(r.y >> 16));
   }
   __device__ static float one(const uint16_t* p) { return bf16_to_f32(*p); }
+  __device__ static uint16_t ninf() { return 0xff80u; }
+  __device__ static Raw pack(const uint16_t (&v)[4]) {
+    return make_uint2(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16);
+  }
 };
 
 
