@@ -22,6 +22,7 @@ constexpr int BNW = BNT / 64;             // waves
 constexpr int BQ = 4;                     // quads per thread and tile
 constexpr uint32_t BSL = BNT * 4;         // tokens per slice (one quad per thread)
 constexpr uint32_t BTILE = BSL * BQ;      // tokens per tile (4096)
+constexpr uint32_t BBT = 8;               // tiles between two looks for candidates
 constexpr uint32_t BCAP = 256;            // candidate slots per wave
 constexpr uint32_t BLIST = 512;           // entries a chunk publishes at most
 constexpr uint32_t BDENSE = 1024;         // entries a group's finisher ranks by counting
@@ -65,6 +66,12 @@ enum { BEAM_ALL = 0, BEAM_MASK = 1, BEAM_MASK_NORM = 2 };   // no mask; candidat
 __device__ __forceinline__ unsigned long long beam_entry(uint32_t key, uint32_t token) {
   return ((unsigned long long)key << 32) | (unsigned long long)(~token);
 }
+// The legal ones of the four tokens from e0, from their mask word.
+__device__ __forceinline__ uint32_t beam_nibble(uint32_t word, uint32_t e0, uint32_t vm) {
+  const uint32_t have = vm > e0 ? vm - e0 : 0u;
+  const uint32_t nib = (word >> (e0 & 31u)) & 15u;
+  return have < 4u ? nib & ((1u << have) - 1u) : nib;
+}
 __device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 // 2^(n - n0) e^r for x = n ln 2 + r, |r| <= ln 2 / 2, in f64: `magic` is 1.5
@@ -84,10 +91,7 @@ __device__ __forceinline__ double beam_weight(float xf, double magic) {
   p = __builtin_fma(p, r, 0x1.fffffffff71cfp-2);
   p = __builtin_fma(p, r, 0x1.ffffffffd38c1p-1);
   p = __builtin_fma(p, r, 1.0);
-  const unsigned long long b = __builtin_bit_cast(unsigned long long, p);
-  const uint32_t n = (uint32_t)__builtin_bit_cast(unsigned long long, t);
-  const uint32_t up = (uint32_t)(b >> 32) + (n << 20);
-  return __builtin_bit_cast(double, ((unsigned long long)up << 32) | (uint32_t)b);
+  return __builtin_ldexp(p, (int)(uint32_t)__builtin_bit_cast(unsigned long long, t));
 }
 
 struct alignas(16) BeamCand {
@@ -97,7 +101,11 @@ struct alignas(16) BeamCand {
 
 struct alignas(16) BeamSmem {
   union {
-    unsigned long long cand[BNW][BCAP];                                    // the chunk's candidates, per wave
+    struct {
+      unsigned long long cand[BNW][BCAP];                                  // the chunk's candidates, per wave
+      float top[BBT][BNT];                                                 // the threads' largest candidate of each tile
+      uint16_t hit[BNW][BBT * 64];                                         // (tile, lane) pairs that reach the threshold
+    } w;
     struct { double ref[BGCH], sum[BGCH]; } c;                             // the finisher: chunks' weights
     BeamCand d[BDENSE];                                                    // ... and its candidates
   } u;
@@ -152,6 +160,20 @@ __device__ __forceinline__ void beam_chunk(const BeamArgs& A, BeamSmem& S, uint3
   const uint32_t vm = MODE == BEAM_ALL ? V : min(V, A.tok_vocab);
   typename Quad<In>::Raw cur[BQ], nxt[BQ];
   uint32_t mcur[BQ] = {}, mnxt[BQ] = {};
+  // the quad at token e0; nothing past the row is read, what is missing is -inf
+  auto load_quad = [&](typename Quad<In>::Raw* raw, uint32_t e0) {
+    if (e0 + 4u <= V) {
+      *raw = Quad<In>::load(src + e0);
+      return;
+    }
+    In v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = Quad<In>::ninf();
+      if (e0 + (uint32_t)e < V) v[e] = src[e0 + (uint32_t)e];
+    }
+    *raw = Quad<In>::pack(v);
+  };
   auto load = [&](typename Quad<In>::Raw (&d)[BQ], uint32_t (&mw)[BQ], uint32_t tile) {
     const uint32_t b = c0 + tile * BTILE;
     if (b + BTILE <= V) {   // uniform
@@ -160,31 +182,21 @@ __device__ __forceinline__ void beam_chunk(const BeamArgs& A, BeamSmem& S, uint3
       if (MODE != BEAM_ALL)
 #pragma unroll
         for (int q = 0; q < BQ; ++q) mw[q] = mrow[(b + (uint32_t)q * BSL + tid * 4u) >> 5];
-    } else {                // the row's last tile: nothing past the row is read, what is missing is -inf
+    } else {                // the row's last tile
 #pragma unroll
       for (int q = 0; q < BQ; ++q) {
         const uint32_t e0 = b + (uint32_t)q * BSL + tid * 4u;
-        In v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = Quad<In>::ninf();
-        if (e0 + 4u <= V) {
-          d[q] = Quad<In>::load(src + e0);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (e0 + (uint32_t)e < V) v[e] = src[e0 + (uint32_t)e];
-          d[q] = Quad<In>::pack(v);
-        }
+        load_quad(&d[q], e0);
         if (MODE != BEAM_ALL) mw[q] = e0 < V ? mrow[e0 >> 5] : 0u;
       }
     }
   };
   load(cur, mcur, 0u);
 
-  unsigned long long* cand = S.u.cand[wave()];
+  unsigned long long* cand = S.u.w.cand[wave()];
+  uint16_t* hit = S.u.w.hit[wave()];
   uint32_t woff = 0u;                 // this wave's candidates (uniform)
   unsigned long long lim = 0ull;      // entries below cannot be among the chunk's n largest
-  float fthr = -INFINITY;             // ... as a logit
   uint32_t thr = 0u;                  // an order key that n of the chunk's candidates reach
   float lm = -INFINITY;               // this lane's largest candidate
   bool bad = false;
@@ -192,49 +204,61 @@ __device__ __forceinline__ void beam_chunk(const BeamArgs& A, BeamSmem& S, uint3
   float ref = -INFINITY, hi = -INFINITY, lo = 0.0f;
   double magic = 0.0;
   bool wide = false;
-  uint32_t slot = 0u;
+  uint32_t slot = 0u, held = 0u, hits = 0u;
+  // Quad i of the hits (four to a hit): its first token, its raw logits and
+  // legal tokens.
+  auto hit_load = [&](uint32_t i, uint32_t first, uint32_t* e0, typename Quad<In>::Raw* raw, uint32_t* nib) {
+    const uint32_t h = hit[min(i >> 2, hits - 1u)];
+    *e0 = c0 + (first + (h >> 6)) * BTILE + (i & 3u) * BSL + (wave() * 64u + (h & 63u)) * 4u;
+    static_assert(BQ == 4, "four quads to a hit");
+    load_quad(raw, *e0);
+    *nib = 0u;
+    if (MODE != BEAM_ALL && *e0 < V) *nib = beam_nibble(mrow[*e0 >> 5], *e0, vm);
+  };
   for (uint32_t tile = 0; tile < tiles; ++tile) {
     if (tile + 1u < tiles) load(nxt, mnxt, tile + 1u);
     const uint32_t tb = c0 + tile * BTILE + tid * 4u;
-    float x[BQ][4], qm[BQ], tm;       // the logits weighed; the quads' largest candidates; the largest weighed
-    uint32_t nib[BQ];
+    float x[BQ][4], tm;   // the logits weighed, the largest of them
     if (MODE == BEAM_ALL) {
+      float qm[BQ];
 #pragma unroll
       for (int q = 0; q < BQ; ++q) {
         Quad<In>::unpack(cur[q], x[q]);
         qm[q] = max_nan(max_nan(max_nan(x[q][0], x[q][1]), x[q][2]), x[q][3]);
       }
       tm = max_nan(max_nan(qm[0], qm[1]), max_nan(qm[2], qm[3]));
+      S.u.w.top[held][tid] = tm;
+      lm = fmaxf(lm, tm);
     } else {
+      float ym = -INFINITY;
       tm = -INFINITY;
 #pragma unroll
       for (int q = 0; q < BQ; ++q) {
-        const uint32_t e0 = tb + (uint32_t)q * BSL;
-        nib[q] = (mcur[q] >> (e0 & 31u)) & 15u;
-        const uint32_t have = vm > e0 ? vm - e0 : 0u;
-        if (have < 4u) nib[q] &= (1u << have) - 1u;
+        const uint32_t e0 = tb + (uint32_t)q * BSL, nib = beam_nibble(mcur[q], e0, vm);
         Quad<In>::unpack(cur[q], x[q]);
-        float y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = ((nib[q] >> e) & 1u) ? x[q][e] : -INFINITY;
-        qm[q] = max_nan(max_nan(max_nan(y[0], y[1]), y[2]), y[3]);
-        if (MODE == BEAM_MASK_NORM) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[q][e] = y[e];
-          tm = max_nan(tm, qm[q]);
-        } else {
-          tm = max_nan(tm, max_nan(max_nan(max_nan(x[q][0], x[q][1]), x[q][2]), x[q][3]));
+        for (int e = 0; e < 4; ++e) {
+          const float y = ((nib >> e) & 1u) ? x[q][e] : -INFINITY;
+          ym = max_nan(ym, y);
+          if (MODE == BEAM_MASK_NORM) x[q][e] = y;
+          else tm = max_nan(tm, x[q][e]);
         }
       }
-      if (MODE == BEAM_MASK) bad |= !(tm < INFINITY);
+      if (MODE == BEAM_MASK_NORM) tm = ym;
+      else bad |= !(tm < INFINITY);
+      S.u.w.top[held][tid] = ym;
+      lm = fmaxf(lm, ym);
     }
-    lm = fmaxf(lm, fmaxf(fmaxf(qm[0], qm[1]), fmaxf(qm[2], qm[3])));
-    if (((tile + 1u) & tile) == 0u) {
-      // After 1, 2, 4, ... tiles: a key that at least n of the chunk's lanes
-      // have reached, so n of its candidates have: each wave's n/4-th largest
-      // lane maximum (0 where fewer lanes hold a candidate), the smallest over
-      // the waves, to its upper 18 bits (a few candidates more, 14 ballots
-      // less).
+    ++held;
+    const bool look = held == BBT || tile + 1u == tiles;
+    const uint32_t first = tile + 1u - held;
+    uint32_t he0 = 0u, hnib = 0u;
+    typename Quad<In>::Raw hraw{};
+    if (look) {
+      // A key that at least n of the chunk's lanes have reached, so n of its
+      // candidates have: each wave's n/4-th largest lane maximum (0 where
+      // fewer lanes hold a candidate), the smallest over the waves, to its
+      // upper 18 bits (a few candidates more, 14 ballots less).
       const uint32_t sh = (n + (uint32_t)BNW - 1u) / (uint32_t)BNW;
       const bool any = lm > -INFINITY;
       uint32_t wthr = 0u;
@@ -255,29 +279,21 @@ __device__ __forceinline__ void beam_chunk(const BeamArgs& A, BeamSmem& S, uint3
       thr = max(thr, t);
       lim = max(lim, (unsigned long long)thr << 32);
       // (a key below the finite ones' is no logit)
-      fthr = okey_value(max((uint32_t)(lim >> 32), okey(-FLT_MAX)));
-    }
-#pragma unroll
-    for (int q = 0; q < BQ; ++q) {
-      if (__builtin_amdgcn_ballot_w64(!(qm[q] < fthr)) == 0ull) continue;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool legal = MODE == BEAM_ALL || ((nib[q] >> e) & 1u);
-        const float v = x[q][e];
-        bad |= legal && !(v < INFINITY);
-        const unsigned long long entry = beam_entry(okey(v + 0.0f), tb + (uint32_t)q * BSL + (uint32_t)e);   // -0 as +0
-        bool c = legal && v > -INFINITY && entry >= lim;
-        uint64_t bal = __builtin_amdgcn_ballot_w64(c);
+      const float fthr = okey_value(max((uint32_t)(lim >> 32), okey(-FLT_MAX)));
+      // The few threads whose largest reaches it take a second look at that
+      // tile's logits, again from memory (a NaN reaches it too): the loads go
+      // out here and are used after the weights.
+      hits = 0u;
+      for (uint32_t k = 0; k < held; ++k) {
+        const bool h = !(S.u.w.top[k][tid] < fthr);
+        const uint64_t bal = __builtin_amdgcn_ballot_w64(h);
         if (bal == 0ull) continue;
-        if (woff + (uint32_t)__builtin_popcountll(bal) > BCAP) {
-          woff = beam_compact(cand, woff, n, &lim);
-          fthr = okey_value(max((uint32_t)(lim >> 32), okey(-FLT_MAX)));
-          c = c && entry >= lim;
-          bal = __builtin_amdgcn_ballot_w64(c);
-        }
-        if (c) cand[woff + lanes_below(bal)] = entry;
-        woff += (uint32_t)__builtin_popcountll(bal);
+        if (h) hit[hits + lanes_below(bal)] = (uint16_t)(k * 64u + lane());
+        hits += (uint32_t)__builtin_popcountll(bal);
       }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (hits) hit_load(lane(), first, &he0, &hraw, &hnib);
     }
     // The weights, relative to a power of two near the first maximum the wave
     // meets: f64 holds e^-700..e^600 of it, so it moves only for a later
@@ -309,6 +325,31 @@ __device__ __forceinline__ void beam_chunk(const BeamArgs& A, BeamSmem& S, uint3
 #pragma unroll
           for (int e = 0; e < 4; ++e) sum += exp_neg_p((double)x[q][e] - unit);
       }
+    }
+    if (look) {
+      for (uint32_t i0 = 0; i0 < 4u * hits; i0 += 64u) {
+        if (i0) hit_load(i0 + lane(), first, &he0, &hraw, &hnib);
+        const bool in = i0 + lane() < 4u * hits;
+        float v[4];
+        Quad<In>::unpack(hraw, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool legal = in && (MODE == BEAM_ALL || ((hnib >> e) & 1u));
+          const unsigned long long entry = beam_entry(okey(v[e] + 0.0f), he0 + (uint32_t)e);   // -0 as +0
+          bad |= legal && !(v[e] < INFINITY);
+          bool c = legal && v[e] > -INFINITY && entry >= lim;
+          uint64_t bal = __builtin_amdgcn_ballot_w64(c);
+          if (bal == 0ull) continue;
+          if (woff + (uint32_t)__builtin_popcountll(bal) > BCAP) {
+            woff = beam_compact(cand, woff, n, &lim);
+            c = c && entry >= lim;
+            bal = __builtin_amdgcn_ballot_w64(c);
+          }
+          if (c) cand[woff + lanes_below(bal)] = entry;
+          woff += (uint32_t)__builtin_popcountll(bal);
+        }
+      }
+      held = 0u;
     }
 #pragma unroll
     for (int q = 0; q < BQ; ++q) {
