@@ -112,6 +112,7 @@ struct alignas(16) BeamSmem {
   double wref[BNW], wsum[BNW];
   uint32_t wthr[2][BNW], wcnt[2][BNW], wtop[BNW], wbad[BNW];
   double score[MXS_BEAM_MAX], scale[MXS_BEAM_MAX], norm[MXS_BEAM_MAX];
+  uint32_t key[BDENSE];                                                    // beam_key of the finisher's candidates
   uint16_t surv[BGCH], cnt[BGCH];
   uint8_t kind[MXS_BEAM_MAX];                                              // 0: not there, 1: live, 2: ended
   uint32_t flags, nsurv, m, last;
@@ -442,6 +443,12 @@ __device__ __forceinline__ bool beam_before(const BeamCand& a, const BeamCand& b
   return (a.rank > b.rank) | ((a.rank == b.rank) & (a.tie > b.tie));   // (no branch around the second read)
 }
 
+// The upper half of a rank's order key; 0 for none.
+__device__ __forceinline__ uint32_t beam_key(double r) {
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, r);
+  return (uint32_t)(((b >> 63) ? ~b : (b | 1ull << 63)) >> 32);
+}
+
 // At most the wave's k-th largest of the lanes' ranks (-inf: none), -inf when
 // it has fewer: a value near it that k of them reach.
 template <int OWN>
@@ -449,8 +456,7 @@ __device__ __forceinline__ double beam_wave_nth(const double (&r)[OWN], uint32_t
   uint32_t key[OWN], most = 0u, have = 0u;   // the upper halves of order keys (0: none)
 #pragma unroll
   for (int i = 0; i < OWN; ++i) {
-    const unsigned long long b = __builtin_bit_cast(unsigned long long, r[i]);
-    key[i] = r[i] > -INFINITY ? (uint32_t)(((b >> 63) ? ~b : (b | 1ull << 63)) >> 32) : 0u;
+    key[i] = r[i] > -INFINITY ? beam_key(r[i]) : 0u;
     most = max(most, key[i]);
     have += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(key[i] != 0u));
   }
@@ -597,15 +603,19 @@ __device__ __forceinline__ void beam_finish(const BeamArgs& A, BeamSmem& S, uint
     if (ccnt[i] && ctr[i] >= gthr) S.surv[atomicAdd(&S.nsurv, 1u)] = (uint16_t)own(i);
   if (tid < W && S.kind[tid] == 2) {
     const double r = S.score[tid] * S.scale[tid];
-    if (r >= gthr) S.u.d[atomicAdd(&S.m, 1u)] = BeamCand{r, beam_tie(tid, 1u, (uint32_t)A.end_token)};   // at most 64
+    if (r >= gthr) {
+      const uint32_t at = atomicAdd(&S.m, 1u);   // at most 64 of them
+      S.u.d[at] = BeamCand{r, beam_tie(tid, 1u, (uint32_t)A.end_token)};
+      S.key[at] = beam_key(r);
+    }
   }
   __syncthreads();
   const uint32_t ns = S.nsurv;
   auto each = [&](auto&& f) {   // every listed entry that reaches gthr, 16 lanes to a chunk
     for (uint32_t k = tid >> 4; k < ns; k += BNT / 16u) {
-      const uint32_t c = S.surv[k], b = c / C;
-      const uint32_t count = S.cnt[c];
+      const uint32_t c = S.surv[k], b = c / C, count = S.cnt[c];
       const double* list = reinterpret_cast<const double*>(&A.list[((uint64_t)g * NC + c) * BLIST]);
+      const double bs = S.score[b], bn = S.norm[b], bc = S.scale[b];   // (live beams only have lists)
       for (uint32_t j0 = tid & 15u; j0 < count; j0 += 64u) {
         double d[4];   // (four loads in flight)
 #pragma unroll
@@ -614,7 +624,7 @@ __device__ __forceinline__ void beam_finish(const BeamArgs& A, BeamSmem& S, uint
         for (uint32_t i = 0; i < 4u; ++i) {
           const unsigned long long e = __builtin_bit_cast(unsigned long long, d[i]);
           const uint32_t key = (uint32_t)(e >> 32);
-          const double r = beam_score(S, b, key) * S.scale[b];
+          const double r = (bs + ((double)okey_value(key) - bn)) * bc;
           if (j0 + 16u * i < count && r >= gthr) f(r, beam_tie(b, key, ~(uint32_t)e));
         }
       }
@@ -622,10 +632,15 @@ __device__ __forceinline__ void beam_finish(const BeamArgs& A, BeamSmem& S, uint
   };
   each([&](double r, unsigned long long t) {
     const uint32_t at = atomicAdd(&S.m, 1u);
-    if (at < BDENSE) S.u.d[at] = BeamCand{r, t};
+    if (at < BDENSE) {
+      S.u.d[at] = BeamCand{r, t};
+      S.key[at] = beam_key(r);
+    }
   });
   __syncthreads();
   const uint32_t m = S.m;
+  if (tid < 8u && m + tid < BDENSE) S.key[m + tid] = 0u;
+  __syncthreads();
   auto put = [&](uint32_t j, unsigned long long t) {
     const uint64_t at = (uint64_t)g * n + j;
     const uint32_t b = MXS_BEAM_MAX - 1u - (uint32_t)(t >> 53);
@@ -636,13 +651,30 @@ __device__ __forceinline__ void beam_finish(const BeamArgs& A, BeamSmem& S, uint
     if (A.oended) A.oended[at] = token == A.end_token ? 1 : 0;
   };
   if (m <= BDENSE) {
+    // Each one's place by counting, on the upper halves of the ranks' order
+    // keys (a 64-bit comparison costs several 32-bit ones); those that share
+    // one compare in full.
     for (uint32_t i = tid; i < m; i += BNT) {
       const BeamCand e = S.u.d[i];
-      uint32_t at = 0, k = 0;
-      for (; k + 8u <= m; k += 8u)   // (eight reads in flight)
+      const uint32_t mine = S.key[i];
+      uint32_t at = 0, same = 0;
+      for (uint32_t k = 0; k < m; k += 8u) {   // (the keys past m are 0)
+        const uint4 v0 = *reinterpret_cast<const uint4*>(&S.key[k]), v1 = *reinterpret_cast<const uint4*>(&S.key[k + 4u]);
+        const uint32_t v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
-        for (uint32_t j = 0; j < 8u; ++j) at += beam_before(S.u.d[k + j], e) ? 1u : 0u;
-      for (; k < m; ++k) at += beam_before(S.u.d[k], e) ? 1u : 0u;
+        for (uint32_t j = 0; j < 8u; ++j) {
+          at += v[j] > mine ? 1u : 0u;
+          same += v[j] == mine ? 1u : 0u;
+        }
+      }
+      if (same > 1u) {
+        at = 0;
+        uint32_t k = 0;
+        for (; k + 8u <= m; k += 8u)   // (eight reads in flight)
+#pragma unroll
+          for (uint32_t j = 0; j < 8u; ++j) at += beam_before(S.u.d[k + j], e) ? 1u : 0u;
+        for (; k < m; ++k) at += beam_before(S.u.d[k], e) ? 1u : 0u;
+      }
       if (at < n) put(at, e.tie);
     }
   } else {
