@@ -9,9 +9,12 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/mx_sampler.h"
 #include "mxs_checks.h"
 #include "mxs_ctx.h"
+#include "mxs_device.h"
 
 namespace mxs {
 
@@ -27,7 +30,9 @@ struct LinArgs {
   uint64_t xs, ws, rs, os;   // strides in elements
   uint32_t R, K, N;
   int32_t act, out_f32, bias_f32;
-  int32_t vec;               // out and residual take 4-element accesses
+  uint32_t P, span;          // the sum over k in P parts of `span` k (a multiple of 64) each
+  float* part;               // [tiles * P][tile] the parts' sums
+  uint32_t* ctr;             // [tiles * CTR_STRIDE] arrivals
 };
 
 // exp(-y) for the sigmoid, to about 2 ulp: exp2 of fl(-y log2(e)), corrected
@@ -40,7 +45,7 @@ __device__ __forceinline__ float exp_minus(float y) {
 }
 
 __device__ __forceinline__ float activate(float y, int32_t act) {
-  switch (act) {   // uniform
+  switch (act) {   // uniform, or known
     case MXS_ACT_RELU: return y < 0.0f ? 0.0f : y;   // (a NaN stays)
     case MXS_ACT_SILU: return y / (1.0f + exp_minus(y));
     case MXS_ACT_GELU: return 0.5f * y * (1.0f + erff(y * 0.707106781f));
@@ -57,19 +62,58 @@ __device__ __forceinline__ float ld_elem(const void* p, uint64_t i, int32_t f32)
   return f32 ? reinterpret_cast<const float*>(p)[i] : (float)reinterpret_cast<const __bf16*>(p)[i];
 }
 
-// Four consecutive features o..o+3 of row r (those below N).
-__device__ __forceinline__ void epilogue4(const LinArgs& A, uint32_t r, uint32_t o, f32x4 v) {
-  const uint32_t have = min(4u, A.N - o);
-  const uint64_t at = (uint64_t)r * A.os + o, rat = (uint64_t)r * A.rs + o;
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef f32x4 f32x4_u __attribute__((aligned(4)));     // (global memory takes unaligned accesses)
+typedef bf16x4 bf16x4_u __attribute__((aligned(2)));
+
+// Four elements of `have` (1..4, the others 0) at i.
+__device__ __forceinline__ f32x4 ld_four(const void* p, uint64_t i, uint32_t have, int32_t f32) {
+  if (have == 4u) {
+    if (f32) return *reinterpret_cast<const f32x4_u*>(reinterpret_cast<const float*>(p) + i);
+    const bf16x4 v = *reinterpret_cast<const bf16x4_u*>(reinterpret_cast<const __bf16*>(p) + i);
+    return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+  }
+  f32x4 v = {};
 #pragma unroll
-  for (uint32_t j = 0; j < 4u; ++j) {
-    if (j >= have) break;
-    float y = v[j];
-    if (A.bias) y += ld_elem(A.bias, o + j, A.bias_f32);
-    y = activate(y, A.act);
-    if (A.res) y += ld_elem(A.res, rat + j, A.out_f32);
-    if (A.out_f32) reinterpret_cast<float*>(A.out)[at + j] = y;
-    else reinterpret_cast<__bf16*>(A.out)[at + j] = (__bf16)y;
+  for (uint32_t j = 0; j < 3u; ++j)
+    if (j < have) v[j] = ld_elem(p, i + j, f32);
+  return v;
+}
+__device__ __forceinline__ void st_four(void* p, uint64_t i, uint32_t have, int32_t f32, f32x4 v) {
+  const bf16x4 h{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+  if (have == 4u) {
+    if (f32) *reinterpret_cast<f32x4_u*>(reinterpret_cast<float*>(p) + i) = v;
+    else *reinterpret_cast<bf16x4_u*>(reinterpret_cast<__bf16*>(p) + i) = h;
+    return;
+  }
+#pragma unroll
+  for (uint32_t j = 0; j < 3u; ++j) {
+    if (j >= have) continue;
+    if (f32) reinterpret_cast<float*>(p)[i + j] = v[j];
+    else reinterpret_cast<__bf16*>(p)[i + j] = h[j];
+  }
+}
+
+// The epilogue of four consecutive features from o in NJ rows, 16 apart from
+// r: the residuals' loads go out together.
+template <int NJ>
+__device__ __forceinline__ void epilogue(const LinArgs& A, int32_t act, uint32_t r, uint32_t o, const f32x4 (&acc)[NJ]) {
+  if (o >= A.N) return;
+  const uint32_t have = min(4u, A.N - o);
+  const f32x4 b = A.bias ? ld_four(A.bias, o, have, A.bias_f32) : f32x4{};
+  f32x4 res[NJ];
+  if (A.res) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) res[j] = ld_four(A.res, (uint64_t)min(r + 16u * (uint32_t)j, A.R - 1u) * A.rs + o, have, A.out_f32);
+  }
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    const uint32_t row = r + 16u * (uint32_t)j;
+    f32x4 v = acc[j] + b;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = activate(v[e], act);
+    if (A.res) v += res[j];
+    if (row < A.R) st_four(A.out, (uint64_t)row * A.os + o, have, A.out_f32, v);
   }
 }
 
@@ -77,40 +121,320 @@ __device__ __forceinline__ void epilogue4(const LinArgs& A, uint32_t r, uint32_t
 __device__ __forceinline__ bf16x8 ld_k(const __bf16* row, uint32_t k, uint32_t K) {
   if (k + 8u <= K) return *reinterpret_cast<const bf16x8*>(row + k);
   bf16x8 v = {};
+  if (k < K) {
 #pragma unroll
-  for (uint32_t j = 0; j < 8u; ++j)
-    if (k + j < K) v[j] = row[k + j];
+    for (uint32_t j = 0; j < 7u; ++j)
+      if (k + j < K) v[j] = row[k + j];
+  }
   return v;
 }
 
-// 64 rows x 64 features per 256-thread workgroup; wave w has 32 x 32 of them
-// as 2 x 2 MFMA blocks, operands straight from memory.
-__global__ __launch_bounds__(256) void linear_kernel(LinArgs A) {
+// At most 16 rows: one MFMA block of 16 features and all rows per workgroup.
+// Its waves split the sum over k, 64 at a time in turn (whole 128-byte lines
+// of a weight row), operands straight from memory, and their parts meet in
+// LDS, added in order.
+constexpr int SW = 8;   // waves
+__global__ __launch_bounds__(SW * 64) void linear_rows_kernel(LinArgs A) {
+  __shared__ f32x4 part[SW][64];
   const uint32_t w = threadIdx.x >> 6, l = threadIdx.x & 63u, lr = l & 15u, lg = l >> 4;
-  const uint32_t o0 = blockIdx.x * 64u + (w & 1u) * 32u, r0 = blockIdx.y * 64u + (w >> 1) * 32u;
-  const __bf16* wp[2];
-  const __bf16* xp[2];
+  const uint32_t o0 = blockIdx.x * 16u;
+  const __bf16* const wp = A.w + (uint64_t)min(o0 + lr, A.N - 1u) * A.ws;
+  const __bf16* const xp = A.x + (uint64_t)min(lr, A.R - 1u) * A.xs;
+  f32x4 acc = {};
+  const uint32_t whole = A.K / 64u;
+  constexpr uint32_t U = 4;   // steps in flight
+  uint32_t s = w;
+  for (; s + (U - 1u) * SW < whole; s += U * SW) {
+    bf16x8 a[U][2], b[U][2];
 #pragma unroll
-  for (uint32_t i = 0; i < 2u; ++i) {
-    wp[i] = A.w + (uint64_t)min(o0 + i * 16u + lr, A.N - 1u) * A.ws;
-    xp[i] = A.x + (uint64_t)min(r0 + i * 16u + lr, A.R - 1u) * A.xs;
+    for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+      for (uint32_t h = 0; h < 2u; ++h) {
+        const uint32_t k = (s + u * SW) * 64u + h * 32u + lg * 8u;
+        a[u][h] = *reinterpret_cast<const bf16x8*>(wp + k);
+        b[u][h] = *reinterpret_cast<const bf16x8*>(xp + k);
+      }
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+      for (uint32_t h = 0; h < 2u; ++h) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[u][h], b[u][h], acc, 0, 0, 0);
   }
-  f32x4 acc[2][2] = {};
-  for (uint32_t k = lg * 8u; k < A.K + lg * 8u; k += 32u) {
-    const bf16x8 a0 = ld_k(wp[0], k, A.K), a1 = ld_k(wp[1], k, A.K);
-    const bf16x8 b0 = ld_k(xp[0], k, A.K), b1 = ld_k(xp[1], k, A.K);
-    acc[0][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, b0, acc[0][0], 0, 0, 0);
-    acc[0][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, b1, acc[0][1], 0, 0, 0);
-    acc[1][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, b0, acc[1][0], 0, 0, 0);
-    acc[1][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, b1, acc[1][1], 0, 0, 0);
-  }
+  for (; s * 64u < A.K; s += SW) {   // the rest, the last 64 perhaps in part
 #pragma unroll
-  for (uint32_t i = 0; i < 2u; ++i)
-#pragma unroll
-    for (uint32_t j = 0; j < 2u; ++j) {
-      const uint32_t o = o0 + i * 16u + lg * 4u, r = r0 + j * 16u + lr;
-      if (o < A.N && r < A.R) epilogue4(A, r, o, acc[i][j]);
+    for (uint32_t h = 0; h < 2u; ++h) {
+      const uint32_t k = s * 64u + h * 32u + lg * 8u;
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ld_k(wp, k, A.K), ld_k(xp, k, A.K), acc, 0, 0, 0);
     }
+  }
+  part[w][l] = acc;
+  __syncthreads();
+  if (w == 0) {
+#pragma unroll
+    for (int q = 1; q < SW; ++q) acc += part[q][l];
+    const f32x4 one[1] = {acc};
+    epilogue<1>(A, A.act, lr, o0 + lg * 4u, one);
+  }
+}
+
+// Sixteen bytes per lane from base + off + at (off: this lane's, at: the
+// wave's) straight into LDS, lane after lane from `lds` on.
+__device__ __forceinline__ void load_lds16(__bf16* lds, const __bf16* base, uint32_t off, uint32_t at) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, -1, 0x27000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, off, at, 0, 0);
+#endif
+}
+// All but the wave's N newest loads into LDS have landed and its reads are
+// done; then the workgroup meets.
+template <int N>
+__device__ __forceinline__ void tile_barrier() {
+  // (the builtin, so that the compiler knows that nothing it tracks is pending)
+  static_assert(N < 64, "a six-bit counter");
+  __asm__ volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4);   // vmcnt(N) lgkmcnt(0), exports not waited for
+  __asm__ volatile("s_barrier" ::: "memory");
+}
+
+// The order in which M products and D LDS reads issue: a read after every
+// product (or every M / D).
+template <int M, int D>
+__device__ __forceinline__ void interleave() {
+  constexpr int P = M >= D ? M / D : 1;
+#pragma unroll
+  for (int i = 0; i < D; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, P, 0);
+  }
+}
+
+// Many rows: BO features x BR rows per workgroup, WO x WR waves.  Tiles of TK
+// k pass through S LDS buffers, written there by the loads themselves, S - 1
+// tiles ahead; a row's 16-byte pieces are permuted by bits of the row so that
+// the 16 rows a fragment takes fall in different banks.
+template <int BO, int BR, int WO, int WR, int TK, int S, int ACT, bool SPLIT>
+__global__ __launch_bounds__(WO * WR * 64, 2) void linear_tile_kernel(LinArgs A) {
+  constexpr int NW = WO * WR, FO = BO / WO / 16, FR = BR / WR / 16;   // waves; 16 x 16 blocks per wave
+  constexpr uint32_t PR = TK / 8, LR = 64 / PR;                       // pieces per row, rows per load
+  constexpr int LA = BO / (int)LR / NW, LB = BR / (int)LR / NW;       // loads per wave
+  static_assert(LA * (int)LR * NW == BO && LB * (int)LR * NW == BR, "the loads cover the tile");
+  __shared__ __align__(1024) __bf16 As[S][BO * TK];
+  __shared__ __align__(1024) __bf16 Bs[S][BR * TK];
+  const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63u, lr = l & 15u, lg = l >> 4;
+  // XCD x (workgroups go to the XCDs in turn) takes a contiguous range of the
+  // tiles, in bands of 8 row tiles, so that what it reads is shared in its L2.
+  const uint32_t no = (A.N + BO - 1u) / BO, nr = (A.R + BR - 1u) / BR, per = gridDim.x / 8u;
+  const uint32_t job = (blockIdx.x & 7u) * per + (blockIdx.x >> 3);
+  const uint32_t t = SPLIT ? job / A.P : job, pt = SPLIT ? job - t * A.P : 0u;
+  if (t >= no * nr) return;
+  const uint32_t band = t / (8u * no), in = t - band * 8u * no, hgt = min(8u, nr - band * 8u);
+  const uint32_t o0 = in / hgt * BO, r0 = (band * 8u + in % hgt) * BR;
+  auto turn = [](uint32_t row) { return TK == 64 ? row & 7u : (row >> 2) & 3u; };
+  const uint32_t ro = l / PR, piece = ((l % PR) ^ turn(ro)) * 8u;   // what this lane loads
+  // (32-bit offsets from the tile's first rows: the strides are below 2^22)
+  const uint32_t k0 = SPLIT ? pt * A.span : 0u, K = SPLIT ? min(A.K - k0, A.span) : A.K;   // this part's k
+  const __bf16* const wt = A.w + (uint64_t)o0 * A.ws + k0;
+  const __bf16* const xt = A.x + (uint64_t)r0 * A.xs + k0;
+  uint32_t ga[LA], gb[LB];
+#pragma unroll
+  for (int i = 0; i < LA; ++i) ga[i] = min((w * LA + i) * LR + ro, A.N - 1u - o0) * (uint32_t)A.ws + piece;
+#pragma unroll
+  for (int i = 0; i < LB; ++i) gb[i] = min((w * LB + i) * LR + ro, A.R - 1u - r0) * (uint32_t)A.xs + piece;
+  auto fetch = [&](const __bf16* __restrict__ wk, const __bf16* __restrict__ xk, __bf16* __restrict__ as,
+                   __bf16* __restrict__ bs, uint32_t k, int which) __attribute__((always_inline)) {
+    if (which == 0) {
+#pragma unroll
+      for (int i = 0; i < LA; ++i) load_lds16(as + (w * LA + i) * LR * TK, wk, ga[i] * 2u, k * 2u);
+    } else {
+#pragma unroll
+      for (int i = 0; i < LB; ++i) load_lds16(bs + (w * LB + i) * LR * TK, xk, gb[i] * 2u, k * 2u);
+    }
+  };
+  auto fetch_part = [&](uint32_t k, __bf16* as, __bf16* bs) {   // the last k, not a whole tile
+#pragma unroll 1
+    for (int i = 0; i < LA; ++i) {
+      const uint32_t row = min((w * LA + i) * LR + ro, A.N - 1u - o0);
+      *reinterpret_cast<bf16x8*>(as + (w * LA + i) * LR * TK + l * 8u) = ld_k(wt + (uint64_t)row * A.ws, k + piece, K);
+    }
+#pragma unroll 1
+    for (int i = 0; i < LB; ++i) {
+      const uint32_t row = min((w * LB + i) * LR + ro, A.R - 1u - r0);
+      *reinterpret_cast<bf16x8*>(bs + (w * LB + i) * LR * TK + l * 8u) = ld_k(xt + (uint64_t)row * A.xs, k + piece, K);
+    }
+  };
+  const uint32_t wo = (w / WR) * (BO / WO), wr = (w % WR) * (BR / WR);
+  f32x4 acc[FO][FR] = {};
+  const uint32_t whole = K / TK, nk = (K + TK - 1u) / TK;
+#pragma unroll
+  for (uint32_t k = 0; k < (uint32_t)S - 1u; ++k) {
+    if (k < whole) {
+      fetch(wt, xt, As[k], Bs[k], k * TK, 0);
+      fetch(wt, xt, As[k], Bs[k], k * TK, 1);
+    } else if (k < nk) fetch_part(k * TK, As[k], Bs[k]);
+  }
+  // Fragments are read one half tile ahead of the products that take them, so
+  // that the reads' latency passes under the products before; the workgroup
+  // meets between the last read of a tile and its last products.
+  bf16x8 a0[FO], b0[FR], a1[FO], b1[FR];
+  auto read = [&](bf16x8 (&a)[FO], bf16x8 (&b)[FR], const __bf16* __restrict__ ac, const __bf16* __restrict__ bc, uint32_t h)
+                  __attribute__((always_inline)) {
+    const uint32_t pc = ((h * 4u + lg) ^ turn(lr)) * 8u;
+#pragma unroll
+    for (int i = 0; i < FO; ++i) a[i] = *reinterpret_cast<const bf16x8*>(ac + (wo + i * 16u + lr) * TK + pc);
+#pragma unroll
+    for (int j = 0; j < FR; ++j) b[j] = *reinterpret_cast<const bf16x8*>(bc + (wr + j * 16u + lr) * TK + pc);
+  };
+  auto mul = [&](const bf16x8 (&a)[FO], const bf16x8 (&b)[FR], int from, int to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < FO; ++i)
+      if (i >= from && i < to) {
+#pragma unroll
+        for (int j = 0; j < FR; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], acc[i][j], 0, 0, 0);
+      }
+  };
+  // The restricted pointers tell the compiler that the loads do not write
+  // what this tile's reads take, which it would wait for otherwise.  The group
+  // barriers have it issue reads and loads between the products.
+  auto step = [&](const __bf16* __restrict__ ac, const __bf16* __restrict__ bc, __bf16* __restrict__ an,
+                  __bf16* __restrict__ bn, const __bf16* __restrict__ wk, const __bf16* __restrict__ xk, uint32_t kt,
+                  auto ahead) __attribute__((always_inline)) {
+    constexpr bool AHEAD = decltype(ahead)::value;
+    constexpr int HALF = FO / 2 * FR, D = FO + FR;
+    if (S == 2) {   // the loads have little time: first
+      if (AHEAD) {
+        fetch(wk, xk, an, bn, kt * TK, 0);
+        fetch(wk, xk, an, bn, kt * TK, 1);
+      }
+      read(a0, b0, ac, bc, 0u);
+      mul(a1, b1, 0, FO);
+      interleave<FO * FR, D>();
+      __builtin_amdgcn_sched_barrier(0);
+    } else {
+      read(a0, b0, ac, bc, 0u);
+      mul(a1, b1, 0, FO / 2);
+      interleave<HALF, D>();
+      __builtin_amdgcn_sched_barrier(0);
+      if (AHEAD) fetch(wk, xk, an, bn, kt * TK, 0);
+      mul(a1, b1, FO / 2, FO * 3 / 4);
+      __builtin_amdgcn_sched_barrier(0);
+      if (AHEAD) fetch(wk, xk, an, bn, kt * TK, 1);
+      mul(a1, b1, FO * 3 / 4, FO);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    read(a1, b1, ac, bc, 1u);
+    mul(a0, b0, 0, FO);
+    interleave<FO * FR, D>();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  static_assert(TK == 64, "two halves to a tile");
+#pragma unroll
+  for (int i = 0; i < FO; ++i) a1[i] = bf16x8{};
+#pragma unroll
+  for (int j = 0; j < FR; ++j) b1[j] = bf16x8{};
+  uint32_t cur = 0u, nxt = S - 1u, kt = 0u;
+  auto turn_buffers = [&] {
+    cur = cur + 1u == (uint32_t)S ? 0u : cur + 1u;
+    nxt = nxt + 1u == (uint32_t)S ? 0u : nxt + 1u;
+  };
+  // Tile kt is there when at most the loads of the tiles after it are still
+  // in flight.
+  for (; kt + (uint32_t)S - 1u < whole; ++kt) {
+    tile_barrier<(S - 2) * (LA + LB)>();
+    step(As[cur], Bs[cur], As[nxt], Bs[nxt], wt, xt, kt + (uint32_t)S - 1u, std::true_type{});
+    turn_buffers();
+  }
+  for (; kt < nk; ++kt) {
+    const uint32_t after = whole > kt + 1u ? whole - 1u - kt : 0u;
+    if (S > 3 && after >= 2u) tile_barrier<2 * (LA + LB)>();
+    else if (S > 2 && after >= 1u) tile_barrier<LA + LB>();
+    else tile_barrier<0>();
+    if (kt + (uint32_t)S - 1u == whole && whole < nk) fetch_part(whole * TK, As[nxt], Bs[nxt]);
+    step(As[cur], Bs[cur], As[nxt], Bs[nxt], wt, xt, 0u, std::false_type{});
+    turn_buffers();
+  }
+  mul(a1, b1, 0, FO);
+  if (SPLIT) {
+    // The parts' sums meet in memory; the tile's last part adds them in order.
+    static_assert(sizeof(As) >= 4, "a word of LDS for the arrival");
+    float* mine = A.part + (uint64_t)job * (BO * BR) + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < FO; ++i)
+#pragma unroll
+      for (int j = 0; j < FR; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st_dev(mine + ((i * FR + j) * 4 + e) * (NW * 64), acc[i][j][e]);
+    if (!arrive_last(&A.ctr[t * CTR_STRIDE], A.P, reinterpret_cast<uint32_t*>(&As[0][0]))) return;
+    const float* from = A.part + (uint64_t)t * A.P * (BO * BR) + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < FO; ++i)
+#pragma unroll
+      for (int j = 0; j < FR; ++j) acc[i][j] = f32x4{};
+    for (uint32_t q = 0; q < A.P; ++q, from += BO * BR) {
+#pragma unroll
+      for (int i = 0; i < FO; ++i)
+#pragma unroll
+        for (int j = 0; j < FR; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] += ld_dev(from + ((i * FR + j) * 4 + e) * (NW * 64));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < FO; ++i) epilogue<FR>(A, ACT, r0 + wr + lr, o0 + wo + (uint32_t)i * 16u + lg * 4u, acc[i]);
+}
+
+template <int BO, int BR, int WO, int WR, int S, bool SPLIT>
+static void tile_go(hipStream_t st, const LinArgs& A) {
+  const uint64_t jobs = (uint64_t)((A.N + BO - 1u) / BO) * ((A.R + BR - 1u) / BR) * (SPLIT ? A.P : 1u);
+  const dim3 grid((uint32_t)((jobs + 7u) / 8u * 8u)), block(WO * WR * 64);
+  switch (A.act) {
+    case MXS_ACT_NONE: hipLaunchKernelGGL((linear_tile_kernel<BO, BR, WO, WR, 64, S, MXS_ACT_NONE, SPLIT>), grid, block, 0, st, A); break;
+    case MXS_ACT_RELU: hipLaunchKernelGGL((linear_tile_kernel<BO, BR, WO, WR, 64, S, MXS_ACT_RELU, SPLIT>), grid, block, 0, st, A); break;
+    case MXS_ACT_SILU: hipLaunchKernelGGL((linear_tile_kernel<BO, BR, WO, WR, 64, S, MXS_ACT_SILU, SPLIT>), grid, block, 0, st, A); break;
+    case MXS_ACT_GELU: hipLaunchKernelGGL((linear_tile_kernel<BO, BR, WO, WR, 64, S, MXS_ACT_GELU, SPLIT>), grid, block, 0, st, A); break;
+    default: hipLaunchKernelGGL((linear_tile_kernel<BO, BR, WO, WR, 64, S, MXS_ACT_GELU_TANH, SPLIT>), grid, block, 0, st, A); break;
+  }
+}
+
+constexpr uint32_t LIN_JOBS = 288;   // workgroups of a split sum, at most
+size_t linear_scratch_bytes() { return (size_t)LIN_JOBS * 64u * 64u * sizeof(float); }
+size_t linear_ctr_words() { return (size_t)LIN_JOBS * CTR_STRIDE; }
+
+// Which kernel a product takes; fills in the split's parts.
+enum LinKernel { LIN_ROWS, LIN_SPLIT, LIN_64, LIN_128, LIN_128_256, LIN_256 };
+static LinKernel linear_choice(LinArgs& A) {
+  auto tiles = [&](uint32_t bo, uint32_t br) { return (uint64_t)((A.N + bo - 1u) / bo) * ((A.R + br - 1u) / br); };
+  const uint32_t steps = (A.K + 63u) / 64u;
+  // Up to 16 rows against weights of moderate size, or up to 4 rows against
+  // up to 16384 features, are latency: no LDS tiles.  us, this kernel / tiles
+  // of 64 (split): 16 x 1024 x 1024 4.1 / 6.0, 16 x 4096 x 4096 9.8 / 11.9,
+  // 4 x 4096 x 14336 26.1 / 30.4; but 16 x 8192 x 1024 16.3 / 11.4, 16 x 4096
+  // x 14336 36.3 / 31.1, 4 x 1024 x 151936 72 / 58.
+  if ((A.R <= 16u && A.N <= 4096u && A.K <= 4096u) || (A.R <= 4u && A.N <= 16384u)) return LIN_ROWS;
+  // Few tiles of 64 and a long sum: at least 16 steps of 64 k to a part, up to
+  // 8 parts.  us, whole / split: 64 x 8192 x 1024 31.4 / 12.4, 256 x 4096 x
+  // 1024 18.5 / 11.3, 2197 x 7797 x 31 35.1 / 17.4; but 256 x 1024 x 1024 6.9
+  // / 7.8, and 64 x 4096 x 4096 12.4 in 256 jobs, 14.6 in 512.
+  const uint64_t t64 = tiles(64, 64);
+  uint32_t parts = steps / 16u;
+  if (parts > 8u) parts = 8u;
+  if (parts > LIN_JOBS / t64) parts = (uint32_t)(LIN_JOBS / t64);
+  if (parts >= 2u) {
+    A.span = (steps + parts - 1u) / parts * 64u;
+    A.P = (A.K + A.span - 1u) / A.span;
+    return LIN_SPLIT;
+  }
+  // Otherwise the tile with the least time: rounds of workgroups over 256 CUs
+  // (three of 64 x 64 share one) times what a step of 64 k takes in each (us,
+  // measured at 8192 x 8192 x 8192, 512 x 4096 x 4096 and 2048 x 4096 x 4096)
+  // and a tile's first loads and epilogue.
+  auto rounds = [](uint64_t t, uint64_t per) { return (double)((t + per - 1u) / per); };
+  const uint64_t last = t64 % 768u;
+  const double at64 = (double)(t64 / 768u) * (0.56 * steps + 3.0) +
+                      (last ? (0.34 + 0.075 * rounds(last, 256)) * steps + 2.0 : 0.0);
+  const double at128 = rounds(tiles(128, 128), 256) * (0.50 * steps + 3.0);
+  const double at128_256 = rounds(tiles(128, 256), 256) * (0.88 * steps + 4.0);
+  const double at256 = rounds(tiles(256, 256), 256) * (1.62 * steps + 6.0);
+  const double least = fmin(fmin(at64, at128), fmin(at128_256, at256));
+  return least == at256 ? LIN_256 : least == at128_256 ? LIN_128_256 : least == at128 ? LIN_128 : LIN_64;
 }
 
 }  // namespace mxs
@@ -137,12 +461,21 @@ extern "C" int mxs_linear_bf16(mxs_ctx* ctx, const mxs_linear* linear) {
   A.act = a.act;
   A.out_f32 = a.out_dtype == MXS_F32;
   A.bias_f32 = a.bias_dtype == MXS_F32;
-  const uint32_t gx = (a.out_features + 63u) / 64u, gy = (a.rows + 63u) / 64u;
-  if (gy > 65535u) return fail(ctx, MXS_EINVAL, "rows must be at most 4194240");
+  if ((uint64_t)((a.rows + 63u) / 64u) * ((a.out_features + 63u) / 64u) >= 1u << 31)
+    return fail(ctx, MXS_EINVAL, "rows x out_features is too large");
   int prev = 0;
   (void)hipGetDevice(&prev);
   if (prev != ctx->device) (void)hipSetDevice(ctx->device);
-  hipLaunchKernelGGL(linear_kernel, dim3(gx, gy), dim3(256), 0, ctx->stream, A);
+  A.part = ctx->linear_scratch;
+  A.ctr = ctx->linear_ctr;
+  switch (linear_choice(A)) {
+    case LIN_ROWS: hipLaunchKernelGGL(linear_rows_kernel, dim3((A.N + 15u) / 16u), dim3(SW * 64), 0, ctx->stream, A); break;
+    case LIN_SPLIT: tile_go<64, 64, 2, 2, 3, true>(ctx->stream, A); break;
+    case LIN_64: tile_go<64, 64, 2, 2, 3, false>(ctx->stream, A); break;
+    case LIN_128: tile_go<128, 128, 2, 4, 3, false>(ctx->stream, A); break;
+    case LIN_128_256: tile_go<128, 256, 2, 4, 3, false>(ctx->stream, A); break;
+    case LIN_256: tile_go<256, 256, 2, 4, 2, false>(ctx->stream, A); break;
+  }
   const hipError_t e = hipGetLastError();
   if (prev != ctx->device) (void)hipSetDevice(prev);
   if (e != hipSuccess) return hip_fail(ctx, e, "linear_kernel launch");

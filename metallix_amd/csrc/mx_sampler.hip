@@ -7069,6 +7069,9 @@ int mxs_create(int device, void* stream, uint32_t max_rows, uint32_t max_vocab, 
   e = e ? e : hipMalloc(&ctx->beam_ctr, (size_t)max_rows * mxs::CTR_STRIDE * sizeof(uint32_t));
   e = e ? e : hipMemset(ctx->beam_ctr, 0, (size_t)max_rows * mxs::CTR_STRIDE * sizeof(uint32_t));
   e = e ? e : hipMalloc(&ctx->beam_scratch, mxs::beam_scratch_bytes(max_rows));
+  e = e ? e : hipMalloc(&ctx->linear_scratch, mxs::linear_scratch_bytes());
+  e = e ? e : hipMalloc(&ctx->linear_ctr, mxs::linear_ctr_words() * sizeof(uint32_t));
+  e = e ? e : hipMemset(ctx->linear_ctr, 0, mxs::linear_ctr_words() * sizeof(uint32_t));
   const size_t nr = (size_t)max_rows + 1, nwords = (size_t)max_vocab / 32 + 2;
   e = e ? e : hipMalloc(&ctx->d_zero_u32, nr * sizeof(uint32_t));
   e = e ? e : hipMalloc(&ctx->d_one_f64, nr * sizeof(double));
@@ -7127,6 +7130,8 @@ int mxs_destroy(mxs_ctx* ctx) {
   hipFree(ctx->race_m);
   hipFree(ctx->beam_ctr);
   hipFree(ctx->beam_scratch);
+  hipFree(ctx->linear_scratch);
+  hipFree(ctx->linear_ctr);
   mxs::mask_release(ctx);
   hipSetDevice(prev);
   delete ctx;

@@ -83,9 +83,8 @@ inline const char* linear_check(const mxs_linear* a) {
     return "x_stride and weight_stride must be multiples of 8 and >= in_features";
   if (a->out_stride < a->out_features || (a->residual && a->residual_stride < a->out_features))
     return "out_stride and residual_stride must be >= out_features";
-  if (a->x_stride >= 1ull << 40 || a->weight_stride >= 1ull << 40 || a->out_stride >= 1ull << 40 ||
-      a->residual_stride >= 1ull << 40)
-    return "strides are out of range";
+  if (a->x_stride >= 1ull << 22 || a->weight_stride >= 1ull << 22) return "x_stride and weight_stride must be below 2^22: out of range";
+  if (a->out_stride >= 1ull << 40 || a->residual_stride >= 1ull << 40) return "strides are out of range";
   if (((uintptr_t)a->x | (uintptr_t)a->weight) % 16u) return "x and weight must be 16-byte aligned";
   const uint64_t es = a->out_dtype == MXS_F32 ? 4u : 2u, bs = a->bias_dtype == MXS_F32 ? 4u : 2u;
   if ((uintptr_t)a->out % es || (uintptr_t)a->residual % es || (a->bias && (uintptr_t)a->bias % bs))

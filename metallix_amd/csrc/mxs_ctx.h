@@ -46,6 +46,8 @@ const char* noalloc_last_error();   // this thread's last mxs_logsoftmax_topn_no
 size_t spec_scratch_bytes(uint32_t max_rows, uint32_t max_vocab);
 size_t race_scratch_bytes(uint32_t max_rows, uint32_t max_vocab);
 size_t beam_scratch_bytes(uint32_t max_rows);
+size_t linear_scratch_bytes();
+size_t linear_ctr_words();
 constexpr uint32_t SPEC_COUNTERS_PER_ROW = 10;   // one per (row, position <= 8), one per row
 
 // Rows' counters and exchange words sit on their own 128-byte lines, so the
@@ -103,6 +105,9 @@ struct mxs_ctx {
   // mxs_beam_select: per-group arrival counters, per-chunk results
   uint32_t* beam_ctr = nullptr;
   void* beam_scratch = nullptr;
+  // mxs_linear_bf16: a split sum's parts and their arrivals
+  float* linear_scratch = nullptr;
+  uint32_t* linear_ctr = nullptr;
   // the uniform of the inverse-CDF draw mxs_sample_race discards (below)
   double* d_race_u = nullptr;
   // grammar-mask staging (mxs_mask_host / mxs_mask_upload, mx_mask.hip):
