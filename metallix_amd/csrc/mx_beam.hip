@@ -761,27 +761,22 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 template <typename T>
 struct Unaligned { typedef T type __attribute__((aligned(1))); };
 
-// Moves one T at `at` (offset `at` of row 0 of the group) between the rows,
-// in the lanes where `act`.  p: lane j holds row j's parent.  Every lane of
-// the wave comes here, so that the ballots see all parents.
-template <typename T, int WMAX>
-__device__ __forceinline__ void move_piece(char* at, uint64_t stride, int32_t p, bool act) {
-  typedef typename Unaligned<T>::type U;
-  const uint32_t l = threadIdx.x & 63u;
-  T v[WMAX];
-#pragma unroll
-  for (int j = 0; j < WMAX; ++j) {
-    const uint64_t to = __builtin_amdgcn_ballot_w64(p == j && l != (uint32_t)j);
-    if (to && act) v[j] = *reinterpret_cast<const U*>(at + (uint64_t)j * stride);
-  }
-#pragma unroll
-  for (int j = 0; j < WMAX; ++j) {
-    uint64_t to = __builtin_amdgcn_ballot_w64(p == j && l != (uint32_t)j);
-    while (to) {
-      const uint32_t d = (uint32_t)__builtin_ctzll(to);
-      to &= to - 1u;
-      if (act) *reinterpret_cast<U*>(at + (uint64_t)d * stride) = v[j];
-    }
+// Moves one T at `at` (in row 0 of the group) between the rows.  to[j]: the
+// rows that take row j over (uniform over the wave, in LDS).  Row J's value is
+// loaded, then the rows' after it, then row J's is stored: all loads before
+// all stores.  (A recursion and no array: an array written under conditions
+// is kept as one value, and copied whole at each: 222 registers for 8 rows.)
+template <typename T, int WMAX, int J>
+__device__ __forceinline__ void move_piece(char* at, uint64_t stride, const unsigned long long* to) {
+  if constexpr (J < WMAX) {
+    typedef typename Unaligned<T>::type U;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)to[J]);
+    const uint32_t hi = WMAX > 32 ? __builtin_amdgcn_readfirstlane((uint32_t)(to[J] >> 32)) : 0u;
+    T v;
+    if (lo | hi) v = *reinterpret_cast<const U*>(at + (uint64_t)J * stride);
+    move_piece<T, WMAX, J + 1>(at, stride, to);
+    for (uint32_t m = lo; m; m &= m - 1u) *reinterpret_cast<U*>(at + (uint64_t)(uint32_t)__builtin_ctz(m) * stride) = v;
+    for (uint32_t m = hi; m; m &= m - 1u) *reinterpret_cast<U*>(at + (uint64_t)(32u + (uint32_t)__builtin_ctz(m)) * stride) = v;
   }
 }
 
@@ -806,22 +801,32 @@ __global__ __launch_bounds__(RO_NT) void reorder_kernel(ReorderArgs A) {
   const uint32_t pieces = (uint32_t)((used + 15u) / 16u);   // per segment
   const uint32_t total = pieces * s.segments;               // < 2^31
   if (blockIdx.x * RO_NT >= total) return;                  // the whole workgroup
-  const uint32_t i = min(blockIdx.x * RO_NT + threadIdx.x, total - 1u);
-  const bool in = blockIdx.x * RO_NT + threadIdx.x < total;
+  __shared__ unsigned long long to[WMAX];
+  if (threadIdx.x < 64u) {
+    unsigned long long mine = 0ull;   // lane j: the rows that take row j over
+    for (uint32_t d = 0; d < W; ++d)
+      if ((uint32_t)__builtin_amdgcn_readlane(p, (int)d) == l && d != l) mine |= 1ull << d;
+    if (l < (uint32_t)WMAX) to[l] = mine;
+  }
+  __syncthreads();
+  const uint32_t i = blockIdx.x * RO_NT + threadIdx.x;
+  if (i >= total) return;
   const uint32_t seg = i / pieces, pc = i - seg * pieces;
   char* at = reinterpret_cast<char*>(s.data) + (uint64_t)g * W * s.row_stride + (uint64_t)seg * s.segment_stride +
              (uint64_t)pc * 16u;
-  const uint32_t have = !in ? 0u : (uint32_t)min((uint64_t)16u, used - (uint64_t)pc * 16u);
-  move_piece<u32x4, WMAX>(at, s.row_stride, p, have == 16u);
-  if (__builtin_amdgcn_ballot_w64(have & 15u)) {   // a segment's last bytes
-    move_piece<u32x2, WMAX>(at, s.row_stride, p, (have & 8u) != 0u);
-    at += have & 8u;
-    move_piece<uint32_t, WMAX>(at, s.row_stride, p, (have & 4u) != 0u);
-    at += have & 4u;
-    move_piece<uint16_t, WMAX>(at, s.row_stride, p, (have & 2u) != 0u);
-    at += have & 2u;
-    move_piece<uint8_t, WMAX>(at, s.row_stride, p, (have & 1u) != 0u);
+  const uint32_t have = (uint32_t)min((uint64_t)16u, used - (uint64_t)pc * 16u);
+  if (have == 16u) {
+    move_piece<u32x4, WMAX, 0>(at, s.row_stride, to);
+    return;
   }
+  // a segment's last bytes
+  if (have & 8u) move_piece<u32x2, WMAX, 0>(at, s.row_stride, to);
+  at += have & 8u;
+  if (have & 4u) move_piece<uint32_t, WMAX, 0>(at, s.row_stride, to);
+  at += have & 4u;
+  if (have & 2u) move_piece<uint16_t, WMAX, 0>(at, s.row_stride, to);
+  at += have & 2u;
+  if (have & 1u) move_piece<uint8_t, WMAX, 0>(at, s.row_stride, to);
 }
 
 template <int WMAX>

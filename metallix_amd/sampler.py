@@ -353,10 +353,15 @@ def reorder_struct(torch, device, states, parent, status, *, beams: Optional[int
     if len(dims) != len(states):
         raise ValueError("length_dim must be one dimension or one per state")
     arr = (MxsState * max(1, len(states)))()
+    last = None   # a cache's layers share one layout
     for i, (t, d) in enumerate(zip(states, dims)):
         if t.device != device:
             raise ValueError(f"states must be on {device}, not {t.device}")
-        arr[i] = state_struct(t, groups * W, d)
+        like = (t.shape, t.stride(), t.dtype, d)
+        if like != last:
+            m, last = state_struct(t, groups * W, d), like
+        m.data = t.data_ptr()
+        arr[i] = m
     r = MxsReorder()
     r.states, r.count = ctypes.cast(arr, ctypes.POINTER(MxsState)), len(states)
     r.groups, r.beams = groups, W
