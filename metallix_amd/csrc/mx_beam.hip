@@ -598,19 +598,7 @@ __device__ __forceinline__ void beam_finish(const BeamArgs& A, BeamSmem& S, uint
     tops = fmin(tops, S.wsum[w]);
   }
   gthr = fmax(gthr, tops);
-#pragma unroll
-  for (int i = 0; i < OWN; ++i)
-    if (ccnt[i] && ctr[i] >= gthr) S.surv[atomicAdd(&S.nsurv, 1u)] = (uint16_t)own(i);
-  if (tid < W && S.kind[tid] == 2) {
-    const double r = S.score[tid] * S.scale[tid];
-    if (r >= gthr) {
-      const uint32_t at = atomicAdd(&S.m, 1u);   // at most 64 of them
-      S.u.d[at] = BeamCand{r, beam_tie(tid, 1u, (uint32_t)A.end_token)};
-      S.key[at] = beam_key(r);
-    }
-  }
-  __syncthreads();
-  const uint32_t ns = S.nsurv;
+  uint32_t ns = 0;
   auto each = [&](auto&& f) {   // every listed entry that reaches gthr, 16 lanes to a chunk
     for (uint32_t k = tid >> 4; k < ns; k += BNT / 16u) {
       const uint32_t c = S.surv[k], b = c / C, count = S.cnt[c];
@@ -630,15 +618,46 @@ __device__ __forceinline__ void beam_finish(const BeamArgs& A, BeamSmem& S, uint
       }
     }
   };
-  each([&](double r, unsigned long long t) {
-    const uint32_t at = atomicAdd(&S.m, 1u);
-    if (at < BDENSE) {
-      S.u.d[at] = BeamCand{r, t};
-      S.key[at] = beam_key(r);
+  uint32_t m = 0;
+  for (int round = 0;; ++round) {
+    // the chunks that reach gthr, the ended beams and the entries that do
+#pragma unroll
+    for (int i = 0; i < OWN; ++i)
+      if (ccnt[i] && ctr[i] >= gthr) S.surv[atomicAdd(&S.nsurv, 1u)] = (uint16_t)own(i);
+    auto keep = [&](double r, unsigned long long t) {
+      const uint32_t at = atomicAdd(&S.m, 1u);
+      if (at < BDENSE) {
+        S.u.d[at] = BeamCand{r, t};
+        S.key[at] = beam_key(r);
+      }
+    };
+    if (tid < W && S.kind[tid] == 2) {
+      const double r = S.score[tid] * S.scale[tid];
+      if (r >= gthr) keep(r, beam_tie(tid, 1u, (uint32_t)A.end_token));
     }
-  });
-  __syncthreads();
-  const uint32_t m = S.m;
+    __syncthreads();
+    ns = S.nsurv;
+    each(keep);
+    __syncthreads();
+    m = S.m;
+    if (m <= 2u * n + 64u || round == 3) break;
+    // Many (few chunks or few of them with candidates, so a loose
+    // threshold): the n-th largest of those kept,
+    // which n candidates reach too, is a closer one.
+    double r[BDENSE / BNT];
+#pragma unroll
+    for (uint32_t i = 0; i < BDENSE / BNT; ++i) r[i] = tid + i * BNT < m ? S.u.d[tid + i * BNT].rank : -INFINITY;
+    const double wnth = beam_wave_nth(r, (n + (uint32_t)BNW - 1u) / (uint32_t)BNW);
+    if (lane() == 0) S.wsum[wave()] = wnth;
+    __syncthreads();   // (S.m and S.nsurv have been read)
+    if (tid == 0) S.m = S.nsurv = 0u;
+    double t = S.wsum[0];
+#pragma unroll
+    for (int w = 1; w < BNW; ++w) t = fmin(t, S.wsum[w]);
+    if (!(t > gthr)) break;   // equal ranks: m stands
+    gthr = t;
+    __syncthreads();
+  }
   if (tid < 8u && m + tid < BDENSE) S.key[m + tid] = 0u;
   __syncthreads();
   auto put = [&](uint32_t j, unsigned long long t) {
@@ -667,14 +686,14 @@ __device__ __forceinline__ void beam_finish(const BeamArgs& A, BeamSmem& S, uint
           same += v[j] == mine ? 1u : 0u;
         }
       }
-      if (same > 1u) {
-        at = 0;
-        uint32_t k = 0;
-        for (; k + 8u <= m; k += 8u)   // (eight reads in flight)
+      if (same > 1u)
+        for (uint32_t k = 0; k < m; k += 8u) {
+          const uint4 v0 = *reinterpret_cast<const uint4*>(&S.key[k]), v1 = *reinterpret_cast<const uint4*>(&S.key[k + 4u]);
+          const uint32_t v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
-          for (uint32_t j = 0; j < 8u; ++j) at += beam_before(S.u.d[k + j], e) ? 1u : 0u;
-        for (; k < m; ++k) at += beam_before(S.u.d[k], e) ? 1u : 0u;
-      }
+          for (uint32_t j = 0; j < 8u; ++j)
+            if (v[j] == mine) at += beam_before(S.u.d[k + j], e) ? 1u : 0u;
+        }
       if (at < n) put(at, e.tie);
     }
   } else {

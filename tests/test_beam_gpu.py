@@ -258,6 +258,20 @@ def test_ties_and_orders(torch_mod, sampler, V, n):
     check(torch_mod, sampler, np.zeros((2 * W, V), np.float32), np.full((2, W), -3.5), n, name="all equal", dtype="bf16")
 
 
+@pytest.mark.parametrize("G,W,V,n,dtype", [(8, 32, 151936, 64, "f32"), (4, 32, 50257, 64, "bf16"), (2, 64, 40000, 128, "f32"),
+                                           (3, 1, 9000, 128, "bf16"), (2, 16, 20000, 100, "bf16")])
+def test_first_steps_and_many_candidates(torch_mod, sampler, G, W, V, n, dtype):
+    """One live beam a group (few chunks hold all candidates), many wanted;
+    a group whose beams are nearly level; rows of few distinct values, whose
+    ties pass every list's length."""
+    rng = np.random.default_rng(V + n)
+    x, s = logits(rng, G * W, V), scores(rng, G, W)
+    s[0, 1:] = -np.inf
+    s[1] = -4.0 - 1e-3 * np.arange(W)
+    x[(G - 1) * W :] = np.round(x[(G - 1) * W :])
+    check(torch_mod, sampler, x, s, n, dtype=dtype, name="many")
+
+
 @pytest.mark.parametrize("top", [-3e38, -1e4, -750.0, -90.0, 0.0, 90.0, 800.0, 1e5, 3e38])
 def test_ranges_of_logits(torch_mod, sampler, top):
     G, W, V, n = 2, 3, 20011, 6
