@@ -44,11 +44,39 @@ __device__ __forceinline__ float exp_minus(float y) {
   return fabsf(t) < 126.0f ? __builtin_fmaf(e, r, e) : e;
 }
 
+// The normal distribution's integral up to y, to 2^-20 relative for y > -3
+// (2^-17 further down): erfc(x) = t exp(q(t) - x^2) with x = |y| / sqrt(2), t =
+// 1 / (1 + 0.4 x) and q the polynomial of degree 8 through its values at the
+// Chebyshev nodes for x in 0..9.3 (1.4e-7).  x^2 = y^2 / 2 in two parts: the
+// exponential would turn its rounding into a relative error.  About 25
+// instructions where the library's erff, whose two branches a wave takes
+// both, made the epilogue of 1032 x 240 x 7236 half of its time.
+__device__ __forceinline__ float normal_cdf(float y) {
+  const float a = fminf(fabsf(y), 17.0f);   // (erfc is 0 there)
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.282842712f, a, 1.0f));
+  float q = -0.218680516f;
+  q = __builtin_fmaf(q, t, 0.978943706f);
+  q = __builtin_fmaf(q, t, -1.59774411f);
+  q = __builtin_fmaf(q, t, 1.12605083f);
+  q = __builtin_fmaf(q, t, -0.530103087f);
+  q = __builtin_fmaf(q, t, 0.336691082f);
+  q = __builtin_fmaf(q, t, 0.390685141f);
+  q = __builtin_fmaf(q, t, 1.00293851f);
+  q = __builtin_fmaf(q, t, -1.48878169f);
+  const float hi = a * a, lo = __builtin_fmaf(a, a, -hi);
+  const float z = __builtin_fmaf(hi, -0.5f, q);
+  const float res = __builtin_fmaf(lo, -0.5f, (-0.5f * hi - z) + q);   // what z and hi have lost
+  const float yh = z * 1.44269504f;
+  const float e = __builtin_amdgcn_exp2f(yh);
+  const float h = 0.5f * t * __builtin_fmaf(e, __builtin_fmaf(yh, -0.693147182f, z) + res, e);
+  return y < 0.0f ? h : 1.0f - h;
+}
+
 __device__ __forceinline__ float activate(float y, int32_t act) {
   switch (act) {   // uniform, or known
     case MXS_ACT_RELU: return y < 0.0f ? 0.0f : y;   // (a NaN stays)
     case MXS_ACT_SILU: return y / (1.0f + exp_minus(y));
-    case MXS_ACT_GELU: return 0.5f * y * (1.0f + erff(y * 0.707106781f));
+    case MXS_ACT_GELU: return y * normal_cdf(y);
     case MXS_ACT_GELU_TANH: {
       // 0.5 (1 + tanh(u)) = 1 / (1 + exp(-2u)), u = sqrt(2/pi) (y + 0.044715 y^3)
       const float u2 = 1.59576912f * __builtin_fmaf(0.044715f * y * y, y, y);
@@ -65,6 +93,7 @@ __device__ __forceinline__ float ld_elem(const void* p, uint64_t i, int32_t f32)
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef f32x4 f32x4_u __attribute__((aligned(4)));     // (global memory takes unaligned accesses)
 typedef bf16x4 bf16x4_u __attribute__((aligned(2)));
+typedef bf16x8 bf16x8_u __attribute__((aligned(2)));
 
 // Four elements of `have` (1..4, the others 0) at i.
 __device__ __forceinline__ f32x4 ld_four(const void* p, uint64_t i, uint32_t have, int32_t f32) {
@@ -117,11 +146,78 @@ __device__ __forceinline__ void epilogue(const LinArgs& A, int32_t act, uint32_t
   }
 }
 
+// The epilogue of a wave's FO x FR blocks, the features from o and rows from
+// r on.  A block's lanes hold four features of 16 rows, 32 bytes of a bf16
+// row: stored like that the output reached 1.3 TB/s (4096 x 128 x 12288).  So
+// 16 rows at a time pass through LDS (the wave's own 16 x 16 FO floats, a row's
+// 16-byte pieces permuted by its low bits) and leave as 16 bytes a lane along the rows.  The bias and activation come
+// before, the residual, loaded along the rows too, after.
+template <int FO, int FR, int ACT, int E>   // E: elements in 16 bytes of output
+__device__ __forceinline__ void epilogue_wave(const LinArgs& A, uint32_t r, uint32_t o, const f32x4 (&acc)[FO][FR], float* lds) {
+  constexpr uint32_t W = 16u * FO, LPR = W / E, RPP = 64u / LPR, NP = 16u / RPP;   // lanes per row, rows per pass, passes
+  const uint32_t l = threadIdx.x & 63u, lr = l & 15u, lg = l >> 4;
+  const uint32_t row = l / LPR, col = o + (l % LPR) * E;   // what this lane stores
+  f32x4 bias[FO];
+#pragma unroll
+  for (int i = 0; i < FO; ++i) {
+    const uint32_t oi = o + 16u * (uint32_t)i + lg * 4u;
+    bias[i] = A.bias && oi < A.N ? ld_four(A.bias, oi, min(4u, A.N - oi), A.bias_f32) : f32x4{};
+  }
+#pragma unroll
+  for (int j = 0; j < FR; ++j) {
+    f32x4 res[NP][E / 4];
+    if (A.res) {
+#pragma unroll
+      for (uint32_t p = 0; p < NP; ++p) {
+        const uint32_t rr = r + 16u * (uint32_t)j + p * RPP + row;
+#pragma unroll
+        for (uint32_t q = 0; q < E / 4u; ++q) {
+          const uint32_t c = col + 4u * q;
+          res[p][q] = rr < A.R && c < A.N ? ld_four(A.res, (uint64_t)rr * A.rs + c, min(4u, A.N - c), E == 4) : f32x4{};
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < FO; ++i) {
+      f32x4 v = acc[i][j] + bias[i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = activate(v[e], ACT);
+      *reinterpret_cast<f32x4*>(lds + lr * W + (((uint32_t)i * 4u + lg) ^ (lr & 7u)) * 4u) = v;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (uint32_t p = 0; p < NP; ++p) {
+      const uint32_t rr = r + 16u * (uint32_t)j + p * RPP + row;
+      f32x4 v[E / 4];
+#pragma unroll
+      for (uint32_t q = 0; q < E / 4u; ++q) {
+        v[q] = *reinterpret_cast<const f32x4*>(lds + (p * RPP + row) * W + (((l % LPR) * (E / 4u) + q) ^ ((p * RPP + row) & 7u)) * 4u);
+        if (A.res) v[q] += res[p][q];
+      }
+      if (rr >= A.R || col >= A.N) continue;
+      const uint64_t at = (uint64_t)rr * A.os + col;
+      if (E == 8 && col + 8u <= A.N) {
+        bf16x8 h;
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; ++e) h[e] = (__bf16)v[e / 4u][e & 3u];
+        *reinterpret_cast<bf16x8_u*>(reinterpret_cast<__bf16*>(A.out) + at) = h;
+      } else {
+#pragma unroll
+        for (uint32_t q = 0; q < E / 4u; ++q)
+          if (col + 4u * q < A.N) st_four(A.out, at + 4u * q, min(4u, A.N - col - 4u * q), E == 4, v[q]);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
 // Sixteen bytes of a row at k, elements from K on as zero.
 __device__ __forceinline__ bf16x8 ld_k(const __bf16* row, uint32_t k, uint32_t K) {
-  if (k + 8u <= K) return *reinterpret_cast<const bf16x8*>(row + k);
   bf16x8 v = {};
-  if (k < K) {
+  if (k + 8u <= K) v = *reinterpret_cast<const bf16x8*>(row + k);
+  if ((K & 7u) && k < K && k + 8u > K) {   // (uniformly not, or one piece of a row)
 #pragma unroll
     for (uint32_t j = 0; j < 7u; ++j)
       if (k + j < K) v[j] = row[k + j];
@@ -217,6 +313,7 @@ __global__ __launch_bounds__(WO * WR * 64, 2) void linear_tile_kernel(LinArgs A)
   constexpr uint32_t PR = TK / 8, LR = 64 / PR;                       // pieces per row, rows per load
   constexpr int LA = BO / (int)LR / NW, LB = BR / (int)LR / NW;       // loads per wave
   static_assert(LA * (int)LR * NW == BO && LB * (int)LR * NW == BR, "the loads cover the tile");
+  // (two arrays: with one, the compiler waits for every load before a read)
   __shared__ __align__(1024) __bf16 As[S][BO * TK];
   __shared__ __align__(1024) __bf16 Bs[S][BR * TK];
   const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63u, lr = l & 15u, lg = l >> 4;
@@ -250,16 +347,16 @@ __global__ __launch_bounds__(WO * WR * 64, 2) void linear_tile_kernel(LinArgs A)
     }
   };
   auto fetch_part = [&](uint32_t k, __bf16* as, __bf16* bs) {   // the last k, not a whole tile
-#pragma unroll 1
-    for (int i = 0; i < LA; ++i) {
-      const uint32_t row = min((w * LA + i) * LR + ro, A.N - 1u - o0);
-      *reinterpret_cast<bf16x8*>(as + (w * LA + i) * LR * TK + l * 8u) = ld_k(wt + (uint64_t)row * A.ws, k + piece, K);
-    }
-#pragma unroll 1
-    for (int i = 0; i < LB; ++i) {
-      const uint32_t row = min((w * LB + i) * LR + ro, A.R - 1u - r0);
-      *reinterpret_cast<bf16x8*>(bs + (w * LB + i) * LR * TK + l * 8u) = ld_k(xt + (uint64_t)row * A.xs, k + piece, K);
-    }
+    auto rows = [&](auto count, const __bf16* from, uint64_t stride, uint32_t last, __bf16* to) {
+      constexpr int C = decltype(count)::value;
+      bf16x8 v[C];
+#pragma unroll
+      for (int i = 0; i < C; ++i) v[i] = ld_k(from + (uint64_t)min((w * C + i) * LR + ro, last) * stride, k + piece, K);
+#pragma unroll
+      for (int i = 0; i < C; ++i) *reinterpret_cast<bf16x8*>(to + (w * C + i) * LR * TK + l * 8u) = v[i];
+    };
+    rows(std::integral_constant<int, LA>{}, wt, A.ws, A.N - 1u - o0, as);
+    rows(std::integral_constant<int, LB>{}, xt, A.xs, A.R - 1u - r0, bs);
   };
   const uint32_t wo = (w / WR) * (BO / WO), wr = (w % WR) * (BR / WR);
   f32x4 acc[FO][FR] = {};
@@ -354,7 +451,6 @@ __global__ __launch_bounds__(WO * WR * 64, 2) void linear_tile_kernel(LinArgs A)
   mul(a1, b1, 0, FO);
   if (SPLIT) {
     // The parts' sums meet in memory; the tile's last part adds them in order.
-    static_assert(sizeof(As) >= 4, "a word of LDS for the arrival");
     float* mine = A.part + (uint64_t)job * (BO * BR) + threadIdx.x;
 #pragma unroll
     for (int i = 0; i < FO; ++i)
@@ -377,8 +473,16 @@ __global__ __launch_bounds__(WO * WR * 64, 2) void linear_tile_kernel(LinArgs A)
           for (int e = 0; e < 4; ++e) acc[i][j][e] += ld_dev(from + ((i * FR + j) * 4 + e) * (NW * 64));
     }
   }
+  if constexpr (FO < 4) {   // 64 bytes of a row per wave: straight away (1024 x 1024 x 1024 8.7 us, through LDS 9.7)
 #pragma unroll
-  for (int i = 0; i < FO; ++i) epilogue<FR>(A, ACT, r0 + wr + lr, o0 + wo + (uint32_t)i * 16u + lg * 4u, acc[i]);
+    for (int i = 0; i < FO; ++i) epilogue<FR>(A, ACT, r0 + wr + lr, o0 + wo + (uint32_t)i * 16u + lg * 4u, acc[i]);
+  } else {
+    static_assert(sizeof(As) >= NW * 16 * 16 * FO * sizeof(float), "the waves' rows fit");
+    __syncthreads();   // the tiles' last reads are done
+    float* const rows = reinterpret_cast<float*>(&As[0][0]) + w * (16u * 16u * FO);
+    if (A.out_f32) epilogue_wave<FO, FR, ACT, 4>(A, r0 + wr, o0 + wo, acc, rows);
+    else epilogue_wave<FO, FR, ACT, 8>(A, r0 + wr, o0 + wo, acc, rows);
+  }
 }
 
 template <int BO, int BR, int WO, int WR, int S, bool SPLIT>
@@ -409,12 +513,12 @@ static LinKernel linear_choice(LinArgs& A) {
   // 4 x 4096 x 14336 26.1 / 30.4; but 16 x 8192 x 1024 16.3 / 11.4, 16 x 4096
   // x 14336 36.3 / 31.1, 4 x 1024 x 151936 72 / 58.
   if ((A.R <= 16u && A.N <= 4096u && A.K <= 4096u) || (A.R <= 4u && A.N <= 16384u)) return LIN_ROWS;
-  // Few tiles of 64 and a long sum: at least 16 steps of 64 k to a part, up to
+  // Few tiles of 64 and a long sum: at least 10 steps of 64 k to a part, up to
   // 8 parts.  us, whole / split: 64 x 8192 x 1024 31.4 / 12.4, 256 x 4096 x
   // 1024 18.5 / 11.3, 2197 x 7797 x 31 35.1 / 17.4; but 256 x 1024 x 1024 6.9
   // / 7.8, and 64 x 4096 x 4096 12.4 in 256 jobs, 14.6 in 512.
   const uint64_t t64 = tiles(64, 64);
-  uint32_t parts = steps / 16u;
+  uint32_t parts = steps / 10u;
   if (parts > 8u) parts = 8u;
   if (parts > LIN_JOBS / t64) parts = (uint32_t)(LIN_JOBS / t64);
   if (parts >= 2u) {
@@ -423,16 +527,20 @@ static LinKernel linear_choice(LinArgs& A) {
     return LIN_SPLIT;
   }
   // Otherwise the tile with the least time: rounds of workgroups over 256 CUs
-  // (three of 64 x 64 share one) times what a step of 64 k takes in each (us,
-  // measured at 8192 x 8192 x 8192, 512 x 4096 x 4096 and 2048 x 4096 x 4096)
-  // and a tile's first loads and epilogue.
+  // (three of 64 x 64 share one) times what a step of 64 k takes in each, a
+  // tile's first loads and stores, and its activations (us; from 8192 x 8192 x
+  // 8192, 512 x 4096 x 4096, 4096 x 128 x 12288 and 8192 x 1024 x 4096).  us
+  // with tiles of 64 / 128 / 128 x 256 / 256: 8192 x 8192 x 8192 1601 / 1187 /
+  // 902 / 785, 2048 x 4096 x 4096 100 / 77 / 64 / 95, 128 x 1024 x 151936 118 /
+  // 98 / 112 / 120, 512 x 4096 x 4096 26 / 29 / 46 / 83.
+  const double act = A.act == MXS_ACT_NONE || A.act == MXS_ACT_RELU ? 0.0 : A.act == MXS_ACT_GELU ? 11.0 : 8.0;   // of 256 x 256
   auto rounds = [](uint64_t t, uint64_t per) { return (double)((t + per - 1u) / per); };
-  const uint64_t last = t64 % 768u;
-  const double at64 = (double)(t64 / 768u) * (0.56 * steps + 3.0) +
-                      (last ? (0.34 + 0.075 * rounds(last, 256)) * steps + 2.0 : 0.0);
-  const double at128 = rounds(tiles(128, 128), 256) * (0.50 * steps + 3.0);
-  const double at128_256 = rounds(tiles(128, 256), 256) * (0.88 * steps + 4.0);
-  const double at256 = rounds(tiles(256, 256), 256) * (1.62 * steps + 6.0);
+  const double left = rounds(t64 % 768u, 256);
+  const double at64 = (double)(t64 / 768u) * (0.565 * steps + 2.6 + act * 0.19) +
+                      (left > 0.0 ? (0.36 + 0.08 * left) * steps + 2.0 + act * 0.0625 * left : 0.0);
+  const double at128 = rounds(tiles(128, 128), 256) * (0.56 * steps + 2.7 + act * 0.25);
+  const double at128_256 = rounds(tiles(128, 256), 256) * (0.85 * steps + 4.2 + act * 0.5);
+  const double at256 = rounds(tiles(256, 256), 256) * (1.46 * steps + 9.0 + act);
   const double least = fmin(fmin(at64, at128), fmin(at128_256, at256));
   return least == at256 ? LIN_256 : least == at128_256 ? LIN_128_256 : least == at128 ? LIN_128 : LIN_64;
 }
