@@ -374,8 +374,8 @@ int mxs_beam_reorder(mxs_ctx* ctx, const mxs_reorder* reorder);
 /* A bf16 matrix product with its epilogue:
  *   out[r][o] = act(sum_k x[r][k] weight[o][k] + bias[o]) + residual[r][o]
  * x rows x in_features and weight out_features x in_features row-major bf16
- * (16-byte aligned, strides multiples of 8 elements; nothing past a row's
- * in_features is read), products summed in f32, the epilogue in f32 with
+ * (16-byte aligned, strides multiples of 8 below 2^22 elements; nothing past a
+ * row's in_features is read), products summed in f32, the epilogue in f32 with
  * one rounding to the output type.  Any number of rows and features.  bias
  * f32 or bf16 (bias_dtype) or NULL; residual of out's type or NULL; it may be
  * out itself (same stride), otherwise out may overlap no input. */

@@ -1,6 +1,49 @@
 // mx_beam.hip -- beam search: the selection of each group's n best
 // continuations over its beams and the vocabulary (mxs_beam_select), and the
 // move of the beams' states to their children (mxs_beam_reorder).
+//
+// The selection.  A live beam b with cumulative score s_b and logits l has
+// the candidates (b, v) of score s_b + (l_v - N_b), N_b = ln sum_u exp(l_u); an
+// ended beam is one candidate of its own score.  A group keeps the n largest
+// by score times the beam's scale.  One launch:
+//
+// - A row is split into C chunks of T tiles of 4096 tokens, one 256-thread
+//   workgroup each (rows that are not live exit).  It streams its chunk once.
+//   The weights are summed in f64, relative to a power of two near the first
+//   maximum met: with f64's exponent range that unit needs no running maximum
+//   (it moves for one 600 nats above).  A weight takes 15 vector instructions
+//   (beam_weight), as many as an f32 exponential with a corrected argument
+//   and its guards, at 2^-39 instead of 2^-22: beams are ordered by sums of
+//   such logarithms over hundreds of steps.
+// - Candidates: each thread keeps its largest logit of every tile in LDS.
+//   After the chunk (or 8 tiles) a threshold that n of the chunk's threads
+//   have reached comes from the threads' maxima, and only the (thread, tile)
+//   pairs that reach it (about n to 1.4 n) look at their 16 logits again, from
+//   L2 or the Infinity Cache; a NaN or +inf reaches it too and is found there.
+//   Scanning every tile against a running threshold instead took 101 us where
+//   this takes 76 (16 x 16 x 262144, n 32).  Near-ties that overflow a wave's
+//   256 slots are cut to its n largest, any number of times.
+// - The group's last workgroup (arrival counter) merges: the rows' N from
+//   their chunks' (unit, sum) in chunk order; a rank that n candidates reach,
+//   the best chunk threshold or the n-th largest chunk maximum; the entries
+//   at or above it, from the chunks whose maximum is; their order by counting
+//   on 32-bit keys.  While more than 2 n + 64 pass, the n-th largest of those
+//   kept is a closer threshold (8 x 32 x 151936, n 64, groups at their first
+//   step: 475 -> 70 us); more than 1024 equal ranks are taken one by one.
+//
+// Bound.  16 x 16 x 262144 f32 (221 MB of live rows), n 32: 73 us, 45 at the
+// 4.92 TB/s of a large copy; vector instructions (40% of the issue slots over
+// the launch) and the tail of the last groups' merges (9 us) keep it off the
+// stream.  253 MB are read, 30 of them second looks.  Small calls are a chain
+// of latencies: 1 x 4 x 50257, n 8, takes 13 us: 3.6 to load and sum, 1.2 to
+// publish, 1.7 to arrive, 6.3 to merge (statistics 1.1, norms 1.3, threshold
+// 1.5, entries 1.1, order and output 0.9).  Also measured, in the first
+// shape: 1024 workgroups 83 us and 4096 97 (2048: 76); five workgroups on a
+// CU 83 (spills); loads two tiles ahead 78; a polynomial of degree 7 the same.
+//
+// The move is a copy: reorder_kernel reads each surviving row and writes each
+// changed row once, at 4.7 to 5.3 TB/s of both from 64 MB on.
+
 #include <hip/hip_runtime.h>
 
 #include <float.h>
@@ -803,7 +846,11 @@ __device__ __forceinline__ void move_piece(char* at, uint64_t stride, const unsi
 // of every row that some other row takes over, then stores them to the rows
 // that take them.  No thread reads what another writes, so any permutation
 // goes in place, each surviving row read once and each changed row written
-// once.  WMAX, the most rows held, is the power of two at or above beams.
+// once.  WMAX, the most rows held, is the power of two at or above beams (20,
+// 36, 68, 133 and 255 registers).  us, and at 4.92 TB/s: 8 groups x 4 beams x
+// 56 states of 8 x 520 x 128 bf16, ragged lengths (1.87 GB) 358-383, 379; 4 x 8
+// 432, 433; 2 x 32 of half the length 508, 499; 1 x 64 607, 576; 1 x 4 x 56
+// states of 8 x 48 x 128 (28 MB) 7.2, 5.6.
 template <int WMAX>
 __global__ __launch_bounds__(RO_NT) void reorder_kernel(ReorderArgs A) {
   const mxs_state& s = A.st[blockIdx.z];
