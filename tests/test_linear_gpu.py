@@ -226,3 +226,85 @@ def test_no_rows_and_refusals(torch_mod, sampler):
         sampler.linear(z(4, 16), z(4, 16).cpu())
     with pytest.raises(ValueError):
         sampler.linear(z(4, 16), z(4, 16), activation="swish")
+
+
+# Sizes whose tiles are 128 x 128, 128 x 256 (features x rows) and 256 x 256,
+# and those summed in parts, each with a last tile that rows, features and k
+# leave unfilled.
+LARGER = [(2999, 31, 1025), (2900, 328, 1100), (257, 72, 12001), (300, 1000, 12003), (1031, 392, 7799),
+          (2999, 200, 4099), (4100, 1032, 2056), (700, 2056, 130), (33, 8200, 1023), (65, 1350, 130)]
+
+
+@pytest.mark.parametrize("R,K,N", LARGER)
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "gelu_tanh"])
+def test_larger_tiles(torch_mod, sampler, R, K, N, act):
+    i = len(act) + R
+    for out in ("bf16", "f32"):
+        check(torch_mod, sampler, R, K, N, act=act, bias=["none", "bf16", "f32"][i % 3], residual=i % 2 == 0, out=out,
+              pad=i % 2, spread=2.0, seed=i)
+        i += 1
+
+
+@pytest.mark.parametrize("R,K,N", [(2999, 72, 1025), (257, 72, 12001), (1031, 392, 7799), (700, 2056, 130)])
+def test_larger_tiles_strides_and_in_place(torch_mod, sampler, R, K, N):
+    torch = torch_mod
+    for dt, name in ((torch.bfloat16, "bf16"), (torch.float32, "f32")):
+        for off, stride in ((0, N + 8 - N % 8), (1, N + 2), (3, N)):
+            x, w, b, res, _ = inputs(torch, R, K, N, off + R, "bf16", True, name)
+            big = torch.full((R * stride + 8,), 7.5, dtype=dt, device="cuda")
+            out = big[off : off + R * stride].view(R, stride)[:, :N]
+            out.copy_(res)
+            say(f"case strides R {R} K {K} N {N} {name} off {off} stride {stride}, in place")
+            sampler.linear(x, w, b, activation="relu", residual=out, out=out)
+            torch.cuda.synchronize()
+            verify(torch, out, x, w, b, res, "relu")
+            keep = torch.ones_like(big, dtype=torch.bool)
+            keep[off : off + R * stride].view(R, stride)[:, :N] = False
+            assert bool((big[keep] == 7.5).all())
+
+
+@pytest.mark.parametrize("R,K,N", [(2999, 72, 1025), (257, 72, 12001), (1031, 392, 7799), (700, 2056, 130)])
+def test_larger_tiles_not_finite_and_repeated(torch_mod, sampler, R, K, N):
+    """A NaN or infinity stays in its row or feature; equal calls give equal
+    bits."""
+    torch = torch_mod
+    x, w, b, _, _ = inputs(torch, R, K, N, R, "f32", False, "f32")
+    x, w = padded(torch, x, 1), padded(torch, w, 2)
+    base = sampler.linear(x, w, b, out_dtype=torch.float32)
+    again = sampler.linear(x, w, b, out_dtype=torch.float32)
+    x2, w2 = x.clone(), w.clone()
+    x2[R - 1, K - 1] = float("nan")
+    w2[N - 1, 0] = float("inf")
+    got = sampler.linear(x2, w2, b, out_dtype=torch.float32)
+    torch.cuda.synchronize()
+    assert torch.equal(base, again)
+    assert bool(got[R - 1].isnan().all()) and bool((~got[: R - 1, N - 1].isfinite()).all())
+    assert torch.equal(got[: R - 1, : N - 1], base[: R - 1, : N - 1])
+
+
+def test_largest_tiles_captured_and_replayed(torch_mod):
+    torch = torch_mod
+    from metallix_amd import Sampler
+
+    stream = torch.cuda.Stream()
+    s = Sampler(max_rows=8, max_vocab=1024, stream=stream)
+    try:
+        for R, K, N in ((2999, 200, 4099), (300, 1000, 12003), (700, 2056, 130)):
+            x, w, b, res, _ = inputs(torch, R, K, N, R, "bf16", True, "bf16")
+            torch.cuda.synchronize()
+            call = s.linear_launcher(x, w, b, activation="gelu", residual=res)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                call(x)
+            for i in range(3):
+                new = inputs(torch, R, K, N, R + i + 1, "none", False, "bf16")[0]
+                torch.cuda.synchronize()
+                with torch.cuda.stream(stream):
+                    x.copy_(new)
+                    s.linear(x, w)
+                    graph.replay()
+                torch.cuda.synchronize()
+                verify(torch, call.out, x, w, b, res, "gelu")
+    finally:
+        s.close()
