@@ -313,7 +313,8 @@ int mxs_finish_tiles(mxs_ctx* ctx, const mxs_batch* batch, const void* tile_stat
  * status[g]: 0, MXS_ROW_PROBABILITIES (a score NaN or +inf, a scale not
  * finite and positive), MXS_ROW_NON_FINITE_LOGIT (a NaN or +inf among the
  * logits that count) or MXS_ROW_EMPTY_SUPPORT (no candidate).  With the first
- * two every entry is token -1, beam -1, score NaN, ended 0. */
+ * two every entry is token -1, beam -1, score NaN, ended 0.  But for the two
+ * arrays named below, the outputs meet neither an input nor one another. */
 #define MXS_BEAM_MAX 64    /* beams per group */
 #define MXS_BEAM_N_MAX 128 /* candidates per group */
 typedef struct {

@@ -10,6 +10,11 @@ namespace mxs {
 
 constexpr uint32_t BEAM_MAX_VOCAB = 2u << 20;   // tokens per row of mxs_beam_select
 
+inline bool ranges_meet(const void* a, uint64_t na, const void* b, uint64_t nb) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return x < y + nb && y < x + na;
+}
+
 inline const char* beam_check(const mxs_beam* b, const mxs_beam_out* o, uint32_t max_rows, uint32_t max_vocab) {
   if (!b || !o) return "beam and out are required";
   if (b->groups == 0) return nullptr;
@@ -22,6 +27,7 @@ inline const char* beam_check(const mxs_beam* b, const mxs_beam_out* o, uint32_t
   if ((uint64_t)b->groups * b->beams > max_rows || b->vocab > max_vocab || b->vocab > BEAM_MAX_VOCAB)
     return "batch exceeds the context's max_rows/max_vocab";
   if (b->row_stride < b->vocab || (b->row_stride & 3u)) return "row_stride must be >= vocab and a multiple of 4";
+  if (b->row_stride >= 1ull << 40 || (b->mask_words && b->mask_stride >= 1ull << 40)) return "strides are out of range";
   if ((uintptr_t)b->logits % (b->dtype == MXS_F32 ? 16u : 8u)) return "logits must be 16-byte (f32) or 8-byte (bf16) aligned";
   if (b->end_token < -1 || (b->end_token >= 0 && (uint32_t)b->end_token >= b->vocab))
     return "end_token must be -1 or a token of the vocabulary";
@@ -33,6 +39,25 @@ inline const char* beam_check(const mxs_beam* b, const mxs_beam_out* o, uint32_t
   }
   if (((const void*)o->score == (const void*)b->score || (o->ended && o->ended == b->ended)) && b->n != b->beams)
     return "out may share the input's score and ended arrays only when n == beams";
+  // A group's results are written while other groups' inputs are still read,
+  // so nothing else may meet.
+  struct Range { const void* p; uint64_t bytes; };
+  const uint64_t rows = (uint64_t)b->groups * b->beams, items = (uint64_t)b->groups * b->n;
+  const Range outs[5] = {{o->token, items * 4u}, {o->beam, items * 4u}, {o->score, items * 8u}, {o->ended, items},
+                         {o->status, b->groups * 4ull}};
+  const Range ins[5] = {{b->logits, ((rows - 1) * b->row_stride + b->vocab) * (b->dtype == MXS_F32 ? 4u : 2u)},
+                        {b->score, rows * 8u}, {b->ended, rows}, {b->scale, rows * 8u},
+                        {b->mask_words, ((rows - 1) * b->mask_stride + (b->vocab + 31u) / 32u) * 4u}};
+  for (int i = 0; i < 5; ++i) {
+    if (!outs[i].p) continue;
+    for (int j = 0; j < 5; ++j) {
+      const bool own = (i == 2 && j == 1) || (i == 3 && j == 2);   // (checked above)
+      if (ins[j].p && !(own && outs[i].p == ins[j].p) && ranges_meet(outs[i].p, outs[i].bytes, ins[j].p, ins[j].bytes))
+        return "out overlaps an input";
+    }
+    for (int j = 0; j < i; ++j)
+      if (outs[j].p && ranges_meet(outs[i].p, outs[i].bytes, outs[j].p, outs[j].bytes)) return "the outputs overlap";
+  }
   return nullptr;
 }
 
@@ -63,11 +88,6 @@ inline const char* reorder_check(const mxs_reorder* r) {
     if (!seg_apart || !(nested || crossed)) return "a state's rows or segments overlap";
   }
   return nullptr;
-}
-
-inline bool ranges_meet(const void* a, uint64_t na, const void* b, uint64_t nb) {
-  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-  return x < y + nb && y < x + na;
 }
 
 inline const char* linear_check(const mxs_linear* a) {

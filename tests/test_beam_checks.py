@@ -27,7 +27,7 @@ def checks(tmp_path_factory):
 
 def beam(**kw):
     b = S.MxsBeam()
-    b.logits, b.dtype, b.groups, b.beams, b.vocab, b.row_stride = 0x1000, 0, 3, 4, 1000, 1000
+    b.logits, b.dtype, b.groups, b.beams, b.vocab, b.row_stride = 0x100000, 0, 3, 4, 1000, 1000
     b.score, b.n, b.end_token = 0x2000, 4, -1
     for k, v in kw.items():
         setattr(b, k, v)
@@ -52,6 +52,11 @@ BEAM_BAD = [
     (dict(logits=0x1004, dtype=1), {}, "aligned"), (dict(end_token=1000), {}, "end_token"),
     (dict(end_token=-2), {}, "end_token"), (dict(ended=0x7000), {}, "end_token"),
     (dict(mask_words=0x8000, mask_stride=31), {}, "mask_stride"), (dict(legal_norm=1), {}, "mask_words"),
+    (dict(row_stride=1 << 62), {}, "range"), (dict(mask_words=0x8000, mask_stride=1 << 62), {}, "range"),
+    ({}, dict(score=0x2008), "overlaps"), ({}, dict(score=0x1ff8), "overlaps"), (dict(scale=0x5058), {}, "overlaps"),
+    (dict(ended=0x7000, end_token=2), dict(ended=0x7001), "overlaps"), ({}, dict(token=0x100000 + 47996), "overlaps"),
+    (dict(mask_words=0x8000, mask_stride=32), dict(status=0x85fc), "overlaps"), ({}, dict(beam=0x302c), "outputs"),
+    ({}, dict(status=0x5000), "outputs"), ({}, dict(ended=0x6004), "outputs"),
     (dict(n=8), dict(score=0x2000), "n == beams"), (dict(n=3, ended=0x7000, end_token=2), dict(ended=0x7000), "n == beams"),
 ]
 
@@ -62,9 +67,11 @@ def test_beam_select_refuses(checks, b, o, word):
     assert msg and word in msg.decode(), msg
 
 
-@pytest.mark.parametrize("b,o", [({}, {}), (dict(groups=0, logits=None), {}), (dict(logits=0x1008, dtype=1), {}),
+@pytest.mark.parametrize("b,o", [({}, {}), (dict(groups=0, logits=None), {}), (dict(logits=0x100008, dtype=1), {}),
                                  ({}, dict(score=0x2000)), (dict(ended=0x7000, end_token=0), dict(ended=0x7000)),
-                                 (dict(mask_words=0x8000, mask_stride=32, legal_norm=1), {})])
+                                 (dict(mask_words=0x8000, mask_stride=32, legal_norm=1), {}),
+                                 (dict(mask_words=0x8000, mask_stride=32), dict(status=0x8600)),
+                                 ({}, dict(beam=0x3030)), ({}, dict(token=0x100000 + 48000))])
 def test_beam_select_accepts(checks, b, o):
     assert checks.check_beam(ctypes.byref(beam(**b)), ctypes.byref(beam_out(**o)), 1000, 262144) is None
 
