@@ -350,8 +350,8 @@ int mxs_beam_select(mxs_ctx* ctx, const mxs_beam* beam, const mxs_beam_out* out)
  * A row of a state is `segments` pieces of segment_bytes, segment_stride
  * apart; all lengths in bytes, at any alignment.  With `lengths`, only the
  * first lengths[g] * position_bytes bytes of each segment move (states with
- * position_bytes 0 move whole).  Each surviving row is read once and each
- * changed row written once, whatever the permutation.  Rows and segments of
+ * position_bytes 0 move whole; it is below 4 GiB).  Each surviving row is read
+ * once and each changed row written once, whatever the permutation.  Rows and segments of
  * a state must not overlap, nor two states (the latter is not checked). */
 typedef struct {
   void* data;

@@ -76,9 +76,12 @@ inline const char* reorder_check(const mxs_reorder* r) {
     if (s.segments == 0 || s.segment_bytes == 0) return "a state's segments and segment_bytes must be positive";
     if (s.segment_bytes >= 1ull << 35 || (s.segment_bytes + 15u) / 16u * s.segments >= 1ull << 31)
       return "a state's row must be below 32 GiB";
+    if (s.position_bytes >= 1ull << 32) return "a state's position_bytes must be below 4 GiB";   // (times a length: 63 bits)
     if (s.position_bytes > s.segment_bytes) return "a state's position_bytes must be at most segment_bytes";
     // segments within a row, rows within a state: apart, or interleaved the other way round
-    if (s.row_stride >= 1ull << 48 || s.segment_stride >= 1ull << 48) return "a state's strides are out of range";
+    // (all below 2^48 from the first byte, so that no sum wraps)
+    if ((s.segments > 1 && s.segment_stride >= (1ull << 48) / (s.segments - 1u)) || (rows > 1 && s.row_stride >= (1ull << 48) / (rows - 1)))
+      return "a state's strides are out of range";
     const uint64_t one = s.segment_bytes;
     const bool seg_apart = s.segments == 1 || s.segment_stride >= one;
     const uint64_t row_span = (s.segments - 1ull) * s.segment_stride + one;

@@ -105,6 +105,9 @@ REORDER_BAD = [
     (dict(row_stride=4095), {}, "overlap"), (dict(segment_stride=511), {}, "overlap"),
     (dict(segment_stride=0), {}, "overlap"), (dict(row_stride=512, segment_stride=4095), {}, "overlap"),
     (dict(row_stride=1 << 50), {}, "range"),
+    # products that wrap 64 bits: segments that would come back to the row's start, positions to no bytes
+    (dict(segments=(1 << 17) + 1, segment_stride=1 << 47, row_stride=4096), {}, "range"),
+    (dict(segment_bytes=1 << 34, position_bytes=1 << 34, segments=1, segment_stride=1 << 34, row_stride=1 << 34), {}, "4 GiB"),
 ]
 
 
@@ -115,7 +118,8 @@ def test_beam_reorder_refuses(checks, s, r, word):
 
 
 @pytest.mark.parametrize("s", [{}, dict(row_stride=512, segment_stride=4096), dict(segments=1, segment_stride=0),
-                               dict(position_bytes=0)])
+                               dict(position_bytes=0), dict(segments=1, segment_stride=1 << 60),
+                               dict(segment_bytes=1 << 32, position_bytes=(1 << 32) - 1, segments=1, row_stride=1 << 32)])
 def test_beam_reorder_accepts(checks, s):
     assert checks.check_reorder(ctypes.byref(reorder([state(**s)]))) is None
 
