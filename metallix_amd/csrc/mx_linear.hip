@@ -593,8 +593,6 @@ extern "C" int mxs_linear_bf16(mxs_ctx* ctx, const mxs_linear* linear) {
   A.act = a.act;
   A.out_f32 = a.out_dtype == MXS_F32;
   A.bias_f32 = a.bias_dtype == MXS_F32;
-  if ((uint64_t)((a.rows + 63u) / 64u) * ((a.out_features + 63u) / 64u) >= 1u << 31)
-    return fail(ctx, MXS_EINVAL, "rows x out_features is too large");
   int prev = 0;
   (void)hipGetDevice(&prev);
   if (prev != ctx->device) (void)hipSetDevice(ctx->device);

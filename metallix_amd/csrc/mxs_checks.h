@@ -99,6 +99,8 @@ inline const char* linear_check(const mxs_linear* a) {
   if (!a->x || !a->weight || !a->out) return "x, weight and out are required";
   if (a->in_features == 0 || a->out_features == 0) return "in_features and out_features must be positive";
   if (a->in_features > 1u << 30 || a->out_features > 1u << 30 || a->rows > 1u << 30) return "rows and features must be at most 2^30";
+  if ((a->rows + 63ull) / 64u * ((a->out_features + 63ull) / 64u) >= 1ull << 23)   // (a launch holds below 2^32 threads)
+    return "rows x out_features must be below 2^35 (counted in whole blocks of 64 x 64)";
   if (a->act < MXS_ACT_NONE || a->act > MXS_ACT_GELU_TANH) return "act must be one of MXS_ACT_*";
   if (a->out_dtype != MXS_F32 && a->out_dtype != MXS_BF16) return "out_dtype must be MXS_F32 or MXS_BF16";
   if (a->bias && a->bias_dtype != MXS_F32 && a->bias_dtype != MXS_BF16) return "bias_dtype must be MXS_F32 or MXS_BF16";

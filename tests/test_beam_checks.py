@@ -142,7 +142,8 @@ LINEAR_BAD = [
     (dict(weight=0x20008), "aligned"), (dict(out=0x40001), "aligned"), (dict(out=0x40002, out_dtype=0), "aligned"),
     (dict(out=0x10010), "overlaps"), (dict(out=0x20ff0), "overlaps"), (dict(bias=0x40010, bias_dtype=1), "overlaps"),
     (dict(residual=0x40002, residual_stride=32), "residual"), (dict(residual=0x40000, residual_stride=48), "residual"),
-    (dict(rows=1 << 31), "2^30"), (dict(x_stride=1 << 41), "range"),
+    (dict(rows=1 << 31), "2^30"), (dict(rows=1 << 30, x_stride=64, in_features=64, out_features=64, out_stride=64), "2^35"),
+    (dict(rows=1 << 18, out_features=1 << 17, out_stride=1 << 17), "2^35"), (dict(x_stride=1 << 41), "range"),
 ]
 
 
@@ -153,7 +154,8 @@ def test_linear_refuses(checks, a, word):
 
 
 @pytest.mark.parametrize("a", [{}, dict(rows=0, x=None), dict(residual=0x40000, residual_stride=32),
-                               dict(in_features=57), dict(out_features=31), dict(bias=0x40400, bias_dtype=0)])
+                               dict(in_features=57), dict(out_features=31), dict(bias=0x40400, bias_dtype=0),
+                               dict(rows=(1 << 29) - 64, out_stride=32, out=1 << 44, x=1 << 45)])
 def test_linear_accepts(checks, a):
     assert checks.check_linear(ctypes.byref(linear(**a))) is None
 
