@@ -352,6 +352,8 @@ def reorder_struct(torch, device, states, parent, status, *, beams: Optional[int
     dims = list(length_dim) if isinstance(length_dim, (list, tuple)) else [length_dim] * len(states)
     if len(dims) != len(states):
         raise ValueError("length_dim must be one dimension or one per state")
+    if len({t.data_ptr() for t in states}) != len(states):
+        raise ValueError("a state is given twice: its rows would move twice at once")
     arr = (MxsState * max(1, len(states)))()
     last = None   # a cache's layers share one layout
     for i, (t, d) in enumerate(zip(states, dims)):

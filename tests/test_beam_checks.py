@@ -204,6 +204,7 @@ def test_reorder_struct_refuses():
     assert (f().groups, f().beams, f().count) == (2, 4, 1)
     assert f(states=[t[:4]], beams=2).parent_stride == 4
     for kw in (dict(parent=p.long()), dict(parent=p[0]), dict(beams=5), dict(beams=0), dict(states=[t[:7]]),
+               dict(states=[t, t]), dict(states=[t, torch.zeros(8, 2), t[:, :2]]),
                dict(lengths=torch.zeros(3, dtype=torch.int32)), dict(lengths=torch.zeros(2)),
                dict(length_dim=[1, 1]), dict(length_dim=2), dict(parent=torch.zeros(4, 2, dtype=torch.int32).t())):
         with pytest.raises(ValueError):
