@@ -61,6 +61,10 @@ class BeamSearch:
             raise ValueError(f"the search holds {self.max_new} tokens")
         s, torch = self.sampler, self.sampler.torch
         with torch.cuda.stream(s.stream):
+            # (the states are checked before anything is queued)
+            dims = list(length_dim) if isinstance(length_dim, (list, tuple)) else [length_dim] * len(states)
+            move = s.reorder_launcher([*states, self.tokens, self.length], self.picked.beam, lengths=lengths,
+                                      length_dim=[*dims, None, None], status=self.moved)
             if self.end_token is not None:
                 rule = dict(rule, ended=self.ended, end_token=self.end_token)
             if self.length_penalty:
@@ -71,9 +75,7 @@ class BeamSearch:
             else:
                 self.length.fill_(self.steps + 1)
             s.beam_select(logits, self.score, self.beams, out=self.picked, **rule)
-            dims = list(length_dim) if isinstance(length_dim, (list, tuple)) else [length_dim] * len(states)
-            s.beam_reorder([*states, self.tokens, self.length], self.picked.beam, lengths=lengths,
-                           length_dim=[*dims, None, None], status=self.moved)
+            move()
             self.tokens[:, self.steps] = self.picked.token.view(-1)
         self.steps += 1
         return self.picked.token.view(-1)

@@ -99,3 +99,34 @@ def test_search(torch_mod, G, W, V, penalty):
     with pytest.raises(ValueError):
         search.step(lgp[:, :V])
     s.close()
+
+
+def test_a_refused_step_leaves_the_search_as_it_was(torch_mod):
+    """States or logits that do not fit raise before anything moves: the step
+    with the right ones gives what a search without the mistakes gives."""
+    torch = torch_mod
+    from metallix_amd import BeamSearch, Sampler
+
+    G, W, V, T = 2, 3, 40, 4
+    s = Sampler(max_rows=G * W, max_vocab=V)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    steps = [torch.randn((G * W, V), generator=g, device="cuda") for _ in range(T)]
+    found = []
+    for mistakes in (False, True):
+        search = BeamSearch(s, G, W, T, end_token=3, length_penalty=0.5)
+        state = torch.arange(G * W * 5, dtype=torch.float32, device="cuda").view(G * W, 5).clone()
+        for lg in steps:
+            if mistakes:
+                for bad in (dict(states=[state[:-1]]), dict(states=[state, state]), dict(states=[state.cpu()]),
+                            dict(states=[state], length_dim=[1, 1]), dict(states=[state], mask=state),
+                            dict(states=[state], lengths=torch.zeros(G, device="cuda"))):
+                    with pytest.raises(ValueError):
+                        search.step(lg, **bad)
+                with pytest.raises(ValueError):
+                    search.step(lg[:-1], [state])
+            search.step(lg, [state])
+        found.append((search.result(), state.cpu()))
+        with pytest.raises(ValueError):
+            search.step(steps[0], [state])
+    assert found[0][0] == found[1][0] and torch.equal(found[0][1], found[1][1])
+    s.close()
