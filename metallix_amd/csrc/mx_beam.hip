@@ -17,7 +17,9 @@
 //   such logarithms over hundreds of steps.
 // - Candidates: each thread keeps its largest logit of every tile in LDS.
 //   After the chunk (or 8 tiles) a threshold that n of the chunk's threads
-//   have reached comes from the threads' maxima, and only the (thread, tile)
+//   have reached comes from the threads' maxima (of the waves that have
+//   enough of them, where a mask or the row's end leaves some without: 24.7 to
+//   22.8 us at 7 x 5 x 151936 bf16 under masks), and only the (thread, tile)
 //   pairs that reach it (about n to 1.4 n) look at their 16 logits again, from
 //   L2 or the Infinity Cache; a NaN or +inf reaches it too and is found there.
 //   Scanning every tile against a running threshold instead took 101 us where
@@ -35,9 +37,9 @@
 // 4.92 TB/s of a large copy; vector instructions (40% of the issue slots over
 // the launch) and the tail of the last groups' merges (9 us) keep it off the
 // stream.  253 MB are read, 30 of them second looks.  Small calls are a chain
-// of latencies: 1 x 4 x 50257, n 8, takes 13 us: 3.6 to load and sum, 1.2 to
-// publish, 1.7 to arrive, 6.3 to merge (statistics 1.1, norms 1.3, threshold
-// 1.5, entries 1.1, order and output 0.9).  Also measured, in the first
+// of latencies: 1 x 4 x 50257, n 8, takes 12.3 us: 3.4 to load and sum, 1.2
+// to publish, 1.8 to arrive, 5.4 to merge (statistics 1.1, norms 0.9,
+// threshold 1.5, entries 1.0, order and output 0.9).  Also measured, in the first
 // shape: 1024 workgroups 83 us and 4096 97 (2048: 76); five workgroups on a
 // CU 83 (spills); loads two tiles ahead 78; a polynomial of degree 7 the same.
 //
@@ -51,6 +53,7 @@
 #include <stdint.h>
 
 #include <string>
+#include <type_traits>
 
 #include "../../include/mx_sampler.h"
 #include "mxs_checks.h"
@@ -153,7 +156,7 @@ struct alignas(16) BeamSmem {
     BeamCand d[BDENSE];                                                    // ... and its candidates
   } u;
   double wref[BNW], wsum[BNW];
-  uint32_t wthr[2][BNW], wcnt[2][BNW], wtop[BNW], wbad[BNW];
+  uint32_t wthr[2][BNW], whave[2][BNW], wfew[BNW], wcnt[2][BNW], wtop[BNW], wbad[BNW];
   double score[MXS_BEAM_MAX], scale[MXS_BEAM_MAX], norm[MXS_BEAM_MAX];
   uint32_t key[BDENSE];                                                    // beam_key of the finisher's candidates
   uint16_t surv[BGCH], cnt[BGCH];
@@ -303,22 +306,54 @@ __device__ __forceinline__ void beam_chunk(const BeamArgs& A, BeamSmem& S, uint3
       // candidates have: each wave's n/4-th largest lane maximum (0 where
       // fewer lanes hold a candidate), the smallest over the waves, to its
       // upper 18 bits (a few candidates more, 14 ballots less).
-      const uint32_t sh = (n + (uint32_t)BNW - 1u) / (uint32_t)BNW;
-      const bool any = lm > -INFINITY;
-      uint32_t wthr = 0u;
-      if ((uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(any)) >= sh) {
-        const uint32_t ak = any ? okey(lm) : 0u;
+      const uint32_t ak = lm > -INFINITY ? okey(lm) : 0u;
+      const uint32_t have = (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(ak != 0u));
+      auto reached = [&](uint32_t by) {   // by `by` of the wave's lanes
+        uint32_t wthr = 0u;
+        if (have >= by) {
 #pragma unroll
-        for (int bit = 31; bit >= 14; --bit) {
-          const uint32_t c = wthr | (1u << bit);
-          if ((uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(ak >= c)) >= sh) wthr = c;
+          for (int bit = 31; bit >= 14; --bit) {
+            const uint32_t c = wthr | (1u << bit);
+            if ((uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(ak >= c)) >= by) wthr = c;
+          }
         }
+        return wthr;
+      };
+      const uint32_t wthr = reached((n + (uint32_t)BNW - 1u) / (uint32_t)BNW);
+      if (lane() == 0) {
+        S.wthr[slot][wave()] = wthr;
+        S.whave[slot][wave()] = have;
       }
-      if (lane() == 0) S.wthr[slot][wave()] = wthr;
       lds_barrier();
       uint32_t t = 0xffffffffu;
 #pragma unroll
       for (int w = 0; w < BNW; ++w) t = min(t, S.wthr[slot][w]);
+      if (t == 0u) {   // uniform: a wave has too few
+        // Fewer waves may have enough (a mask's runs, the row's end): the a-th
+        // largest of the waves' n/a-th largest.
+        uint32_t a = (uint32_t)BNW - 1u;
+        for (; a; --a) {
+          uint32_t ok = 0u;
+#pragma unroll
+          for (int w = 0; w < BNW; ++w) ok += S.whave[slot][w] >= (n + a - 1u) / a ? 1u : 0u;
+          if (ok >= a) break;
+        }
+        if (a) {
+          const uint32_t w1 = reached((n + a - 1u) / a);
+          if (lane() == 0) S.wfew[wave()] = w1;
+          lds_barrier();
+          uint32_t k[BNW];
+#pragma unroll
+          for (int w = 0; w < BNW; ++w) k[w] = S.wfew[w];
+#pragma unroll
+          for (int w = 0; w < BNW; ++w) {
+            uint32_t above = 0u;   // those at or above it
+#pragma unroll
+            for (int v = 0; v < BNW; ++v) above += k[v] >= k[w] ? 1u : 0u;
+            if (above >= a) t = max(t, k[w]);
+          }
+        }
+      }
       slot ^= 1u;
       thr = max(thr, t);
       lim = max(lim, (unsigned long long)thr << 32);
@@ -481,6 +516,21 @@ __device__ __forceinline__ unsigned long long beam_tie(uint32_t beam, uint32_t k
 __device__ __forceinline__ double beam_score(const BeamSmem& S, uint32_t b, uint32_t key) {
   return S.kind[b] == 2 ? S.score[b] : S.score[b] + ((double)okey_value(key) - S.norm[b]);
 }
+__device__ __forceinline__ double beam_rank(const BeamSmem& S, uint32_t b, uint32_t key) {   // of a live beam's candidate
+  return (S.score[b] + ((double)okey_value(key) - S.norm[b])) * S.scale[b];
+}
+
+// Over each 16 lanes, in all of them.
+template <typename F>
+__device__ __forceinline__ double row_all_f64(double v, F f) {
+  auto turned = [](auto ctrl, double x) {
+    return __builtin_bit_cast(double, dpp64<decltype(ctrl)::value>(__builtin_bit_cast(unsigned long long, x)));
+  };
+  v = f(v, turned(std::integral_constant<int, 0x128>{}, v));   // row_ror:8, 4, 2, 1
+  v = f(v, turned(std::integral_constant<int, 0x124>{}, v));
+  v = f(v, turned(std::integral_constant<int, 0x122>{}, v));
+  return f(v, turned(std::integral_constant<int, 0x121>{}, v));
+}
 
 __device__ __forceinline__ bool beam_before(const BeamCand& a, const BeamCand& b) {
   return (a.rank > b.rank) | ((a.rank == b.rank) & (a.tie > b.tie));   // (no branch around the second read)
@@ -509,10 +559,13 @@ __device__ __forceinline__ double beam_wave_nth(const double (&r)[OWN], uint32_t
 #pragma unroll
   for (int i = 0; i < OWN; ++i) least = key[i] ? min(least, key[i]) : least;
   least = ~wave_max_u32(~least);
-  // the bits all keys share, then the twelve after them: within 2^-11 of the
-  // ranks' spread
-  const int first = most == least ? -1 : 31 - __builtin_clz(most ^ least);
-  uint32_t t = first < 0 ? most : most & ~((2u << first) - 1u);
+  // twelve bits of the keys' distance from the least: within 2^-11 of their
+  // spread (a prefix of the keys themselves says nothing across 2.0, where
+  // the exponent's upper bit turns)
+#pragma unroll
+  for (int i = 0; i < OWN; ++i) key[i] = key[i] ? key[i] - least + 1u : 0u;
+  const int first = 31 - __builtin_clz(most - least + 1u);
+  uint32_t t = 0u;
   for (int bit = first; bit >= max(0, first - 11); --bit) {
     const uint32_t c = t | (1u << bit);
     uint32_t count = 0u;
@@ -520,6 +573,7 @@ __device__ __forceinline__ double beam_wave_nth(const double (&r)[OWN], uint32_t
     for (int i = 0; i < OWN; ++i) count += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(key[i] >= c));
     if (count >= k) t = c;
   }
+  t = least + max(t, 1u) - 1u;
   const unsigned long long b = (unsigned long long)t << 32;
   return __builtin_bit_cast(double, (t >> 31) ? b & ~(1ull << 63) : ~b);
 }
@@ -589,32 +643,28 @@ __device__ __forceinline__ void beam_finish(const BeamArgs& A, BeamSmem& S, uint
     if (tid == 0) A.status[g] = (S.flags & 1u) ? MXS_ROW_PROBABILITIES : MXS_ROW_NON_FINITE_LOGIT;
     return;
   }
-  // each chunk's sum relative to its row's largest unit, then the row's sum in chunk order
-  double rel[OWN];
-#pragma unroll
-  for (int i = 0; i < OWN; ++i) {
-    const uint32_t c = own(i);
-    rel[i] = 0.0;
-    if (c < NC && S.kind[c / C] == 1 && ref[i] > -INFINITY) {
-      const uint32_t c0 = c / C * C;
-      double m = ref[i];
-      for (uint32_t k = 0; k < C; ++k) m = fmax(m, S.u.c.ref[c0 + k]);
-      rel[i] = sum[i] * exp_neg_p(ref[i] - m);
+  // The rows' norms: a row's chunks on 16 lanes or 64, relative to the largest
+  // unit, added in an order that the number of chunks alone gives.
+  {
+    const bool few = C <= 16u || W > (uint32_t)BNW;   // (sixteen rows at once, or one per wave)
+    const uint32_t L = few ? 16u : 64u;
+    auto whole = [&](double v, auto f) {
+      v = row_all_f64(v, f);
+      return few ? v : f(f(readlane_t(v, 0), readlane_t(v, 16)), f(readlane_t(v, 32), readlane_t(v, 48)));
+    };
+    for (uint32_t b0 = wave() * (64u / L); b0 < W; b0 += (uint32_t)BNW * (64u / L)) {
+      const uint32_t b = b0 + lane() / L, first = b * C, k0 = lane() % L;
+      const bool live = b < W && S.kind[min(b, W - 1u)] == 1;
+      double m = -INFINITY, t = 0.0;
+      for (uint32_t k = k0; live && k < C; k += L) m = fmax(m, S.u.c.ref[first + k]);
+      m = whole(m, [](double x, double y) { return fmax(x, y); });
+      for (uint32_t k = k0; live && k < C; k += L) {
+        const double r = S.u.c.ref[first + k];
+        if (r > -INFINITY) t += S.u.c.sum[first + k] * exp_neg_p(r - m);
+      }
+      t = whole(t, [](double x, double y) { return x + y; });
+      if (live && k0 == 0u) S.norm[b] = m + log(t);   // (a row without weight has no candidates either)
     }
-  }
-#pragma unroll
-  for (int i = 0; i < OWN; ++i) {
-    const uint32_t c = own(i);
-    if (c < NC) S.u.c.sum[c] = rel[i];
-  }
-  __syncthreads();
-  if (tid < W && S.kind[tid] == 1) {
-    double m = -INFINITY, t = 0.0;
-    for (uint32_t k = 0; k < C; ++k) {
-      m = fmax(m, S.u.c.ref[tid * C + k]);
-      t += S.u.c.sum[tid * C + k];
-    }
-    S.norm[tid] = m + log(t);   // (a row without weight has no candidates either)
   }
   __syncthreads();
   // A rank that n candidates reach: the best chunk threshold, or the n-th
@@ -624,8 +674,8 @@ __device__ __forceinline__ void beam_finish(const BeamArgs& A, BeamSmem& S, uint
 #pragma unroll
   for (int i = 0; i < OWN; ++i) {
     const uint32_t b = min(own(i), NC - 1u) / C;
-    ctr[i] = ccnt[i] ? beam_score(S, b, ctop[i]) * S.scale[b] : -INFINITY;
-    if (cthr[i]) gthr = fmax(gthr, beam_score(S, b, max(cthr[i], okey(-FLT_MAX))) * S.scale[b]);
+    ctr[i] = ccnt[i] ? beam_rank(S, b, ctop[i]) : -INFINITY;
+    if (cthr[i]) gthr = fmax(gthr, beam_rank(S, b, max(cthr[i], okey(-FLT_MAX))));
   }
   gthr = wave_max_f64(gthr);
   const double nth = beam_wave_nth(ctr, (n + (uint32_t)BNW - 1u) / (uint32_t)BNW);
@@ -643,20 +693,38 @@ __device__ __forceinline__ void beam_finish(const BeamArgs& A, BeamSmem& S, uint
   gthr = fmax(gthr, tops);
   uint32_t ns = 0;
   auto each = [&](auto&& f) {   // every listed entry that reaches gthr, 16 lanes to a chunk
-    for (uint32_t k = tid >> 4; k < ns; k += BNT / 16u) {
-      const uint32_t c = S.surv[k], b = c / C, count = S.cnt[c];
-      const double* list = reinterpret_cast<const double*>(&A.list[((uint64_t)g * NC + c) * BLIST]);
-      const double bs = S.score[b], bn = S.norm[b], bc = S.scale[b];   // (live beams only have lists)
-      for (uint32_t j0 = tid & 15u; j0 < count; j0 += 64u) {
-        double d[4];   // (four loads in flight)
+    for (uint32_t k = tid >> 4; k < ns; k += 2u * (BNT / 16u)) {
+      double d[2][4];   // (two chunks' loads in flight)
+      uint32_t c[2], count[2];
+      const double* list[2];
 #pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i) d[i] = ld_dev(&list[min(j0 + 16u * i, count - 1u)]);
+      for (uint32_t h = 0; h < 2u; ++h) {
+        c[h] = S.surv[min(k + h * (BNT / 16u), ns - 1u)];
+        count[h] = k + h * (BNT / 16u) < ns ? S.cnt[c[h]] : 0u;
+        list[h] = reinterpret_cast<const double*>(&A.list[((uint64_t)g * NC + c[h]) * BLIST]);
 #pragma unroll
         for (uint32_t i = 0; i < 4u; ++i) {
-          const unsigned long long e = __builtin_bit_cast(unsigned long long, d[i]);
-          const uint32_t key = (uint32_t)(e >> 32);
-          const double r = (bs + ((double)okey_value(key) - bn)) * bc;
-          if (j0 + 16u * i < count && r >= gthr) f(r, beam_tie(b, key, ~(uint32_t)e));
+          const uint32_t j = (tid & 15u) + 16u * i;
+          if (j < count[h]) d[h][i] = ld_dev(&list[h][j]);
+        }
+      }
+#pragma unroll
+      for (uint32_t h = 0; h < 2u; ++h) {
+        const uint32_t b = c[h] / C;
+        const double bs = S.score[b], bn = S.norm[b], bc = S.scale[b];   // (live beams only have lists)
+        for (uint32_t j0 = tid & 15u; j0 < count[h]; j0 += 64u) {
+          if (j0 >= 64u)
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; ++i)
+              if (j0 + 16u * i < count[h]) d[h][i] = ld_dev(&list[h][j0 + 16u * i]);
+#pragma unroll
+          for (uint32_t i = 0; i < 4u; ++i) {
+            if (j0 + 16u * i >= count[h]) continue;
+            const unsigned long long e = __builtin_bit_cast(unsigned long long, d[h][i]);
+            const uint32_t key = (uint32_t)(e >> 32);
+            const double r = (bs + ((double)okey_value(key) - bn)) * bc;
+            if (r >= gthr) f(r, beam_tie(b, key, ~(uint32_t)e));
+          }
         }
       }
     }
@@ -689,7 +757,10 @@ __device__ __forceinline__ void beam_finish(const BeamArgs& A, BeamSmem& S, uint
     // which n candidates reach too, is a closer one.
     double r[BDENSE / BNT];
 #pragma unroll
-    for (uint32_t i = 0; i < BDENSE / BNT; ++i) r[i] = tid + i * BNT < m ? S.u.d[tid + i * BNT].rank : -INFINITY;
+    for (uint32_t i = 0; i < BDENSE / BNT; ++i) {   // (in turn to the waves: neighbours are of one chunk)
+      const uint32_t at = (uint32_t)own((int)i);
+      r[i] = at < m ? S.u.d[at].rank : -INFINITY;
+    }
     const double wnth = beam_wave_nth(r, (n + (uint32_t)BNW - 1u) / (uint32_t)BNW);
     if (lane() == 0) S.wsum[wave()] = wnth;
     __syncthreads();   // (S.m and S.nsurv have been read)
@@ -733,9 +804,10 @@ __device__ __forceinline__ void beam_finish(const BeamArgs& A, BeamSmem& S, uint
         for (uint32_t k = 0; k < m; k += 8u) {
           const uint4 v0 = *reinterpret_cast<const uint4*>(&S.key[k]), v1 = *reinterpret_cast<const uint4*>(&S.key[k + 4u]);
           const uint32_t v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+          uint32_t eq = 0u;
 #pragma unroll
-          for (uint32_t j = 0; j < 8u; ++j)
-            if (v[j] == mine) at += beam_before(S.u.d[k + j], e) ? 1u : 0u;
+          for (uint32_t j = 0; j < 8u; ++j) eq |= v[j] == mine ? 1u << j : 0u;
+          for (; eq; eq &= eq - 1u) at += beam_before(S.u.d[k + (uint32_t)__builtin_ctz(eq)], e) ? 1u : 0u;
         }
       if (at < n) put(at, e.tie);
     }
