@@ -336,6 +336,7 @@ __global__ __launch_bounds__(WO * WR * 64, 2) void linear_tile_kernel(LinArgs A)
   constexpr int NW = WO * WR, FO = BO / WO / 16, FR = BR / WR / 16;   // waves; 16 x 16 blocks per wave
   constexpr uint32_t PR = TK / 8, LR = 64 / PR;                       // pieces per row, rows per load
   constexpr int LA = BO / (int)LR / NW, LB = BR / (int)LR / NW;       // loads per wave
+  static_assert(S <= 5, "the last tiles' waits");
   static_assert(LA * (int)LR * NW == BO && LB * (int)LR * NW == BR, "the loads cover the tile");
   // (two arrays: with one, the compiler waits for every load before a read)
   __shared__ __align__(1024) __bf16 As[S][BO * TK];
@@ -465,7 +466,8 @@ __global__ __launch_bounds__(WO * WR * 64, 2) void linear_tile_kernel(LinArgs A)
   }
   for (; kt < nk; ++kt) {
     const uint32_t after = whole > kt + 1u ? whole - 1u - kt : 0u;
-    if (S > 3 && after >= 2u) tile_barrier<2 * (LA + LB)>();
+    if (S > 4 && after >= 3u) tile_barrier<3 * (LA + LB)>();
+    else if (S > 3 && after >= 2u) tile_barrier<2 * (LA + LB)>();
     else if (S > 2 && after >= 1u) tile_barrier<LA + LB>();
     else tile_barrier<0>();
     if (kt + (uint32_t)S - 1u == whole && whole < nk) fetch_part(whole * TK, As[nxt], Bs[nxt]);
@@ -527,7 +529,7 @@ size_t linear_scratch_bytes() { return (size_t)LIN_JOBS * 64u * 64u * sizeof(flo
 size_t linear_ctr_words() { return (size_t)LIN_JOBS * CTR_STRIDE; }
 
 // Which kernel a product takes; fills in the split's parts.
-enum LinKernel { LIN_ROWS, LIN_SPLIT, LIN_64, LIN_128, LIN_128_256, LIN_256 };
+enum LinKernel { LIN_ROWS, LIN_SPLIT, LIN_SPLIT_LONG, LIN_64, LIN_64_LONG, LIN_128, LIN_128_256, LIN_256 };
 static LinKernel linear_choice(LinArgs& A) {
   auto tiles = [&](uint32_t bo, uint32_t br) { return (uint64_t)((A.N + bo - 1u) / bo) * ((A.R + br - 1u) / br); };
   const uint32_t steps = (A.K + 63u) / 64u;
@@ -537,6 +539,12 @@ static LinKernel linear_choice(LinArgs& A) {
   // 4 x 4096 x 14336 26.1 / 30.4; but 16 x 8192 x 1024 16.3 / 11.4, 16 x 4096
   // x 14336 36.3 / 31.1, 4 x 1024 x 151936 72 / 58.
   if ((A.R <= 16u && A.N <= 4096u && A.K <= 4096u) || (A.R <= 4u && A.N <= 16384u)) return LIN_ROWS;
+  // One workgroup on a CU and a long sum: four tiles of loads ahead, not two,
+  // for 0.4 us more to begin with.  us, two / four: 256 x 4096 x 4096 19.0 /
+  // 16.4, 256 x 14336 x 4096 83.5 / 68.2, 256 x 1280 x 4096 9.7 / 9.2, 16 x
+  // 14336 x 4096 (in parts) 30.3 / 25.3; but 256 x 1024 x 1024 6.7 / 7.1, and
+  // with two on a CU 512 x 4096 x 4096 26.2 / 26.7, 100 x 11272 x 1025 23.3 / 24.3.
+  constexpr uint32_t LONG = 20;   // steps of 64 k
   // Few tiles of 64 and a long sum: at least 10 steps of 64 k to a part, up to
   // 8 parts.  us, whole / split: 64 x 8192 x 1024 31.4 / 12.4, 256 x 4096 x
   // 1024 18.5 / 11.3, 2197 x 7797 x 31 35.1 / 17.4; but 256 x 1024 x 1024 6.9
@@ -548,7 +556,7 @@ static LinKernel linear_choice(LinArgs& A) {
   if (parts >= 2u) {
     A.span = (steps + parts - 1u) / parts * 64u;
     A.P = (A.K + A.span - 1u) / A.span;
-    return LIN_SPLIT;
+    return A.span >= LONG * 64u && t64 * A.P <= 256u ? LIN_SPLIT_LONG : LIN_SPLIT;
   }
   // Otherwise the tile with the least time: rounds of workgroups over 256 CUs
   // (three of 64 x 64 share one) times what a step of 64 k takes in each, a
@@ -566,7 +574,7 @@ static LinKernel linear_choice(LinArgs& A) {
   const double at128_256 = rounds(tiles(128, 256), 256) * (0.85 * steps + 4.2 + act * 0.5);
   const double at256 = rounds(tiles(256, 256), 256) * (1.46 * steps + 9.0 + act);
   const double least = fmin(fmin(at64, at128), fmin(at128_256, at256));
-  return least == at256 ? LIN_256 : least == at128_256 ? LIN_128_256 : least == at128 ? LIN_128 : LIN_64;
+  return least == at256 ? LIN_256 : least == at128_256 ? LIN_128_256 : least == at128 ? LIN_128 : t64 <= 256u && steps >= LONG ? LIN_64_LONG : LIN_64;
 }
 
 }  // namespace mxs
@@ -601,6 +609,8 @@ extern "C" int mxs_linear_bf16(mxs_ctx* ctx, const mxs_linear* linear) {
   switch (linear_choice(A)) {
     case LIN_ROWS: hipLaunchKernelGGL(linear_rows_kernel, dim3((A.N + 15u) / 16u), dim3(SW * 64), 0, ctx->stream, A); break;
     case LIN_SPLIT: tile_go<64, 64, 2, 2, 3, true>(ctx->stream, A); break;
+    case LIN_SPLIT_LONG: tile_go<64, 64, 2, 2, 5, true>(ctx->stream, A); break;
+    case LIN_64_LONG: tile_go<64, 64, 2, 2, 5, false>(ctx->stream, A); break;
     case LIN_64: tile_go<64, 64, 2, 2, 3, false>(ctx->stream, A); break;
     case LIN_128: tile_go<128, 128, 2, 4, 3, false>(ctx->stream, A); break;
     case LIN_128_256: tile_go<128, 256, 2, 4, 3, false>(ctx->stream, A); break;

@@ -232,7 +232,8 @@ def test_no_rows_and_refusals(torch_mod, sampler):
 # and those summed in parts, each with a last tile that rows, features and k
 # leave unfilled.
 LARGER = [(2999, 31, 1025), (2900, 328, 1100), (257, 72, 12001), (300, 1000, 12003), (1031, 392, 7799),
-          (2999, 200, 4099), (4100, 1032, 2056), (700, 2056, 130), (33, 8200, 1023), (65, 1350, 130)]
+          (2999, 200, 4099), (4100, 1032, 2056), (700, 2056, 130), (33, 8200, 1023), (65, 1350, 130), (130, 1300, 2050), (40, 14344, 200),
+          (20, 11272, 1025)]
 
 
 @pytest.mark.parametrize("R,K,N", LARGER)
