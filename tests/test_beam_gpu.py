@@ -553,3 +553,37 @@ def test_a_move_past_32_bits(torch_mod, sampler):
     assert (t[:, at] - torch.arange(6, dtype=torch.uint8, device="cuda")).cpu()[:, 0].tolist() == [60, 60, 10, 20, 50, 40]
     assert all(len(set(r)) == 1 for r in (t[:, at] - torch.arange(6, dtype=torch.uint8, device="cuda")).cpu().tolist())
     assert [int(t[r].count_nonzero()) for r in range(rows)] == [6] * rows
+
+
+@pytest.mark.parametrize("n", [1, 2, 5, 10, 31, 64, 100, 128])
+@pytest.mark.parametrize("blocks", [(2,), (0, 3), (1, 2, 3), (0, 1, 2, 3)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_legal_tokens_in_some_blocks_only(torch_mod, sampler, n, blocks, dtype):
+    """Legal tokens in some of the 256-token blocks of every 1024, whole,
+    sparse or in runs, so that only some waves hold candidates; the vocabulary
+    ends inside a block."""
+    G, W, V = 3, 2, 3 * 4096 + 300
+    rng = np.random.default_rng(n + 7 * len(blocks))
+    x, s = logits(rng, G * W, V), scores(rng, G, W)
+    at = np.arange(V)
+    mask = np.broadcast_to(np.isin(at // 256 % 4, blocks), (G * W, V)).copy()
+    mask[1] &= rng.random(V) < 0.02       # sparse
+    mask[2] &= at // 40 % 7 == 0          # runs
+    mask[3] &= at % 1024 < 300            # the first two blocks at most
+    mask[5] &= at >= 3 * 4096             # the last tile, which the row's end cuts
+    check(torch_mod, sampler, x, s, n, dtype=dtype, name=f"blocks {blocks}", mask=mask, legal_norm=n % 2 == 0)
+
+
+@pytest.mark.parametrize("W,n", [(1, 64), (1, 100), (2, 32), (6, 7), (20, 24), (64, 128)])
+@pytest.mark.parametrize("centre", [-1.0, 0.0, 0.5, 2.0, 4.0])
+def test_ranks_on_both_sides_of_a_power_of_two(torch_mod, sampler, W, n, centre):
+    """Groups whose listed candidates' ranks straddle 0 and the powers of two
+    (cumulative scores may have any sign), many of them close together."""
+    G, V = 2, 20000
+    rng = np.random.default_rng(W + n)
+    x = (0.3 * rng.standard_normal((G * W, V))).astype(np.float32)
+    ids = rng.integers(0, V, (G * W, 400))
+    np.put_along_axis(x, ids, (9.0 + 0.4 * rng.standard_normal(ids.shape)).astype(np.float32), 1)
+    # candidates near -ln(400): their scores near `centre`
+    s = centre + np.log(400.0) + np.cumsum(rng.uniform(0.0, 0.2, (G, W)), 1)
+    check(torch_mod, sampler, x, s, n, name=f"centre {centre}")
