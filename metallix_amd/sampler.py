@@ -291,6 +291,23 @@ def beam_struct(torch, device, logits, score, n: int, *, ended=None, end_token: 
     return b
 
 
+def beam_out_struct(torch, device, out, groups: int, n: int) -> MxsBeamOut:
+    """The mxs_beam_out of a call's outputs, checked against `device` and the
+    sizes (ValueError)."""
+    for name, dts in (("token", (torch.int32,)), ("beam", (torch.int32,)), ("score", (torch.float64,)),
+                      ("ended", (torch.bool, torch.uint8))):
+        t = getattr(out, name)
+        if t is not None or name != "ended":
+            _need(t, f"out.{name}", device, dts, (groups, n))
+            _dense(t, f"out.{name}")
+    _need(out.status, "out.status", device, (torch.int32,), (groups,))
+    _dense(out.status, "out.status")
+    o = MxsBeamOut()
+    o.token, o.beam, o.score = out.token.data_ptr(), out.beam.data_ptr(), out.score.data_ptr()
+    o.ended, o.status = _ptr(out.ended), out.status.data_ptr()
+    return o
+
+
 def state_struct(t, rows: int, length_dim: Optional[int] = None) -> MxsState:
     """The mxs_state of a tensor whose dimension 0 is the rows: the pieces of
     a row from `length_dim` on (or the longest run of dimensions that lie
@@ -346,6 +363,8 @@ def reorder_struct(torch, device, states, parent, status, *, beams: Optional[int
     W = parent.shape[1] if beams is None else int(beams)
     if not 0 < W <= parent.shape[1] or (parent.shape[1] > 1 and parent.stride(1) != 1):
         raise ValueError("parent rows must hold `beams` consecutive entries")
+    _need(status, "status", device, (torch.int32,), (groups,))
+    _dense(status, "status")
     if lengths is not None:
         _need(lengths, "lengths", device, (torch.int32,), (groups,))
         _dense(lengths, "lengths")
@@ -856,17 +875,7 @@ class Sampler:
                 e = lambda dt: torch.empty((groups, n), dtype=dt, device=dev)
                 out = BeamResult(token=e(torch.int32), beam=e(torch.int32), score=e(torch.float64),
                                  ended=e(torch.bool), status=torch.empty(groups, dtype=torch.int32, device=dev))
-        else:
-            for name, dts in (("token", (torch.int32,)), ("beam", (torch.int32,)), ("score", (torch.float64,)),
-                              ("ended", (torch.bool, torch.uint8))):
-                t = getattr(out, name)
-                if t is not None or name != "ended":
-                    _need(t, f"out.{name}", dev, dts, (groups, n))
-                    _dense(t, f"out.{name}")
-            _need(out.status, "out.status", dev, (torch.int32,), (groups,))
-        o = MxsBeamOut()
-        o.token, o.beam, o.score = out.token.data_ptr(), out.beam.data_ptr(), out.score.data_ptr()
-        o.ended, o.status = _ptr(out.ended), out.status.data_ptr()
+        o = beam_out_struct(torch, dev, out, groups, n)
         fn, ctx, bp, op = self.lib.mxs_beam_select, self.ctx, ctypes.byref(b), ctypes.byref(o)
 
         def launch(t):
@@ -899,8 +908,6 @@ class Sampler:
         if status is None:
             with torch.cuda.stream(self.stream):
                 status = torch.empty(parent.shape[0], dtype=torch.int32, device=dev)
-        else:
-            _need(status, "status", dev, (torch.int32,), (parent.shape[0],))
         r = reorder_struct(torch, dev, states, parent, status, **kw)
         fn, ctx, rp = self.lib.mxs_beam_reorder, self.ctx, ctypes.byref(r)
 
