@@ -67,14 +67,16 @@ class BeamSearch:
                                       length_dim=[*dims, None, None], status=self.moved)
             if self.end_token is not None:
                 rule = dict(rule, ended=self.ended, end_token=self.end_token)
+                going = ~self.ended.view(-1, 1)   # (the selection writes over `ended`)
             if self.length_penalty:
                 n = torch.where(self.ended, self.length.view(self.groups, self.beams), self.steps + 1)
                 rule = dict(rule, scale=((5.0 + n.double()) / 6.0) ** -self.length_penalty)
+            s.beam_select(logits, self.score, self.beams, out=self.picked, **rule)
+            # (the step is accepted: the parents' lengths, which then move with their rows)
             if self.end_token is not None:
-                self.length.masked_fill_(~self.ended.view(-1, 1), self.steps + 1)
+                self.length.masked_fill_(going, self.steps + 1)
             else:
                 self.length.fill_(self.steps + 1)
-            s.beam_select(logits, self.score, self.beams, out=self.picked, **rule)
             move()
             self.tokens[:, self.steps] = self.picked.token.view(-1)
         self.steps += 1
