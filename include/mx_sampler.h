@@ -372,6 +372,10 @@ typedef struct {
   int32_t* status;                /* device: groups; 0 or MXS_ROW_INVALID_PARENT */
 } mxs_reorder;
 int mxs_beam_reorder(mxs_ctx* ctx, const mxs_reorder* reorder);
+/* Whether mxs_beam_reorder takes these arguments (MXS_OK, or MXS_EINVAL with
+ * the reason in mxs_last_error); queues nothing.  For a caller whose selection
+ * writes in place and may not be left without the move that follows it. */
+int mxs_beam_reorder_check(mxs_ctx* ctx, const mxs_reorder* reorder);
 /* A bf16 matrix product with its epilogue:
  *   out[r][o] = act(sum_k x[r][k] weight[o][k] + bias[o]) + residual[r][o]
  * x rows x in_features and weight out_features x in_features row-major bf16

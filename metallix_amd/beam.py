@@ -61,7 +61,7 @@ class BeamSearch:
             raise ValueError(f"the search holds {self.max_new} tokens")
         s, torch = self.sampler, self.sampler.torch
         with torch.cuda.stream(s.stream):
-            # (the states are checked before anything is queued)
+            # (the states and the move are checked before anything is queued)
             dims = list(length_dim) if isinstance(length_dim, (list, tuple)) else [length_dim] * len(states)
             move = s.reorder_launcher([*states, self.tokens, self.length], self.picked.beam, lengths=lengths,
                                       length_dim=[*dims, None, None], status=self.moved)

@@ -1016,6 +1016,12 @@ extern "C" int mxs_beam_select(mxs_ctx* ctx, const mxs_beam* beam, const mxs_bea
   return MXS_OK;
 }
 
+extern "C" int mxs_beam_reorder_check(mxs_ctx* ctx, const mxs_reorder* reorder) {
+  if (!ctx) return MXS_EINVAL;
+  if (const char* m = mxs::reorder_check(reorder)) return fail(ctx, MXS_EINVAL, m);
+  return MXS_OK;
+}
+
 extern "C" int mxs_beam_reorder(mxs_ctx* ctx, const mxs_reorder* reorder) {
   using namespace mxs;
   if (!ctx) return MXS_EINVAL;

@@ -142,6 +142,7 @@ PROTOTYPES = {
     "mxs_finish_tiles": (ctypes.c_int, [_vp, ctypes.POINTER(MxsBatch), _vp, ctypes.POINTER(MxsOut)]),
     "mxs_beam_select": (ctypes.c_int, [_vp, ctypes.POINTER(MxsBeam), ctypes.POINTER(MxsBeamOut)]),
     "mxs_beam_reorder": (ctypes.c_int, [_vp, ctypes.POINTER(MxsReorder)]),
+    "mxs_beam_reorder_check": (ctypes.c_int, [_vp, ctypes.POINTER(MxsReorder)]),
     "mxs_linear_bf16": (ctypes.c_int, [_vp, ctypes.POINTER(MxsLinear)]),
     "mxs_debug_set_timing": (ctypes.c_int, [_vp, _vp]),
     "mxs_debug_floor": (ctypes.c_int, [_vp, _vp, ctypes.c_int32, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32,
@@ -903,13 +904,15 @@ class Sampler:
     def reorder_launcher(self, states, parent, *, status=None, **kw):
         """Pre-built beam_reorder for repeated moves of the same states:
         returns f() that re-issues mxs_beam_reorder with what parent and
-        lengths then hold (f.status holds the status)."""
+        lengths then hold (f.status holds the status).  What the call would
+        refuse is refused here."""
         torch, dev = self.torch, self._device()
         if status is None:
             with torch.cuda.stream(self.stream):
                 status = torch.empty(parent.shape[0], dtype=torch.int32, device=dev)
         r = reorder_struct(torch, dev, states, parent, status, **kw)
         fn, ctx, rp = self.lib.mxs_beam_reorder, self.ctx, ctypes.byref(r)
+        self._check(self.lib.mxs_beam_reorder_check(ctx, rp), "mxs_beam_reorder")
 
         def launch():
             rc = fn(ctx, rp)

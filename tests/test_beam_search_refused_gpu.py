@@ -71,3 +71,35 @@ def test_logits_that_the_selection_refuses(run):
     run.refuses(ValueError, "logits", run.logits()[:-1])
     run.refuses(ValueError, "mask", run.logits(), mask=run.state)
     run.refuses(ValueError, "vocab", run.logits(), vocab=V + 1)
+
+
+def test_states_that_the_move_refuses(run):
+    """Layouts that only the move's own checks look at: they are refused before
+    the selection has written over the scores."""
+    from metallix_amd import SamplerError
+
+    torch = run.torch
+    rows = G * W
+    z = lambda *n: torch.zeros(n, device="cuda")
+    run.refuses(SamplerError, "overlap", run.logits(), [run.state, z(1, 4).expand(rows, 4)])
+    run.refuses(SamplerError, "overlap", run.logits(), [z(rows + 3).unfold(0, 4, 1), run.state])
+    run.refuses(SamplerError, "overlap", run.logits(), [z(rows, 1, 4).expand(rows, 3, 4)], length_dim=2)
+    run.refuses(SamplerError, "overlap", run.logits(), [run.state] * 1 + [z(rows, 9).unfold(1, 4, 1)])
+    run.refuses(ValueError, "rows", run.logits(), [run.state[:-1]])
+    run.refuses(ValueError, "lengths", run.logits(), lengths=z(G))
+
+
+def test_a_move_is_refused_where_it_is_described(torch_mod):
+    """The launcher refuses what its calls would, before the first of them."""
+    from metallix_amd import Sampler, SamplerError
+
+    torch = torch_mod
+    s = Sampler(max_rows=G * W, max_vocab=V)
+    parent = torch.zeros((G, W), dtype=torch.int32, device="cuda")
+    with pytest.raises(SamplerError, match="overlap"):
+        s.reorder_launcher([torch.zeros((1, 4), device="cuda").expand(G * W, 4)], parent)
+    with pytest.raises(SamplerError, match="one state"):
+        s.reorder_launcher([], parent)
+    with pytest.raises(SamplerError, match="65535"):
+        s.reorder_launcher([torch.zeros((1 << 16, 1), device="cuda")], torch.zeros((1 << 16, 1), dtype=torch.int32, device="cuda"))
+    s.close()
