@@ -10,7 +10,7 @@ histories, the lengths) on the sampler's stream; nothing is read back until
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 from typing import List, Optional
 
 from .sampler import BeamResult
@@ -56,7 +56,8 @@ class BeamSearch:
         Sampler.beam_select), moves `states` (tensors of groups * beams rows,
         the first lengths[g] positions of their length_dim) and the search's
         own rows to them.  Returns the rows' next tokens, int32[groups *
-        beams] on the device (-1: no sequence; an ended one's end token)."""
+        beams] on the device (-1: no sequence; an ended one's end token), a
+        tensor of this step's own that later steps leave alone."""
         if self.steps >= self.max_new:
             raise ValueError(f"the search holds {self.max_new} tokens")
         s, torch = self.sampler, self.sampler.torch
@@ -71,13 +72,15 @@ class BeamSearch:
             if self.length_penalty:
                 n = torch.where(self.ended, self.length.view(self.groups, self.beams), self.steps + 1)
                 rule = dict(rule, scale=((5.0 + n.double()) / 6.0) ** -self.length_penalty)
-            s.beam_select(logits, self.score, self.beams, out=self.picked, **rule)
+            picked = replace(self.picked, token=torch.empty_like(self.picked.token))
+            s.beam_select(logits, self.score, self.beams, out=picked, **rule)
             # (the step is accepted: the parents' lengths, which then move with their rows)
             if self.end_token is not None:
                 self.length.masked_fill_(going, self.steps + 1)
             else:
                 self.length.fill_(self.steps + 1)
             move()
+            self.picked = picked
             self.tokens[:, self.steps] = self.picked.token.view(-1)
         self.steps += 1
         return self.picked.token.view(-1)

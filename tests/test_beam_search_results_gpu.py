@@ -1,0 +1,46 @@
+"""What a search gives back: its steps' tokens and its groups' outcomes."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+G, W, V, T, END = 3, 4, 60, 6, 5
+
+
+@pytest.fixture(scope="module")
+def torch_mod():
+    import torch
+
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    return torch
+
+
+@pytest.fixture
+def sampler(torch_mod):
+    from metallix_amd import Sampler
+
+    s = Sampler(max_rows=G * W, max_vocab=V)
+    yield s
+    s.close()
+
+
+def logits(torch, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return 3.0 * torch.randn((G * W, V), generator=g, device="cuda")
+
+
+def test_a_steps_tokens_stay_what_they_were(torch_mod, sampler):
+    """A caller may keep the tensors that the steps return."""
+    from metallix_amd import BeamSearch
+
+    torch = torch_mod
+    search = BeamSearch(sampler, G, W, T)
+    kept, then = [], []
+    for t in range(T):
+        kept.append(search.step(logits(torch, t)))
+        torch.cuda.synchronize()
+        then.append(kept[-1].cpu())
+        assert torch.equal(search.picked.token.view(-1).cpu(), then[-1])
+    assert len({tuple(t.tolist()) for t in then}) == T   # the steps' tokens differ
+    for k, w in zip(kept, then):
+        assert torch.equal(k.cpu(), w)
