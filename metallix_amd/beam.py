@@ -29,7 +29,12 @@ class BeamSearch:
     """groups x beams sequences over one Sampler.  Row g * beams + b of every
     tensor is beam b of group g; a group starts with one live beam, beam 0.
     Ended beams stay in the race with their score.  length_penalty a orders
-    the candidates by score * ((5 + length) / 6) ** -a."""
+    the candidates by score * ((5 + length) / 6) ** -a.
+
+    `status`, int32[groups] on the device, is 0 or what first stopped a group
+    (ROW_STATUS): a NaN or +inf among its logits (-6), no candidate (-3),
+    scores or scales that are no numbers (-14).  Such a group has no
+    hypotheses from then on; the others go on."""
 
     def __init__(self, sampler, groups: int, beams: int, max_new: int, *, end_token: Optional[int] = None,
                  length_penalty: float = 0.0):
@@ -48,7 +53,8 @@ class BeamSearch:
             e = lambda *s: torch.empty(s, dtype=torch.int32, device=dev)
             self.picked = BeamResult(token=e(groups, beams), beam=e(groups, beams), score=self.score, ended=self.ended,
                                      status=e(groups))
-            self.moved = e(groups)
+            self.moved = e(groups)   # (always 0: the parents are the selection's)
+            self.status = torch.zeros(groups, dtype=torch.int32, device=dev)
 
     def step(self, logits, states=(), *, lengths=None, length_dim=None, **rule):
         """Queues one step over `logits` [groups * beams, vocab]: picks each
@@ -81,6 +87,7 @@ class BeamSearch:
                 self.length.fill_(self.steps + 1)
             move()
             self.picked = picked
+            self.status = torch.where(self.status == 0, picked.status, self.status)
             self.tokens[:, self.steps] = self.picked.token.view(-1)
         self.steps += 1
         return self.picked.token.view(-1)
@@ -91,7 +98,8 @@ class BeamSearch:
         return bool((self.ended | (self.score == float("-inf")) | self.score.isnan()).all())
 
     def result(self) -> List[List[Hypothesis]]:
-        """Each group's hypotheses, best first (reads back)."""
+        """Each group's hypotheses, best first (reads back); none for a group
+        whose `status` is not 0."""
         self.sampler.sync()
         tokens, length = self.tokens.cpu().tolist(), self.length.cpu().view(-1).tolist()
         score, ended = self.score.cpu().tolist(), self.ended.cpu().tolist()

@@ -44,3 +44,31 @@ def test_a_steps_tokens_stay_what_they_were(torch_mod, sampler):
     assert len({tuple(t.tolist()) for t in then}) == T   # the steps' tokens differ
     for k, w in zip(kept, then):
         assert torch.equal(k.cpu(), w)
+
+
+@pytest.mark.parametrize("at", [0, 2, T - 1])
+def test_what_stopped_a_group_is_kept(torch_mod, sampler, at):
+    """A group whose logits hold a NaN at one step, and one left without a
+    legal token, say so at the end; the third gives what it gives alone."""
+    from metallix_amd import BeamSearch
+
+    torch = torch_mod
+    alone = BeamSearch(sampler, G, W, T, end_token=END)
+    search = BeamSearch(sampler, G, W, T, end_token=END)
+    mask = torch.full((G * W, (V + 31) // 32), -1, dtype=torch.int32, device="cuda")
+    none = mask.clone()
+    none[2 * W :] = 0
+    for t in range(T):
+        lg = logits(torch, 50 + t)
+        lg[:, END] = -30.0                     # (no beam ends)
+        alone.step(lg, mask=mask)
+        if t == at:
+            lg = lg.clone()
+            lg[0, 7] = float("nan")
+        search.step(lg, mask=none if t == at else mask)
+        torch.cuda.synchronize()
+        assert search.status.cpu().tolist() == ([0, 0, 0] if t < at else [-6, 0, -3]), t
+    assert alone.status.cpu().tolist() == [0, 0, 0]
+    want, got = alone.result(), search.result()
+    assert got == [[], want[1], []] and len(want[1]) == W
+    assert alone.done() is False
