@@ -59,13 +59,17 @@ class BeamSearch:
     def step(self, logits, states=(), *, lengths=None, length_dim=None, **rule):
         """Queues one step over `logits` [groups * beams, vocab]: picks each
         group's best continuations (`rule`: mask, legal_norm, ... of
-        Sampler.beam_select), moves `states` (tensors of groups * beams rows,
+        Sampler.beam_select, but not the end token, the ended beams or, with
+        a length penalty, the scale, which are the search's), moves `states` (tensors of groups * beams rows,
         the first lengths[g] positions of their length_dim) and the search's
         own rows to them.  Returns the rows' next tokens, int32[groups *
         beams] on the device (-1: no sequence; an ended one's end token), a
         tensor of this step's own that later steps leave alone."""
         if self.steps >= self.max_new:
             raise ValueError(f"the search holds {self.max_new} tokens")
+        own = {"ended", "end_token"} | ({"scale"} if self.length_penalty else set())
+        if own & rule.keys():
+            raise ValueError(f"the search itself gives the selection its {' and '.join(sorted(own & rule.keys()))}")
         s, torch = self.sampler, self.sampler.torch
         with torch.cuda.stream(s.stream):
             # (the states and the move are checked before anything is queued)

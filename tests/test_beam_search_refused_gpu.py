@@ -103,3 +103,13 @@ def test_a_move_is_refused_where_it_is_described(torch_mod):
     with pytest.raises(SamplerError, match="65535"):
         s.reorder_launcher([torch.zeros((1 << 16, 1), device="cuda")], torch.zeros((1 << 16, 1), dtype=torch.int32, device="cuda"))
     s.close()
+
+
+def test_rules_that_are_the_searchs_own(run):
+    """An end token, ended beams or a scale given to one step would disagree
+    with the search's flags and lengths."""
+    torch = run.torch
+    run.refuses(ValueError, "end_token", run.logits(), end_token=1)
+    run.refuses(ValueError, "ended", run.logits(), ended=torch.zeros((G, W), dtype=torch.bool, device="cuda"))
+    if run.search.length_penalty:
+        run.refuses(ValueError, "scale", run.logits(), scale=torch.ones((G, W), dtype=torch.float64, device="cuda"))
