@@ -927,7 +927,9 @@ class Sampler:
         x bf16[rows, in_features], weight bf16[out_features, in_features],
         row strides multiples of 8; bias f32 or bf16; activation none, relu,
         silu, gelu or gelu_tanh; residual of out's type (bf16 by default; it
-        may be out itself).  Returns out."""
+        may be out itself).  Returns out; where none is given, a tensor whose
+        row stride is out_features rounded up to a multiple of 8, as
+        beam_select and another linear take it."""
         return self.linear_launcher(x, weight, bias, activation=activation, residual=residual, out=out,
                                     out_dtype=out_dtype).out
 
@@ -938,7 +940,8 @@ class Sampler:
         torch, dev = self.torch, self._device()
         if out is None:
             with torch.cuda.stream(self.stream):
-                out = torch.empty((x.shape[0], weight.shape[0]), dtype=out_dtype or torch.bfloat16, device=dev)
+                N = weight.shape[0]   # (rows start where beam_select and another product take them)
+                out = torch.empty((x.shape[0], -(-N // 8) * 8), dtype=out_dtype or torch.bfloat16, device=dev)[:, :N]
         elif out_dtype is not None and out.dtype != out_dtype:
             raise ValueError(f"out must be {out_dtype}, not {out.dtype}")
         a = linear_struct(torch, dev, x, weight, bias, residual, out, activation)
