@@ -313,7 +313,8 @@ def state_struct(t, rows: int, length_dim: Optional[int] = None) -> MxsState:
     """The mxs_state of a tensor whose dimension 0 is the rows: the pieces of
     a row from `length_dim` on (or the longest run of dimensions that lie
     consecutively in memory), one per index of the dimensions before, which
-    must be evenly spaced.  ValueError for any other layout."""
+    must be evenly spaced; the dimensions are taken in the order of their
+    strides.  ValueError for any other layout."""
     if t.dim() < 1 or t.shape[0] != rows:
         raise ValueError(f"a state must have {rows} rows, not {list(t.shape)}")
     size, stride = list(t.shape), list(t.stride())
@@ -322,6 +323,18 @@ def state_struct(t, rows: int, length_dim: Optional[int] = None) -> MxsState:
     es, nd = t.element_size(), t.dim()
     if length_dim is not None and not 1 <= length_dim < nd:
         raise ValueError(f"length_dim must be in 1..{nd - 1}")
+
+    # Largest stride first, as [rows, positions, heads, dim] seen as [rows,
+    # heads, positions, dim] lies in memory; a dimension of one index goes with
+    # the one after it.  (Stride 0, rows on top of one another, is refused later.)
+    by = stride + [1]
+    for d in range(nd - 1, 0, -1):
+        if size[d] == 1:
+            by[d] = by[d + 1]
+    if all(by[1:nd]):
+        order = [0, *sorted(range(1, nd), key=lambda d: -by[d])]
+        size, stride = [size[d] for d in order], [stride[d] for d in order]
+        length_dim = None if length_dim is None else order.index(length_dim)
 
     def run(d):   # elements of dimensions d.. when they are consecutive, else 0
         n = 1
