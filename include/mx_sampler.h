@@ -352,7 +352,9 @@ int mxs_beam_select(mxs_ctx* ctx, const mxs_beam* beam, const mxs_beam_out* out)
  * first lengths[g] * position_bytes bytes of each segment move (states with
  * position_bytes 0 move whole; it is below 4 GiB).  Each surviving row is read
  * once and each changed row written once, whatever the permutation.  Rows and segments of
- * a state must not overlap, nor two states (the latter is not checked). */
+ * a state must not overlap, nor may status meet parent or lengths; nor two
+ * states, nor a state and parent, lengths or status (these are not checked:
+ * states may lie between one another). */
 typedef struct {
   void* data;
   uint64_t row_stride;

@@ -69,6 +69,10 @@ inline const char* reorder_check(const mxs_reorder* r) {
   if (r->beams == 0 || r->beams > MXS_BEAM_MAX) return "beams must be in 1..64";
   if (r->groups > 65535u) return "groups must be at most 65535";
   if (r->parent_stride < r->beams) return "parent_stride must be >= beams";
+  // A group's status is written while others' parents and lengths are read.
+  const uint64_t nst = r->groups * 4ull, npar = ((r->groups - 1ull) * r->parent_stride + r->beams) * 4u;
+  if (ranges_meet(r->status, nst, r->parent, npar) || (r->lengths && ranges_meet(r->status, nst, r->lengths, nst)))
+    return "status overlaps parent or lengths";
   const uint64_t rows = (uint64_t)r->groups * r->beams;
   for (uint32_t i = 0; i < r->count; ++i) {
     const mxs_state& s = r->states[i];

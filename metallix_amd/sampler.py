@@ -909,7 +909,8 @@ class Sampler:
         parent: int32[groups, >= beams] (its first `beams` columns; default
         all).  lengths: int32[groups], the positions in use along each
         state's length_dim (one dimension, or one per state, None for states
-        that move whole).  Returns the status, int32[groups]."""
+        that move whole).  The states must not share memory with one another,
+        parent, lengths or the status.  Returns the status, int32[groups]."""
         f = self.reorder_launcher(states, parent, status=status, **kw)
         f()
         return f.status
