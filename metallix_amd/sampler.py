@@ -11,6 +11,7 @@ engine::sampling::SamplingError (crates/core/engine/src/sampling.rs:19-43).
 from __future__ import annotations
 
 import ctypes
+import math
 from dataclasses import dataclass
 from pathlib import Path
 from typing import Optional, Sequence
@@ -248,6 +249,14 @@ def _dense(t, name: str) -> None:
         raise ValueError(f"{name} must be contiguous")
 
 
+def _u32(v, name: str) -> int:
+    """v as the ABI's 32-bit count; ctypes would keep its low bits only."""
+    v = int(v)
+    if not 0 <= v < 1 << 32:
+        raise ValueError(f"{name} must be in 0..2^32 - 1, not {v}")
+    return v
+
+
 def _float_code(torch, dtype) -> int:
     return MXS_BF16 if dtype == torch.bfloat16 else MXS_F32
 
@@ -272,7 +281,7 @@ def beam_struct(torch, device, logits, score, n: int, *, ended=None, end_token: 
         _dense(scale, "scale")
     b = MxsBeam()
     b.logits, b.dtype = logits.data_ptr(), _float_code(torch, logits.dtype)
-    b.groups, b.beams, b.vocab = groups, beams, V
+    b.groups, b.beams, b.vocab = _u32(groups, "groups"), _u32(beams, "beams"), _u32(V, "vocab")
     # (a single row's stride says nothing: any multiple of 4 that holds it)
     b.row_stride = logits.stride(0) if groups * beams > 1 else (V + 3) // 4 * 4
     b.score, b.ended, b.scale = score.data_ptr(), _ptr(ended), _ptr(scale)
@@ -285,10 +294,12 @@ def beam_struct(torch, device, logits, score, n: int, *, ended=None, end_token: 
             raise ValueError("mask holds fewer rows than the batch")
         b.mask_words = mask.data_ptr()
         b.mask_stride = mask.stride(0) if groups * beams > 1 else (V + 31) // 32
-        b.tokenizer_vocab = V if tokenizer_vocab is None else int(tokenizer_vocab)
+        b.tokenizer_vocab = V if tokenizer_vocab is None else _u32(tokenizer_vocab, "tokenizer_vocab")
     b.legal_norm = 1 if legal_norm else 0
-    b.n = n
+    b.n = _u32(n, "n")
     b.end_token = -1 if end_token is None else int(end_token)
+    if end_token is not None and b.end_token != int(end_token):
+        raise ValueError(f"end_token must be a token of the vocabulary, not {end_token}")
     return b
 
 
@@ -359,9 +370,7 @@ def state_struct(t, rows: int, length_dim: Optional[int] = None) -> MxsState:
     m = MxsState()
     m.data = t.data_ptr()
     m.segment_bytes = run(first) * es
-    m.segments = 1
-    for n, _ in outer:
-        m.segments *= n
+    m.segments = _u32(math.prod(n for n, _ in outer), "a state's pieces")
     m.segment_stride = outer[-1][1] * es if outer else m.segment_bytes
     m.row_stride = stride[0] * es if rows > 1 else m.segments * m.segment_stride
     m.position_bytes = 0 if length_dim is None else run(first) * es // size[first]
@@ -399,8 +408,9 @@ def reorder_struct(torch, device, states, parent, status, *, beams: Optional[int
         arr[i] = m
     r = MxsReorder()
     r.states, r.count = ctypes.cast(arr, ctypes.POINTER(MxsState)), len(states)
-    r.groups, r.beams = groups, W
-    r.parent, r.parent_stride = parent.data_ptr(), parent.stride(0) if groups > 1 else parent.shape[1]
+    r.groups, r.beams = _u32(groups, "groups"), W
+    r.parent = parent.data_ptr()
+    r.parent_stride = _u32(parent.stride(0) if groups > 1 else parent.shape[1], "parent's row stride")
     r.lengths, r.status = _ptr(lengths), status.data_ptr()
     r.keep = arr
     return r
@@ -433,7 +443,8 @@ def linear_struct(torch, device, x, weight, bias, residual, out, activation) -> 
     a.bias, a.residual = _ptr(bias), _ptr(residual)
     a.residual_stride = rows_of(residual, 1) if residual is not None else 0
     a.out, a.out_stride = out.data_ptr(), rows_of(out, 1)
-    a.rows, a.in_features, a.out_features, a.act = R, K, N, act
+    a.rows, a.in_features, a.out_features = _u32(R, "rows"), _u32(K, "in_features"), _u32(N, "out_features")
+    a.act = act
     a.out_dtype = _float_code(torch, out.dtype)
     a.bias_dtype = _float_code(torch, bias.dtype) if bias is not None else MXS_F32
     return a

@@ -98,3 +98,29 @@ def test_positions_in_any_order_of_the_dimensions():
                    (torch.zeros((4, 5, 6, 7))[:, :, :4].transpose(1, 3), 1)):
         with pytest.raises(ValueError):
             S.state_struct(bad, 4, d)
+
+
+def test_numbers_that_32_bits_do_not_hold():
+    """ctypes keeps the low 32 bits: 2^32 + 4 candidates, rows or pieces would
+    be 4."""
+    big = (1 << 32) + 4
+    meta, bf = torch.device("meta"), torch.bfloat16
+    z = lambda *n, dt=torch.float32: torch.zeros(n, dtype=dt, device="meta")
+    lg, sc = torch.zeros(8, 100), torch.zeros(2, 4, dtype=torch.float64)
+    f = lambda n=4, **kw: S.beam_struct(torch, CPU, lg, sc, n, **kw)
+    mask = torch.zeros(8, 4, dtype=torch.int32)
+    assert f(mask=mask, tokenizer_vocab=(1 << 32) - 1).tokenizer_vocab == (1 << 32) - 1
+    for kw in (dict(n=big), dict(n=-1), dict(end_token=big), dict(end_token=(1 << 32) - 1), dict(mask=mask, tokenizer_vocab=big),
+               dict(mask=mask, tokenizer_vocab=-1)):
+        with pytest.raises(ValueError):
+            f(**kw)
+    with pytest.raises(ValueError, match="groups"):
+        S.beam_struct(torch, meta, z(big, 4), z(big, 1, dt=torch.float64), 1)
+    for R, K, N in ((big, 8, 8), (8, big, 8), (8, 8, big)):
+        with pytest.raises(ValueError, match="2.32"):
+            S.linear_struct(torch, meta, z(R, K, dt=bf), z(N, K, dt=bf), None, None, z(R, N, dt=bf), None)
+    with pytest.raises(ValueError, match="pieces"):
+        S.state_struct(z(2, 1 << 31, 4, 8)[:, :, :, :4], 2)
+    parent, status = z(2, big, dt=torch.int32), z(2, dt=torch.int32)
+    with pytest.raises(ValueError, match="row stride"):
+        S.reorder_struct(torch, meta, [z(8, 4)], parent, status, beams=4)
