@@ -376,7 +376,9 @@ __device__ __forceinline__ void beam_chunk(const BeamArgs& A, BeamSmem& S, uint3
     }
     // The weights, relative to a power of two near the first maximum the wave
     // meets: f64 holds e^-700..e^600 of it, so it moves only for a later
-    // maximum 600 above.
+    // maximum 600 above.  (Logits past 1000 in size: for any later maximum. A
+    // f32 near 2^33 plus 600 rounds to 1024 above, whose weight f64 does not
+    // hold.)
     if (__builtin_amdgcn_ballot_w64(tm > hi)) {
       const float wm = wave_max_f32(tm);
       wide = !(fabsf(wm) <= 1000.0f);
@@ -385,7 +387,7 @@ __device__ __forceinline__ void beam_chunk(const BeamArgs& A, BeamSmem& S, uint3
       if (ref > -INFINITY) sum *= exp_neg_p(unit - u);
       ref = wm;
       unit = u;
-      hi = wm + 600.0f;
+      hi = wide ? wm : wm + 600.0f;
       lo = wm - 700.0f;
       magic = 0x1.8p52 - n0;
     }

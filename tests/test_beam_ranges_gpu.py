@@ -1,0 +1,58 @@
+"""GPU tests of mxs_beam_select where a row's logits are large and its maximum
+comes late.  The oracle's norms are long doubles."""
+import numpy as np
+import pytest
+
+from test_beam_gpu import run
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch_mod():
+    import torch
+
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    return torch
+
+
+@pytest.fixture(scope="module")
+def sampler(torch_mod):
+    from metallix_amd import Sampler
+
+    s = Sampler(max_rows=256, max_vocab=262144)
+    yield s
+    s.close()
+
+
+@pytest.mark.parametrize("base", [2.0 ** k for k in range(10, 40)] + [-(2.0 ** k) for k in range(10, 40, 3)])
+def test_maxima_that_come_late(torch_mod, sampler, base):
+    """Each row rises by steps between its tiles, by the smallest f32 step that
+    is at least 1, 300, 600 or 1000, so that a later maximum lies just below,
+    at and above the point where the weights' unit moves; the last step's
+    tokens are the row's best."""
+    W, V = 64, 100003                       # 25 tiles in chunks of 4
+    x = np.empty((W, V), np.float32)
+    steps = [1.0, 300.0, 600.0, 1000.0]
+    for b in range(W):
+        v = np.float32(base * (1.0 + 0.001 * (b // 4)))
+        for t in range(25):
+            x[b, t * 4096 : (t + 1) * 4096] = v
+            if t % 8 != 7:
+                ulp = np.spacing(np.abs(v))
+                v = np.float32(v + max(ulp, np.float32(np.ceil(steps[b % 4] / ulp) * ulp)))
+    score = np.full((1, W), -np.inf)
+    for b in (0, 1, 2, 3, 21, 42, 63):      # one live beam at a time: its own scores
+        s = score.copy()
+        s[0, b] = -2.0
+        tok, beam, sc, _, st = run(torch_mod, sampler, x, s, 8)
+        l = x[b].astype(np.longdouble)
+        norm = l.max() + np.log(np.sum(np.exp(l - l.max())))
+        assert st.tolist() == [0], (base, b)
+        assert beam.tolist() == [[b] * 8]
+        at = np.nonzero(x[b] == x[b].max())[0][:8]
+        assert tok.tolist() == [at.tolist()]
+        want = -2.0 + (l.max() - norm)
+        # the logarithm of the sum within 2^-39, and its own and the score's roundings
+        assert np.all(np.abs(sc - float(want)) <= 2.0 ** -39 + 2.0 ** -52 * abs(float(norm)) + 2.0 ** -50), (base, b, sc, want)
