@@ -130,7 +130,8 @@ MXS_HD double exp_neg16_t(double x, const double* tab_hi, const double* tab_lo) 
 // (Cody-Waite reduction with a 32-bit high part of ln2, so n * hi is exact
 // for |n| < 2^21), degree-13 Taylor polynomial for e^r (truncation below
 // 5e-18 relative), scaled by 2^n.  Within 2 ulp of glibc's exp (checked in
-// tests).  Returns 0 below -746 and for -inf.
+// tests), which holds for x > 0 too, up to the 709 where f64 ends.  Returns 0
+// below -746 and for -inf.
 MXS_HD double exp_neg_p(double x) {
   if (!(x > -746.0)) return 0.0;
   const double kLn2Hi = 0.6931471803691238;       // ln 2, low 21 bits of the significand clear
