@@ -298,9 +298,10 @@ int mxs_finish_tiles(mxs_ctx* ctx, const mxs_batch* batch, const void* tile_stat
  * an ended beam (`ended` nonzero) is one candidate with end_token and its own
  * score, and its logits are not read.  Candidates are ordered by
  * score * scale[row] (a length penalty; NULL => by score), largest first;
- * equal ones by lower beam, larger logit, lower token.  The logarithm of the
- * sum is within 2^-39 of exact, so candidates of different beams closer than
- * that may come in either order.
+ * equal ones by lower beam, larger logit, lower token.  The logarithm N of the
+ * sum is within 2^-39 + 2^-52 |N| of exact (the second term, an f64's own
+ * rounding, counts from logits of 2^12 in size on), so candidates of different
+ * beams closer than that may come in either order.
  *
  * A score of -inf is a beam that is not there (the first step has one live
  * beam a group).  A logit of -inf is a token that cannot follow: it weighs

@@ -56,3 +56,32 @@ def test_maxima_that_come_late(torch_mod, sampler, base):
         want = -2.0 + (l.max() - norm)
         # the logarithm of the sum within 2^-39, and its own and the score's roundings
         assert np.all(np.abs(sc - float(want)) <= 2.0 ** -39 + 2.0 ** -52 * abs(float(norm)) + 2.0 ** -50), (base, b, sc, want)
+
+
+@pytest.mark.parametrize("size", [1.0, 300.0, 900.0, 2.0 ** 12, 2.0 ** 14, 1e5, 3e6, 2.0 ** 30])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_the_logarithms_stated_bound(torch_mod, sampler, size, sign, dtype):
+    """Scores of single beams against norms in long double: the logarithm N
+    within 2^-39 + 2^-52 |N|; l - N and the score add their own roundings,
+    2^-53 of their sizes each, and the long doubles 2^-60."""
+    G, W, V, n = 6, 1, 30011, 5
+    rng = np.random.default_rng(int(size) % 9973)
+    x = (sign * size + rng.standard_normal((G, V)) * 2.5).astype(np.float32)
+    x[1] = (sign * size * (1.0 + 0.5 * rng.random(V))).astype(np.float32)
+    x[2, :20000] -= np.float32(50.0)
+    if dtype == "bf16":
+        b = x.view(np.uint32)
+        x = ((b + 0x7FFF + ((b >> 16) & 1)) & 0xFFFF0000).astype(np.uint32).view(np.float32)
+    score = -rng.uniform(0.0, 3.0, (G, W))
+    tok, beam, sc, _, st = run(torch_mod, sampler, x, score, n, dtype=dtype)
+    assert st.tolist() == [0] * G
+    for g in range(G):
+        l = x[g].astype(np.longdouble)
+        norm = l.max() + np.log(np.sum(np.exp(l - l.max())))
+        at = np.lexsort((np.arange(V), -x[g]))[:n]
+        assert tok[g].tolist() == at.tolist()
+        lp = l[at] - norm
+        want = score[g, 0] + lp
+        err = 2.0 ** -39 + 2.0 ** -52 * abs(norm) + 2.0 ** -53 * (np.abs(lp) + np.abs(want)) + 2.0 ** -60 * abs(norm)
+        assert np.all(np.abs(sc[g].astype(np.longdouble) - want) <= err), (g, sc[g], want, norm)
