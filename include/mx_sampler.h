@@ -383,8 +383,9 @@ int mxs_beam_reorder_check(mxs_ctx* ctx, const mxs_reorder* reorder);
  *   out[r][o] = act(sum_k x[r][k] weight[o][k] + bias[o]) + residual[r][o]
  * x rows x in_features and weight out_features x in_features row-major bf16
  * (16-byte aligned, strides multiples of 8 below 2^22 elements; nothing past a
- * row's in_features is read), products summed in f32, the epilogue in f32 with
- * one rounding to the output type.  Any number of rows and features, up
+ * row's in_features is read), products summed in f32, the epilogue in f32
+ * (activations within 2^-20 of their value's size plus 2^-30; a NaN stays, and
+ * silu and gelu of -inf are NaN) with one rounding to the output type.  Any number of rows and features, up
  * to 2^35 results (in whole blocks of 64 x 64).  bias f32 or bf16 (bias_dtype)
  * or NULL; residual of out's type or NULL; it may be out itself (same stride),
  * otherwise out may overlap no input. */
