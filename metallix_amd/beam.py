@@ -10,7 +10,7 @@ histories, the lengths) on the sampler's stream; nothing is read back until
 """
 from __future__ import annotations
 
-from dataclasses import dataclass, replace
+from dataclasses import dataclass
 from typing import List, Optional
 
 from .sampler import BeamResult
@@ -51,18 +51,21 @@ class BeamSearch:
             self.tokens = torch.full((rows, max_new), -1, dtype=torch.int32, device=dev)
             self.length = torch.zeros((rows, 1), dtype=torch.int32, device=dev)
             e = lambda *s: torch.empty(s, dtype=torch.int32, device=dev)
+            # each step's own tokens and statuses
+            self._tokens = torch.empty((max_new, groups, beams), dtype=torch.int32, device=dev).unbind(0)
+            self._statuses = torch.zeros((max_new + 1, groups), dtype=torch.int32, device=dev)
+            self._status_rows = self._statuses.unbind(0)
             self.picked = BeamResult(token=e(groups, beams), beam=e(groups, beams), score=self.score, ended=self.ended,
                                      status=e(groups))
             self.moved = e(groups)   # (always 0: the parents are the selection's)
-            self.status = torch.zeros(groups, dtype=torch.int32, device=dev)
 
     def step(self, logits, states=(), *, lengths=None, length_dim=None, **rule):
         """Queues one step over `logits` [groups * beams, vocab]: picks each
         group's best continuations (`rule`: mask, legal_norm, ... of
         Sampler.beam_select, but not the end token, the ended beams or, with
-        a length penalty, the scale, which are the search's), moves `states` (tensors of groups * beams rows,
-        the first lengths[g] positions of their length_dim) and the search's
-        own rows to them.  Returns the rows' next tokens, int32[groups *
+        a length penalty, the scale, which are the search's), moves `states`
+        (tensors of groups * beams rows, the first lengths[g] positions of
+        their length_dim) and the search's own rows to them.  Returns the rows' next tokens, int32[groups *
         beams] on the device (-1: no sequence; an ended one's end token), a
         tensor of this step's own that later steps leave alone."""
         if self.steps >= self.max_new:
@@ -82,7 +85,8 @@ class BeamSearch:
             if self.length_penalty:
                 n = torch.where(self.ended, self.length.view(self.groups, self.beams), self.steps + 1)
                 rule = dict(rule, scale=((5.0 + n.double()) / 6.0) ** -self.length_penalty)
-            picked = replace(self.picked, token=torch.empty_like(self.picked.token))
+            p = self.picked
+            picked = BeamResult(self._tokens[self.steps], p.beam, p.score, p.ended, self._status_rows[self.steps])
             s.beam_select(logits, self.score, self.beams, out=picked, **rule)
             # (the step is accepted: the parents' lengths, which then move with their rows)
             if self.end_token is not None:
@@ -90,11 +94,17 @@ class BeamSearch:
             else:
                 self.length.fill_(self.steps + 1)
             move()
-            self.picked = picked
-            self.status = torch.where(self.status == 0, picked.status, self.status)
-            self.tokens[:, self.steps] = self.picked.token.view(-1)
+            self.picked, tokens = picked, picked.token.view(-1)
+            self.tokens[:, self.steps] = tokens
         self.steps += 1
-        return self.picked.token.view(-1)
+        return tokens
+
+    @property
+    def status(self):
+        torch = self.sampler.torch
+        with torch.cuda.stream(self.sampler.stream):
+            first = (self._statuses != 0).int().argmax(0, keepdim=True)   # (the first of equal ones)
+            return self._statuses.gather(0, first)[0]
 
     def done(self) -> bool:
         """Whether every sequence has ended or is not there (reads back)."""

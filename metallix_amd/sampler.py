@@ -335,17 +335,19 @@ def state_struct(t, rows: int, length_dim: Optional[int] = None) -> MxsState:
     if length_dim is not None and not 1 <= length_dim < nd:
         raise ValueError(f"length_dim must be in 1..{nd - 1}")
 
-    # Largest stride first, as [rows, positions, heads, dim] seen as [rows,
-    # heads, positions, dim] lies in memory; a dimension of one index goes with
-    # the one after it.  (Stride 0, rows on top of one another, is refused later.)
-    by = stride + [1]
-    for d in range(nd - 1, 0, -1):
-        if size[d] == 1:
-            by[d] = by[d + 1]
-    if all(by[1:nd]):
-        order = [0, *sorted(range(1, nd), key=lambda d: -by[d])]
-        size, stride = [size[d] for d in order], [stride[d] for d in order]
-        length_dim = None if length_dim is None else order.index(length_dim)
+    if not t.is_contiguous():
+        # Largest stride first, as [rows, positions, heads, dim] seen as [rows,
+        # heads, positions, dim] lies in memory; a dimension of one index goes
+        # with the one after it.  (Stride 0, rows on top of one another, is
+        # refused later.)
+        by = stride + [1]
+        for d in range(nd - 1, 0, -1):
+            if size[d] == 1:
+                by[d] = by[d + 1]
+        if all(by[1:nd]):
+            order = [0, *sorted(range(1, nd), key=lambda d: -by[d])]
+            size, stride = [size[d] for d in order], [stride[d] for d in order]
+            length_dim = None if length_dim is None else order.index(length_dim)
 
     def run(d):   # elements of dimensions d.. when they are consecutive, else 0
         n = 1
@@ -394,17 +396,18 @@ def reorder_struct(torch, device, states, parent, status, *, beams: Optional[int
     dims = list(length_dim) if isinstance(length_dim, (list, tuple)) else [length_dim] * len(states)
     if len(dims) != len(states):
         raise ValueError("length_dim must be one dimension or one per state")
-    if len({t.data_ptr() for t in states}) != len(states):
+    at = [t.data_ptr() for t in states]
+    if len(set(at)) != len(at):
         raise ValueError("a state is given twice: its rows would move twice at once")
     arr = (MxsState * max(1, len(states)))()
     last = None   # a cache's layers share one layout
-    for i, (t, d) in enumerate(zip(states, dims)):
+    for i, (t, d, p) in enumerate(zip(states, dims, at)):
         if t.device != device:
             raise ValueError(f"states must be on {device}, not {t.device}")
         like = (t.shape, t.stride(), t.dtype, d)
         if like != last:
             m, last = state_struct(t, groups * W, d), like
-        m.data = t.data_ptr()
+        m.data = p
         arr[i] = m
     r = MxsReorder()
     r.states, r.count = ctypes.cast(arr, ctypes.POINTER(MxsState)), len(states)
