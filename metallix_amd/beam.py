@@ -31,10 +31,8 @@ class BeamSearch:
     Ended beams stay in the race with their score.  length_penalty a orders
     the candidates by score * ((5 + length) / 6) ** -a.
 
-    `status`, int32[groups] on the device, is 0 or what first stopped a group
-    (ROW_STATUS): a NaN or +inf among its logits (-6), no candidate (-3),
-    scores or scales that are no numbers (-14).  Such a group has no
-    hypotheses from then on; the others go on."""
+    A group whose selection fails has no hypotheses from then on, and status()
+    says why; the others go on."""
 
     def __init__(self, sampler, groups: int, beams: int, max_new: int, *, end_token: Optional[int] = None,
                  length_penalty: float = 0.0):
@@ -99,12 +97,12 @@ class BeamSearch:
         self.steps += 1
         return tokens
 
-    @property
-    def status(self):
-        torch = self.sampler.torch
-        with torch.cuda.stream(self.sampler.stream):
-            first = (self._statuses != 0).int().argmax(0, keepdim=True)   # (the first of equal ones)
-            return self._statuses.gather(0, first)[0]
+    def status(self) -> List[int]:
+        """What first stopped each group (ROW_STATUS), 0 for one that goes on
+        (reads back): a NaN or +inf among its logits (-6), no candidate (-3),
+        scores or scales that are no numbers (-14)."""
+        self.sampler.sync()
+        return [next((s for s in steps if s), 0) for steps in zip(*self._statuses.cpu().tolist())]
 
     def done(self) -> bool:
         """Whether every sequence has ended or is not there (reads back)."""
@@ -113,7 +111,7 @@ class BeamSearch:
 
     def result(self) -> List[List[Hypothesis]]:
         """Each group's hypotheses, best first (reads back); none for a group
-        whose `status` is not 0."""
+        whose status() is not 0."""
         self.sampler.sync()
         tokens, length = self.tokens.cpu().tolist(), self.length.cpu().view(-1).tolist()
         score, ended = self.score.cpu().tolist(), self.ended.cpu().tolist()

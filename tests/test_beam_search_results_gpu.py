@@ -66,9 +66,26 @@ def test_what_stopped_a_group_is_kept(torch_mod, sampler, at):
             lg = lg.clone()
             lg[0, 7] = float("nan")
         search.step(lg, mask=none if t == at else mask)
-        torch.cuda.synchronize()
-        assert search.status.cpu().tolist() == ([0, 0, 0] if t < at else [-6, 0, -3]), t
-    assert alone.status.cpu().tolist() == [0, 0, 0]
+        assert search.status() == ([0, 0, 0] if t < at else [-6, 0, -3]), t
+    assert alone.status() == [0, 0, 0]
     want, got = alone.result(), search.result()
     assert got == [[], want[1], []] and len(want[1]) == W
     assert alone.done() is False
+
+
+def test_a_search_on_a_stream_of_its_own(torch_mod):
+    """What reads back waits for the steps, whatever stream is current."""
+    from metallix_amd import BeamSearch, Sampler
+
+    torch = torch_mod
+    lgs = [logits(torch, 90 + t) for t in range(T)]
+    lgs[3][W + 1, 9] = float("inf")            # group 1 stops
+    torch.cuda.synchronize()
+    found = []
+    for stream in (None, torch.cuda.Stream()):
+        s = Sampler(max_rows=G * W, max_vocab=V, stream=stream)
+        search = BeamSearch(s, G, W, T, end_token=END, length_penalty=0.3)
+        kept = [search.step(lg) for lg in lgs]
+        found.append((search.status(), search.done(), search.result(), [k.cpu().tolist() for k in kept]))
+        s.close()
+    assert found[0] == found[1] and found[0][0] == [0, -6, 0]
