@@ -538,9 +538,9 @@ __device__ __forceinline__ bool beam_before(const BeamCand& a, const BeamCand& b
   return (a.rank > b.rank) | ((a.rank == b.rank) & (a.tie > b.tie));   // (no branch around the second read)
 }
 
-// The upper half of a rank's order key; 0 for none.
+// The upper half of a rank's order key; 0 for none.  (-0 as +0: equal ranks.)
 __device__ __forceinline__ uint32_t beam_key(double r) {
-  const unsigned long long b = __builtin_bit_cast(unsigned long long, r);
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, r + 0.0);
   return (uint32_t)(((b >> 63) ? ~b : (b | 1ull << 63)) >> 32);
 }
 

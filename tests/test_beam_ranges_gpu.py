@@ -85,3 +85,18 @@ def test_the_logarithms_stated_bound(torch_mod, sampler, size, sign, dtype):
         want = score[g, 0] + lp
         err = 2.0 ** -39 + 2.0 ** -52 * abs(norm) + 2.0 ** -53 * (np.abs(lp) + np.abs(want)) + 2.0 ** -60 * abs(norm)
         assert np.all(np.abs(sc[g].astype(np.longdouble) - want) <= err), (g, sc[g], want, norm)
+
+
+@pytest.mark.parametrize("score,scale", [([-0.0, 0.0, -0.0, 0.0], None), ([0.0, -0.0, 0.0, -0.0], None),
+                                         ([-1e-200, 0.0, -1e-200, 0.0], [1e-200, 1.0, 1e-200, 1.0])])
+def test_ranks_of_either_zero_are_equal(torch_mod, sampler, score, scale):
+    """Ended beams whose rank is 0 of either sign (certain, or a product that
+    underflows) are equal: the lower beam first.  (Live ones are not: their
+    scores are off by up to 2^-39.)"""
+    W, V = 4, 50
+    x = np.zeros((W, V), np.float32)
+    kw = {} if scale is None else dict(scale=np.array([scale]))
+    tok, beam, sc, en, st = run(torch_mod, sampler, x, np.array([score]), W, ended=np.ones((1, W), bool), end_token=7, **kw)
+    assert st.tolist() == [0] and beam.tolist() == [[0, 1, 2, 3]]
+    assert tok.tolist() == [[7] * W] and en.all()
+    assert sc[0].tolist() == score
