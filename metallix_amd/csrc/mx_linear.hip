@@ -16,17 +16,17 @@
 // work.  us at 8192 x 4096 x 14336, step by step: loads into LDS waited for at
 // once 1335; restricted pointers (the compiler otherwise waits for the next
 // tile's loads before this tile's reads) 1045; fragments ahead and the order
-// of issue 803; results through LDS 728, 1321 TFLOP/s (the library's product
-// alone reaches 1528 on the same card).  The matrix pipes are busy for 66 to
-// 70% of the cycles, at the 1.83 GHz the card holds under this load; LDS, 192
-// KB read and 64 written per 2048 cycles of products, is as busy.  Also
+// of issue 803; results through LDS 728 to 746, 1290 to 1321 TFLOP/s (the
+// library's product alone 631 us, 1525).  The matrix pipes are busy for 65% of
+// the cycles, at the 1.83 GHz the card holds under this load; LDS, 192 KB read
+// and 64 written per 2048 cycles of products, is as busy.  Also
 // measured there: 32 x 32 x 16 products 905 us; four waves of 128 x 128 991
 // (registers spill); wave priorities 826; tiles of 32 k 1127.  No LDS bank
 // conflicts.
 //
 // What the other shapes take (us, floor the larger of bytes at 4.92 TB/s and
-// flops at 1248 TFLOP/s): 128 x 1024 x 151936, f32 out, 94 (floor 79: the
-// weight stream); 2048 x 4096 x 4096, gelu_tanh and residual, 64 (55); 333 x
+// flops at 1587 TFLOP/s): 128 x 1024 x 151936, f32 out, 94 (floor 79: the
+// weight stream); 2048 x 4096 x 4096, gelu_tanh and residual, 64 (43); 333 x
 // 1000 x 2050, gelu and residual, 10.8 (1.5: 16 dependent steps, the epilogue,
 // the launch); 1 x 1024 x 1024 4.1 (0.4: one launch).
 #include <hip/hip_runtime.h>
