@@ -385,10 +385,10 @@ int mxs_beam_reorder_check(mxs_ctx* ctx, const mxs_reorder* reorder);
  * (16-byte aligned, strides multiples of 8 below 2^22 elements; nothing past a
  * row's in_features is read), products summed in f32, the epilogue in f32
  * (activations within 2^-20 of their value's size plus 2^-30; a NaN stays, and
- * silu and gelu of -inf are NaN) with one rounding to the output type.  Any number of rows and features, up
- * to 2^35 results (in whole blocks of 64 x 64).  bias f32 or bf16 (bias_dtype)
- * or NULL; residual of out's type or NULL; it may be out itself (same stride),
- * otherwise out may overlap no input. */
+ * silu and gelu of -inf are NaN) with one rounding to the output type.  Any
+ * number of rows and features, up to 2^35 results (in whole blocks of 64 x 64).
+ * bias f32 or bf16 (bias_dtype) or NULL; residual of out's type or NULL; it may
+ * be out itself (same stride), otherwise out may overlap no input. */
 enum { MXS_ACT_NONE = 0, MXS_ACT_RELU = 1, MXS_ACT_SILU = 2, MXS_ACT_GELU = 3 /* erf */, MXS_ACT_GELU_TANH = 4 };
 typedef struct {
   const void* x;

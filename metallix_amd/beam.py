@@ -50,9 +50,8 @@ class BeamSearch:
             self.length = torch.zeros((rows, 1), dtype=torch.int32, device=dev)
             e = lambda *s: torch.empty(s, dtype=torch.int32, device=dev)
             # each step's own tokens and statuses
-            self._tokens = torch.empty((max_new, groups, beams), dtype=torch.int32, device=dev).unbind(0)
+            self._tokens = torch.empty((max_new, groups, beams), dtype=torch.int32, device=dev)
             self._statuses = torch.zeros((max_new + 1, groups), dtype=torch.int32, device=dev)
-            self._status_rows = self._statuses.unbind(0)
             self.picked = BeamResult(token=e(groups, beams), beam=e(groups, beams), score=self.score, ended=self.ended,
                                      status=e(groups))
             self.moved = e(groups)   # (always 0: the parents are the selection's)
@@ -63,9 +62,10 @@ class BeamSearch:
         Sampler.beam_select, but not the end token, the ended beams or, with
         a length penalty, the scale, which are the search's), moves `states`
         (tensors of groups * beams rows, the first lengths[g] positions of
-        their length_dim) and the search's own rows to them.  Returns the rows' next tokens, int32[groups *
-        beams] on the device (-1: no sequence; an ended one's end token), a
-        tensor of this step's own that later steps leave alone."""
+        their length_dim) and the search's own rows to them.  Returns the
+        rows' next tokens, int32[groups * beams] on the device (-1: no
+        sequence; an ended one's end token), a tensor of this step's own that
+        later steps leave alone."""
         if self.steps >= self.max_new:
             raise ValueError(f"the search holds {self.max_new} tokens")
         own = {"ended", "end_token"} | ({"scale"} if self.length_penalty else set())
@@ -84,7 +84,7 @@ class BeamSearch:
                 n = torch.where(self.ended, self.length.view(self.groups, self.beams), self.steps + 1)
                 rule = dict(rule, scale=((5.0 + n.double()) / 6.0) ** -self.length_penalty)
             p = self.picked
-            picked = BeamResult(self._tokens[self.steps], p.beam, p.score, p.ended, self._status_rows[self.steps])
+            picked = BeamResult(self._tokens[self.steps], p.beam, p.score, p.ended, self._statuses[self.steps])
             s.beam_select(logits, self.score, self.beams, out=picked, **rule)
             # (the step is accepted: the parents' lengths, which then move with their rows)
             if self.end_token is not None:
