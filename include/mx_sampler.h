@@ -47,6 +47,9 @@
  *                                vocabulary, and the move of the beams' states.
  *   mxs_linear_bf16           <- the projections around the lm_head (forward.rs:1745-1761)
  *                                with bias, activation and residual in the epilogue.
+ *   mxs_prefix_attention,     <- (no counterpart: the reference's caches belong to one
+ *   mxs_cache_evict              sequence each and only grow.)  Attention of sequences that
+ *                                share a prefix, and caches held to a budget of positions.
  *   mxs_sync                  <- Qwen3TokenPicks::wait (picks.rs:390-401).
  *   mxs_last_error            <- KernelError's message (mlx-kernels/src/lib.rs:444-450).
  *
@@ -406,6 +409,88 @@ typedef struct {
   int32_t bias_dtype;             /* mxs_dtype of bias */
 } mxs_linear;
 int mxs_linear_bf16(mxs_ctx* ctx, const mxs_linear* linear);
+/* One layer's attention of sequences that share a prefix (a request's beams or
+ * choices over its prompt): sequence b of group g is row r = g * beams + b, its
+ * `tokens` newest tokens are the queries, and query head h reads the caches' head
+ * k = h / (heads / kv_heads).  Token t sees the group's first prefix_lengths[g]
+ * prefix positions and the row's suffix positions j < lengths[r] - tokens + t + 1
+ * (its own is the suffix's last but tokens - 1 - t):
+ *   s[i] = scale * sum_d q[d] keys[i][d]    lse = ln sum_i exp(s[i])
+ *   out[d] = sum_i exp(s[i] - lse) values[i][d]
+ * over the positions that it sees; what else the caches hold, NaN included, does
+ * not count.  A score of -inf weighs nothing, and a token that sees nothing, or
+ * only such scores, gets out 0 and lse -inf.  A NaN or +inf among its scores makes
+ * its out and lse NaN.
+ * With prefix_weight or weight every position's weights exp(s - lse), summed over
+ * the queries that read it, are added to its entry (positions that none sees stay as they are;
+ * a query whose lse is NaN makes those that it sees NaN): what mxs_cache_evict goes by.
+ *
+ * q, caches and out are bf16, the elements of a head consecutive, at 16-byte
+ * aligned addresses, strides in elements and multiples of 8; keys and values
+ * have the same strides.  Scores, statistics and sums are f32; the exponentials are
+ * rounded to bf16 where they multiply the values, as the output is (2^-8 each).
+ * Equal calls give equal bits.
+ * The outputs meet neither an input nor one another. */
+typedef struct {
+  const void* q;                  /* [groups * beams][tokens][heads][dim] */
+  uint64_t q_row, q_token, q_head;
+  const void* prefix_keys;        /* [groups][kv_heads][prefix][dim]; NULL with prefix 0 */
+  const void* prefix_values;
+  uint64_t prefix_group, prefix_head, prefix_position;   /* prefix_position below 2^22, as `position` */
+  const int32_t* prefix_lengths;  /* device: groups, clamped to 0..prefix; NULL => prefix */
+  const void* keys;               /* [groups * beams][kv_heads][suffix][dim]; NULL with suffix 0 */
+  const void* values;
+  uint64_t row, head, position;
+  const int32_t* lengths;         /* device: groups * beams, clamped to 0..suffix; NULL => suffix */
+  void* out;                      /* as q */
+  uint64_t out_row, out_token, out_head;
+  float* lse;                     /* [groups * beams][tokens][heads]; NULL => not written */
+  float* prefix_weight;           /* [groups][kv_heads][prefix], added to; NULL => none */
+  float* weight;                  /* [groups * beams][kv_heads][suffix], added to; NULL => none */
+  uint32_t groups, beams, tokens; /* groups * beams * tokens * heads below 2^31 */
+  uint32_t heads, kv_heads;       /* heads a multiple of kv_heads, at most 4096 */
+  uint32_t dim;                   /* multiple of 8, 8..256 */
+  uint32_t prefix, suffix;        /* positions that the caches hold, below 2^30 */
+  float scale;                    /* finite */
+  uint32_t reserved;
+} mxs_attention;
+int mxs_prefix_attention(mxs_ctx* ctx, const mxs_attention* attention);
+/* Brings caches down to `budget` positions.  A cache of a layer is keys and values
+ * [segments][heads][capacity] of position_bytes; segment s uses its first
+ * len = lengths[s] slots, slot i holding position index[i], and has accumulated
+ * weight[i] on each (mxs_prefix_attention).  Where len > budget, each (layer, segment,
+ * head) by itself keeps `budget` of them: first those whose position is below
+ * keep_first or above newest - keep_recent (newest: the largest position in use),
+ * then by weight, largest first (-0 equals 0, NaN comes last), equal ones by lower slot.  Kept
+ * slots below budget stay where they are; the j-th free slot below budget takes what the j-th kept
+ * slot from budget on holds, so a step that frees one slot moves one position.
+ * The order of positions changes (attention does not see it); index_out
+ * tells them apart.  weight_out and index_out get the slots' new contents, 0 and -1 from
+ * the new length min(len, budget) on, so that later positions start
+ * there; of the caches only the slots filled are written.  Caches (data, any
+ * alignment) must not share memory, nor with the arrays; the outputs meet neither
+ * an input nor one another. */
+#define MXS_EVICT_MAX_CAPACITY (1u << 20)
+typedef struct {
+  void* keys;
+  void* values;                   /* NULL: the layer has one array */
+} mxs_cache;
+typedef struct {
+  const mxs_cache* caches;        /* host array of `layers`, read during the call */
+  uint32_t layers, segments, heads;   /* layers * segments * heads below 2^21 */
+  uint32_t capacity;              /* slots, 1..MXS_EVICT_MAX_CAPACITY */
+  uint64_t segment_stride, head_stride, position_stride;   /* bytes, of every array */
+  uint32_t position_bytes;        /* 1..65536 */
+  uint32_t budget;                /* at least 1 */
+  uint32_t keep_first, keep_recent;   /* together at most budget */
+  const float* weight;            /* [layers][segments][heads][capacity] */
+  const int32_t* index;           /* as weight, distinct and not negative; NULL => slot i holds position i */
+  const int32_t* lengths;         /* device: segments, clamped to 0..capacity; NULL => capacity */
+  float* weight_out;              /* as weight */
+  int32_t* index_out;             /* as weight; NULL => not written */
+  int32_t* lengths_out;           /* segments; NULL => not written */
+} mxs_evict;
+int mxs_cache_evict(mxs_ctx* ctx, const mxs_evict* evict);
 int mxs_mask_host(mxs_ctx* ctx, uint32_t slot, uint32_t** words, uint64_t* stride_words);
 int mxs_mask_upload(mxs_ctx* ctx, uint32_t slot, uint32_t rows, const uint32_t** device_words);
 int mxs_sync(mxs_ctx* ctx);

@@ -14,6 +14,7 @@ from .sampler import (  # noqa: F401
     MXS_F32,
     ROW_STATUS,
     BeamResult,
+    EvictResult,
     Sampler,
     SamplerError,
     load_library,

@@ -48,6 +48,7 @@ size_t race_scratch_bytes(uint32_t max_rows, uint32_t max_vocab);
 size_t beam_scratch_bytes(uint32_t max_rows);
 size_t linear_scratch_bytes();
 size_t linear_ctr_words();
+size_t attention_scratch_bytes();
 constexpr uint32_t SPEC_COUNTERS_PER_ROW = 10;   // one per (row, position <= 8), one per row
 
 // Rows' counters and exchange words sit on their own 128-byte lines, so the
@@ -108,6 +109,8 @@ struct mxs_ctx {
   // mxs_linear_bf16: a split sum's parts and their arrivals
   float* linear_scratch = nullptr;
   uint32_t* linear_ctr = nullptr;
+  // mxs_prefix_attention: the parts of queries whose positions are split, and their statistics
+  float* attention_scratch = nullptr;
   // the uniform of the inverse-CDF draw mxs_sample_race discards (below)
   double* d_race_u = nullptr;
   // grammar-mask staging (mxs_mask_host / mxs_mask_upload, mx_mask.hip):

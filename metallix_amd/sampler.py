@@ -116,6 +116,37 @@ class MxsLinear(ctypes.Structure):
     ]
 
 
+class MxsAttention(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("q_row", ctypes.c_uint64), ("q_token", ctypes.c_uint64), ("q_head", ctypes.c_uint64),
+        ("prefix_keys", _vp), ("prefix_values", _vp), ("prefix_group", ctypes.c_uint64),
+        ("prefix_head", ctypes.c_uint64), ("prefix_position", ctypes.c_uint64), ("prefix_lengths", _vp),
+        ("keys", _vp), ("values", _vp), ("row", ctypes.c_uint64), ("head", ctypes.c_uint64),
+        ("position", ctypes.c_uint64), ("lengths", _vp),
+        ("out", _vp), ("out_row", ctypes.c_uint64), ("out_token", ctypes.c_uint64), ("out_head", ctypes.c_uint64),
+        ("lse", _vp), ("prefix_weight", _vp), ("weight", _vp),
+        ("groups", ctypes.c_uint32), ("beams", ctypes.c_uint32), ("tokens", ctypes.c_uint32),
+        ("heads", ctypes.c_uint32), ("kv_heads", ctypes.c_uint32), ("dim", ctypes.c_uint32),
+        ("prefix", ctypes.c_uint32), ("suffix", ctypes.c_uint32), ("scale", ctypes.c_float),
+        ("reserved", ctypes.c_uint32),
+    ]
+
+
+class MxsCache(ctypes.Structure):
+    _fields_ = [("keys", _vp), ("values", _vp)]
+
+
+class MxsEvict(ctypes.Structure):
+    _fields_ = [
+        ("caches", ctypes.POINTER(MxsCache)), ("layers", ctypes.c_uint32), ("segments", ctypes.c_uint32),
+        ("heads", ctypes.c_uint32), ("capacity", ctypes.c_uint32), ("segment_stride", ctypes.c_uint64),
+        ("head_stride", ctypes.c_uint64), ("position_stride", ctypes.c_uint64), ("position_bytes", ctypes.c_uint32),
+        ("budget", ctypes.c_uint32), ("keep_first", ctypes.c_uint32), ("keep_recent", ctypes.c_uint32),
+        ("weight", _vp), ("index", _vp), ("lengths", _vp), ("weight_out", _vp), ("index_out", _vp),
+        ("lengths_out", _vp),
+    ]
+
+
 # Exported symbols and their prototypes, as declared in include/mx_sampler.h.
 PROTOTYPES = {
     "mxs_abi_version": (ctypes.c_int, []),
@@ -145,6 +176,8 @@ PROTOTYPES = {
     "mxs_beam_reorder": (ctypes.c_int, [_vp, ctypes.POINTER(MxsReorder)]),
     "mxs_beam_reorder_check": (ctypes.c_int, [_vp, ctypes.POINTER(MxsReorder)]),
     "mxs_linear_bf16": (ctypes.c_int, [_vp, ctypes.POINTER(MxsLinear)]),
+    "mxs_prefix_attention": (ctypes.c_int, [_vp, ctypes.POINTER(MxsAttention)]),
+    "mxs_cache_evict": (ctypes.c_int, [_vp, ctypes.POINTER(MxsEvict)]),
     "mxs_debug_set_timing": (ctypes.c_int, [_vp, _vp]),
     "mxs_debug_floor": (ctypes.c_int, [_vp, _vp, ctypes.c_int32, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32,
                                        ctypes.c_uint32, _vp, _vp]),
@@ -453,6 +486,128 @@ def linear_struct(torch, device, x, weight, bias, residual, out, activation) -> 
     return a
 
 
+def _cache_pair(torch, device, keys, values, names, shape, dtypes):
+    """Strides of dimensions 0 to 2 of two like caches of 4 dimensions, the last
+    of them consecutive; a dimension of one index has stride 0."""
+    for t, name in ((keys, names[0]), (values, names[1])):
+        _need(t, name, device, dtypes, shape)
+        if t.shape[3] > 1 and t.stride(3) != 1:
+            raise ValueError(f"{name}: a position's elements must be consecutive")
+    st = lambda t: [s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3])]
+    if values.shape != keys.shape or values.dtype != keys.dtype or st(values) != st(keys):
+        raise ValueError(f"{names[0]} and {names[1]} must have the same type, shape and strides")
+    return st(keys)
+
+
+def attention_struct(torch, device, q, prefix_keys, prefix_values, keys, values, out, *, prefix_lengths=None,
+                     lengths=None, scale=None, lse=None, prefix_weight=None, weight=None) -> MxsAttention:
+    """The mxs_attention of a call, its tensors checked against `device` and
+    each other (ValueError)."""
+    bf = (torch.bfloat16,)
+    if q.dim() not in (3, 4):
+        raise ValueError(f"q must have the shape [rows, (tokens,) heads, dim], not {list(q.shape)}")
+    _need(q, "q", device, bf, (None,) * q.dim())
+    _need(out, "out", device, bf, tuple(q.shape))
+    if lse is not None:
+        _need(lse, "lse", device, (torch.float32,), tuple(q.shape[:-1]))
+        _dense(lse, "lse")
+    if q.dim() == 3:
+        q, out = q.unsqueeze(1), out.unsqueeze(1)
+    rows, tokens, heads, dim = q.shape
+    for t, name in ((q, "q"), (out, "out")):
+        if dim > 1 and t.stride(3) != 1:
+            raise ValueError(f"{name}: a head's elements must be consecutive")
+    if (prefix_keys is None) != (prefix_values is None) or (keys is None) != (values is None):
+        raise ValueError("keys and values come together")
+    if prefix_keys is None:
+        raise ValueError("a prefix is required (of no positions, where there is none)")
+    if prefix_keys.dim() != 4:
+        raise ValueError(f"prefix_keys must have the shape [groups, kv_heads, positions, dim], not {list(prefix_keys.shape)}")
+    groups, kv, P, _ = prefix_keys.shape
+    a = MxsAttention()
+    a.prefix_group, a.prefix_head, a.prefix_position = _cache_pair(
+        torch, device, prefix_keys, prefix_values, ("prefix_keys", "prefix_values"), (None, None, None, dim), bf)
+    if rows and (groups == 0 or rows % groups):
+        raise ValueError(f"q's {rows} rows must be the same number for each of the {groups} groups")
+    N = 0
+    if keys is not None:
+        a.row, a.head, a.position = _cache_pair(torch, device, keys, values, ("keys", "values"), (rows, kv, None, dim), bf)
+        N = keys.shape[2]
+        if N:
+            a.keys, a.values = keys.data_ptr(), values.data_ptr()
+    elif lengths is not None or weight is not None:
+        raise ValueError("lengths and weight need keys and values")
+    for t, name, shape, dt in ((prefix_lengths, "prefix_lengths", (groups,), torch.int32),
+                               (lengths, "lengths", (rows,), torch.int32),
+                               (prefix_weight, "prefix_weight", (groups, kv, P), torch.float32),
+                               (weight, "weight", (rows, kv, N), torch.float32)):
+        if t is not None:
+            _need(t, name, device, (dt,), shape)
+            _dense(t, name)
+    st = lambda t: [s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3])]
+    a.q, (a.q_row, a.q_token, a.q_head) = q.data_ptr(), st(q)
+    a.out, (a.out_row, a.out_token, a.out_head) = out.data_ptr(), st(out)
+    if P:
+        a.prefix_keys, a.prefix_values = prefix_keys.data_ptr(), prefix_values.data_ptr()
+        a.prefix_weight = _ptr(prefix_weight)
+    if N:
+        a.weight = _ptr(weight)
+    a.prefix_lengths, a.lengths, a.lse = _ptr(prefix_lengths), _ptr(lengths), _ptr(lse)
+    a.groups, a.beams = _u32(groups, "groups"), _u32(rows // groups if groups else 0, "beams")
+    a.tokens, a.heads, a.kv_heads, a.dim = _u32(tokens, "tokens"), _u32(heads, "heads"), _u32(kv, "kv_heads"), _u32(dim, "dim")
+    a.prefix, a.suffix = _u32(P, "prefix"), _u32(N, "suffix")
+    a.scale = dim ** -0.5 if scale is None else float(scale)
+    return a
+
+
+def evict_struct(torch, device, keys, values, weight, budget, out, *, index=None, lengths=None, keep_first: int = 0,
+                 keep_recent: int = 0) -> MxsEvict:
+    """The mxs_evict of a call, its tensors checked against `device` and each
+    other (ValueError)."""
+    keys, values = list(keys), None if values is None else list(values)
+    _need(weight, "weight", device, (torch.float32,), (None,) * 4)
+    L, S, H, C = weight.shape
+    if len(keys) != L or (values is not None and len(values) != L):
+        raise ValueError(f"keys and values must hold one cache for each of the {L} layers")
+    for t, name, shape, dt in ((weight, "weight", (L, S, H, C), torch.float32), (index, "index", (L, S, H, C), torch.int32),
+                               (lengths, "lengths", (S,), torch.int32), (out.weight, "out.weight", (L, S, H, C), torch.float32),
+                               (out.index, "out.index", (L, S, H, C), torch.int32),
+                               (out.lengths, "out.lengths", (S,), torch.int32)):
+        if t is not None:
+            _need(t, name, device, (dt,), shape)
+            _dense(t, name)
+    every = keys + (values or [])
+    if len({t.data_ptr() for t in every}) != len(every) and 0 not in weight.shape:
+        raise ValueError("a cache is given twice: its positions would move twice at once")
+    e = MxsEvict()
+    arr = (MxsCache * max(1, L))()
+    st = None
+    for i, t in enumerate(every):
+        _need(t, "a cache", device, (every[0].dtype,), (S, H, C, every[0].shape[3] if every[0].dim() == 4 else None))
+        mine = [s if n > 1 else 0 for n, s in zip(t.shape, t.stride())]
+        if t.shape[3] > 1 and t.stride(3) != 1:
+            raise ValueError("a cache's elements of a position must be consecutive")
+        if st is None:
+            st = mine
+        if mine != st:
+            raise ValueError("the caches must have the same strides")
+        if i < L:
+            arr[i].keys = t.data_ptr()
+        else:
+            arr[i - L].values = t.data_ptr()
+    es = every[0].element_size() if every else 1
+    e.caches, e.layers, e.segments, e.heads = ctypes.cast(arr, ctypes.POINTER(MxsCache)), L, S, H
+    e.capacity = _u32(C, "capacity")
+    if every:
+        e.segment_stride, e.head_stride, e.position_stride = (s * es for s in st[:3])
+        e.position_bytes = _u32(every[0].shape[3] * es, "position_bytes")
+    e.budget, e.keep_first, e.keep_recent = _u32(budget, "budget"), _u32(keep_first, "keep_first"), _u32(keep_recent, "keep_recent")
+    e.weight, e.index, e.lengths = weight.data_ptr(), _ptr(index), _ptr(lengths)
+    e.weight_out, e.index_out, e.lengths_out = out.weight.data_ptr(), _ptr(out.index), _ptr(out.lengths)
+    e.keep = arr
+    return e
+
+
 class DeviceWords:
     """A staging slot's device mask words, as `Sampler.sample(mask=...)`
     takes them (a data pointer and a row stride in words)."""
@@ -486,6 +641,16 @@ class BeamResult:
     score: "object"
     ended: "object"
     status: "object"
+
+
+@dataclass
+class EvictResult:
+    """Device tensors of one eviction (mxs_evict): the slots' weights and
+    positions, [layers, segments, heads, capacity], and the new lengths,
+    [segments]."""
+    weight: "object"
+    index: "object"
+    lengths: "object"
 
 
 @dataclass
@@ -983,6 +1148,78 @@ class Sampler:
 
         launch(x)
         launch.out, launch.keep = out, (a, weight, bias, residual)
+        return launch
+
+    def prefix_attention(self, q, prefix_keys, prefix_values, keys=None, values=None, *, out=None, **kw):
+        """Queues one layer's attention of sequences that share a prefix
+        (mxs_prefix_attention): q bf16[groups * beams, (tokens,) heads, dim],
+        the newest tokens of every sequence, over the first prefix_lengths[g]
+        positions of its group's prefix_keys and prefix_values [groups,
+        kv_heads, positions, dim] and, causally, the first lengths[r] of its
+        own keys and values [groups * beams, kv_heads, positions, dim], the
+        queries' own positions last (lengths int32 on the device; default
+        all).  scale: dim ** -0.5 by default.  lse: f32, q's shape without
+        dim, gets the logarithms of the sums.  prefix_weight f32[groups,
+        kv_heads, positions] and weight f32[groups * beams, kv_heads,
+        positions] get the weights of every position added.  Returns out,
+        bf16 of q's shape."""
+        f = self.prefix_attention_launcher(q, prefix_keys, prefix_values, keys, values, out=out, **kw)
+        f()
+        return f.out
+
+    def prefix_attention_launcher(self, q, prefix_keys, prefix_values, keys=None, values=None, *, out=None, **kw):
+        """Pre-built prefix_attention for repeated calls over the same
+        tensors: returns f() that queues it with what they then hold (f.out
+        holds the output).  Nothing is queued here."""
+        torch, dev = self.torch, self._device()
+        if out is None:
+            with torch.cuda.stream(self.stream):
+                out = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
+        a = attention_struct(torch, dev, q, prefix_keys, prefix_values, keys, values, out, **kw)
+        fn, ctx, ap = self.lib.mxs_prefix_attention, self.ctx, ctypes.byref(a)
+
+        def launch():
+            rc = fn(ctx, ap)
+            if rc != 0:
+                self._check(rc, "mxs_prefix_attention")
+
+        launch.out, launch.keep = out, (a, q, prefix_keys, prefix_values, keys, values, kw)
+        return launch
+
+    def cache_evict(self, keys, values, weight, budget: int, *, out: Optional[EvictResult] = None, **kw) -> EvictResult:
+        """Queues the eviction of caches down to `budget` positions
+        (mxs_cache_evict): keys and values, a tensor [segments, heads,
+        capacity, dim] for each layer (values None: the layers have one array
+        each), of which the first lengths[s] slots are in use (int32[segments];
+        default all); weight f32[layers, segments, heads, capacity], their
+        accumulated weights; index int32, the same shape, the slots' positions
+        (default: in order).  The keep_first first positions, the keep_recent
+        newest and the largest weights stay.  The caches change in place;
+        returns the slots' new weights and positions and the new lengths, as
+        the next eviction takes them."""
+        f = self.cache_evict_launcher(keys, values, weight, budget, out=out, **kw)
+        f()
+        return f.out
+
+    def cache_evict_launcher(self, keys, values, weight, budget: int, *, out: Optional[EvictResult] = None, **kw):
+        """Pre-built cache_evict for repeated calls over the same tensors:
+        returns f() that queues it with what they then hold (f.out holds the
+        outputs).  Nothing is queued here."""
+        torch, dev = self.torch, self._device()
+        if out is None:
+            with torch.cuda.stream(self.stream):
+                e = lambda shape, dt: torch.empty(shape, dtype=dt, device=dev)
+                out = EvictResult(weight=e(weight.shape, torch.float32), index=e(weight.shape, torch.int32),
+                                  lengths=e(weight.shape[1:2], torch.int32))
+        m = evict_struct(torch, dev, keys, values, weight, budget, out, **kw)
+        fn, ctx, mp = self.lib.mxs_cache_evict, self.ctx, ctypes.byref(m)
+
+        def launch():
+            rc = fn(ctx, mp)
+            if rc != 0:
+                self._check(rc, "mxs_cache_evict")
+
+        launch.out, launch.keep = out, (m, keys, values, weight, kw)
         return launch
 
     def mask_host(self, slot: int):
