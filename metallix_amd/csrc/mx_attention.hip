@@ -11,23 +11,34 @@
 
 #include "../../include/mx_sampler.h"
 #include "mxs_attention_checks.h"
+#include "mxs_attention_plan.h"
 #include "mxs_ctx.h"
 #include "mxs_device.h"
 
 namespace mxs {
 
-constexpr size_t ATT_SCRATCH = 64u << 20;
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 struct AttArgs {
   const __bf16 *q, *pk, *pv, *k, *v;
   __bf16* out;
-  uint64_t qr, qt, qh, pg, ph, pp, kr, kh, kp, orow, ot, oh;
+  uint64_t qr, qt, qh, pg, ph, pp, kr, kh, kp, orow, ot, oh;   // strides in elements
   const int32_t *plen, *len;
   float *lse, *pw, *w;
-  float* own;                // [rows][tokens][heads] lse of this slice
-  uint32_t W, T, H, KV, D, P, N;
-  uint32_t r0, nr, t0, nt;   // this slice: rows and tokens
-  float scale;
+  uint32_t W, T, H, KV, D, P, N, per;   // per: query heads a cache head has
+  uint32_t g0, ng, b0, wb, t0, nt;      // this launch's groups, rows of each, tokens
+  uint32_t nrb, nsb, sp, ss, slots;     // blocks of queries of a prefix and a suffix, parts of either, of a query
+  uint32_t np, njobs;                   // workgroups of prefixes, of all
+  uint32_t NQ;                          // queries: ng * wb * nt * H
+  float c;                              // |scale| log2(e)
+  uint32_t flip;                        // 0x8000 where the scale is negative: the queries' signs
+  float* part;                          // [slots][NQ][DP] sums of a part's exponentials times its values
+  float2* stat;                         // [slots][NQ] the part's reference (log2) and sum
+  float* ref;                           // [NQ] log2 of a query's whole sum; inf: it has seen nothing
 };
 
 __device__ __forceinline__ uint32_t att_len(const int32_t* len, uint32_t i, uint32_t most) {
@@ -41,92 +52,543 @@ __device__ __forceinline__ uint32_t att_seen(uint32_t len, uint32_t T, uint32_t 
   return n <= 0 ? 0u : (uint32_t)n;
 }
 
-// One workgroup a query: each wave takes every fourth position.
-__global__ __launch_bounds__(256) void attention_simple_kernel(AttArgs A) {
-  __shared__ float sm[4], sl[4], so[4][256];
-  const uint32_t w = threadIdx.x >> 6, l = threadIdx.x & 63u;
-  const uint32_t h = blockIdx.x % A.H, t = A.t0 + blockIdx.x / A.H % A.nt, r = A.r0 + blockIdx.x / A.H / A.nt;
-  const uint32_t g = r / A.W, kv = h / (A.H / A.KV);
-  const __bf16* const q = A.q + r * A.qr + t * A.qt + h * A.qh;
-  const uint32_t P = att_len(A.plen, g, A.P), N = A.N ? att_seen(att_len(A.len, r, A.N), A.T, t) : 0u;
-  const bool in = l * 4u < A.D;
-  float qv[4] = {}, o[4] = {}, m = -INFINITY, sum = 0.0f;
-  if (in)
-    for (int j = 0; j < 4; ++j) qv[j] = (float)q[l * 4u + j];
-  for (uint32_t i = w; i < P + N; i += 4u) {
-    const bool pre = i < P;
-    const uint64_t at = pre ? g * A.pg + kv * A.ph + (uint64_t)i * A.pp : r * A.kr + kv * A.kh + (uint64_t)(i - P) * A.kp;
-    const __bf16* const kk = (pre ? A.pk : A.k) + at;
-    const __bf16* const vv = (pre ? A.pv : A.v) + at;
-    float s = 0.0f;
-    if (in)
-      for (int j = 0; j < 4; ++j) s += qv[j] * (float)kk[l * 4u + j];
-    for (int x = 1; x < 64; x <<= 1) s += __shfl_xor(s, x);
-    s *= A.scale;
-    const float nm = fmaxf(m, s), base = nm == -INFINITY ? 0.0f : nm;
-    const float a = expf(m - base), p = expf(s - base);
-    sum = sum * a + p;
-    if (in)
-      for (int j = 0; j < 4; ++j) o[j] = o[j] * a + (p == 0.0f ? 0.0f : p * (float)vv[l * 4u + j]);
-    m = nm;
+// The largest, or the sum, over the four lanes that hold the same query.
+__device__ __forceinline__ float max4(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float sum4(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+// 2^(m - to) for the references of two parts; 0 for one that has seen nothing.
+__device__ __forceinline__ float share_of(float m, float to) { return m == -INFINITY ? 0.0f : exp2_(m - to); }
+
+__device__ __forceinline__ bf16x8 flipped(bf16x8 v, uint32_t flip) {
+  s16x8 b = __builtin_bit_cast(s16x8, v);
+  b ^= (short)flip;
+  return __builtin_bit_cast(bf16x8, b);
+}
+
+// Sixteen bytes a lane into LDS (see mx_linear.hip).
+__device__ __forceinline__ void att_load_lds(__bf16* lds, const __bf16* base, uint32_t off, uint32_t at) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, -1, 0x27000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, off, at, 0, 0);
+#endif
+}
+// Four rows of a 16-bit array in LDS, transposed: of 16 lanes, lane l gives the
+// address of four elements of row l / 4 from column 4 (l % 4) on and gets
+// column l of the four rows.
+__device__ __forceinline__ s16x4 read_turned(const __bf16* p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+#else
+  return s16x4{};
+#endif
+}
+template <int N>
+__device__ __forceinline__ void att_barrier() {   // all but the wave's N newest loads have landed; the workgroup meets
+  static_assert(N < 64, "a six-bit counter");
+  __asm__ volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4);
+  __asm__ volatile("s_barrier" ::: "memory");
+}
+
+// One job: the queries of a block over positions a..b of one cache head.
+struct AttJob {
+  const __bf16 *k, *v;      // position 0
+  uint64_t stride;          // elements between positions
+  uint32_t a, b;
+  uint32_t g, kv;           // group within the launch, cache head
+  uint32_t m0, m;           // first query of the block, queries of the cache head
+  uint32_t row;             // suffix: the row within the group
+  uint32_t len;             // suffix: its length
+  uint32_t slot;
+  bool pre;
+};
+
+// Where query m of a job belongs: its row within the launch, token and head.
+struct AttQuery {
+  uint32_t row, t, h;
+};
+__device__ __forceinline__ AttQuery att_query(const AttArgs& A, const AttJob& J, uint32_t m) {
+  const uint32_t hh = m % A.per, r = m / A.per, t = r % A.nt, b = J.pre ? r / A.nt : J.row;
+  return {J.g * A.wb + b, A.t0 + t, J.kv * A.per + hh};
+}
+__device__ __forceinline__ uint32_t att_row(const AttArgs& A, uint32_t row) {   // of the whole call
+  return (A.g0 + row / A.wb) * A.W + A.b0 + row % A.wb;
+}
+
+// Scores as S^T = K Q^T on v_mfma_f32_16x16x32_bf16 (a lane holds four
+// positions of one query), sums as O^T = V^T P^T: the exponentials are the second
+// operand as they lie, values are read transposed from LDS.
+template <int DP, int RB, int WQ, int WP, int S>
+__device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J, __bf16* Ks, __bf16* Vs, float2* stats) {
+  constexpr uint32_t PR = DP / 8, LR = 64 / PR;                  // 16-byte pieces of a row, rows a load takes
+  constexpr int KS = DP / 32, DB = DP / 16, NW = WQ * WP;
+  constexpr int PPW = ATT_TILE / WP, NB = PPW >= 32 ? 2 : 1, SUBS = PPW / (16 * NB);   // positions a wave takes of a tile
+  constexpr int LD = ATT_TILE / (int)LR / NW;                    // loads a wave issues for keys, and for values
+  constexpr uint32_t TE = ATT_TILE * DP;                         // elements of a tile
+  static_assert(LD * (int)LR * NW == (int)ATT_TILE, "the loads cover the tile");
+  const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63u, lr = l & 15u, lg = l >> 4;
+  const uint32_t wq = w % WQ, wp = w / WQ;
+  const uint32_t m0 = J.m0 + wq * (16u * RB);
+
+  // the queries, a fragment of each for every 32 elements; and where each one's positions end
+  bf16x8 q[RB][KS];
+  uint32_t lim[RB], least = J.b;
+#pragma unroll
+  for (int j = 0; j < RB; ++j) {
+    const uint32_t m = m0 + 16u * j + lr;
+    lim[j] = 0u;
+    if (m < J.m) {
+      const AttQuery x = att_query(A, J, m);
+      lim[j] = J.pre ? J.b : min(J.b, att_seen(J.len, A.T, x.t));
+      const __bf16* const from = A.q + (uint64_t)att_row(A, x.row) * A.qr + x.t * A.qt + x.h * A.qh;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const uint32_t d = 32u * s + 8u * lg;
+        q[j][s] = d < A.D ? flipped(*reinterpret_cast<const bf16x8*>(from + d), A.flip) : bf16x8{};
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) q[j][s] = bf16x8{};
+    }
   }
-  if (l == 0) { sm[w] = m; sl[w] = sum; }
-  for (int j = 0; j < 4; ++j) so[w][l * 4u + j] = o[j];
-  __syncthreads();
-  float M = -INFINITY, L = 0.0f;
-  for (int x = 0; x < 4; ++x) M = fmaxf(M, sm[x]);
-  const float base = M == -INFINITY ? 0.0f : M;
-  for (int x = 0; x < 4; ++x) L += sl[x] * expf(sm[x] - base);
-  if (threadIdx.x < A.D) {
-    float v = 0.0f;
-    for (int x = 0; x < 4; ++x) v += so[x][threadIdx.x] * expf(sm[x] - base);
-    A.out[r * A.orow + t * A.ot + h * A.oh + threadIdx.x] = (__bf16)(L == 0.0f ? 0.0f : v / L);
+  if (!J.pre) least = min(J.b, att_seen(J.len, A.T, A.t0));   // (of the job's first token: none ends earlier)
+
+  f32x4 acc[DB][RB] = {};
+  float mc[RB], sum[RB];   // reference (log2) and sum of each query, the sum of this lane's positions
+#pragma unroll
+  for (int j = 0; j < RB; ++j) mc[j] = -INFINITY, sum[j] = 0.0f;
+
+  const uint32_t nt = J.b > J.a ? (J.b - J.a + ATT_TILE - 1u) / ATT_TILE : 0u;
+  if (A.D < DP && nt) {   // elements past dim are never loaded: zero
+    for (uint32_t i = threadIdx.x; i < S * TE / 8u; i += NW * 64) {
+      reinterpret_cast<bf16x8*>(Ks)[i] = bf16x8{};
+      reinterpret_cast<bf16x8*>(Vs)[i] = bf16x8{};
+    }
+    att_barrier<0>();
   }
-  if (threadIdx.x == 0) {
-    const float lse = base + logf(L);
-    if (A.lse) A.lse[((uint64_t)r * A.T + t) * A.H + h] = lse;
-    A.own[blockIdx.x] = lse;
+  // A row's pieces lie permuted by its low bits, so that the rows which a read
+  // takes fall in different banks.
+  auto turn_k = [](uint32_t row) { return PR == 8 ? (row >> 1) & 7u : row & 15u; };
+  auto turn_v = [](uint32_t row) { return PR == 8 ? (row >> 1 & 3u) * 2u : (row & 7u) * 2u; };
+  auto fetch = [&](uint32_t tile, const __bf16* __restrict__ from, __bf16* __restrict__ to, bool keys) __attribute__((always_inline)) {
+    const uint32_t p0 = J.a + tile * ATT_TILE, have = min(ATT_TILE, J.b - p0);
+    const __bf16* const base = from + (uint64_t)p0 * J.stride;
+#pragma unroll
+    for (int i = 0; i < LD; ++i) {
+      const uint32_t row = (w * LD + i) * LR + l / PR, piece = (l % PR) ^ (keys ? turn_k(row) : turn_v(row));
+      if (piece * 8u < A.D)
+        att_load_lds(to + (w * LD + i) * LR * DP, base, (min(row, have - 1u) * (uint32_t)J.stride + piece * 8u) * 2u, 0u);
+    }
+  };
+  const uint32_t kt = turn_k(lr);   // (rows of a fragment: lr more than a multiple of 16)
+  const uint32_t vrow = 4u * lg + (lr >> 2), vt = turn_v(vrow);
+
+  auto compute = [&](const __bf16* __restrict__ kb, const __bf16* __restrict__ vb, uint32_t p0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int sub = 0; sub < SUBS; ++sub) {
+      const uint32_t at = wp * PPW + sub * (16u * NB);   // first position within the tile
+      f32x4 s[NB][RB] = {};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        bf16x8 kf[NB];
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+          kf[i] = *reinterpret_cast<const bf16x8*>(kb + (at + 16u * i + lr) * DP + ((4u * ks + lg) ^ kt) * 8u);
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+          for (int j = 0; j < RB; ++j) s[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i], q[j][ks], s[i][j], 0, 0, 0);
+      }
+      const uint32_t first = p0 + at + 4u * lg;
+      const bool edge = p0 + at + 16u * NB > least;   // uniform: some query sees not all of these
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+          for (int j = 0; j < RB; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (first + 16u * i + e >= lim[j]) s[i][j][e] = -INFINITY;
+      }
+      // The reference follows the maximum only where that is 2^8 above it, which
+      // the first tiles settle: no exchange between lanes and no rescaling otherwise.
+      float top[RB];
+      bool grow = false;
+#pragma unroll
+      for (int j = 0; j < RB; ++j) {
+        float t = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) t = fmaxf(t, s[i][j][e]);
+        top[j] = t;
+        grow |= t * A.c > mc[j] + 8.0f;
+      }
+      if (__builtin_amdgcn_ballot_w64(grow)) {
+#pragma unroll
+        for (int j = 0; j < RB; ++j) {
+          const float m = fmaxf(mc[j], max4(top[j]) * A.c);
+          const float f = m == mc[j] ? 1.0f : share_of(mc[j], m);
+          mc[j] = m;
+          sum[j] *= f;
+#pragma unroll
+          for (int d = 0; d < DB; ++d) acc[d][j] *= f;
+        }
+      }
+      s16x4 pb[NB][RB];
+#pragma unroll
+      for (int j = 0; j < RB; ++j) {
+        const float base = mc[j] == -INFINITY ? 0.0f : mc[j];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          bf16x4 h;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float p = exp2_(__builtin_fmaf(s[i][j][e], A.c, -base));
+            sum[j] += p;
+            h[e] = (__bf16)p;
+          }
+          pb[i][j] = __builtin_bit_cast(s16x4, h);
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        s16x4 vf[NB];
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+          vf[i] = read_turned(vb + (at + 16u * i + vrow) * DP + ((2u * d + ((lr & 3u) >> 1)) ^ vt) * 8u + (lr & 1u) * 4u);
+        if (edge && !J.pre && A.T > 1u) {
+          // A value that is no number times a weight of 0 would reach queries that
+          // do not see its position: those that do get it here, the products without.
+#pragma unroll
+          for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const bool odd = (vf[i][e] & 0x7f80) == 0x7f80;
+              unsigned long long b = __builtin_amdgcn_ballot_w64(odd);
+              const uint32_t bits = (uint32_t)(uint16_t)vf[i][e] << 16;
+              if (odd) vf[i][e] = 0;
+              for (; b; b &= b - 1ull) {
+                const uint32_t src = (uint32_t)__builtin_ctzll(b);
+                const float v = __uint_as_float(__builtin_amdgcn_readlane(bits, src));
+                const uint32_t p = p0 + at + 16u * i + 4u * (src >> 4) + e, dd = src & 15u;
+#pragma unroll
+                for (int j = 0; j < RB; ++j)
+#pragma unroll
+                  for (int x = 0; x < 4; ++x)
+                    if (p < lim[j] && dd == 4u * lg + x) acc[d][j][x] += v;
+              }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < RB; ++j) {
+          if constexpr (NB == 2) {
+            const s16x8 v8 = __builtin_shufflevector(vf[0], vf[1], 0, 1, 2, 3, 4, 5, 6, 7);
+            const s16x8 p8 = __builtin_shufflevector(pb[0][j], pb[1][j], 0, 1, 2, 3, 4, 5, 6, 7);
+            acc[d][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v8), __builtin_bit_cast(bf16x8, p8), acc[d][j], 0, 0, 0);
+          } else {
+            acc[d][j] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf[0], pb[0][j], acc[d][j], 0, 0, 0);
+          }
+        }
+      }
+    }
+  };
+
+#pragma unroll
+  for (uint32_t t = 0; t < (uint32_t)S - 1u; ++t)
+    if (t < nt) {
+      fetch(t, J.k, Ks + t * TE, true);
+      fetch(t, J.v, Vs + t * TE, false);
+    }
+  uint32_t cur = 0u, nxt = S - 1u;
+  for (uint32_t t = 0; t < nt; ++t) {
+    const uint32_t after = nt - 1u - t;   // tiles still in flight, at most S - 2
+    if (S > 3 && after >= 2u) att_barrier<4 * LD>();
+    else if (S > 2 && after >= 1u) att_barrier<2 * LD>();
+    else att_barrier<0>();
+    const uint32_t p0 = J.a + t * ATT_TILE;
+    if (t + (uint32_t)S - 1u < nt) {
+      fetch(t + S - 1u, J.k, Ks + nxt * TE, true);
+      fetch(t + S - 1u, J.v, Vs + nxt * TE, false);
+    }
+    if (J.b - p0 < ATT_TILE) {   // values past the end: 0, so that their weights of 0 give 0
+      const uint32_t have = J.b - p0;
+      for (uint32_t i = have * PR + threadIdx.x; i < ATT_TILE * PR; i += NW * 64) reinterpret_cast<bf16x8*>(Vs + cur * TE)[i] = bf16x8{};
+      att_barrier<0>();
+    }
+    compute(Ks + cur * TE, Vs + cur * TE, p0);
+    cur = cur + 1u == (uint32_t)S ? 0u : cur + 1u;
+    nxt = nxt + 1u == (uint32_t)S ? 0u : nxt + 1u;
+  }
+#pragma unroll
+  for (int j = 0; j < RB; ++j) sum[j] = sum4(sum[j]);
+
+  // Waves that took different positions of the same queries meet in LDS.
+  if constexpr (WP > 1) {
+    static_assert((WP / 2) * WQ * 16 * RB * DP * 4 <= 2 * S * (int)TE * 2, "the halves fit");
+    f32x4* const room = reinterpret_cast<f32x4*>(Ks);
+#pragma unroll
+    for (int half = WP / 2; half > 0; half /= 2) {
+      att_barrier<0>();
+      // (Ks and Vs are one array of LDS)
+      const uint32_t pair = (wp % (uint32_t)half) * WQ + wq;
+      f32x4* const at = room + pair * (RB * DB * 64u) + l;
+      float2* const st = stats + pair * (RB * 64u) + l;
+      if (wp >= (uint32_t)half && wp < 2u * half) {
+#pragma unroll
+        for (int j = 0; j < RB; ++j) {
+          st[j * 64u] = make_float2(mc[j], sum[j]);
+#pragma unroll
+          for (int d = 0; d < DB; ++d) at[(j * DB + d) * 64u] = acc[d][j];
+        }
+      }
+      att_barrier<0>();
+      if (wp < (uint32_t)half) {
+#pragma unroll
+        for (int j = 0; j < RB; ++j) {
+          const float2 o = st[j * 64u];
+          const float m = fmaxf(mc[j], o.x);
+          const float fa = share_of(mc[j], m), fb = share_of(o.x, m);
+          mc[j] = m;
+          sum[j] = sum[j] * fa + o.y * fb;
+#pragma unroll
+          for (int d = 0; d < DB; ++d) acc[d][j] = acc[d][j] * fa + at[(j * DB + d) * 64u] * fb;
+        }
+      }
+    }
+    if (wp > 0u) return;
+  }
+#pragma unroll
+  for (int j = 0; j < RB; ++j) {
+    const uint32_t m = m0 + 16u * j + lr;
+    if (m >= J.m) continue;
+    const AttQuery x = att_query(A, J, m);
+    const uint64_t id = (uint64_t)J.slot * A.NQ + ((uint64_t)x.row * A.nt + x.t - A.t0) * A.H + x.h;
+    if (lg == 0u) A.stat[id] = make_float2(mc[j], sum[j]);
+#pragma unroll
+    for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4*>(A.part + id * DP + 16u * d + 4u * lg) = acc[d][j];
   }
 }
 
-// One thread a position.
-template <bool PRE>
-__global__ __launch_bounds__(256) void attention_weight_kernel(AttArgs A, uint32_t g0, uint32_t ng) {
-  const uint32_t n = PRE ? A.P : A.N;
-  const uint64_t id = (uint64_t)blockIdx.x * 256u + threadIdx.x;
-  const uint32_t i = (uint32_t)(id % n), kv = (uint32_t)(id / n % A.KV), seg = (PRE ? g0 : A.r0) + (uint32_t)(id / n / A.KV);
-  if (seg >= (PRE ? g0 + ng : A.r0 + A.nr)) return;
-  const uint32_t len = PRE ? att_len(A.plen, seg, A.P) : att_len(A.len, seg, A.N);
-  if (i >= len) return;
-  const __bf16* const kk = PRE ? A.pk + seg * A.pg + kv * A.ph + (uint64_t)i * A.pp : A.k + seg * A.kr + kv * A.kh + (uint64_t)i * A.kp;
-  const uint32_t ra = PRE ? max(seg * A.W, A.r0) : seg, rb = PRE ? min((seg + 1u) * A.W, A.r0 + A.nr) : seg + 1u, per = A.H / A.KV;
-  float add = 0.0f;
-  for (uint32_t r = ra; r < rb; ++r)
-    for (uint32_t t = A.t0; t < A.t0 + A.nt; ++t) {
-      if (!PRE && i >= att_seen(len, A.T, t)) continue;
-      for (uint32_t h = kv * per; h < (kv + 1u) * per; ++h) {
-        const __bf16* const q = A.q + r * A.qr + t * A.qt + h * A.qh;
-        float s = 0.0f;
-        for (uint32_t d = 0; d < A.D; ++d) s += (float)q[d] * (float)kk[d];
-        const float lse = A.own[((uint64_t)(r - A.r0) * A.nt + t - A.t0) * A.H + h];
-        s *= A.scale;
-        if (lse != -INFINITY) add += expf(s - lse);
+template <int DP, int RB, int WQ, bool SMALL, int S>
+__global__ __launch_bounds__(256, WQ == 1 ? 2 : 1) void attention_tile_kernel(AttArgs A) {
+  __shared__ __align__(1024) __bf16 tiles[2][S * ATT_TILE * DP];
+  __shared__ float2 stats[2 * RB * 64];   // (the waves that meet, at most two at a time)
+  // XCD x (workgroups go to the XCDs in turn) takes a contiguous range of the jobs.
+  const uint32_t per = gridDim.x / 8u, job = (blockIdx.x & 7u) * per + (blockIdx.x >> 3);
+  if (job >= A.njobs) return;
+  AttJob J;
+  J.pre = job < A.np;
+  if (J.pre) {   // blocks of queries together: they read the same positions
+    uint32_t i = job;
+    const uint32_t blk = i % A.nrb;
+    i /= A.nrb;
+    J.slot = i % A.sp;
+    i /= A.sp;
+    J.kv = i % A.KV;
+    J.g = i / A.KV;
+    J.m0 = blk * (16u * RB * WQ);
+    J.m = A.wb * A.nt * A.per;
+    const uint32_t g = A.g0 + J.g, len = att_len(A.plen, g, A.P);
+    const uint64_t at = g * A.pg + J.kv * A.ph;
+    J.k = A.pk + at, J.v = A.pv + at, J.stride = A.pp;
+    const uint32_t tiles_all = (len + ATT_TILE - 1u) / ATT_TILE, each = (tiles_all + A.sp - 1u) / A.sp * ATT_TILE;
+    J.a = min(len, J.slot * each), J.b = min(len, J.a + each);
+    J.row = 0u, J.len = 0u;
+    attention_job<DP, RB, WQ, 4 / WQ, S>(A, J, tiles[0], tiles[1], stats);
+    return;
+  }
+  uint32_t i = job - A.np;
+  const uint32_t blk = i % A.nsb;
+  i /= A.nsb;
+  const uint32_t part = i % A.ss;
+  i /= A.ss;
+  J.kv = i % A.KV;
+  const uint32_t row = i / A.KV;
+  J.g = row / A.wb, J.row = row - J.g * A.wb;
+  J.slot = A.sp + part;
+  J.m0 = blk * (SMALL ? 16u : 16u * RB * WQ);
+  J.m = A.nt * A.per;
+  const uint32_t r = att_row(A, row);
+  J.len = att_len(A.len, r, A.N);
+  const uint64_t at = r * A.kr + J.kv * A.kh;
+  J.k = A.k + at, J.v = A.v + at, J.stride = A.kp;
+  const uint32_t end = min(J.len, att_seen(J.len, A.T, A.t0 + A.nt - 1u));   // of the last token here
+  const uint32_t tiles_all = (end + ATT_TILE - 1u) / ATT_TILE, each = (tiles_all + A.ss - 1u) / A.ss * ATT_TILE;
+  J.a = min(end, part * each), J.b = min(end, J.a + each);
+  if constexpr (SMALL) attention_job<DP, 1, 1, 4, S>(A, J, tiles[0], tiles[1], stats);
+  else attention_job<DP, RB, WQ, 4 / WQ, S>(A, J, tiles[0], tiles[1], stats);
+}
+
+// A query's parts: their common reference and the reciprocal of the sum.
+struct AttTotal {
+  float m, sum;
+};
+__device__ __forceinline__ AttTotal att_total(const AttArgs& A, uint32_t id) {
+  float m = -INFINITY, sum = 0.0f;
+  for (uint32_t s = 0; s < A.slots; ++s) m = fmaxf(m, A.stat[(uint64_t)s * A.NQ + id].x);
+  for (uint32_t s = 0; s < A.slots; ++s) {
+    const float2 v = A.stat[(uint64_t)s * A.NQ + id];
+    sum += v.y * (v.x == m ? 1.0f : share_of(v.x, m));   // (a sum that is NaN stays)
+  }
+  return {m, sum};
+}
+
+// Joins the parts: DP / 4 lanes a query, four elements each.
+template <int DP>
+__device__ __forceinline__ void attention_join(const AttArgs& A, uint32_t block) {
+  constexpr uint32_t LQ = DP / 4;
+  const uint32_t id = block * (256u / LQ) + threadIdx.x / LQ, d = threadIdx.x % LQ * 4u;
+  if (id >= A.NQ) return;
+  const AttTotal x = att_total(A, id);
+  f32x4 o = {};
+  for (uint32_t s = 0; s < A.slots; ++s) {
+    const float2 v = A.stat[(uint64_t)s * A.NQ + id];
+    if (v.y == 0.0f) continue;   // (a part that has seen nothing)
+    const float f = v.x == x.m ? 1.0f : share_of(v.x, x.m);
+    o += *reinterpret_cast<const f32x4*>(A.part + ((uint64_t)s * A.NQ + id) * DP + d) * f;
+  }
+  const uint32_t h = id % A.H, t = A.t0 + id / A.H % A.nt, r = att_row(A, id / A.H / A.nt);
+  if (d == 0u) {
+    const float ref = x.m + __log2f(x.sum);
+    if (A.ref) A.ref[id] = x.sum == 0.0f ? INFINITY : ref;
+    if (A.lse) A.lse[((uint64_t)r * A.T + t) * A.H + h] = x.sum == 0.0f ? -INFINITY : ref * 0.693147181f;
+  }
+  const float inv = x.sum == 0.0f ? 0.0f : 1.0f / x.sum;
+  if (d < A.D) {
+    bf16x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (__bf16)(o[e] * inv);
+    *reinterpret_cast<bf16x4*>(A.out + (uint64_t)r * A.orow + t * A.ot + h * A.oh + d) = v;
+  }
+}
+
+template <int DP>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttArgs A) { attention_join<DP>(A, blockIdx.x); }
+
+// The weights of 64 positions of a cache head: the scores once more, a wave's
+// positions in registers, all queries that read them in turn.
+template <int DP>
+__global__ __launch_bounds__(256) void attention_weight_kernel(AttArgs A, uint32_t tp, uint32_t ts, uint64_t jobs_p, uint64_t jobs) {
+  constexpr int KS = DP / 32;
+  const uint32_t l = threadIdx.x & 63u, lr = l & 15u, lg = l >> 4;
+  for (uint64_t job = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6); job < jobs; job += (uint64_t)gridDim.x * 4u) {
+    const bool pre = job < jobs_p;
+    uint64_t i = pre ? job : job - jobs_p;
+    const uint32_t tile = (uint32_t)(i % (pre ? tp : ts));
+    i /= pre ? tp : ts;
+    AttJob J;
+    J.pre = pre;
+    J.kv = (uint32_t)(i % A.KV);
+    const uint32_t seg = (uint32_t)(i / A.KV);   // group, or row, within the launch
+    J.g = pre ? seg : seg / A.wb;
+    J.row = pre ? 0u : seg - J.g * A.wb;
+    const uint32_t r = pre ? A.g0 + seg : att_row(A, seg);
+    const uint32_t len = pre ? att_len(A.plen, r, A.P) : att_len(A.len, r, A.N), p0 = tile * 32u;
+    if (p0 >= len) continue;
+    const uint64_t stride = pre ? A.pp : A.kp;
+    const __bf16* const kb = pre ? A.pk + r * A.pg + J.kv * A.ph : A.k + r * A.kr + J.kv * A.kh;
+    bf16x8 kf[2][KS];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const __bf16* const from = kb + (uint64_t)min(p0 + 16u * b + lr, len - 1u) * stride;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const uint32_t d = 32u * s + 8u * lg;
+        kf[b][s] = d < A.D ? *reinterpret_cast<const bf16x8*>(from + d) : bf16x8{};
       }
     }
-  float* const to = PRE ? &A.pw[((uint64_t)seg * A.KV + kv) * A.P + i] : &A.w[((uint64_t)seg * A.KV + kv) * A.N + i];
-  *to += add;
+    const uint32_t M = (pre ? A.wb : 1u) * A.nt * A.per;
+    f32x4 add[2] = {};
+    for (uint32_t m0 = 0; m0 < M; m0 += 16u) {
+      const uint32_t m = m0 + lr;
+      bf16x8 q[KS];
+      float ref = INFINITY;    // log2 of the query's whole sum; nothing for a query past the last
+      uint32_t lim = 0u;
+      if (m < M) {
+        const AttQuery x = att_query(A, J, m);
+        const __bf16* const from = A.q + (uint64_t)att_row(A, x.row) * A.qr + x.t * A.qt + x.h * A.qh;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const uint32_t d = 32u * s + 8u * lg;
+          q[s] = d < A.D ? flipped(*reinterpret_cast<const bf16x8*>(from + d), A.flip) : bf16x8{};
+        }
+        ref = A.ref[(x.row * A.nt + x.t - A.t0) * A.H + x.h];
+        lim = pre ? len : min(len, att_seen(len, A.T, x.t));
+      } else {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) q[s] = bf16x8{};
+      }
+      f32x4 s2[2] = {};
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) s2[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[b][s], q[s], s2[b], 0, 0, 0);
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p = exp2_(__builtin_fmaf(s2[b][e], A.c, -ref));
+          if (p0 + 16u * b + 4u * lg + e < lim) add[b][e] += p;
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float v = add[b][e];
+        v += __shfl_xor(v, 1);
+        v += __shfl_xor(v, 2);
+        v += __shfl_xor(v, 4);
+        v += __shfl_xor(v, 8);
+        add[b][e] = v;
+      }
+    if (lr == 0u) {
+      float* const to = (pre ? A.pw + ((uint64_t)r * A.KV + J.kv) * A.P : A.w + ((uint64_t)r * A.KV + J.kv) * A.N) + p0;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t p = 16u * b + 4u * lg + e;
+          if (p0 + p < len) to[p] += add[b][e];
+        }
+    }
+  }
 }
 
 size_t attention_scratch_bytes() { return ATT_SCRATCH; }
 
-static void attention_slice(hipStream_t st, const AttArgs& A) {
-  hipLaunchKernelGGL(attention_simple_kernel, dim3(A.nr * A.nt * A.H), dim3(256), 0, st, A);
-  if (A.pw) {
-    const uint32_t g0 = A.r0 / A.W, ng = (A.r0 + A.nr - 1u) / A.W + 1u - g0;
-    hipLaunchKernelGGL(attention_weight_kernel<true>, dim3((uint32_t)(((uint64_t)ng * A.KV * A.P + 255u) / 256u)), dim3(256), 0, st, A, g0, ng);
+template <int DP, int RB, int WQ, int S>
+static void att_go(hipStream_t st, const AttArgs& A, bool small) {
+  const dim3 grid((A.njobs + 7u) / 8u * 8u), block(256);
+  if (small) hipLaunchKernelGGL((attention_tile_kernel<DP, RB, WQ, true, S>), grid, block, 0, st, A);
+  else hipLaunchKernelGGL((attention_tile_kernel<DP, RB, WQ, false, S>), grid, block, 0, st, A);
+}
+
+template <int DP>
+static void attention_launch(hipStream_t st, const AttArgs& A, const AttPlan& p) {
+  constexpr int S = DP == 64 ? 4 : 2, RL = DP == 256 ? 2 : 4;
+  if (A.njobs) {
+    if (p.rb == 1u) att_go<DP, 1, 1, S>(st, A, p.small);
+    else if (p.rb == 2u && p.wq == 1u) att_go<DP, 2, 1, S>(st, A, p.small);
+    else if (p.wq == 1u) att_go<DP, RL, 1, S>(st, A, p.small);
+    else if (p.wq == 2u) att_go<DP, RL, 2, S>(st, A, p.small);
+    else att_go<DP, RL, 4, S>(st, A, p.small);
   }
-  if (A.w)
-    hipLaunchKernelGGL(attention_weight_kernel<false>, dim3((uint32_t)(((uint64_t)A.nr * A.KV * A.N + 255u) / 256u)), dim3(256), 0, st, A, 0u, 0u);
+  const uint32_t a_block = 256u / (DP / 4u);
+  hipLaunchKernelGGL(attention_join_kernel<DP>, dim3((A.NQ + a_block - 1u) / a_block), dim3(256), 0, st, A);
+  const uint32_t tp = A.pw ? (A.P + 31u) / 32u : 0u, ts = A.w ? (A.N + 31u) / 32u : 0u;
+  const uint64_t jobs_p = (uint64_t)A.ng * A.KV * tp, jobs = jobs_p + (uint64_t)A.ng * A.wb * A.KV * ts;
+  if (jobs) {
+    const uint64_t blocks = (jobs + 3u) / 4u;
+    hipLaunchKernelGGL(attention_weight_kernel<DP>, dim3((uint32_t)(blocks < 1u << 20 ? blocks : 1u << 20)), dim3(256), 0, st, A, tp, ts, jobs_p, jobs);
+  }
 }
 
 }  // namespace mxs
@@ -151,24 +613,35 @@ extern "C" int mxs_prefix_attention(mxs_ctx* ctx, const mxs_attention* attention
   A.plen = a.prefix_lengths, A.len = a.lengths;
   A.lse = a.lse, A.pw = a.prefix_weight, A.w = a.weight;
   A.W = a.beams, A.T = a.tokens, A.H = a.heads, A.KV = a.kv_heads, A.D = a.dim, A.P = a.prefix, A.N = a.suffix;
-  A.scale = a.scale;
-  A.own = ctx->attention_scratch;
+  A.per = a.heads / a.kv_heads;
+  // scale log2(e); 0 becomes so little that no score shows it, since -inf times 0 is no number
+  A.c = fmaxf(fabsf(a.scale) * 1.44269504f, 1e-38f);
+  A.flip = a.scale < 0.0f ? 0x8000u : 0u;
+  const AttPlan p = attention_plan(a.groups, a.beams, a.tokens, a.heads, a.kv_heads, a.dim, a.prefix, a.suffix);
+  A.sp = p.sp, A.ss = p.ss, A.slots = p.slots;
   int prev = 0;
   (void)hipGetDevice(&prev);
   if (prev != ctx->device) (void)hipSetDevice(ctx->device);
-  // slices of whole rows, or of one row's tokens, whose queries fit the scratch and a launch
-  const uint64_t most = 1u << 20;
-  const uint32_t rows = a.groups * a.beams;
-  const uint32_t nt = (uint32_t)(a.tokens < most / a.heads ? a.tokens : most / a.heads);
-  const uint32_t nr = nt < a.tokens ? 1u : (uint32_t)(most / ((uint64_t)nt * a.heads));
   hipError_t e = hipSuccess;
-  for (A.r0 = 0; A.r0 < rows && e == hipSuccess; A.r0 += nr)
-    for (A.t0 = 0; A.t0 < a.tokens && e == hipSuccess; A.t0 += nt) {
-      A.nr = rows - A.r0 < nr ? rows - A.r0 : nr;
-      A.nt = a.tokens - A.t0 < nt ? a.tokens - A.t0 : nt;
-      attention_slice(ctx->stream, A);
-      e = hipGetLastError();
-    }
+  for (uint32_t g = 0; g < a.groups && e == hipSuccess; g += p.ng)
+    for (uint32_t b = 0; b < a.beams && e == hipSuccess; b += p.wb)
+      for (uint32_t t = 0; t < a.tokens && e == hipSuccess; t += p.nt) {
+        A.g0 = g, A.ng = a.groups - g < p.ng ? a.groups - g : p.ng;
+        A.b0 = b, A.wb = a.beams - b < p.wb ? a.beams - b : p.wb;
+        A.t0 = t, A.nt = a.tokens - t < p.nt ? a.tokens - t : p.nt;
+        A.NQ = A.ng * A.wb * A.nt * A.H;
+        const uint32_t rows = 16u * p.rb * p.wq, ms = A.nt * A.per;
+        A.nrb = att_ceil((uint64_t)A.wb * ms, rows), A.nsb = p.small ? 1u : att_ceil(ms, rows);
+        A.np = A.ng * A.KV * A.nrb * A.sp;
+        A.njobs = A.np + A.ng * A.wb * A.KV * A.nsb * A.ss;
+        A.stat = reinterpret_cast<float2*>(ctx->attention_scratch);
+        A.ref = A.pw || A.w ? ctx->attention_scratch + 2ull * A.slots * A.NQ : nullptr;
+        A.part = ctx->attention_scratch + ((2ull * A.slots + 1u) * A.NQ + 3u) / 4u * 4u;
+        if (p.dp == 64u) attention_launch<64>(ctx->stream, A, p);
+        else if (p.dp == 128u) attention_launch<128>(ctx->stream, A, p);
+        else attention_launch<256>(ctx->stream, A, p);
+        e = hipGetLastError();
+      }
   if (prev != ctx->device) (void)hipSetDevice(prev);
   if (e != hipSuccess) return hip_fail(ctx, e, "attention launch");
   return MXS_OK;
