@@ -121,11 +121,17 @@ __device__ __forceinline__ uint32_t att_row(const AttArgs& A, uint32_t row) {   
   return (A.g0 + row / A.wb) * A.W + A.b0 + row % A.wb;
 }
 
+struct AttEntry {
+  uint32_t id, lim;   // of the launch's queries (~0: none); positions below lim are seen
+  uint64_t at;        // its elements
+};
+
 // Scores as S^T = K Q^T on v_mfma_f32_16x16x32_bf16 (a lane holds four
 // positions of one query), sums as O^T = V^T P^T: the exponentials are the second
 // operand as they lie, values are read transposed from LDS.
 template <int DP, int RB, int WQ, int WP, int S>
-__device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J, __bf16* Ks, __bf16* Vs, float2* stats) {
+__device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J, __bf16* Ks, __bf16* Vs, float2* stats,
+                                              AttEntry* table, uint32_t* odd) {
   constexpr uint32_t PR = DP / 8, LR = 64 / PR;                  // 16-byte pieces of a row, rows a load takes
   constexpr int KS = DP / 32, DB = DP / 16, NW = WQ * WP;
   constexpr int PPW = ATT_TILE / WP, NB = PPW >= 32 ? 2 : 1, SUBS = PPW / (16 * NB);   // positions a wave takes of a tile
@@ -134,27 +140,32 @@ __device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J,
   static_assert(LD * (int)LR * NW == (int)ATT_TILE, "the loads cover the tile");
   const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63u, lr = l & 15u, lg = l >> 4;
   const uint32_t wq = w % WQ, wp = w / WQ;
-  const uint32_t m0 = J.m0 + wq * (16u * RB);
+  // What the block's queries are, worked out once.
+  if (threadIdx.x < 16u * RB * WQ) {
+    const uint32_t m = J.m0 + threadIdx.x;
+    AttEntry e{~0u, 0u, 0ull};
+    if (m < J.m) {
+      const AttQuery x = att_query(A, J, m);
+      e.id = (x.row * A.nt + x.t - A.t0) * A.H + x.h;
+      e.lim = J.pre ? J.b : min(J.b, att_seen(J.len, A.T, x.t));
+      e.at = (uint64_t)att_row(A, x.row) * A.qr + x.t * A.qt + x.h * A.qh;
+    }
+    table[threadIdx.x] = e;
+  }
+  if (threadIdx.x == 0) *odd = 0u;
+  __syncthreads();
 
   // the queries, a fragment of each for every 32 elements; and where each one's positions end
   bf16x8 q[RB][KS];
   uint32_t lim[RB], least = J.b;
 #pragma unroll
   for (int j = 0; j < RB; ++j) {
-    const uint32_t m = m0 + 16u * j + lr;
-    lim[j] = 0u;
-    if (m < J.m) {
-      const AttQuery x = att_query(A, J, m);
-      lim[j] = J.pre ? J.b : min(J.b, att_seen(J.len, A.T, x.t));
-      const __bf16* const from = A.q + (uint64_t)att_row(A, x.row) * A.qr + x.t * A.qt + x.h * A.qh;
+    const AttEntry e = table[(wq * RB + j) * 16u + lr];
+    lim[j] = e.lim;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const uint32_t d = 32u * s + 8u * lg;
-        q[j][s] = d < A.D ? flipped(*reinterpret_cast<const bf16x8*>(from + d), A.flip) : bf16x8{};
-      }
-    } else {
-#pragma unroll
-      for (int s = 0; s < KS; ++s) q[j][s] = bf16x8{};
+    for (int s = 0; s < KS; ++s) {
+      const uint32_t d = 32u * s + 8u * lg;
+      q[j][s] = d < A.D && e.id != ~0u ? flipped(*reinterpret_cast<const bf16x8*>(A.q + e.at + d), A.flip) : bf16x8{};
     }
   }
   if (!J.pre) least = min(J.b, att_seen(J.len, A.T, A.t0));   // (of the job's first token: none ends earlier)
@@ -263,29 +274,6 @@ __device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J,
 #pragma unroll
         for (int i = 0; i < NB; ++i)
           vf[i] = read_turned(vb + (at + 16u * i + vrow) * DP + ((2u * d + ((lr & 3u) >> 1)) ^ vt) * 8u + (lr & 1u) * 4u);
-        if (edge && !J.pre && A.T > 1u) {
-          // A value that is no number times a weight of 0 would reach queries that
-          // do not see its position: those that do get it here, the products without.
-#pragma unroll
-          for (int i = 0; i < NB; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const bool odd = (vf[i][e] & 0x7f80) == 0x7f80;
-              unsigned long long b = __builtin_amdgcn_ballot_w64(odd);
-              const uint32_t bits = (uint32_t)(uint16_t)vf[i][e] << 16;
-              if (odd) vf[i][e] = 0;
-              for (; b; b &= b - 1ull) {
-                const uint32_t src = (uint32_t)__builtin_ctzll(b);
-                const float v = __uint_as_float(__builtin_amdgcn_readlane(bits, src));
-                const uint32_t p = p0 + at + 16u * i + 4u * (src >> 4) + e, dd = src & 15u;
-#pragma unroll
-                for (int j = 0; j < RB; ++j)
-#pragma unroll
-                  for (int x = 0; x < 4; ++x)
-                    if (p < lim[j] && dd == 4u * lg + x) acc[d][j][x] += v;
-              }
-            }
-        }
 #pragma unroll
         for (int j = 0; j < RB; ++j) {
           if constexpr (NB == 2) {
@@ -317,9 +305,29 @@ __device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J,
       fetch(t + S - 1u, J.k, Ks + nxt * TE, true);
       fetch(t + S - 1u, J.v, Vs + nxt * TE, false);
     }
-    if (J.b - p0 < ATT_TILE) {   // values past the end: 0, so that their weights of 0 give 0
-      const uint32_t have = J.b - p0;
-      for (uint32_t i = have * PR + threadIdx.x; i < ATT_TILE * PR; i += NW * 64) reinterpret_cast<bf16x8*>(Vs + cur * TE)[i] = bf16x8{};
+    if (p0 + ATT_TILE > least) {
+      // Values that some queries do not see: those past the end become 0, and those
+      // that are no numbers too (their weight of 0 would not be 0 times them); the
+      // queries that do see these get them at the end.
+      const uint32_t have = min(ATT_TILE, J.b - p0);
+      const bool look = !J.pre && A.T > 1u;
+      for (uint32_t i = (look ? 0u : have * PR) + threadIdx.x; i < ATT_TILE * PR; i += NW * 64) {
+        s16x8* const at = reinterpret_cast<s16x8*>(Vs + cur * TE) + i;
+        s16x8 v = {};
+        if (i < have * PR) {
+          v = *at;
+          bool any = false;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const bool bad = (v[e] & 0x7f80) == 0x7f80;
+            any |= bad;
+            v[e] = bad ? 0 : v[e];
+          }
+          if (!any) continue;
+          *odd = 1u;
+        }
+        *at = v;
+      }
       att_barrier<0>();
     }
     compute(Ks + cur * TE, Vs + cur * TE, p0);
@@ -362,17 +370,32 @@ __device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J,
         }
       }
     }
-    if (wp > 0u) return;
   }
+  if (wp == 0u) {
 #pragma unroll
-  for (int j = 0; j < RB; ++j) {
-    const uint32_t m = m0 + 16u * j + lr;
-    if (m >= J.m) continue;
-    const AttQuery x = att_query(A, J, m);
-    const uint64_t id = (uint64_t)J.slot * A.NQ + ((uint64_t)x.row * A.nt + x.t - A.t0) * A.H + x.h;
-    if (lg == 0u) A.stat[id] = make_float2(mc[j], sum[j]);
+    for (int j = 0; j < RB; ++j) {
+      const uint32_t id = table[(wq * RB + j) * 16u + lr].id;
+      if (id == ~0u) continue;
+      const uint64_t to = (uint64_t)J.slot * A.NQ + id;
+      if (lg == 0u) A.stat[to] = make_float2(mc[j], sum[j]);
 #pragma unroll
-    for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4*>(A.part + id * DP + 16u * d + 4u * lg) = acc[d][j];
+      for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4*>(A.part + to * DP + 16u * d + 4u * lg) = acc[d][j];
+    }
+  }
+  if (!J.pre && A.T > 1u) {
+    __syncthreads();
+    if (*odd) {   // rare: values that are no numbers, added where they are seen
+      for (uint32_t i = threadIdx.x; i < 16u * RB * WQ * A.D; i += NW * 64) {
+        const AttEntry e = table[i / A.D];
+        if (e.id == ~0u) continue;
+        float add = 0.0f;
+        for (uint32_t p = max(J.a, least & ~(ATT_TILE - 1u)); p < e.lim; ++p) {
+          const float v = (float)J.v[p * J.stride + i % A.D];
+          if (!(fabsf(v) < INFINITY)) add += v;
+        }
+        A.part[((uint64_t)J.slot * A.NQ + e.id) * DP + i % A.D] += add;
+      }
+    }
   }
 }
 
@@ -380,6 +403,8 @@ template <int DP, int RB, int WQ, bool SMALL, int S>
 __global__ __launch_bounds__(256, WQ == 1 ? 2 : 1) void attention_tile_kernel(AttArgs A) {
   __shared__ __align__(1024) __bf16 tiles[2][S * ATT_TILE * DP];
   __shared__ float2 stats[2 * RB * 64];   // (the waves that meet, at most two at a time)
+  __shared__ AttEntry table[16 * RB * WQ];
+  __shared__ uint32_t odd;
   // XCD x (workgroups go to the XCDs in turn) takes a contiguous range of the jobs.
   const uint32_t per = gridDim.x / 8u, job = (blockIdx.x & 7u) * per + (blockIdx.x >> 3);
   if (job >= A.njobs) return;
@@ -401,7 +426,7 @@ __global__ __launch_bounds__(256, WQ == 1 ? 2 : 1) void attention_tile_kernel(At
     const uint32_t tiles_all = (len + ATT_TILE - 1u) / ATT_TILE, each = (tiles_all + A.sp - 1u) / A.sp * ATT_TILE;
     J.a = min(len, J.slot * each), J.b = min(len, J.a + each);
     J.row = 0u, J.len = 0u;
-    attention_job<DP, RB, WQ, 4 / WQ, S>(A, J, tiles[0], tiles[1], stats);
+    attention_job<DP, RB, WQ, 4 / WQ, S>(A, J, tiles[0], tiles[1], stats, table, &odd);
     return;
   }
   uint32_t i = job - A.np;
@@ -422,45 +447,53 @@ __global__ __launch_bounds__(256, WQ == 1 ? 2 : 1) void attention_tile_kernel(At
   const uint32_t end = min(J.len, att_seen(J.len, A.T, A.t0 + A.nt - 1u));   // of the last token here
   const uint32_t tiles_all = (end + ATT_TILE - 1u) / ATT_TILE, each = (tiles_all + A.ss - 1u) / A.ss * ATT_TILE;
   J.a = min(end, part * each), J.b = min(end, J.a + each);
-  if constexpr (SMALL) attention_job<DP, 1, 1, 4, S>(A, J, tiles[0], tiles[1], stats);
-  else attention_job<DP, RB, WQ, 4 / WQ, S>(A, J, tiles[0], tiles[1], stats);
+  if constexpr (SMALL) attention_job<DP, 1, 1, 4, S>(A, J, tiles[0], tiles[1], stats, table, &odd);
+  else attention_job<DP, RB, WQ, 4 / WQ, S>(A, J, tiles[0], tiles[1], stats, table, &odd);
 }
 
-// A query's parts: their common reference and the reciprocal of the sum.
-struct AttTotal {
-  float m, sum;
-};
-__device__ __forceinline__ AttTotal att_total(const AttArgs& A, uint32_t id) {
+// Joins a query's parts: NWV waves a query, each lane four elements of every
+// 256 NWV / DP-th part.
+template <int DP, int NWV>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttArgs A) {
+  constexpr uint32_t LQ = DP / 4, GR = NWV * 64 / LQ;
+  __shared__ f32x4 meet[4][LQ];
+  const uint32_t w = threadIdx.x >> 6, l = threadIdx.x & 63u;
+  const uint32_t id = min(blockIdx.x * (4u / NWV) + w / NWV, A.NQ - 1u);   // (a last workgroup's other waves: the last query once more)
+  const uint32_t in = w % NWV * 64u + l, d = in % LQ * 4u, grp = in / LQ;
+  // every wave by itself: the parts' common reference and the whole sum
   float m = -INFINITY, sum = 0.0f;
-  for (uint32_t s = 0; s < A.slots; ++s) m = fmaxf(m, A.stat[(uint64_t)s * A.NQ + id].x);
-  for (uint32_t s = 0; s < A.slots; ++s) {
+  for (uint32_t s = l; s < A.slots; s += 64u) m = fmaxf(m, A.stat[(uint64_t)s * A.NQ + id].x);
+  for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+  for (uint32_t s = l; s < A.slots; s += 64u) {
     const float2 v = A.stat[(uint64_t)s * A.NQ + id];
     sum += v.y * (v.x == m ? 1.0f : share_of(v.x, m));   // (a sum that is NaN stays)
   }
-  return {m, sum};
-}
-
-// Joins the parts: DP / 4 lanes a query, four elements each.
-template <int DP>
-__device__ __forceinline__ void attention_join(const AttArgs& A, uint32_t block) {
-  constexpr uint32_t LQ = DP / 4;
-  const uint32_t id = block * (256u / LQ) + threadIdx.x / LQ, d = threadIdx.x % LQ * 4u;
-  if (id >= A.NQ) return;
-  const AttTotal x = att_total(A, id);
+  for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
   f32x4 o = {};
-  for (uint32_t s = 0; s < A.slots; ++s) {
-    const float2 v = A.stat[(uint64_t)s * A.NQ + id];
-    if (v.y == 0.0f) continue;   // (a part that has seen nothing)
-    const float f = v.x == x.m ? 1.0f : share_of(v.x, x.m);
-    o += *reinterpret_cast<const f32x4*>(A.part + ((uint64_t)s * A.NQ + id) * DP + d) * f;
+#pragma unroll 4
+  for (uint32_t s = grp; s < A.slots; s += GR) {
+    const float x = A.stat[(uint64_t)s * A.NQ + id].x;
+    o += *reinterpret_cast<const f32x4*>(A.part + ((uint64_t)s * A.NQ + id) * DP + d) * (x == m ? 1.0f : share_of(x, m));
   }
+#pragma unroll
+  for (uint32_t x = LQ; x < 64u; x <<= 1)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], x);
+  if constexpr (NWV > 1) {
+    if (l < LQ) meet[w][l] = o;
+    __syncthreads();
+    if (w % NWV) return;
+#pragma unroll
+    for (uint32_t x = 1; x < (uint32_t)NWV; ++x) o += meet[w + x][l % LQ];
+  }
+  if (l >= LQ) return;
   const uint32_t h = id % A.H, t = A.t0 + id / A.H % A.nt, r = att_row(A, id / A.H / A.nt);
-  if (d == 0u) {
-    const float ref = x.m + __log2f(x.sum);
-    if (A.ref) A.ref[id] = x.sum == 0.0f ? INFINITY : ref;
-    if (A.lse) A.lse[((uint64_t)r * A.T + t) * A.H + h] = x.sum == 0.0f ? -INFINITY : ref * 0.693147181f;
+  if (l == 0u) {
+    const float ref = m + __log2f(sum);
+    if (A.ref) A.ref[id] = sum == 0.0f ? INFINITY : ref;
+    if (A.lse) A.lse[((uint64_t)r * A.T + t) * A.H + h] = sum == 0.0f ? -INFINITY : ref * 0.693147181f;
   }
-  const float inv = x.sum == 0.0f ? 0.0f : 1.0f / x.sum;
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   if (d < A.D) {
     bf16x4 v;
 #pragma unroll
@@ -468,9 +501,6 @@ __device__ __forceinline__ void attention_join(const AttArgs& A, uint32_t block)
     *reinterpret_cast<bf16x4*>(A.out + (uint64_t)r * A.orow + t * A.ot + h * A.oh + d) = v;
   }
 }
-
-template <int DP>
-__global__ __launch_bounds__(256) void attention_join_kernel(AttArgs A) { attention_join<DP>(A, blockIdx.x); }
 
 // The weights of 64 positions of a cache head: the scores once more, a wave's
 // positions in registers, all queries that read them in turn.
@@ -581,8 +611,8 @@ static void attention_launch(hipStream_t st, const AttArgs& A, const AttPlan& p)
     else if (p.wq == 2u) att_go<DP, RL, 2, S>(st, A, p.small);
     else att_go<DP, RL, 4, S>(st, A, p.small);
   }
-  const uint32_t a_block = 256u / (DP / 4u);
-  hipLaunchKernelGGL(attention_join_kernel<DP>, dim3((A.NQ + a_block - 1u) / a_block), dim3(256), 0, st, A);
+  if (A.slots > 16u) hipLaunchKernelGGL((attention_join_kernel<DP, 4>), dim3(A.NQ), dim3(256), 0, st, A);
+  else hipLaunchKernelGGL((attention_join_kernel<DP, 1>), dim3((A.NQ + 3u) / 4u), dim3(256), 0, st, A);
   const uint32_t tp = A.pw ? (A.P + 31u) / 32u : 0u, ts = A.w ? (A.N + 31u) / 32u : 0u;
   const uint64_t jobs_p = (uint64_t)A.ng * A.KV * tp, jobs = jobs_p + (uint64_t)A.ng * A.wb * A.KV * ts;
   if (jobs) {
