@@ -134,46 +134,12 @@ __device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J,
                                               AttEntry* table, uint32_t* odd) {
   constexpr uint32_t PR = DP / 8, LR = 64 / PR;                  // 16-byte pieces of a row, rows a load takes
   constexpr int KS = DP / 32, DB = DP / 16, NW = WQ * WP;
-  constexpr int PPW = ATT_TILE / WP, NB = PPW >= 32 ? 2 : 1, SUBS = PPW / (16 * NB);   // positions a wave takes of a tile
+  constexpr int PPW = ATT_TILE / WP, NB = PPW / 16;              // positions a wave takes of a tile, blocks of 16
   constexpr int LD = ATT_TILE / (int)LR / NW;                    // loads a wave issues for keys, and for values
   constexpr uint32_t TE = ATT_TILE * DP;                         // elements of a tile
   static_assert(LD * (int)LR * NW == (int)ATT_TILE, "the loads cover the tile");
   const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63u, lr = l & 15u, lg = l >> 4;
   const uint32_t wq = w % WQ, wp = w / WQ;
-  // What the block's queries are, worked out once.
-  if (threadIdx.x < 16u * RB * WQ) {
-    const uint32_t m = J.m0 + threadIdx.x;
-    AttEntry e{~0u, 0u, 0ull};
-    if (m < J.m) {
-      const AttQuery x = att_query(A, J, m);
-      e.id = (x.row * A.nt + x.t - A.t0) * A.H + x.h;
-      e.lim = J.pre ? J.b : min(J.b, att_seen(J.len, A.T, x.t));
-      e.at = (uint64_t)att_row(A, x.row) * A.qr + x.t * A.qt + x.h * A.qh;
-    }
-    table[threadIdx.x] = e;
-  }
-  if (threadIdx.x == 0) *odd = 0u;
-  __syncthreads();
-
-  // the queries, a fragment of each for every 32 elements; and where each one's positions end
-  bf16x8 q[RB][KS];
-  uint32_t lim[RB], least = J.b;
-#pragma unroll
-  for (int j = 0; j < RB; ++j) {
-    const AttEntry e = table[(wq * RB + j) * 16u + lr];
-    lim[j] = e.lim;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const uint32_t d = 32u * s + 8u * lg;
-      q[j][s] = d < A.D && e.id != ~0u ? flipped(*reinterpret_cast<const bf16x8*>(A.q + e.at + d), A.flip) : bf16x8{};
-    }
-  }
-  if (!J.pre) least = min(J.b, att_seen(J.len, A.T, A.t0));   // (of the job's first token: none ends earlier)
-
-  f32x4 acc[DB][RB] = {};
-  float mc[RB], sum[RB];   // reference (log2) and sum of each query, the sum of this lane's positions
-#pragma unroll
-  for (int j = 0; j < RB; ++j) mc[j] = -INFINITY, sum[j] = 0.0f;
 
   const uint32_t nt = J.b > J.a ? (J.b - J.a + ATT_TILE - 1u) / ATT_TILE : 0u;
   if (A.D < DP && nt) {   // elements past dim are never loaded: zero
@@ -197,103 +163,137 @@ __device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J,
         att_load_lds(to + (w * LD + i) * LR * DP, base, (min(row, have - 1u) * (uint32_t)J.stride + piece * 8u) * 2u, 0u);
     }
   };
-  const uint32_t kt = turn_k(lr);   // (rows of a fragment: lr more than a multiple of 16)
-  const uint32_t vrow = 4u * lg + (lr >> 2), vt = turn_v(vrow);
-
-  auto compute = [&](const __bf16* __restrict__ kb, const __bf16* __restrict__ vb, uint32_t p0) __attribute__((always_inline)) {
-#pragma unroll
-    for (int sub = 0; sub < SUBS; ++sub) {
-      const uint32_t at = wp * PPW + sub * (16u * NB);   // first position within the tile
-      f32x4 s[NB][RB] = {};
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        bf16x8 kf[NB];
-#pragma unroll
-        for (int i = 0; i < NB; ++i)
-          kf[i] = *reinterpret_cast<const bf16x8*>(kb + (at + 16u * i + lr) * DP + ((4u * ks + lg) ^ kt) * 8u);
-#pragma unroll
-        for (int i = 0; i < NB; ++i)
-#pragma unroll
-          for (int j = 0; j < RB; ++j) s[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i], q[j][ks], s[i][j], 0, 0, 0);
-      }
-      const uint32_t first = p0 + at + 4u * lg;
-      const bool edge = p0 + at + 16u * NB > least;   // uniform: some query sees not all of these
-      if (edge) {
-#pragma unroll
-        for (int i = 0; i < NB; ++i)
-#pragma unroll
-          for (int j = 0; j < RB; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (first + 16u * i + e >= lim[j]) s[i][j][e] = -INFINITY;
-      }
-      // The reference follows the maximum only where that is 2^8 above it, which
-      // the first tiles settle: no exchange between lanes and no rescaling otherwise.
-      float top[RB];
-      bool grow = false;
-#pragma unroll
-      for (int j = 0; j < RB; ++j) {
-        float t = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < NB; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) t = fmaxf(t, s[i][j][e]);
-        top[j] = t;
-        grow |= t * A.c > mc[j] + 8.0f;
-      }
-      if (__builtin_amdgcn_ballot_w64(grow)) {
-#pragma unroll
-        for (int j = 0; j < RB; ++j) {
-          const float m = fmaxf(mc[j], max4(top[j]) * A.c);
-          const float f = m == mc[j] ? 1.0f : share_of(mc[j], m);
-          mc[j] = m;
-          sum[j] *= f;
-#pragma unroll
-          for (int d = 0; d < DB; ++d) acc[d][j] *= f;
-        }
-      }
-      s16x4 pb[NB][RB];
-#pragma unroll
-      for (int j = 0; j < RB; ++j) {
-        const float base = mc[j] == -INFINITY ? 0.0f : mc[j];
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          bf16x4 h;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float p = exp2_(__builtin_fmaf(s[i][j][e], A.c, -base));
-            sum[j] += p;
-            h[e] = (__bf16)p;
-          }
-          pb[i][j] = __builtin_bit_cast(s16x4, h);
-        }
-      }
-#pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        s16x4 vf[NB];
-#pragma unroll
-        for (int i = 0; i < NB; ++i)
-          vf[i] = read_turned(vb + (at + 16u * i + vrow) * DP + ((2u * d + ((lr & 3u) >> 1)) ^ vt) * 8u + (lr & 1u) * 4u);
-#pragma unroll
-        for (int j = 0; j < RB; ++j) {
-          if constexpr (NB == 2) {
-            const s16x8 v8 = __builtin_shufflevector(vf[0], vf[1], 0, 1, 2, 3, 4, 5, 6, 7);
-            const s16x8 p8 = __builtin_shufflevector(pb[0][j], pb[1][j], 0, 1, 2, 3, 4, 5, 6, 7);
-            acc[d][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v8), __builtin_bit_cast(bf16x8, p8), acc[d][j], 0, 0, 0);
-          } else {
-            acc[d][j] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf[0], pb[0][j], acc[d][j], 0, 0, 0);
-          }
-        }
-      }
-    }
-  };
-
+  // The first tiles' loads are under way while the queries are found.
 #pragma unroll
   for (uint32_t t = 0; t < (uint32_t)S - 1u; ++t)
     if (t < nt) {
       fetch(t, J.k, Ks + t * TE, true);
       fetch(t, J.v, Vs + t * TE, false);
     }
+  // What the block's queries are, worked out once.
+  if (threadIdx.x < 16u * RB * WQ) {
+    const uint32_t m = J.m0 + threadIdx.x;
+    AttEntry e{~0u, 0u, 0ull};
+    if (m < J.m) {
+      const AttQuery x = att_query(A, J, m);
+      e.id = (x.row * A.nt + x.t - A.t0) * A.H + x.h;
+      e.lim = J.pre ? J.b : min(J.b, att_seen(J.len, A.T, x.t));
+      e.at = (uint64_t)att_row(A, x.row) * A.qr + x.t * A.qt + x.h * A.qh;
+    }
+    table[threadIdx.x] = e;
+  }
+  if (threadIdx.x == 0) *odd = 0u;
+  att_barrier<63>();
+
+  // the queries, a fragment of each for every 32 elements; and where each one's positions end
+  bf16x8 q[RB][KS];
+  uint32_t lim[RB], least = J.b;
+#pragma unroll
+  for (int j = 0; j < RB; ++j) {
+    const AttEntry e = table[(wq * RB + j) * 16u + lr];
+    lim[j] = e.lim;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) q[j][s] = *reinterpret_cast<const bf16x8*>(A.q + e.at + min(32u * s + 8u * lg, A.D - 8u));
+  }
+#pragma unroll
+  for (int j = 0; j < RB; ++j)
+#pragma unroll
+    for (int s = 0; s < KS; ++s) q[j][s] = 32u * s + 8u * lg < A.D ? flipped(q[j][s], A.flip) : bf16x8{};
+  if (!J.pre) least = min(J.b, att_seen(J.len, A.T, A.t0));   // (of the job's first token: none ends earlier)
+
+  f32x4 acc[DB][RB] = {};
+  float mc[RB], sum[RB];   // reference (log2) and sum of each query, the sum of this lane's positions
+#pragma unroll
+  for (int j = 0; j < RB; ++j) mc[j] = -INFINITY, sum[j] = 0.0f;
+  const uint32_t kt = turn_k(lr);   // (rows of a fragment: lr more than a multiple of 16)
+  const uint32_t vrow = 4u * lg + (lr >> 2), vt = turn_v(vrow);
+
+  auto compute = [&](const __bf16* __restrict__ kb, const __bf16* __restrict__ vb, uint32_t p0) __attribute__((always_inline)) {
+    const uint32_t at = wp * PPW;   // first position within the tile
+    f32x4 s[NB][RB] = {};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      bf16x8 kf[NB];
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+        kf[i] = *reinterpret_cast<const bf16x8*>(kb + (at + 16u * i + lr) * DP + ((4u * ks + lg) ^ kt) * 8u);
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int j = 0; j < RB; ++j) s[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i], q[j][ks], s[i][j], 0, 0, 0);
+    }
+    const uint32_t first = p0 + at + 4u * lg;
+    if (p0 + at + 16u * NB > least) {   // uniform: some query sees not all of these
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int j = 0; j < RB; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (first + 16u * i + e >= lim[j]) s[i][j][e] = -INFINITY;
+    }
+    // The reference follows the maximum only where that is 2^8 above it, which
+    // the first tiles settle: no exchange between lanes and no rescaling otherwise.
+    float top[RB];
+    bool grow = false;
+#pragma unroll
+    for (int j = 0; j < RB; ++j) {
+      float t = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t = fmaxf(t, s[i][j][e]);
+      top[j] = t;
+      grow |= t * A.c > mc[j] + 8.0f;
+    }
+    if (__builtin_amdgcn_ballot_w64(grow)) {
+#pragma unroll
+      for (int j = 0; j < RB; ++j) {
+        const float m = fmaxf(mc[j], max4(top[j]) * A.c);
+        const float f = m == mc[j] ? 1.0f : share_of(mc[j], m);
+        mc[j] = m;
+        sum[j] *= f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc[d][j] *= f;
+      }
+    }
+    s16x4 pb[NB][RB];
+#pragma unroll
+    for (int j = 0; j < RB; ++j) {
+      const float base = mc[j] == -INFINITY ? 0.0f : mc[j];
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        bf16x4 h;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p = exp2_(__builtin_fmaf(s[i][j][e], A.c, -base));
+          sum[j] += p;
+          h[e] = (__bf16)p;
+        }
+        pb[i][j] = __builtin_bit_cast(s16x4, h);
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      s16x4 vf[NB];
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+        vf[i] = read_turned(vb + (at + 16u * i + vrow) * DP + ((2u * d + ((lr & 3u) >> 1)) ^ vt) * 8u + (lr & 1u) * 4u);
+#pragma unroll
+      for (int i = 0; i < NB; i += 2)
+#pragma unroll
+        for (int j = 0; j < RB; ++j) {
+          if constexpr (NB > 1) {
+            const s16x8 v8 = __builtin_shufflevector(vf[i], vf[i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+            const s16x8 p8 = __builtin_shufflevector(pb[i][j], pb[i + 1][j], 0, 1, 2, 3, 4, 5, 6, 7);
+            acc[d][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v8), __builtin_bit_cast(bf16x8, p8), acc[d][j], 0, 0, 0);
+          } else {
+            acc[d][j] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf[0], pb[0][j], acc[d][j], 0, 0, 0);
+          }
+        }
+    }
+  };
+
   uint32_t cur = 0u, nxt = S - 1u;
   for (uint32_t t = 0; t < nt; ++t) {
     const uint32_t after = nt - 1u - t;   // tiles still in flight, at most S - 2
@@ -399,11 +399,11 @@ __device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J,
   }
 }
 
-template <int DP, int RB, int WQ, bool SMALL, int S>
-__global__ __launch_bounds__(256, WQ == 1 ? 2 : 1) void attention_tile_kernel(AttArgs A) {
+template <int DP, int RB, int WQ, int WP, bool SMALL, int S>
+__global__ __launch_bounds__(WQ * WP * 64, 2) void attention_tile_kernel(AttArgs A) {
   __shared__ __align__(1024) __bf16 tiles[2][S * ATT_TILE * DP];
-  __shared__ float2 stats[2 * RB * 64];   // (the waves that meet, at most two at a time)
-  __shared__ AttEntry table[16 * RB * WQ];
+  __shared__ float2 stats[4 * RB * 64];   // (the waves that meet, at most four at a time)
+  __shared__ AttEntry table[16 * RB * WQ < 32 ? 32 : 16 * RB * WQ];
   __shared__ uint32_t odd;
   // XCD x (workgroups go to the XCDs in turn) takes a contiguous range of the jobs.
   const uint32_t per = gridDim.x / 8u, job = (blockIdx.x & 7u) * per + (blockIdx.x >> 3);
@@ -426,7 +426,7 @@ __global__ __launch_bounds__(256, WQ == 1 ? 2 : 1) void attention_tile_kernel(At
     const uint32_t tiles_all = (len + ATT_TILE - 1u) / ATT_TILE, each = (tiles_all + A.sp - 1u) / A.sp * ATT_TILE;
     J.a = min(len, J.slot * each), J.b = min(len, J.a + each);
     J.row = 0u, J.len = 0u;
-    attention_job<DP, RB, WQ, 4 / WQ, S>(A, J, tiles[0], tiles[1], stats, table, &odd);
+    attention_job<DP, RB, WQ, WP, S>(A, J, tiles[0], tiles[1], stats, table, &odd);
     return;
   }
   uint32_t i = job - A.np;
@@ -438,7 +438,7 @@ __global__ __launch_bounds__(256, WQ == 1 ? 2 : 1) void attention_tile_kernel(At
   const uint32_t row = i / A.KV;
   J.g = row / A.wb, J.row = row - J.g * A.wb;
   J.slot = A.sp + part;
-  J.m0 = blk * (SMALL ? 16u : 16u * RB * WQ);
+  J.m0 = blk * (SMALL ? 16u : 16u * RB * WQ);   // (one block, where it is small)
   J.m = A.nt * A.per;
   const uint32_t r = att_row(A, row);
   J.len = att_len(A.len, r, A.N);
@@ -447,8 +447,8 @@ __global__ __launch_bounds__(256, WQ == 1 ? 2 : 1) void attention_tile_kernel(At
   const uint32_t end = min(J.len, att_seen(J.len, A.T, A.t0 + A.nt - 1u));   // of the last token here
   const uint32_t tiles_all = (end + ATT_TILE - 1u) / ATT_TILE, each = (tiles_all + A.ss - 1u) / A.ss * ATT_TILE;
   J.a = min(end, part * each), J.b = min(end, J.a + each);
-  if constexpr (SMALL) attention_job<DP, 1, 1, 4, S>(A, J, tiles[0], tiles[1], stats, table, &odd);
-  else attention_job<DP, RB, WQ, 4 / WQ, S>(A, J, tiles[0], tiles[1], stats, table, &odd);
+  if constexpr (SMALL) attention_job<DP, 1, WQ * WP / 4, 4, S>(A, J, tiles[0], tiles[1], stats, table, &odd);
+  else attention_job<DP, RB, WQ, WP, S>(A, J, tiles[0], tiles[1], stats, table, &odd);
 }
 
 // Joins a query's parts: NWV waves a query, each lane four elements of every
@@ -594,22 +594,29 @@ __global__ __launch_bounds__(256) void attention_weight_kernel(AttArgs A, uint32
 
 size_t attention_scratch_bytes() { return ATT_SCRATCH; }
 
-template <int DP, int RB, int WQ, int S>
+template <int DP, int RB, int WQ, int WP, int S>
 static void att_go(hipStream_t st, const AttArgs& A, bool small) {
-  const dim3 grid((A.njobs + 7u) / 8u * 8u), block(256);
-  if (small) hipLaunchKernelGGL((attention_tile_kernel<DP, RB, WQ, true, S>), grid, block, 0, st, A);
-  else hipLaunchKernelGGL((attention_tile_kernel<DP, RB, WQ, false, S>), grid, block, 0, st, A);
+  const dim3 grid((A.njobs + 7u) / 8u * 8u), block(WQ * WP * 64);
+  if (small) hipLaunchKernelGGL((attention_tile_kernel<DP, RB, WQ, WP, true, S>), grid, block, 0, st, A);
+  else hipLaunchKernelGGL((attention_tile_kernel<DP, RB, WQ, WP, false, S>), grid, block, 0, st, A);
 }
 
 template <int DP>
 static void attention_launch(hipStream_t st, const AttArgs& A, const AttPlan& p) {
-  constexpr int S = DP == 64 ? 4 : 2, RL = DP == 256 ? 2 : 4;
+  constexpr int S = DP == 64 ? 4 : 2, S8 = DP == 256 ? 2 : 4;
   if (A.njobs) {
-    if (p.rb == 1u) att_go<DP, 1, 1, S>(st, A, p.small);
-    else if (p.rb == 2u && p.wq == 1u) att_go<DP, 2, 1, S>(st, A, p.small);
-    else if (p.wq == 1u) att_go<DP, RL, 1, S>(st, A, p.small);
-    else if (p.wq == 2u) att_go<DP, RL, 2, S>(st, A, p.small);
-    else att_go<DP, RL, 4, S>(st, A, p.small);
+    if constexpr (DP == 256) {
+      if (p.wq == 1u) att_go<DP, 1, 1, 4, S>(st, A, p.small);
+      else if (p.wq == 2u) att_go<DP, 1, 2, 2, S>(st, A, p.small);
+      else if (p.wq == 4u) att_go<DP, 1, 4, 1, S>(st, A, p.small);
+      else att_go<DP, 1, 8, 1, S8>(st, A, p.small);
+    } else {
+      if (p.rb == 1u) att_go<DP, 1, 1, 4, S>(st, A, p.small);
+      else if (p.wq == 1u) att_go<DP, 2, 1, 4, S>(st, A, p.small);
+      else if (p.wq == 2u) att_go<DP, 2, 2, 2, S>(st, A, p.small);
+      else if (p.wq == 4u) att_go<DP, 2, 4, 1, S>(st, A, p.small);
+      else att_go<DP, 2, 8, 1, S8>(st, A, p.small);
+    }
   }
   if (A.slots > 16u) hipLaunchKernelGGL((attention_join_kernel<DP, 4>), dim3(A.NQ), dim3(256), 0, st, A);
   else hipLaunchKernelGGL((attention_join_kernel<DP, 1>), dim3((A.NQ + 3u) / 4u), dim3(256), 0, st, A);

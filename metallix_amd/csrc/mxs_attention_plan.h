@@ -37,16 +37,15 @@ inline AttPlan attention_plan(uint32_t G, uint32_t W, uint32_t T, uint32_t H, ui
     if (row > room) p.nt = (uint32_t)(room / H);
   }
   const uint32_t ms = p.nt * per, m = P ? p.wb * ms : ms;   // queries that share a suffix, a prefix
-  if (m <= 16u) p.rb = 1u, p.wq = 1u;
-  else if (m <= 32u) p.rb = 2u, p.wq = 1u;
-  else if (p.dp == 256u) p.rb = 2u, p.wq = m <= 64u ? 2u : 4u;
-  else p.rb = 4u, p.wq = m <= 64u ? 1u : m <= 128u ? 2u : 4u;
+  p.rb = p.dp == 256u || m <= 16u ? 1u : 2u;
+  const uint32_t blocks = att_ceil(m, 16u * p.rb);
+  p.wq = blocks <= 1u ? 1u : blocks <= 2u ? 2u : blocks <= 4u ? 4u : 8u;
   p.small = ms <= 16u;
   const uint32_t rows = 16u * p.rb * p.wq, nrb = att_ceil(m, rows), nsb = p.small ? 1u : att_ceil(ms, rows);
   const uint32_t tp = att_ceil(P, ATT_TILE), ts = att_ceil(N, ATT_TILE);
   // Tiles of a part: so many that the parts fill the chip about once.
   const uint64_t jobs_p = (uint64_t)p.ng * KV * nrb, jobs_s = (uint64_t)p.ng * p.wb * KV * nsb;
-  const uint64_t target = p.wq == 1u ? 512u : 256u;
+  const uint64_t target = p.wq == 8u || p.dp == 256u ? 256u : 512u;
   uint32_t each = att_ceil(jobs_p * tp + jobs_s * ts, target);
   if (each < 1u) each = 1u;
   for (;; each += each / 8u + 1u) {
