@@ -32,7 +32,7 @@ struct AttArgs {
   uint32_t W, T, H, KV, D, P, N, per;   // per: query heads a cache head has
   uint32_t g0, ng, b0, wb, t0, nt;      // this launch's groups, rows of each, tokens
   uint32_t nrb, nsb, sp, ss, slots;     // blocks of queries of a prefix and a suffix, parts of either, of a query
-  uint32_t np, njobs;                   // workgroups of prefixes, of all
+  uint32_t np, ns;                      // workgroups of prefixes, of suffixes
   uint32_t NQ;                          // queries: ng * wb * nt * H
   float c;                              // |scale| log2(e)
   uint32_t flip;                        // 0x8000 where the scale is negative: the queries' signs
@@ -405,11 +405,13 @@ __global__ __launch_bounds__(WQ * WP * 64, 2) void attention_tile_kernel(AttArgs
   __shared__ float2 stats[4 * RB * 64];   // (the waves that meet, at most four at a time)
   __shared__ AttEntry table[16 * RB * WQ < 32 ? 32 : 16 * RB * WQ];
   __shared__ uint32_t odd;
-  // XCD x (workgroups go to the XCDs in turn) takes a contiguous range of the jobs.
-  const uint32_t per = gridDim.x / 8u, job = (blockIdx.x & 7u) * per + (blockIdx.x >> 3);
-  if (job >= A.njobs) return;
+  // XCD x (workgroups go to the XCDs in turn) takes a contiguous range of the
+  // prefixes' jobs, then one of the suffixes'.
+  const uint32_t xcd = blockIdx.x & 7u, at = blockIdx.x >> 3, pp = (A.np + 7u) / 8u, ps = (A.ns + 7u) / 8u;
   AttJob J;
-  J.pre = job < A.np;
+  J.pre = at < pp;
+  const uint32_t job = J.pre ? xcd * pp + at : xcd * ps + at - pp;
+  if (job >= (J.pre ? A.np : A.ns)) return;
   if (J.pre) {   // blocks of queries together: they read the same positions
     uint32_t i = job;
     const uint32_t blk = i % A.nrb;
@@ -421,15 +423,15 @@ __global__ __launch_bounds__(WQ * WP * 64, 2) void attention_tile_kernel(AttArgs
     J.m0 = blk * (16u * RB * WQ);
     J.m = A.wb * A.nt * A.per;
     const uint32_t g = A.g0 + J.g, len = att_len(A.plen, g, A.P);
-    const uint64_t at = g * A.pg + J.kv * A.ph;
-    J.k = A.pk + at, J.v = A.pv + at, J.stride = A.pp;
+    const uint64_t from = g * A.pg + J.kv * A.ph;
+    J.k = A.pk + from, J.v = A.pv + from, J.stride = A.pp;
     const uint32_t tiles_all = (len + ATT_TILE - 1u) / ATT_TILE, each = (tiles_all + A.sp - 1u) / A.sp * ATT_TILE;
     J.a = min(len, J.slot * each), J.b = min(len, J.a + each);
     J.row = 0u, J.len = 0u;
     attention_job<DP, RB, WQ, WP, S>(A, J, tiles[0], tiles[1], stats, table, &odd);
     return;
   }
-  uint32_t i = job - A.np;
+  uint32_t i = job;
   const uint32_t blk = i % A.nsb;
   i /= A.nsb;
   const uint32_t part = i % A.ss;
@@ -442,8 +444,8 @@ __global__ __launch_bounds__(WQ * WP * 64, 2) void attention_tile_kernel(AttArgs
   J.m = A.nt * A.per;
   const uint32_t r = att_row(A, row);
   J.len = att_len(A.len, r, A.N);
-  const uint64_t at = r * A.kr + J.kv * A.kh;
-  J.k = A.k + at, J.v = A.v + at, J.stride = A.kp;
+  const uint64_t from = r * A.kr + J.kv * A.kh;
+  J.k = A.k + from, J.v = A.v + from, J.stride = A.kp;
   const uint32_t end = min(J.len, att_seen(J.len, A.T, A.t0 + A.nt - 1u));   // of the last token here
   const uint32_t tiles_all = (end + ATT_TILE - 1u) / ATT_TILE, each = (tiles_all + A.ss - 1u) / A.ss * ATT_TILE;
   J.a = min(end, part * each), J.b = min(end, J.a + each);
@@ -596,7 +598,7 @@ size_t attention_scratch_bytes() { return ATT_SCRATCH; }
 
 template <int DP, int RB, int WQ, int WP, int S>
 static void att_go(hipStream_t st, const AttArgs& A, bool small) {
-  const dim3 grid((A.njobs + 7u) / 8u * 8u), block(WQ * WP * 64);
+  const dim3 grid(((A.np + 7u) / 8u + (A.ns + 7u) / 8u) * 8u), block(WQ * WP * 64);
   if (small) hipLaunchKernelGGL((attention_tile_kernel<DP, RB, WQ, WP, true, S>), grid, block, 0, st, A);
   else hipLaunchKernelGGL((attention_tile_kernel<DP, RB, WQ, WP, false, S>), grid, block, 0, st, A);
 }
@@ -604,7 +606,7 @@ static void att_go(hipStream_t st, const AttArgs& A, bool small) {
 template <int DP>
 static void attention_launch(hipStream_t st, const AttArgs& A, const AttPlan& p) {
   constexpr int S = DP == 64 ? 4 : 2, S8 = DP == 256 ? 2 : 4;
-  if (A.njobs) {
+  if (A.np + A.ns) {
     if constexpr (DP == 256) {
       if (p.wq == 1u) att_go<DP, 1, 1, 4, S>(st, A, p.small);
       else if (p.wq == 2u) att_go<DP, 1, 2, 2, S>(st, A, p.small);
@@ -670,7 +672,7 @@ extern "C" int mxs_prefix_attention(mxs_ctx* ctx, const mxs_attention* attention
         const uint32_t rows = 16u * p.rb * p.wq, ms = A.nt * A.per;
         A.nrb = att_ceil((uint64_t)A.wb * ms, rows), A.nsb = p.small ? 1u : att_ceil(ms, rows);
         A.np = A.ng * A.KV * A.nrb * A.sp;
-        A.njobs = A.np + A.ng * A.wb * A.KV * A.nsb * A.ss;
+        A.ns = A.ng * A.wb * A.KV * A.nsb * A.ss;
         A.stat = reinterpret_cast<float2*>(ctx->attention_scratch);
         A.ref = A.pw || A.w ? ctx->attention_scratch + 2ull * A.slots * A.NQ : nullptr;
         A.part = ctx->attention_scratch + ((2ull * A.slots + 1u) * A.NQ + 3u) / 4u * 4u;
