@@ -42,48 +42,19 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+constexpr uint32_t EV_BINS = 2048;   // values of a digit
+
 template <int TH>
 struct EvictSmem {
-  uint32_t hist[256];
+  union {
+    uint32_t hist[EV_BINS];
+    struct {
+      uint32_t holes[EV_LIST], late[EV_LIST];
+    };
+  };
   uint32_t wave[TH / 64];
-  uint32_t pick[2];          // the digit, how many are left to take within it
-  uint32_t holes[EV_LIST], late[EV_LIST];
+  uint32_t pick[3];          // the digit, how many are left to take within it, how many have it
 };
-
-// The `need`-th largest of f(slot) over the slots, digit by digit from bit
-// `top` on down, among the slots where f is true.  f(slot, &key).  On return
-// need is how many of the keys equal to the result are among the first `need`.
-template <int TH, typename F>
-__device__ uint32_t nth_largest(EvictSmem<TH>& S, uint32_t len, uint32_t& need, F f) {
-  uint32_t prefix = 0u;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (uint32_t i = threadIdx.x; i < 256u; i += TH) S.hist[i] = 0u;
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < len; i += TH) {
-      uint32_t key;
-      if (!f(i, key)) continue;
-      if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&S.hist[(key >> shift) & 255u], 1u);
-    }
-    __syncthreads();
-    if (threadIdx.x < 64u) {   // lane l holds digits 255 - 4 l down
-      uint32_t c[4], sum = 0u;
-      for (int j = 0; j < 4; ++j) sum += c[j] = S.hist[255u - 4u * threadIdx.x - j];
-      uint32_t before = wave_scan_u32(sum) - sum;
-      for (int j = 0; j < 4; ++j) {
-        if (before < need && before + c[j] >= need) {
-          S.pick[0] = 255u - 4u * threadIdx.x - j;
-          S.pick[1] = need - before;
-        }
-        before += c[j];
-      }
-    }
-    __syncthreads();
-    prefix |= S.pick[0] << shift;
-    need = S.pick[1];
-    __syncthreads();
-  }
-  return prefix;
-}
 
 // Sum over the threads before this one; total: over all.
 template <int TH>
@@ -101,6 +72,34 @@ __device__ uint32_t before_me(EvictSmem<TH>& S, uint32_t v, uint32_t& total) {
   return base + sc - v;
 }
 
+// One digit of the `need`-th largest: f(count) calls count(digit) for each key
+// that is still in question.  Returns the digit; need becomes how many to take of
+// those that have it, same how many there are.
+template <int TH, typename F>
+__device__ uint32_t next_digit(EvictSmem<TH>& S, uint32_t& need, uint32_t& same, F f) {
+  constexpr uint32_t B = EV_BINS / TH;
+  for (uint32_t i = threadIdx.x; i < EV_BINS; i += TH) S.hist[i] = 0u;
+  __syncthreads();
+  f([&](uint32_t digit) { atomicAdd(&S.hist[digit], 1u); });
+  __syncthreads();
+  uint32_t c[B], sum = 0u, total;   // the thread's digits, largest first
+#pragma unroll
+  for (uint32_t j = 0; j < B; ++j) sum += c[j] = S.hist[EV_BINS - 1u - threadIdx.x * B - j];
+  uint32_t before = before_me<TH>(S, sum, total);
+#pragma unroll
+  for (uint32_t j = 0; j < B; ++j) {
+    if (before < need && before + c[j] >= need) {
+      S.pick[0] = EV_BINS - 1u - threadIdx.x * B - j;
+      S.pick[1] = need - before;
+      S.pick[2] = c[j];
+    }
+    before += c[j];
+  }
+  __syncthreads();
+  need = S.pick[1], same = S.pick[2];
+  return S.pick[0];
+}
+
 __device__ __forceinline__ void copy_piece(char* to, const char* from, uint32_t have) {
   if (have >= 16u) {
     *reinterpret_cast<ev_u32x4_u*>(to) = *reinterpret_cast<const ev_u32x4_u*>(from);
@@ -112,11 +111,14 @@ __device__ __forceinline__ void copy_piece(char* to, const char* from, uint32_t 
   if (have & 1u) *to = *from;
 }
 
-template <int TH>
+// A row (layer, segment, head) and one of its parts a workgroup; KR: the keys
+// a thread holds, 0 where there are more than registers hold and they are worked out
+// again for each look.
+template <int TH, int KR>
 __global__ __launch_bounds__(TH) void evict_kernel(EvictArgs A) {
   extern __shared__ unsigned long long kept[];   // a bit a slot
   __shared__ EvictSmem<TH> S;
-  const uint32_t tid = threadIdx.x, part = blockIdx.x % A.parts, row = blockIdx.x / A.parts;   // row: (layer, segment, head)
+  const uint32_t tid = threadIdx.x, part = blockIdx.x % A.parts, row = blockIdx.x / A.parts;
   const uint32_t h = row % A.H, seg = row / A.H % A.S, layer = row / A.H / A.S, n = A.n;
   const int32_t l0 = A.lengths ? A.lengths[seg] : (int32_t)A.C;
   const uint32_t len = l0 <= 0 ? 0u : min((uint32_t)l0, A.C), now = min(len, n);
@@ -139,11 +141,35 @@ __global__ __launch_bounds__(TH) void evict_kernel(EvictArgs A) {
     }
     return;
   }
+  // The slots' keys: the protected ones above all, then by weight.
   int64_t recent_from = INT64_MAX;   // positions past it are protected
+  auto key_of = [&](float w, int32_t p) {
+    return p < (int64_t)A.first || p > recent_from ? 0xffffffffu : weight_key(w);
+  };
+  constexpr int U = KR ? KR : 8;     // slots in flight
+  uint32_t keys[U];
+  int32_t where[U];
+  auto load = [&](uint32_t i0, float (&w)[U], int32_t (&p)[U]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t i = min(i0 + u * TH + tid, len - 1u);
+      w[u] = weight[i];
+      p[u] = index ? index[i] : (int32_t)i;
+    }
+  };
+  float held[U];
+  if (KR) load(0u, held, where);
   if (A.recent) {
     int32_t newest = index ? -1 : (int32_t)len - 1;
-    if (index)
-      for (uint32_t i = tid; i < len; i += TH) newest = max(newest, index[i]);
+    if (index) {
+      if (KR) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) newest = max(newest, where[u]);
+      } else {
+#pragma unroll 8
+        for (uint32_t i = tid; i < len; i += TH) newest = max(newest, index[i]);
+      }
+    }
     for (int x = 1; x < 64; x <<= 1) newest = max(newest, __shfl_xor(newest, x));
     if ((tid & 63u) == 0u) S.wave[tid >> 6] = (uint32_t)newest;
     __syncthreads();
@@ -151,56 +177,106 @@ __global__ __launch_bounds__(TH) void evict_kernel(EvictArgs A) {
     __syncthreads();
     recent_from = (int64_t)newest - A.recent;
   }
-  auto key_of = [&](uint32_t i) {
-    const int64_t p = index ? index[i] : (int32_t)i;
-    if (p < (int64_t)A.first || p > recent_from) return 0xffffffffu;
-    return weight_key(weight[i]);
-  };
-  uint32_t need = n;
-  const uint32_t edge = nth_largest<TH>(S, len, need, [&](uint32_t i, uint32_t& k) { k = key_of(i); return true; });
-  // of the slots with the edge's key the `need` lowest: down to the need-th largest ~slot
-  const uint32_t last = ~nth_largest<TH>(S, len, need, [&](uint32_t i, uint32_t& k) { k = ~i; return key_of(i) == edge; });
-  const uint32_t words = (len + 63u) / 64u;
-  for (uint32_t i = tid; i < words * 64u; i += TH) {
-    const uint32_t k = i < len ? key_of(i) : 0u;
-    const unsigned long long b = __builtin_amdgcn_ballot_w64(i < len && (k > edge || (k == edge && i <= last)));
-    if ((tid & 63u) == 0u) kept[i >> 6] = b;
+  if (KR) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) keys[u] = key_of(held[u], where[u]);
   }
+  // f(slot, key, valid) for all slots of a whole number of waves.
+  auto each = [&](auto f) __attribute__((always_inline)) {
+    if (KR) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if ((uint32_t)u * TH < len) f(u * TH + tid, keys[u], u * TH + tid < len);
+    } else {
+      for (uint32_t i0 = 0; i0 < len; i0 += U * TH) {
+        float w[U];
+        int32_t p[U];
+        load(i0, w, p);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (i0 + u * TH < len) f(i0 + u * TH + tid, key_of(w[u], p[u]), i0 + u * TH + tid < len);
+      }
+    }
+  };
+  // The n-th largest key, 11, 11 and 10 bits at a time, and of the slots that
+  // have it the need-th lowest.
+  uint32_t need = n, same, edge = 0u;
+#pragma unroll 1
+  for (uint32_t r = 0; r < 3u; ++r) {
+    const uint32_t shift = r == 0u ? 21u : r == 1u ? 10u : 0u, bits = r == 2u ? 10u : 11u;
+    const uint32_t above = shift + bits;   // the digits found so far
+    edge |= next_digit<TH>(S, need, same, [&](auto count) {
+      each([&](uint32_t, uint32_t k, bool valid) {
+        if (valid && (above == 32u || k >> above == edge >> above)) count(k >> shift & ((1u << bits) - 1u));
+      });
+    }) << shift;
+  }
+  uint32_t last = ~0u;
+  if (need < same) {
+    uint32_t low = 0u;   // of ~slot's 20 bits
+#pragma unroll 1
+    for (uint32_t r = 0; r < 2u; ++r) {
+      const uint32_t shift = r == 0u ? 10u : 0u;
+      low |= next_digit<TH>(S, need, same, [&](auto count) {
+        each([&](uint32_t i, uint32_t k, bool valid) {
+          const uint32_t c = ~i & 0xfffffu;
+          if (valid && k == edge && (r == 0u || c >> 10 == low >> 10)) count(c >> shift & 0x3ffu);
+        });
+      }) << shift;
+    }
+    last = ~low & 0xfffffu;
+  }
+  each([&](uint32_t i, uint32_t k, bool valid) {
+    const unsigned long long b = __builtin_amdgcn_ballot_w64(valid && (k > edge || (k == edge && i <= last)));
+    if ((tid & 63u) == 0u && i < len) kept[i >> 6] = b;   // (a wave's slots: 64 consecutive ones)
+  });
   __syncthreads();
   for (uint32_t i = sa + tid; i < min(sb, n); i += TH)
     if (kept[i >> 6] >> (i & 63u) & 1u) {
       weight_out[i] = weight[i];
       if (index_out) index_out[i] = index ? index[i] : (int32_t)i;
     }
-  // Each thread takes some words; their free slots below n and kept ones from n on, counted.
-  const uint32_t own = (words + TH - 1u) / TH, wa = min(tid * own, words), wb = min(wa + own, words);
-  auto free_of = [&](uint32_t w) {
-    const uint32_t s = w * 64u;
-    return s >= n ? 0ull : ~kept[w] & (n - s >= 64u ? ~0ull : (1ull << (n - s)) - 1ull);
+  // Each thread takes some units of 2^us slots; their free slots below n and kept
+  // ones from n on, counted.
+  uint32_t us = 0u;
+  while (us < 6u && (len + (1u << us) - 1u) >> us > TH) ++us;
+  const uint32_t units = (len + (1u << us) - 1u) >> us, own = (units + TH - 1u) / TH;
+  const uint32_t ua = min(tid * own, units), ub = min(ua + own, units), unit = 1u << us;
+  auto bits_of = [&](uint32_t x) { return kept[x << us >> 6] >> (x << us & 63u) & (unit == 64u ? ~0ull : (1ull << unit) - 1ull); };
+  auto below = [&](uint32_t x) {   // of the unit's slots those below n
+    const uint32_t s = x << us;
+    return s >= n ? 0ull : n - s >= unit ? (unit == 64u ? ~0ull : (1ull << unit) - 1ull) : (1ull << (n - s)) - 1ull;
   };
-  auto late_of = [&](uint32_t w) {
-    const uint32_t s = w * 64u;
-    return s + 64u <= n ? 0ull : s >= n ? kept[w] : kept[w] & ~((1ull << (n - s)) - 1ull);
-  };
-  uint32_t nf = 0u, nl = 0u, moves, same;
-  for (uint32_t w = wa; w < wb; ++w) {
-    nf += __builtin_popcountll(free_of(w));
-    nl += __builtin_popcountll(late_of(w));
+  auto free_of = [&](uint32_t x) { return ~bits_of(x) & below(x); };
+  auto late_of = [&](uint32_t x) { return bits_of(x) & ~below(x); };
+  uint32_t nf = 0u, nl = 0u, moves, all;
+  for (uint32_t x = ua; x < ub; ++x) {
+    nf += __builtin_popcountll(free_of(x));
+    nl += __builtin_popcountll(late_of(x));
   }
-  const uint32_t f0 = before_me<TH>(S, nf, same), m0 = before_me<TH>(S, nl, moves);
-  const uint32_t share = (moves + A.parts - 1u) / A.parts, ja = part * share, jb = min(moves, ja + share);
+  // (both counts at once where they fit: fewer than 2^16 slots)
+  uint32_t f0, m0;
+  if (len < 1u << 16) {
+    const uint32_t both = before_me<TH>(S, nl << 16 | nf, all);
+    f0 = both & 0xffffu, m0 = both >> 16, moves = all >> 16;
+  } else {
+    f0 = before_me<TH>(S, nf, all);
+    m0 = before_me<TH>(S, nl, moves);
+  }
+  const uint32_t share = (moves + A.parts - 1u) / A.parts, ja = min(moves, part * share), jb = min(moves, ja + share);
   const mxs_cache c = A.cache[layer];
   const uint64_t off = seg * A.ss + h * A.hs;
   char* const ck = reinterpret_cast<char*>(c.keys) + off;
   char* const cv = c.values ? reinterpret_cast<char*>(c.values) + off : nullptr;
   const uint32_t pieces = (A.bytes + 15u) / 16u, both = cv ? 2u * pieces : pieces;
+  const uint32_t bb = min(both, (uint32_t)TH), ppi = TH / bb, k0 = tid / bb, p0 = tid - k0 * bb;   // this thread's pairs and piece
   for (uint32_t j = ja; j < jb; j += EV_LIST) {
     const uint32_t m = min(EV_LIST, jb - j);
-    auto list = [&](uint32_t rank, uint32_t count, uint32_t* to, auto bits_of) {
+    auto list = [&](uint32_t rank, uint32_t count, uint32_t* to, auto bits) {
       if (rank >= j + m || rank + count <= j) return;
-      for (uint32_t w = wa; w < wb; ++w)
-        for (unsigned long long b = bits_of(w); b; b &= b - 1ull, ++rank)
-          if (rank >= j && rank < j + m) to[rank - j] = w * 64u + (uint32_t)__builtin_ctzll(b);
+      for (uint32_t x = ua; x < ub; ++x)
+        for (unsigned long long b = bits(x); b; b &= b - 1ull, ++rank)
+          if (rank >= j && rank < j + m) to[rank - j] = (x << us) + (uint32_t)__builtin_ctzll(b);
     };
     list(f0, nf, S.holes, free_of);
     list(m0, nl, S.late, late_of);
@@ -210,14 +286,37 @@ __global__ __launch_bounds__(TH) void evict_kernel(EvictArgs A) {
       weight_out[to] = weight[from];
       if (index_out) index_out[to] = index ? index[from] : (int32_t)from;
     }
-    for (uint32_t i = tid; i < m * both; i += TH) {
-      const uint32_t k = i / both, p = i - k * both;
-      char* const base = p < pieces ? ck : cv;
-      const uint32_t pc = (p < pieces ? p : p - pieces) * 16u;
-      copy_piece(base + S.holes[k] * A.ps + pc, base + S.late[k] * A.ps + pc, A.bytes - pc);
-    }
+    if (k0 < ppi)
+      for (uint32_t p = p0; p < both; p += bb) {
+        char* const base = (p < pieces ? ck : cv) + (p < pieces ? p : p - pieces) * 16u;
+        const uint32_t have = A.bytes - (p < pieces ? p : p - pieces) * 16u;
+        if (have >= 16u) {
+          constexpr uint32_t V = 4;   // loads in flight
+          for (uint32_t k = k0; k < m; k += V * ppi) {
+            ev_u32x4 v[V];
+#pragma unroll
+            for (uint32_t x = 0; x < V; ++x) v[x] = *reinterpret_cast<const ev_u32x4_u*>(base + S.late[min(k + x * ppi, m - 1u)] * A.ps);
+#pragma unroll
+            for (uint32_t x = 0; x < V; ++x)
+              if (k + x * ppi < m) *reinterpret_cast<ev_u32x4_u*>(base + S.holes[k + x * ppi] * A.ps) = v[x];
+          }
+        } else {
+          for (uint32_t k = k0; k < m; k += ppi) copy_piece(base + S.holes[k] * A.ps, base + S.late[k] * A.ps, have);
+        }
+      }
     __syncthreads();
   }
+}
+
+template <int TH, int KR>
+static hipError_t evict_go(hipStream_t st, uint32_t rows, EvictArgs& A, uint32_t want) {
+  const uint32_t lds = (A.C + 63u) / 64u * 8u;
+  hipError_t e = hipSuccess;
+  if (lds > 32u << 10) e = hipFuncSetAttribute((const void*)evict_kernel<TH, KR>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  if (e != hipSuccess) return e;
+  A.parts = rows >= want ? 1u : want / rows;
+  hipLaunchKernelGGL((evict_kernel<TH, KR>), dim3(rows * A.parts), dim3(TH), lds, st, A);
+  return hipGetLastError();
 }
 
 }  // namespace mxs
@@ -248,13 +347,10 @@ extern "C" int mxs_cache_evict(mxs_ctx* ctx, const mxs_evict* evict) {
     A.S = v.segments, A.H = v.heads, A.C = v.capacity, A.bytes = v.position_bytes;
     A.n = v.budget, A.first = v.keep_first, A.recent = v.keep_recent;
     const uint32_t rows = (uint32_t)(here * a_layer);
-    A.parts = rows >= 256u ? 1u : 256u / rows;
-    const uint32_t lds = (A.C + 63u) / 64u * 8u;
-    if (lds > 32u << 10)
-      e = hipFuncSetAttribute((const void*)evict_kernel<1024>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) break;
-    hipLaunchKernelGGL(evict_kernel<1024>, dim3(rows * A.parts), dim3(1024), lds, ctx->stream, A);
-    e = hipGetLastError();
+    if (A.C <= 2048u) e = evict_go<256, 8>(ctx->stream, rows, A, 256u);
+    else if (A.C <= 8192u) e = evict_go<1024, 8>(ctx->stream, rows, A, 256u);
+    else if (A.C <= 32768u) e = evict_go<1024, 32>(ctx->stream, rows, A, 256u);
+    else e = evict_go<1024, 0>(ctx->stream, rows, A, 256u);
   }
   if (prev != ctx->device) (void)hipSetDevice(prev);
   if (e != hipSuccess) return hip_fail(ctx, e, "evict_kernel launch");
