@@ -27,6 +27,7 @@ struct EvictArgs {
   uint32_t S, H, C, bytes;   // segments, heads, capacity, bytes of a position
   uint32_t n, first, recent;
   uint32_t parts;            // workgroups a row
+  uint32_t list;             // entries of the list of slots in question
 };
 
 typedef uint32_t ev_u32x4 __attribute__((ext_vector_type(4)));
@@ -142,9 +143,9 @@ __global__ __launch_bounds__(TH) void evict_kernel(EvictArgs A) {
     return;
   }
   // The slots' keys: the protected ones above all, then by weight.
-  int64_t recent_from = INT64_MAX;   // positions past it are protected
+  int32_t recent_from = INT32_MAX;   // positions past it are protected (budget < len: 20 bits)
   auto key_of = [&](float w, int32_t p) {
-    return p < (int64_t)A.first || p > recent_from ? 0xffffffffu : weight_key(w);
+    return p < (int32_t)A.first || p > recent_from ? 0xffffffffu : weight_key(w);
   };
   constexpr int U = KR ? KR : 8;     // slots in flight
   uint32_t keys[U];
@@ -175,7 +176,7 @@ __global__ __launch_bounds__(TH) void evict_kernel(EvictArgs A) {
     __syncthreads();
     for (uint32_t i = 0; i < TH / 64u; ++i) newest = max(newest, (int32_t)S.wave[i]);
     __syncthreads();
-    recent_from = (int64_t)newest - A.recent;
+    recent_from = newest - (int32_t)A.recent;
   }
   if (KR) {
 #pragma unroll
@@ -200,36 +201,63 @@ __global__ __launch_bounds__(TH) void evict_kernel(EvictArgs A) {
   };
   // The n-th largest key, 11, 11 and 10 bits at a time, and of the slots that
   // have it the need-th lowest.
-  uint32_t need = n, same, edge = 0u;
-#pragma unroll 1
-  for (uint32_t r = 0; r < 3u; ++r) {
+  uint32_t need = n, same, edge = 0u, last = ~0u;
+  auto round = [&](uint32_t r, auto each_one) {
     const uint32_t shift = r == 0u ? 21u : r == 1u ? 10u : 0u, bits = r == 2u ? 10u : 11u;
     const uint32_t above = shift + bits;   // the digits found so far
     edge |= next_digit<TH>(S, need, same, [&](auto count) {
-      each([&](uint32_t, uint32_t k, bool valid) {
+      each_one([&](uint32_t, uint32_t k, bool valid) {
         if (valid && (above == 32u || k >> above == edge >> above)) count(k >> shift & ((1u << bits) - 1u));
       });
     }) << shift;
-  }
-  uint32_t last = ~0u;
-  if (need < same) {
+  };
+  auto settle = [&](auto each_one) {
+    if (need >= same) return;
     uint32_t low = 0u;   // of ~slot's 20 bits
 #pragma unroll 1
     for (uint32_t r = 0; r < 2u; ++r) {
       const uint32_t shift = r == 0u ? 10u : 0u;
       low |= next_digit<TH>(S, need, same, [&](auto count) {
-        each([&](uint32_t i, uint32_t k, bool valid) {
+        each_one([&](uint32_t i, uint32_t k, bool valid) {
           const uint32_t c = ~i & 0xfffffu;
           if (valid && k == edge && (r == 0u || c >> 10 == low >> 10)) count(c >> shift & 0x3ffu);
         });
       }) << shift;
     }
     last = ~low & 0xfffffu;
+  };
+  round(0u, each);
+  if (KR == 0 && same <= A.list) {
+    // The slots with the edge's first digit go into a list, and the rest is done
+    // on that: two looks at all slots instead of four or more.
+    uint2* const list = reinterpret_cast<uint2*>(kept + (A.C + 63u) / 64u);
+    if (tid == 0) S.wave[0] = 0u;
+    __syncthreads();
+    each([&](uint32_t i, uint32_t k, bool valid) {
+      const unsigned long long b = __builtin_amdgcn_ballot_w64(valid && k >> 21 > edge >> 21);
+      if ((tid & 63u) == 0u && i < len) kept[i >> 6] = b;
+      if (valid && k >> 21 == edge >> 21) list[atomicAdd(&S.wave[0], 1u)] = make_uint2(i, k);
+    });
+    __syncthreads();
+    const uint32_t count = S.wave[0];
+    auto listed = [&](auto f) {
+      for (uint32_t x = tid; x < count; x += TH) f(list[x].x, list[x].y, true);
+    };
+    round(1u, listed);
+    round(2u, listed);
+    settle(listed);
+    listed([&](uint32_t i, uint32_t k, bool) {
+      if (k > edge || (k == edge && i <= last)) atomicOr(&kept[i >> 6], 1ull << (i & 63u));
+    });
+  } else {
+    round(1u, each);
+    round(2u, each);
+    settle(each);
+    each([&](uint32_t i, uint32_t k, bool valid) {
+      const unsigned long long b = __builtin_amdgcn_ballot_w64(valid && (k > edge || (k == edge && i <= last)));
+      if ((tid & 63u) == 0u && i < len) kept[i >> 6] = b;   // (a wave's slots: 64 consecutive ones)
+    });
   }
-  each([&](uint32_t i, uint32_t k, bool valid) {
-    const unsigned long long b = __builtin_amdgcn_ballot_w64(valid && (k > edge || (k == edge && i <= last)));
-    if ((tid & 63u) == 0u && i < len) kept[i >> 6] = b;   // (a wave's slots: 64 consecutive ones)
-  });
   __syncthreads();
   for (uint32_t i = sa + tid; i < min(sb, n); i += TH)
     if (kept[i >> 6] >> (i & 63u) & 1u) {
@@ -310,7 +338,9 @@ __global__ __launch_bounds__(TH) void evict_kernel(EvictArgs A) {
 
 template <int TH, int KR>
 static hipError_t evict_go(hipStream_t st, uint32_t rows, EvictArgs& A, uint32_t want) {
-  const uint32_t lds = (A.C + 63u) / 64u * 8u;
+  const uint32_t bits = (A.C + 63u) / 64u * 8u, room = (148u << 10) - bits;   // (of 160 KB, less the rest)
+  A.list = KR ? 0u : room / 8u < 8192u ? room / 8u : 8192u;
+  const uint32_t lds = bits + A.list * 8u;
   hipError_t e = hipSuccess;
   if (lds > 32u << 10) e = hipFuncSetAttribute((const void*)evict_kernel<TH, KR>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   if (e != hipSuccess) return e;
