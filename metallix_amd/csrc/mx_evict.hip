@@ -26,7 +26,7 @@ struct EvictArgs {
   uint64_t ss, hs, ps;       // strides in bytes
   uint32_t S, H, C, bytes;   // segments, heads, capacity, bytes of a position
   uint32_t n, first, recent;
-  uint32_t parts;            // workgroups a row
+  uint32_t parts, jobs;      // workgroups a row, of all
   uint32_t list;             // entries of the list of slots in question
 };
 
@@ -119,7 +119,11 @@ template <int TH, int KR>
 __global__ __launch_bounds__(TH) void evict_kernel(EvictArgs A) {
   extern __shared__ unsigned long long kept[];   // a bit a slot
   __shared__ EvictSmem<TH> S;
-  const uint32_t tid = threadIdx.x, part = blockIdx.x % A.parts, row = blockIdx.x / A.parts;
+  // XCD x (workgroups go to the XCDs in turn) takes a contiguous range of the
+  // rows, so that a row's parts read its weights from one L2.
+  const uint32_t job = (blockIdx.x & 7u) * (gridDim.x / 8u) + (blockIdx.x >> 3);
+  if (job >= A.jobs) return;
+  const uint32_t tid = threadIdx.x, part = job % A.parts, row = job / A.parts;
   const uint32_t h = row % A.H, seg = row / A.H % A.S, layer = row / A.H / A.S, n = A.n;
   const int32_t l0 = A.lengths ? A.lengths[seg] : (int32_t)A.C;
   const uint32_t len = l0 <= 0 ? 0u : min((uint32_t)l0, A.C), now = min(len, n);
@@ -345,7 +349,8 @@ static hipError_t evict_go(hipStream_t st, uint32_t rows, EvictArgs& A, uint32_t
   if (lds > 32u << 10) e = hipFuncSetAttribute((const void*)evict_kernel<TH, KR>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   if (e != hipSuccess) return e;
   A.parts = rows >= want ? 1u : want / rows;
-  hipLaunchKernelGGL((evict_kernel<TH, KR>), dim3(rows * A.parts), dim3(TH), lds, st, A);
+  A.jobs = rows * A.parts;
+  hipLaunchKernelGGL((evict_kernel<TH, KR>), dim3((A.jobs + 7u) / 8u * 8u), dim3(TH), lds, st, A);
   return hipGetLastError();
 }
 
