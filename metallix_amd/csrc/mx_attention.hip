@@ -38,7 +38,7 @@ struct AttArgs {
   uint32_t flip;                        // 0x8000 where the scale is negative: the queries' signs
   float* part;                          // [slots][NQ][DP] sums of a part's exponentials times its values
   float2* stat;                         // [slots][NQ] the part's reference (log2) and sum
-  float* ref;                           // [NQ] log2 of a query's whole sum; inf: it has seen nothing
+  float* ref;                           // [NQ] log2 of a query's whole sum, inf for one that has seen nothing; NULL: no weights
 };
 
 __device__ __forceinline__ uint32_t att_len(const int32_t* len, uint32_t i, uint32_t most) {
@@ -142,13 +142,6 @@ __device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J,
   const uint32_t wq = w % WQ, wp = w / WQ;
 
   const uint32_t nt = J.b > J.a ? (J.b - J.a + ATT_TILE - 1u) / ATT_TILE : 0u;
-  if (A.D < DP && nt) {   // elements past dim are never loaded: zero
-    for (uint32_t i = threadIdx.x; i < S * TE / 8u; i += NW * 64) {
-      reinterpret_cast<bf16x8*>(Ks)[i] = bf16x8{};
-      reinterpret_cast<bf16x8*>(Vs)[i] = bf16x8{};
-    }
-    att_barrier<0>();
-  }
   // A row's pieces lie permuted by its low bits, so that the rows which a read
   // takes fall in different banks.
   auto turn_k = [](uint32_t row) { return PR == 8 ? (row >> 1) & 7u : row & 15u; };
@@ -163,6 +156,13 @@ __device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J,
         att_load_lds(to + (w * LD + i) * LR * DP, base, (min(row, have - 1u) * (uint32_t)J.stride + piece * 8u) * 2u, 0u);
     }
   };
+  if (A.D < DP && nt) {   // the keys' elements past dim are never loaded: zero (the values' reach only sums past dim)
+    const uint32_t pad = PR - A.D / 8u;
+    for (uint32_t i = threadIdx.x; i < S * ATT_TILE * pad; i += NW * 64) {
+      const uint32_t row = i / pad, piece = A.D / 8u + i - row * pad;
+      reinterpret_cast<bf16x8*>(Ks)[row * PR + (piece ^ turn_k(row % ATT_TILE))] = bf16x8{};
+    }
+  }
   // The first tiles' loads are under way while the queries are found.
 #pragma unroll
   for (uint32_t t = 0; t < (uint32_t)S - 1u; ++t)
@@ -456,11 +456,10 @@ __global__ __launch_bounds__(WQ * WP * 64, 2) void attention_tile_kernel(AttArgs
 // Joins a query's parts: NWV waves a query, each lane four elements of every
 // 256 NWV / DP-th part.
 template <int DP, int NWV>
-__global__ __launch_bounds__(256) void attention_join_kernel(AttArgs A) {
+__device__ __forceinline__ void attention_join(const AttArgs& A, uint32_t block, f32x4 (&meet)[4][DP / 4]) {
   constexpr uint32_t LQ = DP / 4, GR = NWV * 64 / LQ;
-  __shared__ f32x4 meet[4][LQ];
   const uint32_t w = threadIdx.x >> 6, l = threadIdx.x & 63u;
-  const uint32_t id = min(blockIdx.x * (4u / NWV) + w / NWV, A.NQ - 1u);   // (a last workgroup's other waves: the last query once more)
+  const uint32_t id = min(block * (4u / NWV) + w / NWV, A.NQ - 1u);   // (a last workgroup's other waves: the last query once more)
   const uint32_t in = w % NWV * 64u + l, d = in % LQ * 4u, grp = in / LQ;
   // every wave by itself: the parts' common reference and the whole sum
   float m = -INFINITY, sum = 0.0f;
@@ -504,94 +503,122 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttArgs A) {
   }
 }
 
-// The weights of 64 positions of a cache head: the scores once more, a wave's
-// positions in registers, all queries that read them in turn.
-template <int DP>
-__global__ __launch_bounds__(256) void attention_weight_kernel(AttArgs A, uint32_t tp, uint32_t ts, uint64_t jobs_p, uint64_t jobs) {
+// The sum over 16 lanes of a row, in each of them.
+template <int N>
+__device__ __forceinline__ float plus_turned(float v) {
+  return v + __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x120 + N, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float row_sum(float v) { return plus_turned<1>(plus_turned<2>(plus_turned<4>(plus_turned<8>(v)))); }
+
+struct AttWeights {
+  uint32_t cp, cs;        // chunks of a prefix and of a suffix, 0 where it has no weights
+  uint32_t tiles;         // 32 positions each, of a chunk
+  uint64_t jobs_p, jobs;  // chunks of all prefixes, of all
+};
+
+// The weights of a chunk of positions of a cache head, by one wave: the scores
+// once more, 16 MB queries held in registers, the next positions' keys on
+// their way.
+template <int DP, int MB>
+__device__ __forceinline__ void attention_weights(const AttArgs& A, const AttWeights& G, uint64_t job) {
   constexpr int KS = DP / 32;
   const uint32_t l = threadIdx.x & 63u, lr = l & 15u, lg = l >> 4;
-  for (uint64_t job = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6); job < jobs; job += (uint64_t)gridDim.x * 4u) {
-    const bool pre = job < jobs_p;
-    uint64_t i = pre ? job : job - jobs_p;
-    const uint32_t tile = (uint32_t)(i % (pre ? tp : ts));
-    i /= pre ? tp : ts;
-    AttJob J;
-    J.pre = pre;
-    J.kv = (uint32_t)(i % A.KV);
-    const uint32_t seg = (uint32_t)(i / A.KV);   // group, or row, within the launch
-    J.g = pre ? seg : seg / A.wb;
-    J.row = pre ? 0u : seg - J.g * A.wb;
-    const uint32_t r = pre ? A.g0 + seg : att_row(A, seg);
-    const uint32_t len = pre ? att_len(A.plen, r, A.P) : att_len(A.len, r, A.N), p0 = tile * 32u;
-    if (p0 >= len) continue;
-    const uint64_t stride = pre ? A.pp : A.kp;
-    const __bf16* const kb = pre ? A.pk + r * A.pg + J.kv * A.ph : A.k + r * A.kr + J.kv * A.kh;
-    bf16x8 kf[2][KS];
+  AttJob J;
+  J.pre = job < G.jobs_p;
+  uint64_t i = J.pre ? job : job - G.jobs_p;
+  const uint32_t chunks = J.pre ? G.cp : G.cs, chunk = (uint32_t)(i % chunks);
+  i /= chunks;
+  J.kv = (uint32_t)(i % A.KV);
+  const uint32_t seg = (uint32_t)(i / A.KV);   // group, or row, within the launch
+  J.g = J.pre ? seg : seg / A.wb;
+  J.row = J.pre ? 0u : seg - J.g * A.wb;
+  const uint32_t r = J.pre ? A.g0 + seg : att_row(A, seg);
+  const uint32_t len = J.pre ? att_len(A.plen, r, A.P) : att_len(A.len, r, A.N);
+  const uint32_t from = min(len, chunk * G.tiles * 32u), to = min(len, from + G.tiles * 32u);
+  if (from >= to) return;
+  const uint64_t stride = J.pre ? A.pp : A.kp;
+  const __bf16* const kb = J.pre ? A.pk + r * A.pg + J.kv * A.ph : A.k + r * A.kr + J.kv * A.kh;
+  float* const out = J.pre ? A.pw + ((uint64_t)r * A.KV + J.kv) * A.P : A.w + ((uint64_t)r * A.KV + J.kv) * A.N;
+  const uint32_t mine = 16u * (lr >> 2 & 1u) + 4u * lg + (lr & 3u);   // the position that this lane writes (lr < 8)
+  auto load = [&](bf16x8 (&k)[2][KS], uint32_t p0) __attribute__((always_inline)) {
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      const __bf16* const from = kb + (uint64_t)min(p0 + 16u * b + lr, len - 1u) * stride;
+      const __bf16* const at = kb + (uint64_t)min(p0 + 16u * b + lr, len - 1u) * stride;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const uint32_t d = 32u * s + 8u * lg;
-        kf[b][s] = d < A.D ? *reinterpret_cast<const bf16x8*>(from + d) : bf16x8{};
-      }
+      for (int s = 0; s < KS; ++s) k[b][s] = *reinterpret_cast<const bf16x8*>(at + min(32u * s + 8u * lg, A.D - 8u));
     }
-    const uint32_t M = (pre ? A.wb : 1u) * A.nt * A.per;
-    f32x4 add[2] = {};
-    for (uint32_t m0 = 0; m0 < M; m0 += 16u) {
-      const uint32_t m = m0 + lr;
-      bf16x8 q[KS];
-      float ref = INFINITY;    // log2 of the query's whole sum; nothing for a query past the last
-      uint32_t lim = 0u;
-      if (m < M) {
-        const AttQuery x = att_query(A, J, m);
-        const __bf16* const from = A.q + (uint64_t)att_row(A, x.row) * A.qr + x.t * A.qt + x.h * A.qh;
+  };
+  const uint32_t M = (J.pre ? A.wb : 1u) * A.nt * A.per;
+  for (uint32_t m0 = 0; m0 < M; m0 += 16u * MB) {
+    bf16x8 q[MB][KS];
+    float ref[MB];
+    uint32_t lim[MB];   // positions below it are seen
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const uint32_t d = 32u * s + 8u * lg;
-          q[s] = d < A.D ? flipped(*reinterpret_cast<const bf16x8*>(from + d), A.flip) : bf16x8{};
-        }
-        ref = A.ref[(x.row * A.nt + x.t - A.t0) * A.H + x.h];
-        lim = pre ? len : min(len, att_seen(len, A.T, x.t));
-      } else {
+    for (int j = 0; j < MB; ++j) {
+      const uint32_t m = m0 + 16u * j + lr;
+      const AttQuery x = att_query(A, J, min(m, M - 1u));
+      const uint32_t id = (x.row * A.nt + x.t - A.t0) * A.H + x.h;
+      const __bf16* const at = A.q + (uint64_t)att_row(A, x.row) * A.qr + x.t * A.qt + x.h * A.qh;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) q[s] = bf16x8{};
+      for (int s = 0; s < KS; ++s) q[j][s] = *reinterpret_cast<const bf16x8*>(at + min(32u * s + 8u * lg, A.D - 8u));
+      ref[j] = A.ref[id];
+      lim[j] = m >= M ? 0u : J.pre ? len : min(len, att_seen(len, A.T, x.t));
+    }
+    // (elements past dim: zero in the queries and, lest they be no numbers, in the keys)
+#pragma unroll
+    for (int j = 0; j < MB; ++j)
+#pragma unroll
+      for (int s = 0; s < KS; ++s) q[j][s] = 32u * s + 8u * lg < A.D ? flipped(q[j][s], A.flip) : bf16x8{};
+    bf16x8 next[2][KS];
+    load(next, from);
+    for (uint32_t p0 = from; p0 < to; p0 += 32u) {
+      bf16x8 k[2][KS];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int s = 0; s < KS; ++s) k[b][s] = 32u * s + 8u * lg < A.D ? next[b][s] : bf16x8{};
+      const bool write = lr < 8u && p0 + mine < to;
+      const float old = write ? out[p0 + mine] : 0.0f;
+      if (p0 + 32u < to) load(next, p0 + 32u);
+      f32x4 add[2] = {};
+#pragma unroll
+      for (int j = 0; j < MB; ++j) {
+        f32x4 x[2] = {};
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) x[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[b][s], q[j][s], x[b], 0, 0, 0);
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float p = exp2_(__builtin_fmaf(x[b][e], A.c, -ref[j]));
+            if (p0 + 16u * b + 4u * lg + e < lim[j]) add[b][e] += p;
+          }
       }
-      f32x4 s2[2] = {};
-#pragma unroll
-      for (int s = 0; s < KS; ++s)
-#pragma unroll
-        for (int b = 0; b < 2; ++b) s2[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[b][s], q[s], s2[b], 0, 0, 0);
+      float v = 0.0f;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = exp2_(__builtin_fmaf(s2[b][e], A.c, -ref));
-          if (p0 + 16u * b + 4u * lg + e < lim) add[b][e] += p;
+          const float all = row_sum(add[b][e]);
+          if (lr == 4u * b + e) v = all;
         }
-    }
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float v = add[b][e];
-        v += __shfl_xor(v, 1);
-        v += __shfl_xor(v, 2);
-        v += __shfl_xor(v, 4);
-        v += __shfl_xor(v, 8);
-        add[b][e] = v;
-      }
-    if (lr == 0u) {
-      float* const to = (pre ? A.pw + ((uint64_t)r * A.KV + J.kv) * A.P : A.w + ((uint64_t)r * A.KV + J.kv) * A.N) + p0;
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t p = 16u * b + 4u * lg + e;
-          if (p0 + p < len) to[p] += add[b][e];
-        }
+      if (write) out[p0 + mine] = old + v;
     }
   }
+}
+
+template <int DP, int NWV>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttArgs A) {
+  __shared__ f32x4 meet[4][DP / 4];
+  attention_join<DP, NWV>(A, blockIdx.x, meet);
+}
+
+template <int DP, int MB>
+__global__ __launch_bounds__(256) void attention_weights_kernel(AttArgs A, AttWeights G) {
+  for (uint64_t job = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6); job < G.jobs; job += (uint64_t)gridDim.x * 4u)
+    attention_weights<DP, MB>(A, G, job);
 }
 
 size_t attention_scratch_bytes() { return ATT_SCRATCH; }
@@ -622,12 +649,20 @@ static void attention_launch(hipStream_t st, const AttArgs& A, const AttPlan& p)
   }
   if (A.slots > 16u) hipLaunchKernelGGL((attention_join_kernel<DP, 4>), dim3(A.NQ), dim3(256), 0, st, A);
   else hipLaunchKernelGGL((attention_join_kernel<DP, 1>), dim3((A.NQ + 3u) / 4u), dim3(256), 0, st, A);
-  const uint32_t tp = A.pw ? (A.P + 31u) / 32u : 0u, ts = A.w ? (A.N + 31u) / 32u : 0u;
-  const uint64_t jobs_p = (uint64_t)A.ng * A.KV * tp, jobs = jobs_p + (uint64_t)A.ng * A.wb * A.KV * ts;
-  if (jobs) {
-    const uint64_t blocks = (jobs + 3u) / 4u;
-    hipLaunchKernelGGL(attention_weight_kernel<DP>, dim3((uint32_t)(blocks < 1u << 20 ? blocks : 1u << 20)), dim3(256), 0, st, A, tp, ts, jobs_p, jobs);
-  }
+  if (!A.pw && !A.w) return;
+  AttWeights G;
+  const uint64_t tp = A.pw ? att_ceil(A.P, 32u) : 0u, ts = A.w ? att_ceil(A.N, 32u) : 0u;
+  const uint64_t segs_p = (uint64_t)A.ng * A.KV, segs_s = segs_p * A.wb;
+  // so many tiles a wave that the waves fill the chip about once
+  const uint64_t each = (segs_p * tp + segs_s * ts) / 2048u;
+  G.tiles = each < 1u ? 1u : each > 64u ? 64u : (uint32_t)each;
+  G.cp = att_ceil(tp, G.tiles), G.cs = att_ceil(ts, G.tiles);
+  G.jobs_p = segs_p * G.cp, G.jobs = G.jobs_p + segs_s * G.cs;
+  const uint64_t blocks = (G.jobs + 3u) / 4u;
+  const dim3 grid((uint32_t)(blocks < 1u << 20 ? blocks : 1u << 20));
+  const uint32_t m = (A.pw ? A.wb : 1u) * A.nt * A.per;
+  if (m <= 16u) hipLaunchKernelGGL((attention_weights_kernel<DP, 1>), grid, dim3(256), 0, st, A, G);
+  else hipLaunchKernelGGL((attention_weights_kernel<DP, DP == 256 ? 2 : 4>), grid, dim3(256), 0, st, A, G);
 }
 
 }  // namespace mxs

@@ -23,6 +23,20 @@ inline uint32_t att_ceil(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1u
 // Bytes of the parts of so many queries: sums, statistics, and the queries' references.
 inline uint64_t att_bytes(uint64_t queries, uint32_t slots, uint32_t dp) { return (queries * (slots * (dp + 2ull) + 1u) + 3u) * 4u; }
 
+// How long `np` workgroups of `a` tiles and then `ns` of `b` take on `places`
+// at once, in tiles; starting and ending one takes as long as two.
+inline uint64_t att_time(uint64_t np, uint64_t a, uint64_t ns, uint64_t b, uint64_t places) {
+  a += 2u, b += 2u;
+  const uint64_t rem = np % places;
+  uint64_t t = np / places * a;
+  if (rem) {   // the others' places take workgroups of the second kind meanwhile
+    const uint64_t fit = (places - rem) * (a / b);
+    ns = ns > fit ? ns - fit : 0u;
+    t += a;
+  }
+  return t + (ns + places - 1u) / places * b;
+}
+
 inline AttPlan attention_plan(uint32_t G, uint32_t W, uint32_t T, uint32_t H, uint32_t KV, uint32_t D, uint32_t P, uint32_t N) {
   AttPlan p{};
   const uint32_t per = H / KV;
@@ -43,17 +57,33 @@ inline AttPlan attention_plan(uint32_t G, uint32_t W, uint32_t T, uint32_t H, ui
   p.small = ms <= 16u;
   const uint32_t rows = 16u * p.rb * p.wq, nrb = att_ceil(m, rows), nsb = p.small ? 1u : att_ceil(ms, rows);
   const uint32_t tp = att_ceil(P, ATT_TILE), ts = att_ceil(N, ATT_TILE);
-  // Tiles of a part: so many that the parts fill the chip about once.
+  // Parts: the candidates fill the chip's places once or twice with the prefixes'
+  // workgroups, or once with these and the suffixes'.
   const uint64_t jobs_p = (uint64_t)p.ng * KV * nrb, jobs_s = (uint64_t)p.ng * p.wb * KV * nsb;
-  const uint64_t target = p.wq == 8u || p.dp == 256u ? 256u : 512u;
-  uint32_t each = att_ceil(jobs_p * tp + jobs_s * ts, target);
-  if (each < 1u) each = 1u;
-  for (;; each += each / 8u + 1u) {
-    p.sp = att_ceil(tp, each), p.ss = att_ceil(ts, each);
-    p.slots = p.sp + p.ss;
-    if (each >= tp && each >= ts) break;
-    if (att_bytes((uint64_t)p.ng * p.wb * p.nt * H, p.slots, p.dp) <= ATT_SCRATCH) break;
+  const uint64_t places = p.wq == 8u || p.dp == 256u ? 256u : 512u;
+  const auto fit = [](uint64_t workgroups, uint64_t jobs, uint32_t tiles) {   // parts, evened out
+    if (tiles == 0u) return 0u;
+    const uint64_t most = workgroups / jobs;
+    const uint32_t n = most < 1u ? 1u : most < tiles ? (uint32_t)most : tiles;
+    return att_ceil(tiles, att_ceil(tiles, n));
+  };
+  uint64_t best = ~0ull;
+  for (uint32_t s = 0; s < 3u; ++s) {
+    const uint32_t ss = fit(s == 0u ? 0u : places * s / 2u, jobs_s, ts);
+    for (uint32_t k = 0; k < 3u; ++k) {
+      const uint64_t room_p = k < 2u ? places * (k + 1u) : places > jobs_s * ss ? places - jobs_s * ss : 0u;
+      const uint32_t sp = fit(room_p, jobs_p, tp);
+      const uint64_t t = att_time(jobs_p * sp, sp ? att_ceil(tp, sp) : 0u, jobs_s * ss, ss ? att_ceil(ts, ss) : 0u, places);
+      // (a part more costs its join: a hundredth of a tile's time)
+      const uint64_t cost = t * 100u + sp + ss;
+      if (cost < best) best = cost, p.sp = sp, p.ss = ss;
+    }
   }
+  while (att_bytes((uint64_t)p.ng * p.wb * p.nt * H, p.sp + p.ss, p.dp) > ATT_SCRATCH && p.sp + p.ss > least) {
+    if (p.sp >= p.ss) p.sp -= (p.sp + 7u) / 8u;   // (1 stays: sp > 1 where it is the larger of more than `least`)
+    else p.ss -= (p.ss + 7u) / 8u;
+  }
+  p.slots = p.sp + p.ss;
   return p;
 }
 
