@@ -109,13 +109,24 @@ struct AttJob {
   bool pre;
 };
 
-// Where query m of a job belongs: its row within the launch, token and head.
+// Where query m of a job belongs: its row within the group, token and head.
 struct AttQuery {
-  uint32_t row, t, h;
+  uint32_t b, t, h;
 };
 __device__ __forceinline__ AttQuery att_query(const AttArgs& A, const AttJob& J, uint32_t m) {
-  const uint32_t hh = m % A.per, r = m / A.per, t = r % A.nt, b = J.pre ? r / A.nt : J.row;
-  return {J.g * A.wb + b, A.t0 + t, J.kv * A.per + hh};
+  uint32_t r = m, hh = 0u, t = 0u;
+  if (A.per > 1u) r = m / A.per, hh = m - r * A.per;   // (uniform)
+  if (A.nt > 1u) {
+    const uint32_t x = r / A.nt;
+    t = r - x * A.nt, r = x;
+  }
+  return {J.pre ? r : J.row, A.t0 + t, J.kv * A.per + hh};
+}
+__device__ __forceinline__ uint32_t att_id(const AttArgs& A, const AttJob& J, const AttQuery& x) {   // of the launch's queries
+  return ((J.g * A.wb + x.b) * A.nt + x.t - A.t0) * A.H + x.h;
+}
+__device__ __forceinline__ uint64_t att_elements(const AttArgs& A, const AttJob& J, const AttQuery& x) {
+  return (uint64_t)((A.g0 + J.g) * A.W + A.b0 + x.b) * A.qr + x.t * A.qt + x.h * A.qh;
 }
 __device__ __forceinline__ uint32_t att_row(const AttArgs& A, uint32_t row) {   // of the whole call
   return (A.g0 + row / A.wb) * A.W + A.b0 + row % A.wb;
@@ -137,6 +148,7 @@ __device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J,
   constexpr int PPW = ATT_TILE / WP, NB = PPW / 16;              // positions a wave takes of a tile, blocks of 16
   constexpr int LD = ATT_TILE / (int)LR / NW;                    // loads a wave issues for keys, and for values
   constexpr uint32_t TE = ATT_TILE * DP;                         // elements of a tile
+  constexpr uint32_t B = NW == 8 && S == 4 ? 2u : 1u;            // tiles between meetings
   static_assert(LD * (int)LR * NW == (int)ATT_TILE, "the loads cover the tile");
   const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63u, lr = l & 15u, lg = l >> 4;
   const uint32_t wq = w % WQ, wp = w / WQ;
@@ -165,7 +177,7 @@ __device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J,
   }
   // The first tiles' loads are under way while the queries are found.
 #pragma unroll
-  for (uint32_t t = 0; t < (uint32_t)S - 1u; ++t)
+  for (uint32_t t = 0; t < (uint32_t)S - B; ++t)
     if (t < nt) {
       fetch(t, J.k, Ks + t * TE, true);
       fetch(t, J.v, Vs + t * TE, false);
@@ -176,9 +188,9 @@ __device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J,
     AttEntry e{~0u, 0u, 0ull};
     if (m < J.m) {
       const AttQuery x = att_query(A, J, m);
-      e.id = (x.row * A.nt + x.t - A.t0) * A.H + x.h;
+      e.id = att_id(A, J, x);
       e.lim = J.pre ? J.b : min(J.b, att_seen(J.len, A.T, x.t));
-      e.at = (uint64_t)att_row(A, x.row) * A.qr + x.t * A.qt + x.h * A.qh;
+      e.at = att_elements(A, J, x);
     }
     table[threadIdx.x] = e;
   }
@@ -208,20 +220,54 @@ __device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J,
   const uint32_t kt = turn_k(lr);   // (rows of a fragment: lr more than a multiple of 16)
   const uint32_t vrow = 4u * lg + (lr >> 2), vt = turn_v(vrow);
 
-  auto compute = [&](const __bf16* __restrict__ kb, const __bf16* __restrict__ vb, uint32_t p0) __attribute__((always_inline)) {
-    const uint32_t at = wp * PPW;   // first position within the tile
-    f32x4 s[NB][RB] = {};
+  const uint32_t at = wp * PPW;   // this wave's first position within a tile
+  auto read_k = [&](bf16x8 (&kf)[NB], const __bf16* __restrict__ kb, int ks) __attribute__((always_inline)) {
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      bf16x8 kf[NB];
+    for (int i = 0; i < NB; ++i)
+      kf[i] = *reinterpret_cast<const bf16x8*>(kb + (at + 16u * i + lr) * DP + ((4u * ks + lg) ^ kt) * 8u);
+  };
+  auto mul_k = [&](f32x4 (&s)[NB][RB], const bf16x8 (&kf)[NB], int ks) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < NB; ++i)
-        kf[i] = *reinterpret_cast<const bf16x8*>(kb + (at + 16u * i + lr) * DP + ((4u * ks + lg) ^ kt) * 8u);
+    for (int i = 0; i < NB; ++i)
 #pragma unroll
-      for (int i = 0; i < NB; ++i)
+      for (int j = 0; j < RB; ++j)
+        s[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i], q[j][ks], ks ? s[i][j] : f32x4{}, 0, 0, 0);
+  };
+  auto read_v = [&](s16x4 (&vf)[NB], const __bf16* __restrict__ vb, int d) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < RB; ++j) s[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i], q[j][ks], s[i][j], 0, 0, 0);
+    for (int i = 0; i < NB; ++i)
+      vf[i] = read_turned(vb + (at + 16u * i + vrow) * DP + ((2u * d + ((lr & 3u) >> 1)) ^ vt) * 8u + (lr & 1u) * 4u);
+  };
+  auto mul_v = [&](const s16x4 (&pb)[NB][RB], const s16x4 (&vf)[NB], int d) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NB; i += 2)
+#pragma unroll
+      for (int j = 0; j < RB; ++j) {
+        if constexpr (NB > 1) {
+          const s16x8 v8 = __builtin_shufflevector(vf[i], vf[i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+          const s16x8 p8 = __builtin_shufflevector(pb[i][j], pb[i + 1][j], 0, 1, 2, 3, 4, 5, 6, 7);
+          acc[d][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v8), __builtin_bit_cast(bf16x8, p8), acc[d][j], 0, 0, 0);
+        } else {
+          acc[d][j] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf[0], pb[0][j], acc[d][j], 0, 0, 0);
+        }
+      }
+  };
+  // The exponentials of block i of the positions.
+  auto weigh = [&](const f32x4 (&s)[NB][RB], s16x4 (&pb)[NB][RB], int i) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < RB; ++j) {
+      const float base = mc[j] == -INFINITY ? 0.0f : mc[j];
+      bf16x4 h;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p = exp2_(__builtin_fmaf(s[i][j][e], A.c, -base));
+        sum[j] += p;
+        h[e] = (__bf16)p;
+      }
+      pb[i][j] = __builtin_bit_cast(s16x4, h);
     }
+  };
+  auto refer = [&](f32x4 (&s)[NB][RB], uint32_t p0) __attribute__((always_inline)) {
     const uint32_t first = p0 + at + 4u * lg;
     if (p0 + at + 16u * NB > least) {   // uniform: some query sees not all of these
 #pragma unroll
@@ -257,129 +303,129 @@ __device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J,
         for (int d = 0; d < DB; ++d) acc[d][j] *= f;
       }
     }
-    s16x4 pb[NB][RB];
+  };
+  // Values that some queries do not see: those past the end become 0, and those
+  // that are no numbers too (their weight of 0 would not be 0 times them); the
+  // queries that do see these get them at the end.
+  auto clean = [&](__bf16* vb, uint32_t p0) {
+    const uint32_t have = min(ATT_TILE, J.b - p0);
+    const bool look = !J.pre && A.T > 1u;
+    for (uint32_t i = (look ? 0u : have * PR) + threadIdx.x; i < ATT_TILE * PR; i += NW * 64) {
+      s16x8* const to = reinterpret_cast<s16x8*>(vb) + i;
+      s16x8 v = {};
+      if (i < have * PR) {
+        if (((i % PR) ^ turn_v(i / PR)) * 8u >= A.D) continue;   // (never loaded)
+        v = *to;
+        bool any = false;
 #pragma unroll
-    for (int j = 0; j < RB; ++j) {
-      const float base = mc[j] == -INFINITY ? 0.0f : mc[j];
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        bf16x4 h;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p = exp2_(__builtin_fmaf(s[i][j][e], A.c, -base));
-          sum[j] += p;
-          h[e] = (__bf16)p;
+        for (int e = 0; e < 8; ++e) {
+          const bool bad = (v[e] & 0x7f80) == 0x7f80;
+          any |= bad;
+          v[e] = bad ? 0 : v[e];
         }
-        pb[i][j] = __builtin_bit_cast(s16x4, h);
+        if (!any) continue;
+        *odd = 1u;
       }
+      *to = v;
     }
-#pragma unroll
-    for (int d = 0; d < DB; ++d) {
-      s16x4 vf[NB];
-#pragma unroll
-      for (int i = 0; i < NB; ++i)
-        vf[i] = read_turned(vb + (at + 16u * i + vrow) * DP + ((2u * d + ((lr & 3u) >> 1)) ^ vt) * 8u + (lr & 1u) * 4u);
-#pragma unroll
-      for (int i = 0; i < NB; i += 2)
-#pragma unroll
-        for (int j = 0; j < RB; ++j) {
-          if constexpr (NB > 1) {
-            const s16x8 v8 = __builtin_shufflevector(vf[i], vf[i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
-            const s16x8 p8 = __builtin_shufflevector(pb[i][j], pb[i + 1][j], 0, 1, 2, 3, 4, 5, 6, 7);
-            acc[d][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v8), __builtin_bit_cast(bf16x8, p8), acc[d][j], 0, 0, 0);
-          } else {
-            acc[d][j] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf[0], pb[0][j], acc[d][j], 0, 0, 0);
-          }
-        }
-    }
+    att_barrier<0>();
   };
 
-  uint32_t cur = 0u, nxt = S - 1u;
-  for (uint32_t t = 0; t < nt; ++t) {
-    const uint32_t after = nt - 1u - t;   // tiles still in flight, at most S - 2
-    if (S > 3 && after >= 2u) att_barrier<4 * LD>();
-    else if (S > 2 && after >= 1u) att_barrier<2 * LD>();
+  // The workgroup meets once in B tiles.
+  uint32_t cur = 0u, nxt = S - B;
+  for (uint32_t t0 = 0; t0 < nt; t0 += B) {
+    const uint32_t after = nt - t0;
+    if (S > 3 && B == 1u && after > 2u) att_barrier<4 * LD>();
+    else if (S > 2 && B == 1u && after > 1u) att_barrier<2 * LD>();
     else att_barrier<0>();
-    const uint32_t p0 = J.a + t * ATT_TILE;
-    if (t + (uint32_t)S - 1u < nt) {
-      fetch(t + S - 1u, J.k, Ks + nxt * TE, true);
-      fetch(t + S - 1u, J.v, Vs + nxt * TE, false);
-    }
-    if (p0 + ATT_TILE > least) {
-      // Values that some queries do not see: those past the end become 0, and those
-      // that are no numbers too (their weight of 0 would not be 0 times them); the
-      // queries that do see these get them at the end.
-      const uint32_t have = min(ATT_TILE, J.b - p0);
-      const bool look = !J.pre && A.T > 1u;
-      for (uint32_t i = (look ? 0u : have * PR) + threadIdx.x; i < ATT_TILE * PR; i += NW * 64) {
-        s16x8* const at = reinterpret_cast<s16x8*>(Vs + cur * TE) + i;
-        s16x8 v = {};
-        if (i < have * PR) {
-          v = *at;
-          bool any = false;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const bool bad = (v[e] & 0x7f80) == 0x7f80;
-            any |= bad;
-            v[e] = bad ? 0 : v[e];
-          }
-          if (!any) continue;
-          *odd = 1u;
-        }
-        *at = v;
+    for (uint32_t t = t0 + S - B; t < t0 + S; ++t) {
+      if (t < nt) {
+        fetch(t, J.k, Ks + nxt * TE, true);
+        fetch(t, J.v, Vs + nxt * TE, false);
       }
-      att_barrier<0>();
+      nxt = nxt + 1u == (uint32_t)S ? 0u : nxt + 1u;
     }
-    compute(Ks + cur * TE, Vs + cur * TE, p0);
-    cur = cur + 1u == (uint32_t)S ? 0u : cur + 1u;
-    nxt = nxt + 1u == (uint32_t)S ? 0u : nxt + 1u;
+#pragma unroll 1
+    for (uint32_t t = t0; t < min(nt, t0 + B); ++t) {
+      const uint32_t p0 = J.a + t * ATT_TILE;
+      if (p0 + ATT_TILE > least) clean(Vs + cur * TE, p0);
+      const __bf16* __restrict__ const kb = Ks + cur * TE;
+      const __bf16* __restrict__ const vb = Vs + cur * TE;
+      f32x4 s[NB][RB];
+      s16x4 pb[NB][RB];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        bf16x8 kf[NB];
+        read_k(kf, kb, ks);
+        mul_k(s, kf, ks);
+      }
+      refer(s, p0);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) weigh(s, pb, i);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        s16x4 vf[NB];
+        read_v(vf, vb, d);
+        mul_v(pb, vf, d);
+      }
+      cur = cur + 1u == (uint32_t)S ? 0u : cur + 1u;
+    }
   }
 #pragma unroll
   for (int j = 0; j < RB; ++j) sum[j] = sum4(sum[j]);
 
-  // Waves that took different positions of the same queries meet in LDS.
+  auto put = [&](uint32_t id, int d, f32x4 v) { *reinterpret_cast<f32x4*>(A.part + ((uint64_t)J.slot * A.NQ + id) * DP + 16u * d + 4u * lg) = v; };
+  auto tell = [&](uint32_t id, float m, float x) {
+    if (lg == 0u) A.stat[(uint64_t)J.slot * A.NQ + id] = make_float2(m, x);
+  };
   if constexpr (WP > 1) {
-    static_assert((WP / 2) * WQ * 16 * RB * DP * 4 <= 2 * S * (int)TE * 2, "the halves fit");
+    // Waves that took different positions of the same queries meet in LDS; each
+    // joins some of the elements.
+    static_assert(NW * 16 * RB * DP * 4 <= 2 * S * (int)TE * 2, "the waves' sums fit (Ks and Vs are one array)");
     f32x4* const room = reinterpret_cast<f32x4*>(Ks);
+    att_barrier<0>();
 #pragma unroll
-    for (int half = WP / 2; half > 0; half /= 2) {
-      att_barrier<0>();
-      // (Ks and Vs are one array of LDS)
-      const uint32_t pair = (wp % (uint32_t)half) * WQ + wq;
-      f32x4* const at = room + pair * (RB * DB * 64u) + l;
-      float2* const st = stats + pair * (RB * 64u) + l;
-      if (wp >= (uint32_t)half && wp < 2u * half) {
+    for (int j = 0; j < RB; ++j) {
+      if (lg == 0u) stats[(w * RB + j) * 16u + lr] = make_float2(mc[j], sum[j]);
 #pragma unroll
-        for (int j = 0; j < RB; ++j) {
-          st[j * 64u] = make_float2(mc[j], sum[j]);
-#pragma unroll
-          for (int d = 0; d < DB; ++d) at[(j * DB + d) * 64u] = acc[d][j];
-        }
-      }
-      att_barrier<0>();
-      if (wp < (uint32_t)half) {
-#pragma unroll
-        for (int j = 0; j < RB; ++j) {
-          const float2 o = st[j * 64u];
-          const float m = fmaxf(mc[j], o.x);
-          const float fa = share_of(mc[j], m), fb = share_of(o.x, m);
-          mc[j] = m;
-          sum[j] = sum[j] * fa + o.y * fb;
-#pragma unroll
-          for (int d = 0; d < DB; ++d) acc[d][j] = acc[d][j] * fa + at[(j * DB + d) * 64u] * fb;
-        }
-      }
+      for (int d = 0; d < DB; ++d) room[((w * RB + j) * DB + d) * 64u + l] = acc[d][j];
     }
-  }
-  if (wp == 0u) {
+    att_barrier<0>();
+#pragma unroll
+    for (int j = 0; j < RB; ++j) {
+      const uint32_t id = table[(wq * RB + j) * 16u + lr].id;
+      float2 st[WP];
+      float m = -INFINITY, total = 0.0f;
+#pragma unroll
+      for (int x = 0; x < WP; ++x) {
+        st[x] = stats[((x * WQ + wq) * RB + j) * 16u + lr];
+        m = fmaxf(m, st[x].x);
+      }
+#pragma unroll
+      for (int x = 0; x < WP; ++x) {
+        const float f = st[x].x == m ? 1.0f : share_of(st[x].x, m);
+        total += st[x].y * f;   // (a sum that is NaN stays)
+        st[x].x = f;
+      }
+#pragma unroll
+      for (int y = 0; y < DB / WP; ++y) {
+        const uint32_t d = wp * (DB / WP) + y;
+        f32x4 v = {};
+#pragma unroll
+        for (int x = 0; x < WP; ++x) v += room[(((x * WQ + wq) * RB + j) * DB + d) * 64u + l] * st[x].x;
+        if (id != ~0u) put(id, d, v);
+      }
+      if (wp == 0u && id != ~0u) tell(id, m, total);
+    }
+  } else {
 #pragma unroll
     for (int j = 0; j < RB; ++j) {
       const uint32_t id = table[(wq * RB + j) * 16u + lr].id;
       if (id == ~0u) continue;
-      const uint64_t to = (uint64_t)J.slot * A.NQ + id;
-      if (lg == 0u) A.stat[to] = make_float2(mc[j], sum[j]);
+      tell(id, mc[j], sum[j]);
 #pragma unroll
-      for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4*>(A.part + to * DP + 16u * d + 4u * lg) = acc[d][j];
+      for (int d = 0; d < DB; ++d) put(id, d, acc[d][j]);
     }
   }
   if (!J.pre && A.T > 1u) {
@@ -402,7 +448,7 @@ __device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J,
 template <int DP, int RB, int WQ, int WP, bool SMALL, int S>
 __global__ __launch_bounds__(WQ * WP * 64, 2) void attention_tile_kernel(AttArgs A) {
   __shared__ __align__(1024) __bf16 tiles[2][S * ATT_TILE * DP];
-  __shared__ float2 stats[4 * RB * 64];   // (the waves that meet, at most four at a time)
+  __shared__ float2 stats[WQ * WP * RB * 16];
   __shared__ AttEntry table[16 * RB * WQ < 32 ? 32 : 16 * RB * WQ];
   __shared__ uint32_t odd;
   // XCD x (workgroups go to the XCDs in turn) takes a contiguous range of the
@@ -557,11 +603,10 @@ __device__ __forceinline__ void attention_weights(const AttArgs& A, const AttWei
     for (int j = 0; j < MB; ++j) {
       const uint32_t m = m0 + 16u * j + lr;
       const AttQuery x = att_query(A, J, min(m, M - 1u));
-      const uint32_t id = (x.row * A.nt + x.t - A.t0) * A.H + x.h;
-      const __bf16* const at = A.q + (uint64_t)att_row(A, x.row) * A.qr + x.t * A.qt + x.h * A.qh;
+      const __bf16* const at = A.q + att_elements(A, J, x);
 #pragma unroll
       for (int s = 0; s < KS; ++s) q[j][s] = *reinterpret_cast<const bf16x8*>(at + min(32u * s + 8u * lg, A.D - 8u));
-      ref[j] = A.ref[id];
+      ref[j] = A.ref[att_id(A, J, x)];
       lim[j] = m >= M ? 0u : J.pre ? len : min(len, att_seen(len, A.T, x.t));
     }
     // (elements past dim: zero in the queries and, lest they be no numbers, in the keys)
@@ -626,8 +671,22 @@ size_t attention_scratch_bytes() { return ATT_SCRATCH; }
 template <int DP, int RB, int WQ, int WP, int S>
 static void att_go(hipStream_t st, const AttArgs& A, bool small) {
   const dim3 grid(((A.np + 7u) / 8u + (A.ns + 7u) / 8u) * 8u), block(WQ * WP * 64);
+  if (A.np + A.ns == 0u) return;
   if (small) hipLaunchKernelGGL((attention_tile_kernel<DP, RB, WQ, WP, true, S>), grid, block, 0, st, A);
   else hipLaunchKernelGGL((attention_tile_kernel<DP, RB, WQ, WP, false, S>), grid, block, 0, st, A);
+}
+
+// Workgroups of eight waves leave no room beside them: small suffixes go by
+// themselves, two workgroups a CU.
+template <int DP, int RB, int S, int S8>
+static void att_go_apart(hipStream_t st, const AttArgs& A, bool small) {
+  if (!small) return att_go<DP, RB, 8, 1, S8>(st, A, false);
+  AttArgs B = A;
+  B.ns = 0u;
+  att_go<DP, RB, 8, 1, S8>(st, B, false);
+  B = A;
+  B.np = 0u;
+  att_go<DP, 1, 1, 4, S>(st, B, true);
 }
 
 template <int DP>
@@ -638,13 +697,13 @@ static void attention_launch(hipStream_t st, const AttArgs& A, const AttPlan& p)
       if (p.wq == 1u) att_go<DP, 1, 1, 4, S>(st, A, p.small);
       else if (p.wq == 2u) att_go<DP, 1, 2, 2, S>(st, A, p.small);
       else if (p.wq == 4u) att_go<DP, 1, 4, 1, S>(st, A, p.small);
-      else att_go<DP, 1, 8, 1, S8>(st, A, p.small);
+      else att_go_apart<DP, 1, S, S8>(st, A, p.small);
     } else {
       if (p.rb == 1u) att_go<DP, 1, 1, 4, S>(st, A, p.small);
       else if (p.wq == 1u) att_go<DP, 2, 1, 4, S>(st, A, p.small);
       else if (p.wq == 2u) att_go<DP, 2, 2, 2, S>(st, A, p.small);
       else if (p.wq == 4u) att_go<DP, 2, 4, 1, S>(st, A, p.small);
-      else att_go<DP, 2, 8, 1, S8>(st, A, p.small);
+      else att_go_apart<DP, 2, S, S8>(st, A, p.small);
     }
   }
   if (A.slots > 16u) hipLaunchKernelGGL((attention_join_kernel<DP, 4>), dim3(A.NQ), dim3(256), 0, st, A);
