@@ -54,6 +54,7 @@ class BeamSearch:
             self._statuses = torch.zeros((max_new + 1, groups), dtype=torch.int32, device=dev)
             self.picked = BeamResult(token=e(groups, beams), beam=e(groups, beams), score=self.score, ended=self.ended,
                                      status=e(groups))
+            self._own, self._filled = e(rows), 0   # the positions of each row's own cache (attention)
             self.moved = e(groups)   # (always 0: the parents are the selection's)
 
     def step(self, logits, states=(), *, lengths=None, length_dim=None, **rule):
@@ -96,6 +97,33 @@ class BeamSearch:
             self.tokens[:, self.steps] = tokens
         self.steps += 1
         return tokens
+
+    def attention(self, q, prefix_keys, prefix_values, keys, values, *, weight=None, **kw):
+        """Queues one layer's attention of all sequences after a step
+        (Sampler.prefix_attention): q bf16[groups * beams, heads, dim], the
+        queries of the tokens that step() returned; prefix_keys and
+        prefix_values [groups, kv_heads, positions, dim], the prompts', one for
+        each group; keys and values [groups * beams, kv_heads, at least
+        max_new, dim], the sequences' own, of which the steps so far have
+        filled the first self.steps positions (these move as step's states, the
+        prompts' stay).  weight f32[groups * beams, kv_heads, max_new or more]
+        gets the own positions' weights added (a state too); the other
+        arguments are prefix_attention's.  Returns out, of q's shape."""
+        if self.steps == 0:
+            raise ValueError("the first step comes before the sequences have tokens of their own")
+        for t, name in ((q, "q"), (keys, "keys"), (values, "values")):
+            if t.shape[0] != self.groups * self.beams:
+                raise ValueError(f"{name} must have {self.groups * self.beams} rows, not {t.shape[0]}")
+        if keys.dim() != 4 or values.dim() != 4 or min(keys.shape[2], values.shape[2]) < self.steps:
+            raise ValueError(f"keys and values must hold {self.steps} positions")
+        if "lengths" in kw:
+            raise ValueError("the search itself gives the sequences' lengths")
+        with self.sampler.torch.cuda.stream(self.sampler.stream):
+            if self._filled != self.steps:   # every row's positions, the ended ones' too
+                self._filled = self.steps
+                self._own.fill_(self.steps)
+            return self.sampler.prefix_attention(q, prefix_keys, prefix_values, keys, values, lengths=self._own,
+                                                 weight=weight, **kw)
 
     def status(self) -> List[int]:
         """What first stopped each group (ROW_STATUS), 0 for one that goes on

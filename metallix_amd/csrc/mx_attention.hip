@@ -148,7 +148,6 @@ __device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J,
   constexpr int PPW = ATT_TILE / WP, NB = PPW / 16;              // positions a wave takes of a tile, blocks of 16
   constexpr int LD = ATT_TILE / (int)LR / NW;                    // loads a wave issues for keys, and for values
   constexpr uint32_t TE = ATT_TILE * DP;                         // elements of a tile
-  constexpr uint32_t B = NW == 8 && S == 4 ? 2u : 1u;            // tiles between meetings
   static_assert(LD * (int)LR * NW == (int)ATT_TILE, "the loads cover the tile");
   const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63u, lr = l & 15u, lg = l >> 4;
   const uint32_t wq = w % WQ, wp = w / WQ;
@@ -177,7 +176,7 @@ __device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J,
   }
   // The first tiles' loads are under way while the queries are found.
 #pragma unroll
-  for (uint32_t t = 0; t < (uint32_t)S - B; ++t)
+  for (uint32_t t = 0; t < (uint32_t)S - 1u; ++t)
     if (t < nt) {
       fetch(t, J.k, Ks + t * TE, true);
       fetch(t, J.v, Vs + t * TE, false);
@@ -331,46 +330,39 @@ __device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J,
     att_barrier<0>();
   };
 
-  // The workgroup meets once in B tiles.
-  uint32_t cur = 0u, nxt = S - B;
-  for (uint32_t t0 = 0; t0 < nt; t0 += B) {
-    const uint32_t after = nt - t0;
-    if (S > 3 && B == 1u && after > 2u) att_barrier<4 * LD>();
-    else if (S > 2 && B == 1u && after > 1u) att_barrier<2 * LD>();
+  uint32_t cur = 0u, nxt = S - 1u;
+  for (uint32_t t = 0; t < nt; ++t) {
+    const uint32_t after = nt - 1u - t;   // tiles still in flight, at most S - 2
+    if (S > 3 && after >= 2u) att_barrier<4 * LD>();
+    else if (S > 2 && after >= 1u) att_barrier<2 * LD>();
     else att_barrier<0>();
-#pragma unroll
-    for (uint32_t t = t0 + S - B; t < t0 + S; ++t) {
-      if (t < nt) {
-        fetch(t, J.k, Ks + nxt * TE, true);
-        fetch(t, J.v, Vs + nxt * TE, false);
-      }
-      nxt = nxt + 1u == (uint32_t)S ? 0u : nxt + 1u;
+    const uint32_t p0 = J.a + t * ATT_TILE;
+    if (t + (uint32_t)S - 1u < nt) {
+      fetch(t + S - 1u, J.k, Ks + nxt * TE, true);
+      fetch(t + S - 1u, J.v, Vs + nxt * TE, false);
     }
-#pragma unroll 1
-    for (uint32_t t = t0; t < min(nt, t0 + B); ++t) {
-      const uint32_t p0 = J.a + t * ATT_TILE;
-      if (p0 + ATT_TILE > least) clean(Vs + cur * TE, p0);
-      const __bf16* __restrict__ const kb = Ks + cur * TE;
-      const __bf16* __restrict__ const vb = Vs + cur * TE;
-      f32x4 s[NB][RB];
-      s16x4 pb[NB][RB];
+    if (p0 + ATT_TILE > least) clean(Vs + cur * TE, p0);
+    const __bf16* __restrict__ const kb = Ks + cur * TE;
+    const __bf16* __restrict__ const vb = Vs + cur * TE;
+    f32x4 s[NB][RB];
+    s16x4 pb[NB][RB];
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        bf16x8 kf[NB];
-        read_k(kf, kb, ks);
-        mul_k(s, kf, ks);
-      }
-      refer(s, p0);
-#pragma unroll
-      for (int i = 0; i < NB; ++i) weigh(s, pb, i);
-#pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        s16x4 vf[NB];
-        read_v(vf, vb, d);
-        mul_v(pb, vf, d);
-      }
-      cur = cur + 1u == (uint32_t)S ? 0u : cur + 1u;
+    for (int ks = 0; ks < KS; ++ks) {
+      bf16x8 kf[NB];
+      read_k(kf, kb, ks);
+      mul_k(s, kf, ks);
     }
+    refer(s, p0);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) weigh(s, pb, i);
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      s16x4 vf[NB];
+      read_v(vf, vb, d);
+      mul_v(pb, vf, d);
+    }
+    cur = cur + 1u == (uint32_t)S ? 0u : cur + 1u;
+    nxt = nxt + 1u == (uint32_t)S ? 0u : nxt + 1u;
   }
 #pragma unroll
   for (int j = 0; j < RB; ++j) sum[j] = sum4(sum[j]);
@@ -671,39 +663,24 @@ size_t attention_scratch_bytes() { return ATT_SCRATCH; }
 template <int DP, int RB, int WQ, int WP, int S>
 static void att_go(hipStream_t st, const AttArgs& A, bool small) {
   const dim3 grid(((A.np + 7u) / 8u + (A.ns + 7u) / 8u) * 8u), block(WQ * WP * 64);
-  if (A.np + A.ns == 0u) return;
   if (small) hipLaunchKernelGGL((attention_tile_kernel<DP, RB, WQ, WP, true, S>), grid, block, 0, st, A);
   else hipLaunchKernelGGL((attention_tile_kernel<DP, RB, WQ, WP, false, S>), grid, block, 0, st, A);
 }
 
-// Workgroups of eight waves leave no room beside them: small suffixes go by
-// themselves, two workgroups a CU.
-template <int DP, int RB, int S, int S8>
-static void att_go_apart(hipStream_t st, const AttArgs& A, bool small) {
-  if (!small) return att_go<DP, RB, 8, 1, S8>(st, A, false);
-  AttArgs B = A;
-  B.ns = 0u;
-  att_go<DP, RB, 8, 1, S8>(st, B, false);
-  B = A;
-  B.np = 0u;
-  att_go<DP, 1, 1, 4, S>(st, B, true);
-}
-
 template <int DP>
 static void attention_launch(hipStream_t st, const AttArgs& A, const AttPlan& p) {
-  constexpr int S = DP == 64 ? 4 : 2, S8 = DP == 256 ? 2 : 4;
+  constexpr int S = DP == 64 ? 4 : 2;   // tiles in LDS: 64 KB, or 128 where dim is above 128
   if (A.np + A.ns) {
     if constexpr (DP == 256) {
       if (p.wq == 1u) att_go<DP, 1, 1, 4, S>(st, A, p.small);
       else if (p.wq == 2u) att_go<DP, 1, 2, 2, S>(st, A, p.small);
       else if (p.wq == 4u) att_go<DP, 1, 4, 1, S>(st, A, p.small);
-      else att_go_apart<DP, 1, S, S8>(st, A, p.small);
+      else att_go<DP, 1, 8, 1, S>(st, A, p.small);
     } else {
       if (p.rb == 1u) att_go<DP, 1, 1, 4, S>(st, A, p.small);
       else if (p.wq == 1u) att_go<DP, 2, 1, 4, S>(st, A, p.small);
       else if (p.wq == 2u) att_go<DP, 2, 2, 2, S>(st, A, p.small);
-      else if (p.wq == 4u) att_go<DP, 2, 4, 1, S>(st, A, p.small);
-      else att_go_apart<DP, 2, S, S8>(st, A, p.small);
+      else att_go<DP, 2, 4, 1, S>(st, A, p.small);
     }
   }
   if (A.slots > 16u) hipLaunchKernelGGL((attention_join_kernel<DP, 4>), dim3(A.NQ), dim3(256), 0, st, A);

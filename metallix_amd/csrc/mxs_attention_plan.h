@@ -53,7 +53,7 @@ inline AttPlan attention_plan(uint32_t G, uint32_t W, uint32_t T, uint32_t H, ui
   const uint32_t ms = p.nt * per, m = P ? p.wb * ms : ms;   // queries that share a suffix, a prefix
   p.rb = p.dp == 256u || m <= 16u ? 1u : 2u;
   const uint32_t blocks = att_ceil(m, 16u * p.rb);
-  p.wq = blocks <= 1u ? 1u : blocks <= 2u ? 2u : blocks <= 4u ? 4u : 8u;
+  p.wq = blocks <= 1u ? 1u : blocks <= 2u ? 2u : blocks <= 4u || p.dp < 256u ? 4u : 8u;
   p.small = ms <= 16u;
   const uint32_t rows = 16u * p.rb * p.wq, nrb = att_ceil(m, rows), nsb = p.small ? 1u : att_ceil(ms, rows);
   const uint32_t tp = att_ceil(P, ATT_TILE), ts = att_ceil(N, ATT_TILE);

@@ -162,7 +162,8 @@ SHAPES = [
     (1, 64, 1, 20, 2, 80, 200, 33), (1, 4, 1, 4, 2, 256, 300, 40), (2, 20, 1, 8, 2, 256, 190, 10), (1, 9, 1, 4, 1, 192, 100, 66),
     (1, 3, 1, 2, 2, 136, 77, 8), (1, 2, 1, 2, 1, 72, 50, 50), (1, 2, 2, 2, 1, 64, 40, 2), (2, 3, 6, 6, 2, 80, 99, 30),
     (1, 4, 8, 8, 1, 128, 210, 70), (1, 2, 33, 4, 1, 64, 70, 90), (1, 1, 65, 5, 1, 128, 10, 65), (4, 1, 130, 2, 2, 64, 0, 130),
-    (1, 1, 1, 4, 1, 128, 4000, None), (5, 1, 3, 3, 3, 64, 200, 100),
+    (1, 1, 1, 4, 1, 128, 4000, None), (5, 1, 3, 3, 3, 64, 200, 100), (1, 6, 1, 8, 2, 256, 100, 12), (1, 7, 5, 4, 1, 256, 130, 40),
+    (2, 2, 3, 12, 2, 160, 70, 20), (1, 2, 9, 4, 2, 64, 75, 33),
 ]
 
 
