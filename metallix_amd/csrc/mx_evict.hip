@@ -28,6 +28,16 @@ struct EvictArgs {
   uint32_t n, first, recent;
   uint32_t parts, jobs;      // workgroups a row, of all
   uint32_t list;             // entries of the list of slots in question
+  // Where several workgroups share a long row, what earlier launches found:
+  int32_t* newest;           // [rows * parts]
+  uint32_t* counts;          // [rows * parts][EV_BINS] keys by first digit
+  struct EvictFound* found;  // [rows]; NULL: nothing was found ahead
+  unsigned long long* bits;  // [rows][words] slots with a first digit above the edge's
+  uint2* lists;              // [rows][list] slots and keys with the edge's, in any order
+};
+
+struct EvictFound {
+  uint32_t edge, need, same, count;   // the edge's first digit, how many of those that have it stay, how many there are; listed
 };
 
 typedef uint32_t ev_u32x4 __attribute__((ext_vector_type(4)));
@@ -73,16 +83,11 @@ __device__ uint32_t before_me(EvictSmem<TH>& S, uint32_t v, uint32_t& total) {
   return base + sc - v;
 }
 
-// One digit of the `need`-th largest: f(count) calls count(digit) for each key
-// that is still in question.  Returns the digit; need becomes how many to take of
-// those that have it, same how many there are.
-template <int TH, typename F>
-__device__ uint32_t next_digit(EvictSmem<TH>& S, uint32_t& need, uint32_t& same, F f) {
+// The digit of the `need`-th largest, from the digits' counts; need becomes how
+// many to take of those that have it, same how many there are.
+template <int TH>
+__device__ uint32_t pick_digit(EvictSmem<TH>& S, uint32_t& need, uint32_t& same) {
   constexpr uint32_t B = EV_BINS / TH;
-  for (uint32_t i = threadIdx.x; i < EV_BINS; i += TH) S.hist[i] = 0u;
-  __syncthreads();
-  f([&](uint32_t digit) { atomicAdd(&S.hist[digit], 1u); });
-  __syncthreads();
   uint32_t c[B], sum = 0u, total;   // the thread's digits, largest first
 #pragma unroll
   for (uint32_t j = 0; j < B; ++j) sum += c[j] = S.hist[EV_BINS - 1u - threadIdx.x * B - j];
@@ -101,6 +106,16 @@ __device__ uint32_t next_digit(EvictSmem<TH>& S, uint32_t& need, uint32_t& same,
   return S.pick[0];
 }
 
+// One digit: f(count) calls count(digit) for each key that is still in question.
+template <int TH, typename F>
+__device__ uint32_t next_digit(EvictSmem<TH>& S, uint32_t& need, uint32_t& same, F f) {
+  for (uint32_t i = threadIdx.x; i < EV_BINS; i += TH) S.hist[i] = 0u;
+  __syncthreads();
+  f([&](uint32_t digit) { atomicAdd(&S.hist[digit], 1u); });
+  __syncthreads();
+  return pick_digit<TH>(S, need, same);
+}
+
 __device__ __forceinline__ void copy_piece(char* to, const char* from, uint32_t have) {
   if (have >= 16u) {
     *reinterpret_cast<ev_u32x4_u*>(to) = *reinterpret_cast<const ev_u32x4_u*>(from);
@@ -110,6 +125,105 @@ __device__ __forceinline__ void copy_piece(char* to, const char* from, uint32_t 
   if (have & 4u) { *reinterpret_cast<ev_u32_u*>(to) = *reinterpret_cast<const ev_u32_u*>(from); to += 4; from += 4; }
   if (have & 2u) { *reinterpret_cast<ev_u16_u*>(to) = *reinterpret_cast<const ev_u16_u*>(from); to += 2; from += 2; }
   if (have & 1u) *to = *from;
+}
+
+__device__ __forceinline__ uint32_t evict_len(const EvictArgs& A, uint32_t seg) {
+  const int32_t n = A.lengths ? A.lengths[seg] : (int32_t)A.C;
+  return n <= 0 ? 0u : min((uint32_t)n, A.C);
+}
+__device__ __forceinline__ uint32_t slot_key(const EvictArgs& A, int32_t recent_from, float w, int32_t p) {
+  return p < (int32_t)A.first || p > recent_from ? 0xffffffffu : weight_key(w);
+}
+
+// Long rows that several workgroups share would each be looked at whole by all of
+// them, three times (131072 slots: 26 us a look).  Instead every workgroup looks
+// at its own slots: STEP 0 finds the newest position, 1 counts the keys' first
+// digits, 2 marks what lies above the edge's digit and lists what has it.
+template <int STEP>
+__global__ __launch_bounds__(1024) void evict_ahead_kernel(EvictArgs A) {
+  constexpr uint32_t TH = 1024u;
+  extern __shared__ unsigned long long room[];
+  __shared__ EvictSmem<1024> S;
+  const uint32_t job = (blockIdx.x & 7u) * (gridDim.x / 8u) + (blockIdx.x >> 3), tid = threadIdx.x;
+  if (job >= A.jobs) return;
+  const uint32_t part = job % A.parts, row = job / A.parts, len = evict_len(A, row / A.H % A.S);
+  if (len <= A.n) return;
+  const uint32_t span = ((len + A.parts - 1u) / A.parts + 63u) / 64u * 64u, sa = min(len, part * span), sb = min(len, sa + span);
+  const uint64_t at = (uint64_t)row * A.C;
+  const float* const weight = A.weight + at;
+  const int32_t* const index = A.index ? A.index + at : nullptr;
+  if (STEP == 0) {
+    int32_t newest = -1;
+#pragma unroll 8
+    for (uint32_t i = sa + tid; i < sb; i += TH) newest = max(newest, index[i]);
+    for (int x = 1; x < 64; x <<= 1) newest = max(newest, __shfl_xor(newest, x));
+    if ((tid & 63u) == 0u) S.wave[tid >> 6] = (uint32_t)newest;
+    __syncthreads();
+    if (tid == 0) {
+      for (uint32_t i = 1; i < TH / 64u; ++i) newest = max(newest, (int32_t)S.wave[i]);
+      A.newest[job] = newest;
+    }
+    return;
+  }
+  int32_t recent_from = INT32_MAX;
+  if (A.recent) {
+    int32_t newest = index ? -1 : (int32_t)len - 1;
+    if (index)
+      for (uint32_t i = 0; i < A.parts; ++i) newest = max(newest, A.newest[row * A.parts + i]);   // (uniform)
+    recent_from = newest - (int32_t)A.recent;
+  }
+  uint32_t need = A.n, same = 0u, edge = 0u;
+  uint2* const list = reinterpret_cast<uint2*>(room);
+  for (uint32_t i = tid; i < EV_BINS; i += TH) {
+    uint32_t c = 0u;
+    if (STEP == 2)
+#pragma unroll 8
+      for (uint32_t x = 0; x < A.parts; ++x) c += A.counts[(uint64_t)(row * A.parts + x) * EV_BINS + i];
+    S.hist[i] = c;
+  }
+  if (STEP == 1 && part == 0 && tid == 0) A.found[row].count = 0u;
+  __syncthreads();
+  if (STEP == 2) {
+    edge = pick_digit<1024>(S, need, same);
+    __syncthreads();
+    if (tid == 0) {
+      if (part == 0) A.found[row].edge = edge, A.found[row].need = need, A.found[row].same = same;
+      S.wave[0] = 0u;
+    }
+    __syncthreads();
+    if (same > A.list) return;   // (more than a list holds: the last launch looks at all of the row)
+  }
+  constexpr int U = 8;
+  for (uint32_t i0 = sa; i0 < sb; i0 += U * TH) {
+    float w[U];
+    int32_t p[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t i = min(i0 + u * TH + tid, sb - 1u);
+      w[u] = weight[i];
+      p[u] = index ? index[i] : (int32_t)i;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t i = i0 + u * TH + tid, k = slot_key(A, recent_from, w[u], p[u]);
+      if (STEP == 1) {
+        if (i < sb) atomicAdd(&S.hist[k >> 21], 1u);
+      } else {
+        const unsigned long long b = __builtin_amdgcn_ballot_w64(i < sb && k >> 21 > edge);
+        if ((tid & 63u) == 0u && i < sb) A.bits[(uint64_t)row * ((A.C + 63u) / 64u) + (i >> 6)] = b;
+        if (i < sb && k >> 21 == edge) list[atomicAdd(&S.wave[0], 1u)] = make_uint2(i, k);
+      }
+    }
+  }
+  __syncthreads();
+  if (STEP == 1) {
+    for (uint32_t i = tid; i < EV_BINS; i += TH) A.counts[(uint64_t)job * EV_BINS + i] = S.hist[i];
+    return;
+  }
+  const uint32_t count = S.wave[0];
+  if (tid == 0) S.wave[1] = atomicAdd(&A.found[row].count, count);
+  __syncthreads();
+  for (uint32_t i = tid; i < count; i += TH) A.lists[(uint64_t)row * A.list + S.wave[1] + i] = list[i];
 }
 
 // A row (layer, segment, head) and one of its parts a workgroup; KR: the keys
@@ -125,8 +239,7 @@ __global__ __launch_bounds__(TH) void evict_kernel(EvictArgs A) {
   if (job >= A.jobs) return;
   const uint32_t tid = threadIdx.x, part = job % A.parts, row = job / A.parts;
   const uint32_t h = row % A.H, seg = row / A.H % A.S, layer = row / A.H / A.S, n = A.n;
-  const int32_t l0 = A.lengths ? A.lengths[seg] : (int32_t)A.C;
-  const uint32_t len = l0 <= 0 ? 0u : min((uint32_t)l0, A.C), now = min(len, n);
+  const uint32_t len = evict_len(A, seg), now = min(len, n);
   const uint64_t at = (uint64_t)row * A.C;
   const float* const weight = A.weight + at;
   const int32_t* const index = A.index ? A.index + at : nullptr;
@@ -148,9 +261,7 @@ __global__ __launch_bounds__(TH) void evict_kernel(EvictArgs A) {
   }
   // The slots' keys: the protected ones above all, then by weight.
   int32_t recent_from = INT32_MAX;   // positions past it are protected (budget < len: 20 bits)
-  auto key_of = [&](float w, int32_t p) {
-    return p < (int32_t)A.first || p > recent_from ? 0xffffffffu : weight_key(w);
-  };
+  auto key_of = [&](float w, int32_t p) { return slot_key(A, recent_from, w, p); };
   constexpr int U = KR ? KR : 8;     // slots in flight
   uint32_t keys[U];
   int32_t where[U];
@@ -164,7 +275,9 @@ __global__ __launch_bounds__(TH) void evict_kernel(EvictArgs A) {
   };
   float held[U];
   if (KR) load(0u, held, where);
-  if (A.recent) {
+  // (a row that was listed ahead is not looked at again)
+  const bool ahead = KR == 0 && A.found && A.found[row].same <= A.list;
+  if (A.recent && !ahead) {
     int32_t newest = index ? -1 : (int32_t)len - 1;
     if (index) {
       if (KR) {
@@ -230,20 +343,30 @@ __global__ __launch_bounds__(TH) void evict_kernel(EvictArgs A) {
     }
     last = ~low & 0xfffffu;
   };
-  round(0u, each);
+  if (ahead) {
+    edge = A.found[row].edge << 21, need = A.found[row].need, same = A.found[row].same;
+  } else {
+    round(0u, each);
+  }
   if (KR == 0 && same <= A.list) {
     // The slots with the edge's first digit go into a list, and the rest is done
     // on that: two looks at all slots instead of four or more.
     uint2* const list = reinterpret_cast<uint2*>(kept + (A.C + 63u) / 64u);
-    if (tid == 0) S.wave[0] = 0u;
+    uint32_t count = same;
+    if (ahead) {
+      const uint32_t words = (A.C + 63u) / 64u;
+      for (uint32_t i = tid; i < (len + 63u) / 64u; i += TH) kept[i] = A.bits[(uint64_t)row * words + i];
+      for (uint32_t i = tid; i < count; i += TH) list[i] = A.lists[(uint64_t)row * A.list + i];
+    } else {
+      if (tid == 0) S.wave[0] = 0u;
+      __syncthreads();
+      each([&](uint32_t i, uint32_t k, bool valid) {
+        const unsigned long long b = __builtin_amdgcn_ballot_w64(valid && k >> 21 > edge >> 21);
+        if ((tid & 63u) == 0u && i < len) kept[i >> 6] = b;
+        if (valid && k >> 21 == edge >> 21) list[atomicAdd(&S.wave[0], 1u)] = make_uint2(i, k);
+      });
+    }
     __syncthreads();
-    each([&](uint32_t i, uint32_t k, bool valid) {
-      const unsigned long long b = __builtin_amdgcn_ballot_w64(valid && k >> 21 > edge >> 21);
-      if ((tid & 63u) == 0u && i < len) kept[i >> 6] = b;
-      if (valid && k >> 21 == edge >> 21) list[atomicAdd(&S.wave[0], 1u)] = make_uint2(i, k);
-    });
-    __syncthreads();
-    const uint32_t count = S.wave[0];
     auto listed = [&](auto f) {
       for (uint32_t x = tid; x < count; x += TH) f(list[x].x, list[x].y, true);
     };
@@ -341,16 +464,39 @@ __global__ __launch_bounds__(TH) void evict_kernel(EvictArgs A) {
 }
 
 template <int TH, int KR>
-static hipError_t evict_go(hipStream_t st, uint32_t rows, EvictArgs& A, uint32_t want) {
-  const uint32_t bits = (A.C + 63u) / 64u * 8u, room = (148u << 10) - bits;   // (of 160 KB, less the rest)
+static hipError_t evict_go(mxs_ctx* ctx, uint32_t rows, EvictArgs& A) {
+  const hipStream_t st = ctx->stream;
+  const uint32_t words = (A.C + 63u) / 64u, room = (148u << 10) - words * 8u;   // (of 160 KB, less the rest)
   A.list = KR ? 0u : room / 8u < 8192u ? room / 8u : 8192u;
-  const uint32_t lds = bits + A.list * 8u;
+  const uint32_t lds = words * 8u + A.list * 8u;
   hipError_t e = hipSuccess;
   if (lds > 32u << 10) e = hipFuncSetAttribute((const void*)evict_kernel<TH, KR>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   if (e != hipSuccess) return e;
-  A.parts = rows >= want ? 1u : want / rows;
+  A.parts = rows >= 256u ? 1u : 256u / rows;   // a workgroup a CU
   A.jobs = rows * A.parts;
-  hipLaunchKernelGGL((evict_kernel<TH, KR>), dim3((A.jobs + 7u) / 8u * 8u), dim3(TH), lds, st, A);
+  const dim3 grid((A.jobs + 7u) / 8u * 8u);
+  if (KR == 0 && A.parts > 1u) {
+    // (at most 255 rows: 2 MB of counts, 33 MB of bits and 17 MB of lists)
+    char* at = reinterpret_cast<char*>(ctx->attention_scratch);
+    auto take = [&](uint64_t bytes) {
+      char* const p = at;
+      at += (bytes + 255u) / 256u * 256u;
+      return p;
+    };
+    A.counts = reinterpret_cast<uint32_t*>(take((uint64_t)A.jobs * EV_BINS * 4u));
+    A.newest = reinterpret_cast<int32_t*>(take(A.jobs * 4u));
+    A.found = reinterpret_cast<EvictFound*>(take(rows * sizeof(EvictFound)));
+    A.bits = reinterpret_cast<unsigned long long*>(take((uint64_t)rows * words * 8u));
+    A.lists = reinterpret_cast<uint2*>(take((uint64_t)rows * A.list * 8u));
+    if ((uint64_t)(at - reinterpret_cast<char*>(ctx->attention_scratch)) > attention_scratch_bytes()) return hipErrorOutOfMemory;
+    const uint32_t lds2 = A.list * 8u;
+    e = hipFuncSetAttribute((const void*)evict_ahead_kernel<2>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds2);
+    if (e != hipSuccess) return e;
+    if (A.index && A.recent) hipLaunchKernelGGL(evict_ahead_kernel<0>, grid, dim3(1024), 0, st, A);
+    hipLaunchKernelGGL(evict_ahead_kernel<1>, grid, dim3(1024), 0, st, A);
+    hipLaunchKernelGGL(evict_ahead_kernel<2>, grid, dim3(1024), lds2, st, A);
+  }
+  hipLaunchKernelGGL((evict_kernel<TH, KR>), grid, dim3(TH), lds, st, A);
   return hipGetLastError();
 }
 
@@ -382,10 +528,10 @@ extern "C" int mxs_cache_evict(mxs_ctx* ctx, const mxs_evict* evict) {
     A.S = v.segments, A.H = v.heads, A.C = v.capacity, A.bytes = v.position_bytes;
     A.n = v.budget, A.first = v.keep_first, A.recent = v.keep_recent;
     const uint32_t rows = (uint32_t)(here * a_layer);
-    if (A.C <= 2048u) e = evict_go<256, 8>(ctx->stream, rows, A, 256u);
-    else if (A.C <= 8192u) e = evict_go<1024, 8>(ctx->stream, rows, A, 256u);
-    else if (A.C <= 32768u) e = evict_go<1024, 32>(ctx->stream, rows, A, 256u);
-    else e = evict_go<1024, 0>(ctx->stream, rows, A, 256u);
+    if (A.C <= 2048u) e = evict_go<256, 8>(ctx, rows, A);
+    else if (A.C <= 8192u) e = evict_go<1024, 8>(ctx, rows, A);
+    else if (A.C <= 32768u) e = evict_go<1024, 32>(ctx, rows, A);
+    else e = evict_go<1024, 0>(ctx, rows, A);
   }
   if (prev != ctx->device) (void)hipSetDevice(prev);
   if (e != hipSuccess) return hip_fail(ctx, e, "evict_kernel launch");

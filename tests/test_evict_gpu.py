@@ -201,6 +201,19 @@ def test_long_caches(torch_mod, sampler):
     check(torch, sampler, [big], None, torch.rand((1, 2, 1, 9000), generator=g, device="cuda"), None, [9000, 8500], 8000, 4, 100)
 
 
+@pytest.mark.parametrize("ties", [0.0, 4.0, 0.02])
+def test_long_rows_of_few_caches(torch_mod, sampler, ties):
+    """Rows that several workgroups share: some within the budget, distinct
+    weights, many equal ones, and nearly all equal."""
+    torch = torch_mod
+    for L, S, H, C, lengths, n, first, recent in ((1, 3, 1, 50001, [50001, 900, 33000], 1000, 4, 300), (2, 1, 2, 40000, None, 39000, 0, 0),
+                                                  (1, 2, 1, 100000, [99999, 65537], 65536, 0, 64)):
+        say(f"long rows {C} {ties}")
+        keys, values, w, index = inputs(torch, L, S, H, C, 8, seed=6, ties=ties)
+        check(torch, sampler, keys, values, w, index, lengths, n, first, recent)
+        check(torch, sampler, keys, None, w, None, lengths, n, first, recent)
+
+
 def test_nothing_to_do_and_refusals(torch_mod, sampler):
     torch = torch_mod
     from metallix_amd import SamplerError
