@@ -528,7 +528,7 @@ extern "C" int mxs_cache_evict(mxs_ctx* ctx, const mxs_evict* evict) {
     A.S = v.segments, A.H = v.heads, A.C = v.capacity, A.bytes = v.position_bytes;
     A.n = v.budget, A.first = v.keep_first, A.recent = v.keep_recent;
     const uint32_t rows = (uint32_t)(here * a_layer);
-    if (A.C <= 2048u) e = evict_go<256, 8>(ctx, rows, A);
+    if (A.C <= 2048u) e = evict_go<512, 4>(ctx, rows, A);
     else if (A.C <= 8192u) e = evict_go<1024, 8>(ctx, rows, A);
     else if (A.C <= 32768u) e = evict_go<1024, 32>(ctx, rows, A);
     else e = evict_go<1024, 0>(ctx, rows, A);
