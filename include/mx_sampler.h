@@ -418,8 +418,8 @@ int mxs_linear_bf16(mxs_ctx* ctx, const mxs_linear* linear);
  *   s[i] = scale * sum_d q[d] keys[i][d]    lse = ln sum_i exp(s[i])
  *   out[d] = sum_i exp(s[i] - lse) values[i][d]
  * over the positions that it sees; what else the caches hold, NaN included, does
- * not count.  A score of -inf weighs nothing, and a token that sees nothing, or
- * only such scores, gets out 0 and lse -inf.  A NaN or +inf among its scores makes
+ * not count.  A score of -inf weighs 0, and a token that sees nothing, or
+ * only such scores of finite values, gets out 0 and lse -inf.  A NaN or +inf among its scores makes
  * its out and lse NaN.
  * With prefix_weight or weight every position's weights exp(s - lse), summed over
  * the queries that read it, are added to its entry (positions that none sees stay as they are;

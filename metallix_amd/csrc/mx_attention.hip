@@ -5,6 +5,32 @@
 //   out = sum_i exp(s[i] - lse) values[i],  weight[i] += exp(s[i] - lse)
 //
 // over the group's prefix and, causally, the row's suffix.
+//
+// The prefix is read once for all the queries of a group that share a cache head
+// (beams x tokens x query heads a cache head), each suffix once for its own.  What
+// bounds it is that stream, 4 dim bytes a position and cache head, up to about 300
+// queries a cache head; with more, the products (4 dim flops a query and position).
+//
+// attention_tile_kernel: a workgroup takes a block of queries over a part of the
+// positions, 64 at a time, which loads write straight into LDS.  The softmax goes
+// along in one pass: scores of a tile, exponentials against a running reference,
+// products with the values.  attention_join_kernel joins a query's parts;
+// attention_weights_kernel makes the weights from the scores once more: storing the
+// scores would write and read 4 bytes a query and position, reading the keys again
+// takes 2 dim bytes a position, often still in a cache.  Parts, and not one workgroup
+// a cache head, because 8 cache heads of one request would leave 248 of 256 CUs idle.
+//
+// us a pass, dim 128 and 8 cache heads: 4 beams of 4 heads a cache head on 131072
+// positions 96 (at a large copy's 4.80 TB/s the keys and values alone take 112); 8
+// groups of these on up to 4096 positions 31.6 (24.6), with weights 48; 64 sequences of
+// 8 heads on 32768 positions 94: 733 TFLOP/s, matrix pipes 34% busy (52 at a large
+// product's rate); one request of 4 beams of 2 heads on 512 positions 8.9.
+// The 64 sequences step by step: one wave a query 27463; 64 queries a wave, whose sums
+// went back and forth between the two kinds of registers, 370; 32 a wave 249; jobs
+// spread over the XCDs (a prefix's had been on three of them) 99; two workgroups of four
+// waves a CU instead of one of eight 94.  Tried there and left, us of the tile
+// kernel's prefixes: the next tile's scores beside this one's exponentials 84, in a fixed
+// order of issue 112, as it is 78; a meeting every second tile 78.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -138,8 +164,15 @@ struct AttEntry {
 };
 
 // Scores as S^T = K Q^T on v_mfma_f32_16x16x32_bf16 (a lane holds four
-// positions of one query), sums as O^T = V^T P^T: the exponentials are the second
-// operand as they lie, values are read transposed from LDS.
+// positions of one query), sums as O^T = V^T P^T: a lane's exponentials are the
+// second operand as they lie (which positions a product takes together is free, as long
+// as both operands agree), so that they never leave the registers; values are
+// read transposed from LDS.  The exponentials are rounded to bf16 there, once: a
+// second term would cost half as many products again, and its sign would make
+// infinite values NaN; the sum and lse keep f32.
+// WQ waves take other queries (16 RB each), WP waves other positions of the tile and
+// meet at the end: with few queries the four waves split positions, so that LDS is read
+// once; 32 queries a wave is what registers hold beside the sums of 128 elements.
 template <int DP, int RB, int WQ, int WP, int S>
 __device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J, __bf16* Ks, __bf16* Vs, float2* stats,
                                               AttEntry* table, uint32_t* odd) {
@@ -492,7 +525,8 @@ __global__ __launch_bounds__(WQ * WP * 64, 2) void attention_tile_kernel(AttArgs
 }
 
 // Joins a query's parts: NWV waves a query, each lane four elements of every
-// 256 NWV / DP-th part.
+// 256 NWV / DP-th part.  Four waves from 17 parts on (128 queries of 64 parts: 4.8 us,
+// where one lane an element, part after part, took 56).
 template <int DP, int NWV>
 __device__ __forceinline__ void attention_join(const AttArgs& A, uint32_t block, f32x4 (&meet)[4][DP / 4]) {
   constexpr uint32_t LQ = DP / 4, GR = NWV * 64 / LQ;
@@ -556,7 +590,9 @@ struct AttWeights {
 
 // The weights of a chunk of positions of a cache head, by one wave: the scores
 // once more, 16 MB queries held in registers, the next positions' keys on
-// their way.
+// their way.  No two waves write one entry and the sums' order is fixed.  8 groups of 4
+// sequences, up to 4096 positions of 8 heads of 128: 17 us (62 MB read); a wave for
+// each 32 positions, which found its queries anew, took 26.
 template <int DP, int MB>
 __device__ __forceinline__ void attention_weights(const AttArgs& A, const AttWeights& G, uint64_t job) {
   constexpr int KS = DP / 32;
