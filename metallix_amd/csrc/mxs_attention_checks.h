@@ -66,7 +66,7 @@ inline const char* attention_check(const mxs_attention* a) {
   if (a->suffix && (!a->keys || !a->values)) return "a suffix needs its keys and values";
   if (a->prefix_weight && !a->prefix) return "prefix_weight needs a prefix";
   if (a->weight && !a->suffix) return "weight needs a suffix";
-  if (!(fabsf(a->scale) <= 3.0e38f)) return "scale must be finite";
+  if (!(fabsf(a->scale) <= 2.0e38f)) return "scale must be a number of at most 2e38";   // (times log2(e): finite)
   const uint64_t st[12] = {a->q_row, a->q_token, a->q_head, a->out_row, a->out_token, a->out_head,
                            a->prefix_group, a->prefix_head, a->prefix_position, a->row, a->head, a->position};
   const int used = 6 + (a->prefix ? 3 : 0);

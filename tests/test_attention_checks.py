@@ -34,7 +34,7 @@ def attention(**kw):
     a.out, a.out_row, a.out_token, a.out_head = 0x110000, 1024, 512, 64
     a.prefix_keys, a.prefix_values = 0x200000, 0x300000                                  # 102400 bytes each
     a.prefix_group, a.prefix_head, a.prefix_position = 25600, 6400, 64
-    a.keys, a.values, a.row, a.head, a.position = 0x400000, 0x500000, 2560, 640, 64      # 30720 bytes each
+    a.keys, a.values, a.row, a.head, a.position = 0x400000, 0x500000, 2560, 640, 64
     for k, v in kw.items():
         setattr(a, k, v)
     return a
@@ -49,7 +49,7 @@ ATTENTION_BAD = [
     (dict(prefix_keys=None), "prefix needs"), (dict(prefix_values=None), "prefix needs"),
     (dict(keys=None), "suffix needs"), (dict(values=None), "suffix needs"),
     (dict(prefix=0, prefix_weight=0x600000), "needs a prefix"), (dict(suffix=0, weight=0x600000), "needs a suffix"),
-    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
+    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(scale=-2.5e38), "scale"),
     (dict(q_row=1028), "multiples of 8"), (dict(out_token=516), "multiples of 8"), (dict(prefix_group=25601), "multiples of 8"),
     (dict(position=65), "multiples of 8"), (dict(q_head=1 << 41), "range"), (dict(prefix_head=1 << 41), "range"),
     (dict(prefix_position=1 << 22), "2^22"), (dict(position=1 << 22), "2^22"),

@@ -356,6 +356,41 @@ def run_only(torch, s, x):
     return out, lse, pw, w
 
 
+def test_nothing_to_see(torch_mod, sampler):
+    """No position at all: caches of none, with and without a suffix's."""
+    torch = torch_mod
+    for N in (None, 0):
+        got = run(torch, sampler, inputs(torch, 2, 3, 2, 4, 2, 64, 0, N))
+        assert bool((got["out"] == 0).all()) and bool((got["lse"] == -math.inf).all())
+
+
+def test_calls_in_a_row(torch_mod, sampler):
+    """Calls of different kinds that nothing waits between share the context's
+    scratch in turn."""
+    torch = torch_mod
+    shapes = [(1, 4, 1, 8, 4, 128, 700, 30), (2, 40, 1, 8, 2, 64, 300, 20), (1, 3, 4, 6, 2, 200, 150, 40)]
+    xs = [inputs(torch, *shape, seed=50 + i) for i, shape in enumerate(shapes)]
+    want = [run_only(torch, sampler, x) for x in xs]
+    w = torch.rand((1, 1, 2, 40000), device="cuda")
+    cache = torch.randn((1, 2, 40000, 8), device="cuda")
+    alone = sampler.cache_evict([cache.clone()], None, w, 500)
+    sampler.sync()
+    args = [(x, torch.zeros_like(a[1]), torch.zeros_like(a[2]), torch.zeros_like(a[3])) for x, a in zip(xs, want)]
+    outs = []
+    for i in range(6):
+        x, lse, pw, ww = args[i % 3]
+        pw.zero_(), ww.zero_()
+        outs.append(sampler.prefix_attention(x["q"], x["prefix_keys"], x["prefix_values"], x["keys"], x["values"], lse=lse,
+                                             prefix_weight=pw, weight=ww))
+        gone = sampler.cache_evict([cache.clone()], None, w, 500)
+    sampler.sync()
+    assert torch.equal(gone.weight, alone.weight) and torch.equal(gone.index, alone.index)
+    for i, o in enumerate(outs):
+        assert torch.equal(o, want[i % 3][0])
+    for (x, lse, pw, ww), a in zip(args, want):
+        assert torch.equal(lse, a[1]) and torch.equal(pw, a[2]) and torch.equal(ww, a[3])
+
+
 def test_nothing_to_do(torch_mod, sampler):
     torch = torch_mod
     x = inputs(torch, 2, 2, 1, 4, 2, 64, 50, 10)

@@ -232,31 +232,32 @@ def test_nothing_to_do_and_refusals(torch_mod, sampler):
     assert e.weight.shape == (0, 2, 2, 30) and torch.equal(keys[0], before)
 
 
-def test_captured_and_replayed(torch_mod):
+@pytest.mark.parametrize("C,n", [(200, 80), (50000, 3000)])
+def test_captured_and_replayed(torch_mod, C, n):
     torch = torch_mod
     from metallix_amd import Sampler
 
     side = torch.cuda.Stream()
     s = Sampler(max_rows=8, max_vocab=1024, stream=side)
     try:
-        keys, values, w, index = inputs(torch, 3, 2, 2, 200, 16, seed=1)
-        lens = torch.tensor([200, 150], dtype=torch.int32, device="cuda")
+        keys, values, w, index = inputs(torch, 3, 2, 2, C, 16, seed=1)
+        lens = torch.tensor([C, C - 50], dtype=torch.int32, device="cuda")
         torch.cuda.synchronize()
-        call = s.cache_evict_launcher(keys, values, w, 80, index=index, lengths=lens, keep_first=2, keep_recent=10)
+        call = s.cache_evict_launcher(keys, values, w, n, index=index, lengths=lens, keep_first=2, keep_recent=10)
         call()
         s.sync()
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=side):
             call()
         for i in range(4):
-            k, v, w1, i1 = inputs(torch, 3, 2, 2, 200, 16, seed=20 + i)
-            n1 = torch.tensor([200 - 50 * i, 190], dtype=torch.int32, device="cuda")
+            k, v, w1, i1 = inputs(torch, 3, 2, 2, C, 16, seed=20 + i)
+            n1 = torch.tensor([C - 50 * i, C - 10], dtype=torch.int32, device="cuda")
             for a, b in zip(keys + values + [w, index, lens], k + v + [w1, i1, n1]):
                 a.copy_(b)
             torch.cuda.synchronize()
             graph.replay()
             torch.cuda.synchronize()
-            want = check(torch, s, k, v, w1, i1, n1.tolist(), 80, 2, 10)
+            want = check(torch, s, k, v, w1, i1, n1.tolist(), n, 2, 10)
             assert torch.equal(call.out.weight, want.weight) and torch.equal(call.out.index, want.index)
             assert all(torch.equal(a, b) for a, b in zip(keys + values, k + v))
     finally:
