@@ -22,13 +22,13 @@
 //
 // us a pass, dim 128 and 8 cache heads: 4 beams of 4 heads a cache head on 131072
 // positions 96 (at a large copy's 4.80 TB/s the keys and values alone take 112); 8
-// groups of these on up to 4096 positions 31.6 (24.6), with weights 48; 64 sequences of
-// 8 heads on 32768 positions 94: 733 TFLOP/s, matrix pipes 34% busy (52 at a large
-// product's rate); one request of 4 beams of 2 heads on 512 positions 8.9.
+// groups of these on up to 4096 positions 31.5 (24.6), with weights 48; 64 sequences of
+// 8 heads on 32768 positions 93: 743 TFLOP/s, matrix pipes 34% busy (52 at a large
+// product's rate); one request of 4 beams of 2 heads on 512 positions 8.6.
 // The 64 sequences step by step: one wave a query 27463; 64 queries a wave, whose sums
 // went back and forth between the two kinds of registers, 370; 32 a wave 249; jobs
 // spread over the XCDs (a prefix's had been on three of them) 99; two workgroups of four
-// waves a CU instead of one of eight 94.  Tried there and left, us of the tile
+// waves a CU instead of one of eight 94; the join's first loads early 93.  Tried there and left, us of the tile
 // kernel's prefixes: the next tile's scores beside this one's exponentials 84, in a fixed
 // order of issue 112, as it is 78; a meeting every second tile 78.
 #include <hip/hip_runtime.h>
@@ -533,18 +533,36 @@ __device__ __forceinline__ void attention_join(const AttArgs& A, uint32_t block,
   const uint32_t w = threadIdx.x >> 6, l = threadIdx.x & 63u;
   const uint32_t id = min(block * (4u / NWV) + w / NWV, A.NQ - 1u);   // (a last workgroup's other waves: the last query once more)
   const uint32_t in = w % NWV * 64u + l, d = in % LQ * 4u, grp = in / LQ;
-  // every wave by itself: the parts' common reference and the whole sum
-  float m = -INFINITY, sum = 0.0f;
-  for (uint32_t s = l; s < A.slots; s += 64u) m = fmaxf(m, A.stat[(uint64_t)s * A.NQ + id].x);
-  for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
-  for (uint32_t s = l; s < A.slots; s += 64u) {
-    const float2 v = A.stat[(uint64_t)s * A.NQ + id];
-    sum += v.y * (v.x == m ? 1.0f : share_of(v.x, m));   // (a sum that is NaN stays)
+  // The first parts are on their way while the references are compared.
+  constexpr uint32_t AHEAD = 4;
+  f32x4 v[AHEAD] = {};
+  float at[AHEAD] = {};
+  float2 mine = make_float2(-INFINITY, 0.0f);
+  if (A.slots) {
+    if (l < A.slots) mine = A.stat[(uint64_t)l * A.NQ + id];
+#pragma unroll
+    for (uint32_t u = 0; u < AHEAD; ++u) {
+      const uint64_t s = (uint64_t)min(grp + u * GR, A.slots - 1u) * A.NQ + id;
+      v[u] = *reinterpret_cast<const f32x4*>(A.part + s * DP + d);
+      at[u] = A.stat[s].x;
+    }
   }
-  for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
+  // every wave by itself: the parts' common reference and the whole sum
+  float m = mine.x;
+  for (uint32_t s = l + 64u; s < A.slots; s += 64u) m = fmaxf(m, A.stat[(uint64_t)s * A.NQ + id].x);
+  m = wave_max_f32(m);
+  float sum = mine.y * (mine.x == m ? 1.0f : share_of(mine.x, m));   // (a sum that is NaN stays)
+  for (uint32_t s = l + 64u; s < A.slots; s += 64u) {
+    const float2 x = A.stat[(uint64_t)s * A.NQ + id];
+    sum += x.y * (x.x == m ? 1.0f : share_of(x.x, m));
+  }
+  sum = wave_sum_f32(sum);
   f32x4 o = {};
+#pragma unroll
+  for (uint32_t u = 0; u < AHEAD; ++u)
+    if (grp + u * GR < A.slots) o += v[u] * (at[u] == m ? 1.0f : share_of(at[u], m));
 #pragma unroll 4
-  for (uint32_t s = grp; s < A.slots; s += GR) {
+  for (uint32_t s = grp + AHEAD * GR; s < A.slots; s += GR) {
     const float x = A.stat[(uint64_t)s * A.NQ + id].x;
     o += *reinterpret_cast<const f32x4*>(A.part + ((uint64_t)s * A.NQ + id) * DP + d) * (x == m ? 1.0f : share_of(x, m));
   }
@@ -568,10 +586,10 @@ __device__ __forceinline__ void attention_join(const AttArgs& A, uint32_t block,
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   if (d < A.D) {
-    bf16x4 v;
+    bf16x4 to;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = (__bf16)(o[e] * inv);
-    *reinterpret_cast<bf16x4*>(A.out + (uint64_t)r * A.orow + t * A.ot + h * A.oh + d) = v;
+    for (int e = 0; e < 4; ++e) to[e] = (__bf16)(o[e] * inv);
+    *reinterpret_cast<bf16x4*>(A.out + (uint64_t)r * A.orow + t * A.ot + h * A.oh + d) = to;
   }
 }
 
