@@ -114,6 +114,9 @@ class BeamSearch:
         for t, name in ((q, "q"), (keys, "keys"), (values, "values")):
             if t.shape[0] != self.groups * self.beams:
                 raise ValueError(f"{name} must have {self.groups * self.beams} rows, not {t.shape[0]}")
+        for t, name in ((prefix_keys, "prefix_keys"), (prefix_values, "prefix_values")):
+            if t.shape[0] != self.groups:
+                raise ValueError(f"{name} must hold a prompt for each of the {self.groups} groups, not {t.shape[0]}")
         if keys.dim() != 4 or values.dim() != 4 or min(keys.shape[2], values.shape[2]) < self.steps:
             raise ValueError(f"keys and values must hold {self.steps} positions")
         if "lengths" in kw:

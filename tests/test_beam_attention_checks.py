@@ -1,0 +1,52 @@
+"""What BeamSearch.attention hands to the sampler and what it refuses, without a
+GPU: a search whose sampler only writes down what it is asked for."""
+import contextlib
+import types
+
+import pytest
+import torch
+
+from metallix_amd import BeamSearch
+
+BF, I32 = torch.bfloat16, torch.int32
+G, W, H, KV, D, P, N = 2, 3, 4, 2, 16, 20, 6
+
+
+class Recorder:
+    """Stands in for a Sampler: notes each prefix_attention call."""
+
+    def __init__(self):
+        cuda = types.SimpleNamespace(stream=lambda s: contextlib.nullcontext(), is_current_stream_capturing=lambda: False)
+        t = {n: getattr(torch, n) for n in ("full", "zeros", "empty", "arange", "int32", "bool", "float64")}
+        self.torch = types.SimpleNamespace(cuda=cuda, device=lambda *a: torch.device("cpu"), **t)
+        self.stream, self.device, self.calls = None, 0, []
+
+    def prefix_attention(self, q, *caches, **kw):
+        self.calls.append((q, caches, kw))
+        return q
+
+
+def search(steps=2, max_new=5):
+    s = BeamSearch(Recorder(), G, W, max_new)
+    s.steps = steps
+    s.score.zero_()
+    return s
+
+
+def args(groups=G):
+    return (torch.zeros(G * W, H, D, dtype=BF), torch.zeros(groups, KV, P, D, dtype=BF), torch.zeros(groups, KV, P, D, dtype=BF),
+            torch.zeros(G * W, KV, N, D, dtype=BF), torch.zeros(G * W, KV, N, D, dtype=BF))
+
+
+@pytest.mark.parametrize("groups", [0, 1, 3, G * W])
+def test_prompts_of_another_number_of_groups_are_refused(groups):
+    """(one prompt, or one for each sequence, would be read by the wrong groups without an error)"""
+    s = search()
+    with pytest.raises(ValueError, match="prefix_keys"):
+        s.attention(*args(groups))
+    q, pk, _, k, v = args()
+    with pytest.raises(ValueError, match="prefix_values"):
+        s.attention(q, pk, torch.zeros(groups, KV, P, D, dtype=BF), k, v)
+    assert not s.sampler.calls
+    s.attention(*args())
+    assert len(s.sampler.calls) == 1
