@@ -111,12 +111,12 @@ class BeamSearch:
         arguments are prefix_attention's.  Returns out, of q's shape."""
         if self.steps == 0:
             raise ValueError("the first step comes before the sequences have tokens of their own")
-        for t, name in ((q, "q"), (keys, "keys"), (values, "values")):
-            if t.shape[0] != self.groups * self.beams:
-                raise ValueError(f"{name} must have {self.groups * self.beams} rows, not {t.shape[0]}")
-        for t, name in ((prefix_keys, "prefix_keys"), (prefix_values, "prefix_values")):
-            if t.shape[0] != self.groups:
-                raise ValueError(f"{name} must hold a prompt for each of the {self.groups} groups, not {t.shape[0]}")
+        rows = self.groups * self.beams
+        for t, name, n, what in ((q, "q", rows, "rows"), (keys, "keys", rows, "rows"), (values, "values", rows, "rows"),
+                                 (prefix_keys, "prefix_keys", self.groups, "prompts, one for each group"),
+                                 (prefix_values, "prefix_values", self.groups, "prompts, one for each group")):
+            if t is None or t.dim() == 0 or t.shape[0] != n:
+                raise ValueError(f"{name} must have {n} {what}, not {None if t is None else list(t.shape)}")
         if keys.dim() != 4 or values.dim() != 4 or min(keys.shape[2], values.shape[2]) < self.steps:
             raise ValueError(f"keys and values must hold {self.steps} positions")
         if "lengths" in kw:

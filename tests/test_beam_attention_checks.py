@@ -50,3 +50,14 @@ def test_prompts_of_another_number_of_groups_are_refused(groups):
     assert not s.sampler.calls
     s.attention(*args())
     assert len(s.sampler.calls) == 1
+
+
+@pytest.mark.parametrize("i", range(5))
+@pytest.mark.parametrize("bad", [None, torch.zeros((), dtype=BF), torch.zeros(0, KV, P, D, dtype=BF)], ids=["none", "scalar", "empty"])
+def test_arguments_that_are_missing_or_have_no_rows(i, bad):
+    a = list(args())
+    a[i] = bad
+    s = search()
+    with pytest.raises(ValueError, match=("q", "prefix_keys", "prefix_values", "keys", "values")[i]):
+        s.attention(*a)
+    assert not s.sampler.calls
