@@ -54,7 +54,8 @@ class BeamSearch:
             self._statuses = torch.zeros((max_new + 1, groups), dtype=torch.int32, device=dev)
             self.picked = BeamResult(token=e(groups, beams), beam=e(groups, beams), score=self.score, ended=self.ended,
                                      status=e(groups))
-            self._own, self._filled = e(rows), 0   # the positions of each row's own cache (attention)
+            # the positions of each row's own cache after so many steps, the ended ones' too (attention)
+            self._own = torch.arange(max_new + 1, dtype=torch.int32, device=dev).view(-1, 1).repeat(1, rows)
             self.moved = e(groups)   # (always 0: the parents are the selection's)
 
     def step(self, logits, states=(), *, lengths=None, length_dim=None, **rule):
@@ -122,11 +123,8 @@ class BeamSearch:
         if "lengths" in kw:
             raise ValueError("the search itself gives the sequences' lengths")
         with self.sampler.torch.cuda.stream(self.sampler.stream):
-            if self._filled != self.steps:   # every row's positions, the ended ones' too
-                self._filled = self.steps
-                self._own.fill_(self.steps)
-            return self.sampler.prefix_attention(q, prefix_keys, prefix_values, keys, values, lengths=self._own,
-                                                 weight=weight, **kw)
+            return self.sampler.prefix_attention(q, prefix_keys, prefix_values, keys, values,
+                                                 lengths=self._own[self.steps], weight=weight, **kw)
 
     def status(self) -> List[int]:
         """What first stopped each group (ROW_STATUS), 0 for one that goes on

@@ -61,3 +61,13 @@ def test_arguments_that_are_missing_or_have_no_rows(i, bad):
     with pytest.raises(ValueError, match=("q", "prefix_keys", "prefix_values", "keys", "values")[i]):
         s.attention(*a)
     assert not s.sampler.calls
+
+
+def test_each_step_has_lengths_of_its_own():
+    """A call that is captured, and so runs later or again, keeps its step's lengths."""
+    s = search(steps=0, max_new=4)
+    s.sampler.calls.clear()
+    for s.steps in (1, 2, 2, 4):
+        s.attention(*args())
+    for (_, _, kw), n in zip(s.sampler.calls, (1, 2, 2, 4)):
+        assert kw["lengths"].tolist() == [n] * (G * W) and kw["lengths"].dtype == I32 and kw["lengths"].is_contiguous()
