@@ -99,7 +99,7 @@ class BeamSearch:
         self.steps += 1
         return tokens
 
-    def attention(self, q, prefix_keys, prefix_values, keys, values, *, weight=None, **kw):
+    def attention(self, q, prefix_keys, prefix_values, keys, values, *, lengths=None, weight=None, **kw):
         """Queues one layer's attention of all sequences after a step
         (Sampler.prefix_attention): q bf16[groups * beams, heads, dim], the
         queries of the tokens that step() returned; prefix_keys and
@@ -107,9 +107,12 @@ class BeamSearch:
         each group; keys and values [groups * beams, kv_heads, at least
         max_new, dim], the sequences' own, of which the steps so far have
         filled the first self.steps positions (these move as step's states, the
-        prompts' stay).  weight f32[groups * beams, kv_heads, max_new or more]
-        gets the own positions' weights added (a state too); the other
-        arguments are prefix_attention's.  Returns out, of q's shape."""
+        prompts' stay).  Own caches that were evicted since hold lengths[r]
+        positions, int32[groups * beams] on the device (a state too, as
+        [groups * beams, 1]), and need no room for max_new.  weight
+        f32[groups * beams, kv_heads, keys' positions] gets the own positions'
+        weights added (a state too); the other arguments are
+        prefix_attention's.  Returns out, of q's shape."""
         if self.steps == 0:
             raise ValueError("the first step comes before the sequences have tokens of their own")
         rows = self.groups * self.beams
@@ -118,13 +121,13 @@ class BeamSearch:
                                  (prefix_values, "prefix_values", self.groups, "prompts, one for each group")):
             if t is None or t.dim() == 0 or t.shape[0] != n:
                 raise ValueError(f"{name} must have {n} {what}, not {None if t is None else list(t.shape)}")
-        if keys.dim() != 4 or values.dim() != 4 or min(keys.shape[2], values.shape[2]) < self.steps:
-            raise ValueError(f"keys and values must hold {self.steps} positions")
-        if "lengths" in kw:
-            raise ValueError("the search itself gives the sequences' lengths")
+        if lengths is None:
+            if keys.dim() != 4 or values.dim() != 4 or min(keys.shape[2], values.shape[2]) < self.steps:
+                raise ValueError(f"keys and values must hold {self.steps} positions")
+            lengths = self._own[self.steps]
         with self.sampler.torch.cuda.stream(self.sampler.stream):
             return self.sampler.prefix_attention(q, prefix_keys, prefix_values, keys, values,
-                                                 lengths=self._own[self.steps], weight=weight, **kw)
+                                                 lengths=lengths, weight=weight, **kw)
 
     def status(self) -> List[int]:
         """What first stopped each group (ROW_STATUS), 0 for one that goes on

@@ -71,3 +71,14 @@ def test_each_step_has_lengths_of_its_own():
         s.attention(*args())
     for (_, _, kw), n in zip(s.sampler.calls, (1, 2, 2, 4)):
         assert kw["lengths"].tolist() == [n] * (G * W) and kw["lengths"].dtype == I32 and kw["lengths"].is_contiguous()
+
+
+def test_own_lengths():
+    """Own caches that were evicted hold fewer positions than there were steps."""
+    s = search(steps=5)
+    q, pk, pv, k, v = args()
+    own = torch.tensor([4] * (G * W), dtype=I32)
+    s.attention(q, pk, pv, k[:, :, :4], v[:, :, :4], lengths=own)
+    assert s.sampler.calls[-1][2]["lengths"] is own
+    with pytest.raises(ValueError, match="5 positions"):
+        s.attention(q, pk, pv, k[:, :, :4], v[:, :, :4])

@@ -70,3 +70,36 @@ def test_a_captured_call_says_nothing_about_eager_ones(torch_mod):
                 search.step(logits())
     finally:
         s.close()
+
+
+def test_own_caches_that_are_evicted(torch_mod):
+    """The search goes on over own caches that are held to a budget: their
+    lengths come from the eviction, and a new position goes behind what is left."""
+    torch = torch_mod
+    s, search, logits, x = setup(torch)
+    rows, budget = G * W, 4
+    try:
+        keys, values = x["keys"][:, :, :budget + 2].clone(), x["values"][:, :, :budget + 2].clone()
+        C = budget + 2
+        w = torch.zeros((1, rows, KV, C), device="cuda")
+        index = torch.arange(C, dtype=torch.int32, device="cuda").expand(1, rows, KV, C).contiguous()
+        n = torch.zeros((rows, 1), dtype=torch.int32, device="cuda")
+        for step in range(N):
+            search.step(logits(), [keys, values, w[0], index[0], n])
+            at = n.long().view(rows, 1, 1).expand(rows, KV, 1)
+            keys.scatter_(2, at[..., None].expand(-1, -1, -1, D), x["keys"][:, :, step:step + 1])
+            values.scatter_(2, at[..., None].expand(-1, -1, -1, D), x["values"][:, :, step:step + 1])
+            index[0].scatter_(2, at, step)
+            n += 1
+            w0 = w.clone()
+            out = call(search, dict(x, keys=keys, values=values), weight=w[0], lengths=n.view(-1))
+            s.sync()
+            y = dict(x, keys=keys, values=values)
+            o = definition(torch, y, n.view(-1))
+            near(torch, out[:, None], o["out"], o["tout"], f"step {step}: out")
+            near(torch, w[0], w0[0].double() + o["w"], o["tw"] + (w0[0] + 1).double() * 2.0 ** -23, f"step {step}: weight")
+            assert n.view(-1).tolist() == [min(step + 1, budget + 1)] * rows
+            e = s.cache_evict([keys], [values], w, budget, index=index, lengths=n.view(-1), keep_recent=2)
+            w, index, n = e.weight, e.index, e.lengths.view(-1, 1)
+    finally:
+        s.close()
