@@ -455,6 +455,10 @@ typedef struct {
   uint32_t reserved;
 } mxs_attention;
 int mxs_prefix_attention(mxs_ctx* ctx, const mxs_attention* attention);
+/* mxs_prefix_attention of which some rows' queries add no weights (sequences that have
+ * ended, rows that hold none): those whose entry of counted (device: groups * beams bytes;
+ * NULL => every row counts) is 0.  Their out and lse are as ever. */
+int mxs_prefix_attention_counted(mxs_ctx* ctx, const mxs_attention* attention, const uint8_t* counted);
 /* Brings caches down to `budget` positions.  A cache of a layer is keys and values
  * [segments][heads][capacity] of position_bytes; segment s uses its first
  * len = lengths[s] slots, slot i holding position index[i], and has accumulated

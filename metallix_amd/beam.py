@@ -54,6 +54,7 @@ class BeamSearch:
             self._statuses = torch.zeros((max_new + 1, groups), dtype=torch.int32, device=dev)
             self.picked = BeamResult(token=e(groups, beams), beam=e(groups, beams), score=self.score, ended=self.ended,
                                      status=e(groups))
+            self._live = None   # the step and which rows' sequences went on after it (attention)
             # the positions of each row's own cache after so many steps, the ended ones' too (attention)
             self._own = torch.arange(max_new + 1, dtype=torch.int32, device=dev).view(-1, 1).repeat(1, rows)
             self.moved = e(groups)   # (always 0: the parents are the selection's)
@@ -111,8 +112,10 @@ class BeamSearch:
         positions, int32[groups * beams] on the device (a state too, as
         [groups * beams, 1]), and need no room for max_new.  weight
         f32[groups * beams, kv_heads, keys' positions] gets the own positions'
-        weights added (a state too); the other arguments are
-        prefix_attention's.  Returns out, of q's shape."""
+        weights added (a state too).  Only rows whose sequence goes on add
+        weights: the queries of ended ones and of beams without a sequence say
+        nothing of what later tokens need (counted: other rows).  The other
+        arguments are prefix_attention's.  Returns out, of q's shape."""
         if self.steps == 0:
             raise ValueError("the first step comes before the sequences have tokens of their own")
         rows = self.groups * self.beams
@@ -126,8 +129,19 @@ class BeamSearch:
                 raise ValueError(f"keys and values must hold {self.steps} positions")
             lengths = self._own[self.steps]
         with self.sampler.torch.cuda.stream(self.sampler.stream):
+            if kw.get("counted") is None and (weight is not None or kw.get("prefix_weight") is not None):
+                kw["counted"] = self._counted()
             return self.sampler.prefix_attention(q, prefix_keys, prefix_values, keys, values,
                                                  lengths=lengths, weight=weight, **kw)
+
+    def _counted(self):
+        """The rows whose sequence goes on, bool[groups * beams], worked out once
+        a step, or in the graph where the call is captured."""
+        if self.sampler.torch.cuda.is_current_stream_capturing():
+            return ((self.score > float("-inf")) & ~self.ended).view(-1)
+        if self._live is None or self._live[0] != self.steps:
+            self._live = self.steps, ((self.score > float("-inf")) & ~self.ended).view(-1)
+        return self._live[1]
 
     def status(self) -> List[int]:
         """What first stopped each group (ROW_STATUS), 0 for one that goes on

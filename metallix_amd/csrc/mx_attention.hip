@@ -54,6 +54,7 @@ struct AttArgs {
   __bf16* out;
   uint64_t qr, qt, qh, pg, ph, pp, kr, kh, kp, orow, ot, oh;   // strides in elements
   const int32_t *plen, *len;
+  const uint8_t* counted;               // rows whose queries add to the weights; NULL: all
   float *lse, *pw, *w;
   uint32_t W, T, H, KV, D, P, N, per;   // per: query heads a cache head has
   uint32_t g0, ng, b0, wb, t0, nt;      // this launch's groups, rows of each, tokens
@@ -64,7 +65,7 @@ struct AttArgs {
   uint32_t flip;                        // 0x8000 where the scale is negative: the queries' signs
   float* part;                          // [slots][NQ][DP] sums of a part's exponentials times its values
   float2* stat;                         // [slots][NQ] the part's reference (log2) and sum
-  float* ref;                           // [NQ] log2 of a query's whole sum, inf for one that has seen nothing; NULL: no weights
+  float* ref;                           // [NQ] log2 of a query's whole sum, inf for one that has seen nothing or does not count; NULL: no weights
 };
 
 __device__ __forceinline__ uint32_t att_len(const int32_t* len, uint32_t i, uint32_t most) {
@@ -581,7 +582,7 @@ __device__ __forceinline__ void attention_join(const AttArgs& A, uint32_t block,
   const uint32_t h = id % A.H, t = A.t0 + id / A.H % A.nt, r = att_row(A, id / A.H / A.nt);
   if (l == 0u) {
     const float ref = m + __log2f(sum);
-    if (A.ref) A.ref[id] = sum == 0.0f ? INFINITY : ref;
+    if (A.ref) A.ref[id] = sum == 0.0f || (A.counted && !A.counted[r]) ? INFINITY : ref;
     if (A.lse) A.lse[((uint64_t)r * A.T + t) * A.H + h] = sum == 0.0f ? -INFINITY : ref * 0.693147181f;
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -653,7 +654,8 @@ __device__ __forceinline__ void attention_weights(const AttArgs& A, const AttWei
 #pragma unroll
       for (int s = 0; s < KS; ++s) q[j][s] = *reinterpret_cast<const bf16x8*>(at + min(32u * s + 8u * lg, A.D - 8u));
       ref[j] = A.ref[att_id(A, J, x)];
-      lim[j] = m >= M ? 0u : J.pre ? len : min(len, att_seen(len, A.T, x.t));
+      // (a reference of inf: no weights, of scores that are no numbers neither)
+      lim[j] = m >= M || ref[j] == INFINITY ? 0u : J.pre ? len : min(len, att_seen(len, A.T, x.t));
     }
     // (elements past dim: zero in the queries and, lest they be no numbers, in the keys)
 #pragma unroll
@@ -758,9 +760,13 @@ static void attention_launch(hipStream_t st, const AttArgs& A, const AttPlan& p)
 }  // namespace mxs
 
 extern "C" int mxs_prefix_attention(mxs_ctx* ctx, const mxs_attention* attention) {
+  return mxs_prefix_attention_counted(ctx, attention, nullptr);
+}
+
+extern "C" int mxs_prefix_attention_counted(mxs_ctx* ctx, const mxs_attention* attention, const uint8_t* counted) {
   using namespace mxs;
   if (!ctx) return MXS_EINVAL;
-  if (const char* m = attention_check(attention)) return fail(ctx, MXS_EINVAL, m);
+  if (const char* m = attention_check(attention, counted)) return fail(ctx, MXS_EINVAL, m);
   const mxs_attention& a = *attention;
   if (a.groups == 0 || a.beams == 0 || a.tokens == 0) return MXS_OK;
   AttArgs A{};
@@ -774,7 +780,7 @@ extern "C" int mxs_prefix_attention(mxs_ctx* ctx, const mxs_attention* attention
   A.pg = a.prefix_group, A.ph = a.prefix_head, A.pp = a.prefix_position;
   A.kr = a.row, A.kh = a.head, A.kp = a.position;
   A.orow = a.out_row, A.ot = a.out_token, A.oh = a.out_head;
-  A.plen = a.prefix_lengths, A.len = a.lengths;
+  A.plen = a.prefix_lengths, A.len = a.lengths, A.counted = counted;
   A.lse = a.lse, A.pw = a.prefix_weight, A.w = a.weight;
   A.W = a.beams, A.T = a.tokens, A.H = a.heads, A.KV = a.kv_heads, A.D = a.dim, A.P = a.prefix, A.N = a.suffix;
   A.per = a.heads / a.kv_heads;

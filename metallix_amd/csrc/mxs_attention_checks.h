@@ -51,7 +51,7 @@ inline bool rows_apart(uint64_t n0, uint64_t s0, uint64_t n1, uint64_t s1, uint6
   return true;
 }
 
-inline const char* attention_check(const mxs_attention* a) {
+inline const char* attention_check(const mxs_attention* a, const uint8_t* counted = nullptr) {
   if (!a) return "attention is required";
   if (a->groups == 0 || a->beams == 0 || a->tokens == 0) return nullptr;
   if (!a->q || !a->out) return "q and out are required";
@@ -100,10 +100,10 @@ inline const char* attention_check(const mxs_attention* a) {
                             {a->lse, queries * 4u},
                             {a->prefix_weight, (uint64_t)a->groups * a->kv_heads * a->prefix * 4u},
                             {a->weight, rows * a->kv_heads * a->suffix * 4u}};
-  const MemRange ins[7] = {{a->q, span3(rows, a->q_row * 2u, a->tokens, a->q_token * 2u, a->heads, a->q_head * 2u, D2)},
+  const MemRange ins[8] = {{a->q, span3(rows, a->q_row * 2u, a->tokens, a->q_token * 2u, a->heads, a->q_head * 2u, D2)},
                            {a->prefix ? a->prefix_keys : nullptr, pre}, {a->prefix ? a->prefix_values : nullptr, pre},
                            {a->suffix ? a->keys : nullptr, suf}, {a->suffix ? a->values : nullptr, suf},
-                           {a->prefix_lengths, a->groups * 4ull}, {a->lengths, rows * 4u}};
+                           {a->prefix_lengths, a->groups * 4ull}, {a->lengths, rows * 4u}, {counted, rows}};
   return outputs_apart(outs, ins);
 }
 

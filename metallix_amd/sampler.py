@@ -177,6 +177,7 @@ PROTOTYPES = {
     "mxs_beam_reorder_check": (ctypes.c_int, [_vp, ctypes.POINTER(MxsReorder)]),
     "mxs_linear_bf16": (ctypes.c_int, [_vp, ctypes.POINTER(MxsLinear)]),
     "mxs_prefix_attention": (ctypes.c_int, [_vp, ctypes.POINTER(MxsAttention)]),
+    "mxs_prefix_attention_counted": (ctypes.c_int, [_vp, ctypes.POINTER(MxsAttention), _vp]),
     "mxs_cache_evict": (ctypes.c_int, [_vp, ctypes.POINTER(MxsEvict)]),
     "mxs_debug_set_timing": (ctypes.c_int, [_vp, _vp]),
     "mxs_debug_floor": (ctypes.c_int, [_vp, _vp, ctypes.c_int32, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32,
@@ -500,9 +501,9 @@ def _cache_pair(torch, device, keys, values, names, shape, dtypes):
 
 
 def attention_struct(torch, device, q, prefix_keys, prefix_values, keys, values, out, *, prefix_lengths=None,
-                     lengths=None, scale=None, lse=None, prefix_weight=None, weight=None) -> MxsAttention:
-    """The mxs_attention of a call, its tensors checked against `device` and
-    each other (ValueError)."""
+                     lengths=None, scale=None, lse=None, prefix_weight=None, weight=None, counted=None) -> MxsAttention:
+    """The mxs_attention of a call (and, as its attribute, the address of
+    `counted`), its tensors checked against `device` and each other (ValueError)."""
     bf = (torch.bfloat16,)
     if q.dim() not in (3, 4):
         raise ValueError(f"q must have the shape [rows, (tokens,) heads, dim], not {list(q.shape)}")
@@ -544,6 +545,10 @@ def attention_struct(torch, device, q, prefix_keys, prefix_values, keys, values,
         if t is not None:
             _need(t, name, device, (dt,), shape)
             _dense(t, name)
+    if counted is not None:
+        _need(counted, "counted", device, (torch.bool, torch.uint8), (rows,))
+        _dense(counted, "counted")
+    a.counted = _ptr(counted)
     st = lambda t: [s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3])]
     a.q, (a.q_row, a.q_token, a.q_head) = q.data_ptr(), st(q)
     a.out, (a.out_row, a.out_token, a.out_head) = out.data_ptr(), st(out)
@@ -1161,8 +1166,9 @@ class Sampler:
         all).  scale: dim ** -0.5 by default.  lse: f32, q's shape without
         dim, gets the logarithms of the sums.  prefix_weight f32[groups,
         kv_heads, positions] and weight f32[groups * beams, kv_heads,
-        positions] get the weights of every position added.  Returns out,
-        bf16 of q's shape."""
+        positions] get the weights of every position added, those of all rows'
+        queries or, with counted (bool or uint8[groups * beams] on the device),
+        of the rows whose entry is not 0.  Returns out, bf16 of q's shape."""
         f = self.prefix_attention_launcher(q, prefix_keys, prefix_values, keys, values, out=out, **kw)
         f()
         return f.out
@@ -1176,10 +1182,10 @@ class Sampler:
             with torch.cuda.stream(self.stream):
                 out = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
         a = attention_struct(torch, dev, q, prefix_keys, prefix_values, keys, values, out, **kw)
-        fn, ctx, ap = self.lib.mxs_prefix_attention, self.ctx, ctypes.byref(a)
+        fn, ctx, ap, counted = self.lib.mxs_prefix_attention_counted, self.ctx, ctypes.byref(a), a.counted
 
         def launch():
-            rc = fn(ctx, ap)
+            rc = fn(ctx, ap, counted)
             if rc != 0:
                 self._check(rc, "mxs_prefix_attention")
 

@@ -82,3 +82,30 @@ def test_own_lengths():
     assert s.sampler.calls[-1][2]["lengths"] is own
     with pytest.raises(ValueError, match="5 positions"):
         s.attention(q, pk, pv, k[:, :, :4], v[:, :, :4])
+
+
+def test_only_live_sequences_count():
+    """Rows whose sequence has ended, or that hold none, add no weights."""
+    s = search(steps=3)
+    s.ended[0, 1] = True
+    s.score[1, 2], s.score[1, 0] = float("-inf"), float("nan")
+    w, pw = torch.zeros(G * W, KV, N), torch.zeros(G, KV, P)
+    s.attention(*args())
+    assert s.sampler.calls[-1][2].get("counted") is None   # (no weights: nothing to count)
+    for kw in (dict(weight=w), dict(prefix_weight=pw), dict(weight=w, prefix_weight=pw)):
+        s.attention(*args(), **kw)
+        assert s.sampler.calls[-1][2]["counted"].tolist() == [True, False, True, False, True, False]
+    first = s.sampler.calls[-1][2]["counted"]
+    s.steps, s.ended[0, 0] = 4, True
+    s.attention(*args(), weight=w)
+    assert s.sampler.calls[-1][2]["counted"].tolist() == [False, False, True, False, True, False]
+    assert first.tolist() == [True, False, True, False, True, False]
+    # captured: looked at when it is replayed, so worked out in the graph, each time
+    s.sampler.torch.cuda.is_current_stream_capturing = lambda: True
+    s.attention(*args(), weight=w)
+    s.attention(*args(), weight=w)
+    a, b = (c[2]["counted"] for c in s.sampler.calls[-2:])
+    assert a.tolist() == b.tolist() and a.data_ptr() != b.data_ptr()
+    every = torch.ones(G * W, dtype=torch.bool)
+    s.attention(*args(), weight=w, counted=every)
+    assert s.sampler.calls[-1][2]["counted"] is every

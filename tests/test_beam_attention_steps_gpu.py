@@ -103,3 +103,80 @@ def test_own_caches_that_are_evicted(torch_mod):
             w, index, n = e.weight, e.index, e.lengths.view(-1, 1)
     finally:
         s.close()
+
+
+def test_ended_and_empty_beams_add_no_weights(torch_mod):
+    """Of a group, one sequence that has ended, one beam without a sequence, whose
+    query is NaN, and one that goes on: the weights are the last one's."""
+    torch = torch_mod
+    end = 7
+    s, search, _, x = setup(torch, end_token=end)
+    try:
+        logits = torch.full((G * W, V), -float("inf"), device="cuda")
+        logits[0, [end, 3]] = torch.tensor([1.0, 0.5], device="cuda")          # group 0: two sequences, one of them ended
+        logits[W, [end, 4, 5]] = torch.tensor([0.1, 1.0, 0.5], device="cuda")  # group 1: three
+        search.step(logits)
+        live = [False, True, False, True, True, False]
+        assert ((search.score > -float("inf")) & ~search.ended).view(-1).tolist() == live
+        x["q"][2] = float("nan")
+        pw, w = torch.rand((G, KV, P), device="cuda"), torch.rand((G * W, KV, N), device="cuda")
+        pw0, w0 = pw.clone(), w.clone()
+        lse = torch.empty((G * W, H), device="cuda")
+        out = call(search, x, prefix_weight=pw, weight=w, lse=lse)
+        s.sync()
+        o = definition(torch, x, torch.ones(G * W))
+        near(torch, out[:, None], o["out"], o["tout"], "out")      # every row's
+        near(torch, lse[:, None], o["lse"], o["tlse"], "lse")
+        add, tol = torch.zeros_like(o["pw"]), torch.zeros_like(o["pw"])
+        for r in range(G * W):
+            g = r // W
+            if not live[r]:
+                assert torch.equal(w[r], w0[r])
+                continue
+            y = {k: v[g:g + 1] if k.startswith("prefix") else v[r:r + 1] for k, v in x.items()}
+            one = definition(torch, y, torch.ones(1))
+            add[g] += one["pw"][0]
+            tol[g] += one["tpw"][0]
+            near(torch, w[r], w0[r].double() + one["w"][0], one["tw"][0] + (w0[r] + 1).double() * 2.0 ** -23, f"weight {r}")
+        near(torch, pw, pw0.double() + add, tol + (pw0 + 1).double() * 2.0 ** -22, "prefix_weight")
+    finally:
+        s.close()
+
+
+@pytest.mark.parametrize("shape", [(2, 3, 1, 8, 2, 64, 200, 20), (1, 20, 3, 4, 1, 128, 300, 30), (2, 2, 2, 6, 1, 256, 70, 40)], ids=str)
+def test_rows_that_do_not_count(torch_mod, shape):
+    """Sampler.prefix_attention with `counted`: the weights of the rows that
+    count, bit for bit what these add where they are all there is to add."""
+    torch = torch_mod
+    from metallix_amd import Sampler
+    from test_attention_gpu import inputs
+
+    G, W, T, H, KV, D, P, N = shape
+    x = inputs(torch, *shape, seed=3, lens=[N - r % 5 for r in range(G * W)])
+    counted = torch.tensor([r % 3 != 1 for r in range(G * W)], device="cuda")
+    s = Sampler(max_rows=8, max_vocab=1024)
+    try:
+        def go(x, **kw):
+            pw, w = torch.zeros((G, KV, P), device="cuda"), torch.zeros((G * W, KV, N), device="cuda")
+            out = s.prefix_attention(x["q"], x["prefix_keys"], x["prefix_values"], x["keys"], x["values"], lengths=x["lengths"],
+                                     prefix_weight=pw, weight=w, **kw)
+            s.sync()
+            return out, pw, w
+
+        every, some, as_bytes = go(x), go(x, counted=counted), go(x, counted=counted.to(torch.uint8) * 5)
+        assert torch.equal(some[0], every[0]) and all(torch.equal(a, b) for a, b in zip(some, as_bytes))
+        assert torch.equal(some[2][counted], every[2][counted]) and not bool(some[2][~counted].any())
+        o = oracle(torch, x)
+        pw = torch.zeros_like(o["pw"])
+        for r in counted.nonzero().view(-1).tolist():
+            y = {k: v[r // W:r // W + 1] if k.startswith("prefix") else v[r:r + 1] for k, v in x.items()}
+            pw[r // W] += oracle(torch, y)["pw"][0]
+        near(torch, some[1], pw, o["tpw"], "prefix_weight")
+        poisoned = dict(x, q=x["q"].clone())
+        poisoned["q"][~counted] = float("nan")
+        got = go(poisoned, counted=counted)
+        assert torch.equal(got[1], some[1]) and torch.equal(got[2], some[2])
+        assert not bool(go(x, counted=torch.zeros_like(counted))[1].any())
+        assert all(torch.equal(a, b) for a, b in zip(go(x, counted=torch.ones_like(counted)), every))
+    finally:
+        s.close()
