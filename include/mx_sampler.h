@@ -421,6 +421,8 @@ int mxs_linear_bf16(mxs_ctx* ctx, const mxs_linear* linear);
  * not count.  A score of -inf weighs 0, and a token that sees nothing, or
  * only such scores of finite values, gets out 0 and lse -inf.  A NaN or +inf among its scores makes
  * its out and lse NaN.
+ * A value that is no number counts times its weight as any other does: an infinite one gives
+ * NaN where its weight is 0 (a score of -inf, or an exponential below 2^-126).
  * With prefix_weight or weight every position's weights exp(s - lse), summed over
  * the queries that read it, are added to its entry (positions that none sees stay as they are;
  * a query whose lse is NaN makes those that it sees NaN): what mxs_cache_evict goes by.

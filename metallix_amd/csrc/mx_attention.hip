@@ -456,16 +456,37 @@ __device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J,
   }
   if (!J.pre && A.T > 1u) {
     __syncthreads();
-    if (*odd) {   // rare: values that are no numbers, added where they are seen
-      for (uint32_t i = threadIdx.x; i < 16u * RB * WQ * A.D; i += NW * 64) {
-        const AttEntry e = table[i / A.D];
+    if (*odd) {
+      // Rare: values that are no numbers, times their weights, added where they are
+      // seen.  A wave a query: the position's score once more, its weight rounded
+      // as `weigh` does.
+      constexpr int EL = (DP + 63) / 64;   // elements a lane
+#pragma unroll 1
+      for (uint32_t x = w; x < 16u * RB * WQ; x += NW) {
+        const AttEntry e = table[x];
         if (e.id == ~0u) continue;
-        float add = 0.0f;
+        const uint64_t entry = (uint64_t)J.slot * A.NQ + e.id;
+        const float ref = A.stat[entry].x, base = ref == -INFINITY ? 0.0f : ref;
+        float add[EL] = {};
+#pragma unroll 1
         for (uint32_t p = max(J.a, least & ~(ATT_TILE - 1u)); p < e.lim; ++p) {
-          const float v = (float)J.v[p * J.stride + i % A.D];
-          if (!(fabsf(v) < INFINITY)) add += v;
+          const __bf16* const v = J.v + p * J.stride;
+          bool bad = false;
+          for (uint32_t d = l; d < A.D; d += 64u) bad |= !(fabsf((float)v[d]) < INFINITY);
+          if (!__builtin_amdgcn_ballot_w64(bad)) continue;
+          float s = 0.0f;
+          for (uint32_t d = l; d < A.D; d += 64u) s = __builtin_fmaf((float)A.q[e.at + d], (float)J.k[p * J.stride + d], s);
+          s = wave_sum_f32(s);
+          const float weight = (float)(__bf16)exp2_(__builtin_fmaf(A.flip ? -s : s, A.c, -base));
+#pragma unroll
+          for (int y = 0; y < EL; ++y) {
+            const float value = 64u * y + l < A.D ? (float)v[64u * y + l] : 0.0f;
+            if (!(fabsf(value) < INFINITY)) add[y] += weight * value;
+          }
         }
-        A.part[((uint64_t)J.slot * A.NQ + e.id) * DP + i % A.D] += add;
+#pragma unroll
+        for (int y = 0; y < EL; ++y)
+          if (add[y] != 0.0f) A.part[entry * DP + 64u * y + l] += add[y];   // (inf or NaN where it is not 0: within dim)
       }
     }
   }
