@@ -740,8 +740,9 @@ size_t attention_scratch_bytes() { return ATT_SCRATCH; }
 template <int DP, int RB, int WQ, int WP, int S>
 static void att_go(hipStream_t st, const AttArgs& A, bool small) {
   const dim3 grid(((A.np + 7u) / 8u + (A.ns + 7u) / 8u) * 8u), block(WQ * WP * 64);
-  if (small) hipLaunchKernelGGL((attention_tile_kernel<DP, RB, WQ, WP, true, S>), grid, block, 0, st, A);
-  else hipLaunchKernelGGL((attention_tile_kernel<DP, RB, WQ, WP, false, S>), grid, block, 0, st, A);
+  // (16 queries a workgroup: all that share a prefix, so that a suffix has no more)
+  if (RB * WQ == 1 || small) hipLaunchKernelGGL((attention_tile_kernel<DP, RB, WQ, WP, true, S>), grid, block, 0, st, A);
+  else if constexpr (RB * WQ > 1) hipLaunchKernelGGL((attention_tile_kernel<DP, RB, WQ, WP, false, S>), grid, block, 0, st, A);
 }
 
 template <int DP>
