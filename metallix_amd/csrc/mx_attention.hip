@@ -806,8 +806,10 @@ extern "C" int mxs_prefix_attention_counted(mxs_ctx* ctx, const mxs_attention* a
   A.lse = a.lse, A.pw = a.prefix_weight, A.w = a.weight;
   A.W = a.beams, A.T = a.tokens, A.H = a.heads, A.KV = a.kv_heads, A.D = a.dim, A.P = a.prefix, A.N = a.suffix;
   A.per = a.heads / a.kv_heads;
-  // scale log2(e); 0 becomes so little that no score shows it, since -inf times 0 is no number
-  A.c = fmaxf(fabsf(a.scale) * 1.44269504f, 1e-38f);
+  // scale log2(e); 0 becomes the least number above it (at most 5e-7 in a score), since
+  // -inf times 0 is no number
+  const float c = fabsf(a.scale) * 1.44269504f;
+  A.c = c > 0.0f ? c : 1.4013e-45f;
   A.flip = a.scale < 0.0f ? 0x8000u : 0u;
   const AttPlan p = attention_plan(a.groups, a.beams, a.tokens, a.heads, a.kv_heads, a.dim, a.prefix, a.suffix);
   A.sp = p.sp, A.ss = p.ss, A.slots = p.slots;
