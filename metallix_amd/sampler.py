@@ -1117,7 +1117,7 @@ class Sampler:
             if rc != 0:
                 self._check(rc, "mxs_beam_reorder")
 
-        launch.status, launch.keep = status, (r, states, parent, kw)
+        launch.status, launch.keep = status, (r, list(states), parent, kw)
         return launch
 
     def linear(self, x, weight, bias=None, *, activation=None, residual=None, out=None, out_dtype=None):
@@ -1212,6 +1212,7 @@ class Sampler:
         returns f() that queues it with what they then hold (f.out holds the
         outputs).  Nothing is queued here."""
         torch, dev = self.torch, self._device()
+        keys, values = list(keys), None if values is None else list(values)   # (the caller's may change)
         if out is None:
             with torch.cuda.stream(self.stream):
                 e = lambda shape, dt: torch.empty(shape, dtype=dt, device=dev)
@@ -1225,7 +1226,7 @@ class Sampler:
             if rc != 0:
                 self._check(rc, "mxs_cache_evict")
 
-        launch.out, launch.keep = out, (m, keys, values, weight, kw)
+        launch.out, launch.keep = out, (m, keys, values, weight, (out.weight, out.index, out.lengths), kw)
         return launch
 
     def mask_host(self, slot: int):
