@@ -561,7 +561,7 @@ def attention_struct(torch, device, q, prefix_keys, prefix_values, keys, values,
     a.groups, a.beams = _u32(groups, "groups"), _u32(rows // groups if groups else 0, "beams")
     a.tokens, a.heads, a.kv_heads, a.dim = _u32(tokens, "tokens"), _u32(heads, "heads"), _u32(kv, "kv_heads"), _u32(dim, "dim")
     a.prefix, a.suffix = _u32(P, "prefix"), _u32(N, "suffix")
-    a.scale = dim ** -0.5 if scale is None else float(scale)
+    a.scale = float(scale) if scale is not None else dim ** -0.5 if dim else 0.0   # (dim 0 is refused by the call)
     return a
 
 
