@@ -429,7 +429,9 @@ int mxs_linear_bf16(mxs_ctx* ctx, const mxs_linear* linear);
  *
  * q, caches and out are bf16, the elements of a head consecutive, at 16-byte
  * aligned addresses, strides in elements and multiples of 8; keys and values
- * have the same strides.  Scores, statistics and sums are f32; the exponentials are
+ * have the same strides.  Scores, statistics and sums are f32, so that an exponent is off by
+ * up to 2^-22 of the largest score; scores are to stay below 2^30 in size, from where on out,
+ * lse and weights may be no numbers.  The exponentials are
  * rounded to bf16 where they multiply the values, as the output is (2^-8 each).
  * Equal calls give equal bits.
  * The outputs meet neither an input nor one another. */
