@@ -54,7 +54,6 @@ struct AttArgs {
   __bf16* out;
   uint64_t qr, qt, qh, pg, ph, pp, kr, kh, kp, orow, ot, oh;   // strides in elements
   const int32_t *plen, *len;
-  const uint8_t* counted;               // rows whose queries add to the weights; NULL: all
   float *lse, *pw, *w;
   uint32_t W, T, H, KV, D, P, N, per;   // per: query heads a cache head has
   uint32_t g0, ng, b0, wb, t0, nt;      // this launch's groups, rows of each, tokens
@@ -244,7 +243,7 @@ __device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J,
   for (int j = 0; j < RB; ++j)
 #pragma unroll
     for (int s = 0; s < KS; ++s) q[j][s] = 32u * s + 8u * lg < A.D ? flipped(q[j][s], A.flip) : bf16x8{};
-  if (!J.pre) least = min(J.b, att_seen(J.len, A.T, A.t0));   // (of the job's first token: none ends earlier)
+  if (!J.pre) least = min(J.b, att_seen(J.len, A.T, A.t0));   // (of the launch's first token: none ends earlier)
 
   f32x4 acc[DB][RB] = {};
   float mc[RB], sum[RB];   // reference (log2) and sum of each query, the sum of this lane's positions
@@ -461,32 +460,41 @@ __device__ __forceinline__ void attention_job(const AttArgs& A, const AttJob& J,
       // seen.  A wave a query: the position's score once more, its weight rounded
       // as `weigh` does.
       constexpr int EL = (DP + 63) / 64;   // elements a lane
+      // (the kernel's first argument, read once more: held for this, it cost the loop scalar registers, one short request
+      // 8.65 -> 8.83 us)
+      const __attribute__((address_space(4))) AttArgs* B = (const __attribute__((address_space(4))) AttArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+      __asm__("" : "+s"(B));
+      const uint32_t D = B->D, NQ = B->NQ, flip = B->flip;
+      const float c = B->c;
+      const __bf16* const q = B->q;
+      float* const part = B->part;
+      const float2* const stat = B->stat;
 #pragma unroll 1
       for (uint32_t x = w; x < 16u * RB * WQ; x += NW) {
         const AttEntry e = table[x];
         if (e.id == ~0u) continue;
-        const uint64_t entry = (uint64_t)J.slot * A.NQ + e.id;
-        const float ref = A.stat[entry].x, base = ref == -INFINITY ? 0.0f : ref;
+        const uint64_t entry = (uint64_t)J.slot * NQ + e.id;
+        const float ref = stat[entry].x, base = ref == -INFINITY ? 0.0f : ref;
         float add[EL] = {};
 #pragma unroll 1
         for (uint32_t p = max(J.a, least & ~(ATT_TILE - 1u)); p < e.lim; ++p) {
           const __bf16* const v = J.v + p * J.stride;
           bool bad = false;
-          for (uint32_t d = l; d < A.D; d += 64u) bad |= !(fabsf((float)v[d]) < INFINITY);
+          for (uint32_t d = l; d < D; d += 64u) bad |= !(fabsf((float)v[d]) < INFINITY);
           if (!__builtin_amdgcn_ballot_w64(bad)) continue;
           float s = 0.0f;
-          for (uint32_t d = l; d < A.D; d += 64u) s = __builtin_fmaf((float)A.q[e.at + d], (float)J.k[p * J.stride + d], s);
+          for (uint32_t d = l; d < D; d += 64u) s = __builtin_fmaf((float)q[e.at + d], (float)J.k[p * J.stride + d], s);
           s = wave_sum_f32(s);
-          const float weight = (float)(__bf16)exp2_(__builtin_fmaf(A.flip ? -s : s, A.c, -base));
+          const float weight = (float)(__bf16)exp2_(__builtin_fmaf(flip ? -s : s, c, -base));
 #pragma unroll
           for (int y = 0; y < EL; ++y) {
-            const float value = 64u * y + l < A.D ? (float)v[64u * y + l] : 0.0f;
+            const float value = 64u * y + l < D ? (float)v[64u * y + l] : 0.0f;
             if (!(fabsf(value) < INFINITY)) add[y] += weight * value;
           }
         }
 #pragma unroll
         for (int y = 0; y < EL; ++y)
-          if (add[y] != 0.0f) A.part[entry * DP + 64u * y + l] += add[y];   // (inf or NaN where it is not 0: within dim)
+          if (add[y] != 0.0f) part[entry * DP + 64u * y + l] += add[y];   // (inf or NaN where it is not 0: within dim)
       }
     }
   }
@@ -550,7 +558,7 @@ __global__ __launch_bounds__(WQ * WP * 64, 2) void attention_tile_kernel(AttArgs
 // 256 NWV / DP-th part.  Four waves from 17 parts on (128 queries of 64 parts: 4.8 us,
 // where one lane an element, part after part, took 56).
 template <int DP, int NWV>
-__device__ __forceinline__ void attention_join(const AttArgs& A, uint32_t block, f32x4 (&meet)[4][DP / 4]) {
+__device__ __forceinline__ void attention_join(const AttArgs& A, const uint8_t* counted, uint32_t block, f32x4 (&meet)[4][DP / 4]) {
   constexpr uint32_t LQ = DP / 4, GR = NWV * 64 / LQ;
   const uint32_t w = threadIdx.x >> 6, l = threadIdx.x & 63u;
   const uint32_t id = min(block * (4u / NWV) + w / NWV, A.NQ - 1u);   // (a last workgroup's other waves: the last query once more)
@@ -603,7 +611,11 @@ __device__ __forceinline__ void attention_join(const AttArgs& A, uint32_t block,
   const uint32_t h = id % A.H, t = A.t0 + id / A.H % A.nt, r = att_row(A, id / A.H / A.nt);
   if (l == 0u) {
     const float ref = m + __log2f(sum);
-    if (A.ref) A.ref[id] = sum == 0.0f || (A.counted && !A.counted[r]) ? INFINITY : ref;
+    if (A.ref) {
+      bool none = sum == 0.0f;
+      if (counted) none |= counted[r] == 0;
+      A.ref[id] = none ? INFINITY : ref;
+    }
     if (A.lse) A.lse[((uint64_t)r * A.T + t) * A.H + h] = sum == 0.0f ? -INFINITY : ref * 0.693147181f;
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -633,7 +645,7 @@ struct AttWeights {
 // their way.  No two waves write one entry and the sums' order is fixed.  8 groups of 4
 // sequences, up to 4096 positions of 8 heads of 128: 17 us (62 MB read); a wave for
 // each 32 positions, which found its queries anew, took 26.
-template <int DP, int MB>
+template <int DP, int MB, bool SOME>
 __device__ __forceinline__ void attention_weights(const AttArgs& A, const AttWeights& G, uint64_t job) {
   constexpr int KS = DP / 32;
   const uint32_t l = threadIdx.x & 63u, lr = l & 15u, lg = l >> 4;
@@ -675,8 +687,7 @@ __device__ __forceinline__ void attention_weights(const AttArgs& A, const AttWei
 #pragma unroll
       for (int s = 0; s < KS; ++s) q[j][s] = *reinterpret_cast<const bf16x8*>(at + min(32u * s + 8u * lg, A.D - 8u));
       ref[j] = A.ref[att_id(A, J, x)];
-      // (a reference of inf: no weights, of scores that are no numbers neither)
-      lim[j] = m >= M || ref[j] == INFINITY ? 0u : J.pre ? len : min(len, att_seen(len, A.T, x.t));
+      lim[j] = m >= M ? 0u : J.pre ? len : min(len, att_seen(len, A.T, x.t));
     }
     // (elements past dim: zero in the queries and, lest they be no numbers, in the keys)
 #pragma unroll
@@ -685,6 +696,10 @@ __device__ __forceinline__ void attention_weights(const AttArgs& A, const AttWei
       for (int s = 0; s < KS; ++s) q[j][s] = 32u * s + 8u * lg < A.D ? flipped(q[j][s], A.flip) : bf16x8{};
     bf16x8 next[2][KS];
     load(next, from);
+    if constexpr (SOME) {   // a row that does not count: no weights, of scores that are no numbers neither
+#pragma unroll
+      for (int j = 0; j < MB; ++j) lim[j] = ref[j] == INFINITY ? 0u : lim[j];
+    }
     for (uint32_t p0 = from; p0 < to; p0 += 32u) {
       bf16x8 k[2][KS];
 #pragma unroll
@@ -724,15 +739,15 @@ __device__ __forceinline__ void attention_weights(const AttArgs& A, const AttWei
 }
 
 template <int DP, int NWV>
-__global__ __launch_bounds__(256) void attention_join_kernel(AttArgs A) {
+__global__ __launch_bounds__(256) void attention_join_kernel(AttArgs A, const uint8_t* counted) {   // (rows whose queries add to the weights; NULL: all)
   __shared__ f32x4 meet[4][DP / 4];
-  attention_join<DP, NWV>(A, blockIdx.x, meet);
+  attention_join<DP, NWV>(A, counted, blockIdx.x, meet);
 }
 
-template <int DP, int MB>
+template <int DP, int MB, bool SOME>
 __global__ __launch_bounds__(256) void attention_weights_kernel(AttArgs A, AttWeights G) {
   for (uint64_t job = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6); job < G.jobs; job += (uint64_t)gridDim.x * 4u)
-    attention_weights<DP, MB>(A, G, job);
+    attention_weights<DP, MB, SOME>(A, G, job);
 }
 
 size_t attention_scratch_bytes() { return ATT_SCRATCH; }
@@ -746,7 +761,7 @@ static void att_go(hipStream_t st, const AttArgs& A, bool small) {
 }
 
 template <int DP>
-static void attention_launch(hipStream_t st, const AttArgs& A, const AttPlan& p) {
+static void attention_launch(hipStream_t st, const AttArgs& A, const uint8_t* counted, const AttPlan& p) {
   constexpr int S = DP == 64 ? 4 : 2;   // tiles in LDS: 64 KB, or 128 where dim is above 128
   if (A.np + A.ns) {
     if constexpr (DP == 256) {
@@ -761,8 +776,8 @@ static void attention_launch(hipStream_t st, const AttArgs& A, const AttPlan& p)
       else att_go<DP, 2, 4, 1, S>(st, A, p.small);
     }
   }
-  if (A.slots > 16u) hipLaunchKernelGGL((attention_join_kernel<DP, 4>), dim3(A.NQ), dim3(256), 0, st, A);
-  else hipLaunchKernelGGL((attention_join_kernel<DP, 1>), dim3((A.NQ + 3u) / 4u), dim3(256), 0, st, A);
+  if (A.slots > 16u) hipLaunchKernelGGL((attention_join_kernel<DP, 4>), dim3(A.NQ), dim3(256), 0, st, A, counted);
+  else hipLaunchKernelGGL((attention_join_kernel<DP, 1>), dim3((A.NQ + 3u) / 4u), dim3(256), 0, st, A, counted);
   if (!A.pw && !A.w) return;
   AttWeights G;
   const uint64_t tp = A.pw ? att_ceil(A.P, 32u) : 0u, ts = A.w ? att_ceil(A.N, 32u) : 0u;
@@ -775,8 +790,15 @@ static void attention_launch(hipStream_t st, const AttArgs& A, const AttPlan& p)
   const uint64_t blocks = (G.jobs + 3u) / 4u;
   const dim3 grid((uint32_t)(blocks < 1u << 20 ? blocks : 1u << 20));
   const uint32_t m = (A.pw ? A.wb : 1u) * A.nt * A.per;
-  if (m <= 16u) hipLaunchKernelGGL((attention_weights_kernel<DP, 1>), grid, dim3(256), 0, st, A, G);
-  else hipLaunchKernelGGL((attention_weights_kernel<DP, DP == 256 ? 2 : 4>), grid, dim3(256), 0, st, A, G);
+  constexpr int MB = DP == 256 ? 2 : 4;
+  // (its own kernels where not all rows count: the test costs the others 0.35 of 27.3 us)
+  if (counted) {
+    if (m <= 16u) hipLaunchKernelGGL((attention_weights_kernel<DP, 1, true>), grid, dim3(256), 0, st, A, G);
+    else hipLaunchKernelGGL((attention_weights_kernel<DP, MB, true>), grid, dim3(256), 0, st, A, G);
+  } else {
+    if (m <= 16u) hipLaunchKernelGGL((attention_weights_kernel<DP, 1, false>), grid, dim3(256), 0, st, A, G);
+    else hipLaunchKernelGGL((attention_weights_kernel<DP, MB, false>), grid, dim3(256), 0, st, A, G);
+  }
 }
 
 }  // namespace mxs
@@ -802,7 +824,7 @@ extern "C" int mxs_prefix_attention_counted(mxs_ctx* ctx, const mxs_attention* a
   A.pg = a.prefix_group, A.ph = a.prefix_head, A.pp = a.prefix_position;
   A.kr = a.row, A.kh = a.head, A.kp = a.position;
   A.orow = a.out_row, A.ot = a.out_token, A.oh = a.out_head;
-  A.plen = a.prefix_lengths, A.len = a.lengths, A.counted = counted;
+  A.plen = a.prefix_lengths, A.len = a.lengths;
   A.lse = a.lse, A.pw = a.prefix_weight, A.w = a.weight;
   A.W = a.beams, A.T = a.tokens, A.H = a.heads, A.KV = a.kv_heads, A.D = a.dim, A.P = a.prefix, A.N = a.suffix;
   A.per = a.heads / a.kv_heads;
@@ -831,9 +853,9 @@ extern "C" int mxs_prefix_attention_counted(mxs_ctx* ctx, const mxs_attention* a
         A.stat = reinterpret_cast<float2*>(ctx->attention_scratch);
         A.ref = A.pw || A.w ? ctx->attention_scratch + 2ull * A.slots * A.NQ : nullptr;
         A.part = ctx->attention_scratch + ((2ull * A.slots + 1u) * A.NQ + 3u) / 4u * 4u;
-        if (p.dp == 64u) attention_launch<64>(ctx->stream, A, p);
-        else if (p.dp == 128u) attention_launch<128>(ctx->stream, A, p);
-        else attention_launch<256>(ctx->stream, A, p);
+        if (p.dp == 64u) attention_launch<64>(ctx->stream, A, counted, p);
+        else if (p.dp == 128u) attention_launch<128>(ctx->stream, A, counted, p);
+        else attention_launch<256>(ctx->stream, A, counted, p);
         e = hipGetLastError();
       }
   if (prev != ctx->device) (void)hipSetDevice(prev);
