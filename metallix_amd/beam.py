@@ -57,6 +57,7 @@ class BeamSearch:
             self._live = None   # the step and which rows' sequences went on after it (attention)
             # the positions of each row's own cache after so many steps, the ended ones' too (attention)
             self._own = torch.arange(max_new + 1, dtype=torch.int32, device=dev).view(-1, 1).repeat(1, rows)
+            self._now = None    # a step and its row of them
             self.moved = e(groups)   # (always 0: the parents are the selection's)
 
     def step(self, logits, states=(), *, lengths=None, length_dim=None, **rule):
@@ -127,7 +128,9 @@ class BeamSearch:
         if lengths is None:
             if keys.dim() != 4 or values.dim() != 4 or min(keys.shape[2], values.shape[2]) < self.steps:
                 raise ValueError(f"keys and values must hold {self.steps} positions")
-            lengths = self._own[self.steps]
+            if self._now is None or self._now[0] != self.steps:
+                self._now = self.steps, self._own[self.steps]
+            lengths = self._now[1]
         with self.sampler.torch.cuda.stream(self.sampler.stream):
             if kw.get("counted") is None and (weight is not None or kw.get("prefix_weight") is not None):
                 kw["counted"] = self._counted()
