@@ -454,7 +454,7 @@ typedef struct {
   uint32_t groups, beams, tokens; /* groups * beams * tokens * heads below 2^31 */
   uint32_t heads, kv_heads;       /* heads a multiple of kv_heads, at most 4096 */
   uint32_t dim;                   /* multiple of 8, 8..256 */
-  uint32_t prefix, suffix;        /* positions that the caches hold, below 2^30 */
+  uint32_t prefix, suffix;        /* positions that the caches hold, at most 2^30 */
   float scale;                    /* a number up to 2e38 in size; with 0 a product of -inf weighs 0 as well */
   uint32_t reserved;
 } mxs_attention;

@@ -21,10 +21,11 @@
 // a cache head, because 8 cache heads of one request would leave 248 of 256 CUs idle.
 //
 // us a pass, dim 128 and 8 cache heads: 4 beams of 4 heads a cache head on 131072
-// positions 96 (at a large copy's 4.80 TB/s the keys and values alone take 112); 8
-// groups of these on up to 4096 positions 31.5 (24.6), with weights 48; 64 sequences of
-// 8 heads on 32768 positions 93: 743 TFLOP/s, matrix pipes 34% busy (52 at a large
-// product's rate); one request of 4 beams of 2 heads on 512 positions 8.6.
+// positions 96 (at a large copy's 4.92 TB/s the keys and values alone would take 110: a
+// stream that is only read is faster); 8 groups of these on up to 4096 positions 31.2
+// (24.0), with weights 47.7; 64 sequences of 8 heads on 32768 positions 93: 742 TFLOP/s,
+// matrix pipes 34% busy (44 at a large product's rate); one request of 4 beams of 2 heads
+// on 512 positions 8.4.
 // The 64 sequences step by step: one wave a query 27463; 64 queries a wave, whose sums
 // went back and forth between the two kinds of registers, 370; 32 a wave 249; jobs
 // spread over the XCDs (a prefix's had been on three of them) 99; two workgroups of four
